@@ -843,6 +843,83 @@ int mega_block_decode_supported(int dtype, int64_t B, int64_t D, int64_t S, int6
 int64_t mega_block_decode_workspace_bytes(const mega_block_decode_args* args);
 int mega_block_decode(const mega_block_decode_args* args, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Paged key / value cache: sequences of different lengths in one pool.
+ *
+ * Stands beside the contiguous cache of the reference's attention
+ * (megalodon/modules/moving_average_gated_attention.py:92-101), which holds
+ * one length for a whole batch.  A page holds `page_size` consecutive positions
+ * of one sequence; keys (pages, page_size, heads, k_width), values (pages,
+ * page_size, heads, v_width); entry i of a sequence's row of `table` is the page
+ * of its positions i * page_size and up.  Sequences may share pages that
+ * are only read.
+ *
+ *   - 16 bits (the exponent pointers null): elements of the call's dtype;
+ *   - 8 bits: e4m3 codes and for each position and head one exponent byte e for
+ *     its key row and one for its value row: an element is code * 2^(e - 127),
+ *     e in 1 .. 254.  mega_paged_cache_write takes the smallest e that keeps the
+ *     row's largest finite magnitude at or below 448; e = 127 for a row of zeros.
+ *     Infinities and NaN become NaN.  A code that would stand for more than the
+ *     largest number of the new rows' type is rounded towards zero instead.
+ *
+ * Strides are in elements (of the pool's type; bytes for the exponents), the
+ * last axis is contiguous.  page_size is a power of two, 16 .. 65536; widths are
+ * multiples of 16, at most 4096 (k_width of an attention call: 512); pools are
+ * 16-byte aligned and their strides multiples of 16 elements.
+ *
+ * Metadata lies on the device and is not checked by the host.  Every kernel
+ * stays inside the pool and the table whatever it says: a table entry that names
+ * no page has nothing behind it (writes are dropped, reads give zeros, attention
+ * does not see its keys), positions at or behind table_width * page_size have no
+ * place, and rows that `cu` gives to no sequence are left alone.
+ * cu (batch + 1): rows cu[b] .. cu[b + 1] - 1 of the packed operands belong to
+ * sequence b; cu[0] = 0, not decreasing.
+ */
+typedef struct mega_paged_cache {
+  void *k, *v;                        /* pools: 16-bit elements of the call's dtype, or e4m3 codes */
+  uint8_t *k_exponents, *v_exponents; /* (pages, page_size, heads); both null: 16 bits */
+  int64_t k_stride[3], v_stride[3];   /* of a page, a position, a head */
+  int64_t ke_stride[3], ve_stride[3];
+  int64_t pages, page_size, heads, k_width, v_width;
+  const int32_t* table;               /* (batch, table_width) */
+  int64_t table_stride, table_width, batch;
+} mega_paged_cache;
+
+/* New rows to their places: sequence b's n = cu[b + 1] - cu[b] rows are its
+ * positions lengths[b] - n .. lengths[b] - 1 (a negative one has no place).
+ * k_new (rows, heads, k_width), v_new (rows, heads, v_width) of dtype MEGA_BF16 /
+ * MEGA_F16 with the given strides (multiples of 8 elements; 16-byte aligned).
+ * No place may be written twice in one call. */
+int mega_paged_cache_write(const mega_paged_cache* cache, int dtype, const void* k_new, int64_t k_row, int64_t k_head,
+                           const void* v_new, int64_t v_row, int64_t v_head, const int32_t* lengths, const int32_t* cu,
+                           int64_t rows, void* stream);
+
+/* Stored rows to contiguous ones: row cu[b] + i of k_out (rows, heads, k_width)
+ * and v_out (rows, heads, v_width) is position begins[b] + i of sequence b, in
+ * dtype (16-bit pools: their own type).  clear_rest = 1: rows behind cu[batch]
+ * become zeros; 0: they are left as they are. */
+int mega_paged_cache_read(const mega_paged_cache* cache, int dtype, const int32_t* begins, const int32_t* cu, int64_t rows,
+                          void* k_out, void* v_out, int clear_rest, void* stream);
+
+/* Attention of new tokens over the stored positions of their sequences, the new
+ * ones included (they are written first).  Row cu[b] + t of q (rows, q_heads,
+ * k_width) is position p = lengths[b] - n + t and sees positions lo .. p, lo the
+ * start of its chunk of `chunk` positions (chunk = 0: 0), as _InnerAttention
+ * does (moving_average_gated_attention.py:43-142):
+ *   out = sum_j softmax_j(scale q . k_j) v_j
+ * q_heads is a multiple of the cache's heads; query head h reads head
+ * h / (q_heads / heads).  A row that sees nothing, or whose scores are all -inf,
+ * becomes zeros.  What a row does not see cannot reach it, NaN and infinities
+ * included.  float32 scores, softmax and sums; probabilities are rounded to
+ * dtype for the matrix cores.
+ * out (rows, q_heads, v_width) contiguous; clear_rest as above.  workspace:
+ * mega_paged_attention_workspace_bytes(...) bytes (0: none is needed), used by
+ * this call alone while it runs. */
+int64_t mega_paged_attention_workspace_bytes(const mega_paged_cache* cache, int64_t rows, int64_t q_heads, int64_t chunk);
+int mega_paged_attention_fwd(const mega_paged_cache* cache, int dtype, const void* q, int64_t q_row, int64_t q_head,
+                             const int32_t* lengths, const int32_t* cu, int64_t rows, int64_t q_heads, double scale,
+                             int64_t chunk, void* out, int clear_rest, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -51,5 +51,6 @@ inline bool has_tangent(const Tensor& t) { return t._fw_grad(/*level=*/0).define
 
 void bind_decode(py::module_& m);
 void bind_ops(py::module_& m);
+void bind_paged(py::module_& m);
 
 }  // namespace mega_host

@@ -4,4 +4,5 @@
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   mega_host::bind_decode(m);
   mega_host::bind_ops(m);
+  mega_host::bind_paged(m);
 }

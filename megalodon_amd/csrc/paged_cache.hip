@@ -1,0 +1,290 @@
+// Rows into and out of the paged key / value cache.
+//
+// A row is one position's key or value of one head.  16 bits: a copy.  8 bits: the row's largest finite
+// magnitude a gives the exponent, e = min { e : a <= 448 2^e }, read off a's own bits (448 = 0.875 * 2^9:
+// with a = f 2^x, 0.5 <= f < 1, it is x - 9 where f <= 0.875 and x - 8 above); code = e4m3(x 2^-e), to nearest,
+// ties to even.  A power of two costs an e4m3 number nothing (its relative step is the same at every scale short of
+// its subnormals), makes both the division and the way back exact, and takes one byte a row.
+//
+// Bound by HBM: a row is read once and written once.  A group of 16, 32 or 64 lanes takes a row, each lane
+// pieces of eight elements (one 16-byte access of 16-bit ones), which it keeps in registers between the maximum
+// and the codes.  Keys and values are rows of the same launch: the first workgroups take keys, the others values.
+#include "paged.hpp"
+
+namespace mega {
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kPieces = kMaxCacheWidth / (8 * kWave);  // of a row of the greatest width, to a lane
+
+struct Side {
+  PagedPool pool;
+  void* rows;          // packed rows: new ones (write) or those handed out (read)
+  int64_t row, head;   // their strides
+  int lanes, lanes_log2;     // to a row
+};
+struct CacheArgs {
+  PagedView view;
+  Side side[2];
+  const int32_t *first, *cu;  // first: lengths (write), begins (read)
+  int32_t rows, heads;
+  uint32_t key_groups;        // workgroups that take keys
+  int clear_rest;
+};
+
+// Where a lane's row is.
+struct Place {
+  int64_t slot, eslot;  // element offsets of the position's row in the pool, -1: nowhere
+  int64_t packed;       // ... and in the packed operand
+  bool row, owned;      // there is such a row; a sequence has it
+};
+
+template <bool kWrite>
+__device__ __forceinline__ Place find_place(const CacheArgs& a, const Side& s, uint32_t group) {
+  const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
+  const int per_wave = kWave >> s.lanes_log2;
+  const int64_t items = static_cast<int64_t>(a.rows) * a.heads;
+  const int64_t item0 = (static_cast<int64_t>(group) * kWaves + wave) * per_wave, item = item0 + (lane >> s.lanes_log2);
+  Place p{-1, -1, 0, item < items, false};
+  if (item0 >= items) return p;  // (the whole wave)
+  const int32_t* cu = a.cu;
+  const int t0 = static_cast<int>(item0 / a.heads);
+  int b = last_not_above(a.view.batch, t0, [&](int i) { return static_cast<int64_t>(cu[i]); });
+  if (!p.row) return p;
+  const int t = static_cast<int>(item / a.heads), h = static_cast<int>(item - static_cast<int64_t>(t) * a.heads);
+  p.packed = t * s.row + h * s.head;
+  while (b + 1 < a.view.batch && cu[b + 1] <= t) ++b;  // (a wave's rows may be of several sequences)
+  const int start = row_bound(cu, b, a.rows), end = row_bound(cu, b + 1, a.rows);
+  if (t < start || t >= end) return p;
+  p.owned = true;
+  const int64_t position = kWrite ? static_cast<int64_t>(a.first[b]) - (end - t) : static_cast<int64_t>(a.first[b]) + (t - start);
+  if (position < 0 || (position >> a.view.page_shift) >= a.view.table_width) return p;
+  const uint32_t page = static_cast<uint32_t>(a.view.table[b * a.view.table_stride + (position >> a.view.page_shift)]);
+  if (page >= static_cast<uint32_t>(a.view.pages)) return p;
+  const int64_t in_page = position & ((int64_t{1} << a.view.page_shift) - 1);
+  p.slot = page * s.pool.page + in_page * s.pool.slot + static_cast<int64_t>(h) * s.pool.head;
+  p.eslot = page * s.pool.ePage + in_page * s.pool.eSlot + static_cast<int64_t>(h) * s.pool.eHead;
+  return p;
+}
+
+// |x| of a 16-bit pattern, 0 where it is not finite
+template <int DT>
+__device__ __forceinline__ uint32_t finite_magnitude(uint32_t bits) {
+  const uint32_t top = DT == MEGA_BF16 ? 0x7f80u : 0x7c00u, m = bits & 0x7fffu;
+  return m < top ? m : 0;
+}
+
+template <int DT, bool kEight>
+__global__ __launch_bounds__(kThreads) void paged_write_kernel(CacheArgs a) {
+  const bool values = blockIdx.x >= a.key_groups;
+  const Side& s = a.side[values];
+  const Place p = find_place<true>(a, s, blockIdx.x - (values ? a.key_groups : 0));
+  const int l = (static_cast<int>(threadIdx.x) & (s.lanes - 1)) * 8, stride = s.lanes * 8, width = s.pool.width;
+  const uint16_t* from = static_cast<const uint16_t*>(s.rows) + p.packed;
+  if (!kEight) {
+    if (p.slot < 0) return;
+    uint16_t* to = static_cast<uint16_t*>(s.pool.rows) + p.slot;
+    uint4 x[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (l + i * stride < width) x[i] = *reinterpret_cast<const uint4*>(from + l + i * stride);
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      if (l + i * stride < width) *reinterpret_cast<uint4*>(to + l + i * stride) = x[i];
+    return;
+  }
+  uint4 x[kPieces];
+  uint32_t top = 0;  // (bit patterns of non-negative numbers are ordered as the numbers are)
+  if (p.slot >= 0) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      if (l + i * stride < width) {
+        x[i] = *reinterpret_cast<const uint4*>(from + l + i * stride);
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = max(top, max(finite_magnitude<DT>(w[j] & 0xffffu), finite_magnitude<DT>(w[j] >> 16)));
+      }
+  }
+  for (int off = 1; off < s.lanes; off <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
+  if (p.slot < 0) return;
+  int e = 0;
+  if (top != 0) {
+    int power;
+    const float fraction = frexpf(DT == MEGA_BF16 ? bf16_bits_to_float(top) : f16_bits_to_float(top), &power);
+    e = max(fraction > 0.875f ? power - 8 : power - 9, -126);
+  }
+  const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  // 256 2^e is twice the type's greatest power of two: a magnitude that would round to it stays at 240
+  const float limit = e == (DT == MEGA_BF16 ? 120 : 8) ? 240.f : 448.f;
+  uint8_t* to = static_cast<uint8_t*>(s.pool.rows) + p.slot;
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i)
+    if (l + i * stride < width) {
+      float v[8];
+      unpack8<DT>(x[i], v);
+      int code[2] = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float y = v[j] * down;
+        v[j] = fabsf(v[j]) < __builtin_inff() ? fminf(fmaxf(y, -limit), limit) : __builtin_nanf("");
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        code[j] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j], v[4 * j + 1], 0, false);
+        code[j] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j + 2], v[4 * j + 3], code[j], true);
+      }
+      *reinterpret_cast<uint2*>(to + l + i * stride) = make_uint2(static_cast<uint32_t>(code[0]), static_cast<uint32_t>(code[1]));
+    }
+  if (l == 0) s.pool.exponents[p.eslot] = static_cast<uint8_t>(e + 127);
+}
+
+// two e4m3 codes of a word's lower or upper half times a power of two, as 16-bit numbers
+template <int DT, bool kUpper>
+__device__ __forceinline__ uint32_t widen(uint32_t codes, float scale) {
+  if (DT == MEGA_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, kUpper));
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, kUpper));
+}
+
+template <int DT, bool kEight>
+__global__ __launch_bounds__(kThreads) void paged_read_kernel(CacheArgs a) {
+  const bool values = blockIdx.x >= a.key_groups;
+  const Side& s = a.side[values];
+  const Place p = find_place<false>(a, s, blockIdx.x - (values ? a.key_groups : 0));
+  if (!p.row || !(p.owned || a.clear_rest)) return;
+  const int l = (static_cast<int>(threadIdx.x) & (s.lanes - 1)) * 8, stride = s.lanes * 8, width = s.pool.width;
+  uint16_t* to = static_cast<uint16_t*>(s.rows) + p.packed;
+  uint4 x[kPieces];
+  float scale = 0.f;
+  if (kEight && p.slot >= 0) scale = exponent_value(s.pool.exponents[p.eslot]);
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i)
+    if (l + i * stride < width) {
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (p.slot < 0) continue;
+      if (kEight) {
+        const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.pool.rows) + p.slot + l + i * stride);
+        x[i].x = c.x, x[i].y = c.y;
+      } else {
+        x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(s.pool.rows) + p.slot + l + i * stride);
+      }
+    }
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i)
+    if (l + i * stride < width) {
+      if (kEight)
+        x[i] = make_uint4(widen<DT, false>(x[i].x, scale), widen<DT, true>(x[i].x, scale), widen<DT, false>(x[i].y, scale),
+                          widen<DT, true>(x[i].y, scale));
+      *reinterpret_cast<uint4*>(to + l + i * stride) = x[i];
+    }
+}
+
+// lanes to a row: as few as take it in one piece each, 16 at the least
+void split_row(Side& s) {
+  s.lanes = 16, s.lanes_log2 = 4;
+  while (s.lanes < kWave && s.lanes * 8 < s.pool.width) s.lanes *= 2, ++s.lanes_log2;
+}
+int64_t groups_of(const Side& s, int64_t rows, int64_t heads) {
+  const int64_t per_group = static_cast<int64_t>(kWaves) * (kWave / s.lanes);
+  return (rows * heads + per_group - 1) / per_group;
+}
+
+template <typename K>
+int launch(K kernel, const CacheArgs& a, int64_t groups, void* stream) {
+  kernel<<<dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, static_cast<hipStream_t>(stream)>>>(a);
+  MEGA_CHECK_LAUNCH();
+  return MEGA_OK;
+}
+
+bool unaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
+
+}  // namespace
+
+int check_paged_cache(const mega_paged_cache* c, int dtype, const char* who) {
+  MEGA_CHECK_ARG(c != nullptr, "%s: null cache", who);
+  MEGA_CHECK_ARG(dtype == MEGA_BF16 || dtype == MEGA_F16, "%s: dtype must be MEGA_BF16 or MEGA_F16", who);
+  MEGA_CHECK_ARG(c->batch >= 0 && c->batch <= 0x7fffffff && c->heads >= 1 && c->heads <= 65536, "%s: bad batch or heads", who);
+  MEGA_CHECK_ARG(c->page_size >= kMinPage && c->page_size <= kMaxPage && (c->page_size & (c->page_size - 1)) == 0,
+                 "%s: page_size must be a power of two, 16 .. 65536", who);
+  MEGA_CHECK_ARG(c->pages >= 1 && c->pages <= 0x7fffffff, "%s: bad number of pages", who);
+  MEGA_CHECK_ARG(c->table_width >= 0 && c->table_width * c->page_size <= 0x7fffffff && c->table_stride >= 0,
+                 "%s: a row of the table holds up to 2^31 - 1 positions", who);
+  for (const int64_t w : {c->k_width, c->v_width})
+    MEGA_CHECK_ARG(w >= 16 && w <= kMaxCacheWidth && w % 16 == 0, "%s: widths must be multiples of 16, 16 .. 4096", who);
+  MEGA_CHECK_ARG(c->k != nullptr && c->v != nullptr && (c->table != nullptr || c->batch == 0 || c->table_width == 0), "%s: null pointer", who);
+  MEGA_CHECK_ARG((c->k_exponents == nullptr) == (c->v_exponents == nullptr), "%s: exponents of keys and values go together", who);
+  MEGA_CHECK_ARG(!unaligned(c->k) && !unaligned(c->v), "%s: pools must be 16-byte aligned", who);
+  // (offsets inside a page are 32-bit numbers)
+  const auto fits = [&](const int64_t* st, int64_t unit) {
+    for (int i = 0; i < 3; ++i)
+      if (st[i] < 0 || st[i] % unit != 0 || st[i] > (int64_t{1} << 40)) return false;
+    return st[1] <= 0x3fffffff / c->page_size && st[2] <= 0x7fffffff;
+  };
+  MEGA_CHECK_ARG(fits(c->k_stride, 16) && fits(c->v_stride, 16), "%s: pool strides must be multiples of 16 elements, a page's positions within 2^30", who);
+  MEGA_CHECK_ARG(c->k_exponents == nullptr || (fits(c->ke_stride, 1) && fits(c->ve_stride, 1)), "%s: bad exponent strides", who);
+  return MEGA_OK;
+}
+
+PagedView paged_view(const mega_paged_cache* c) {
+  PagedView v{c->table, c->table_stride, static_cast<int32_t>(c->table_width), static_cast<int32_t>(c->batch), static_cast<int32_t>(c->pages), 0};
+  while ((int64_t{1} << v.page_shift) < c->page_size) ++v.page_shift;
+  return v;
+}
+
+PagedPool paged_pool(const mega_paged_cache* c, bool values) {
+  const int64_t *st = values ? c->v_stride : c->k_stride, *est = values ? c->ve_stride : c->ke_stride;
+  PagedPool p{values ? c->v : c->k, values ? c->v_exponents : c->k_exponents, st[0], 0, static_cast<int32_t>(st[1]), static_cast<int32_t>(st[2]), 0, 0,
+              static_cast<int32_t>(values ? c->v_width : c->k_width)};
+  if (p.exponents != nullptr) p.ePage = est[0], p.eSlot = static_cast<int32_t>(est[1]), p.eHead = static_cast<int32_t>(est[2]);
+  return p;
+}
+
+}  // namespace mega
+
+using namespace mega;
+
+extern "C" int mega_paged_cache_write(const mega_paged_cache* cache, int dtype, const void* k_new, int64_t k_row, int64_t k_head,
+                                      const void* v_new, int64_t v_row, int64_t v_head, const int32_t* lengths, const int32_t* cu,
+                                      int64_t rows, void* stream) {
+  if (const int rc = check_paged_cache(cache, dtype, "mega_paged_cache_write"); rc != MEGA_OK) return rc;
+  MEGA_CHECK_ARG(rows >= 0 && rows <= 0x7fffffff, "mega_paged_cache_write: bad number of rows");
+  if (rows == 0 || cache->batch == 0) return MEGA_OK;
+  MEGA_CHECK_ARG(k_new != nullptr && v_new != nullptr && lengths != nullptr && cu != nullptr, "mega_paged_cache_write: null pointer");
+  MEGA_CHECK_ARG(!unaligned(k_new) && !unaligned(v_new) && k_row % 8 == 0 && k_head % 8 == 0 && v_row % 8 == 0 && v_head % 8 == 0,
+                 "mega_paged_cache_write: new rows must be 16-byte aligned");
+  CacheArgs a{paged_view(cache), {{paged_pool(cache, false), const_cast<void*>(k_new), k_row, k_head, 0, 0},
+                                  {paged_pool(cache, true), const_cast<void*>(v_new), v_row, v_head, 0, 0}},
+              lengths, cu, static_cast<int32_t>(rows), static_cast<int32_t>(cache->heads), 0, 0};
+  split_row(a.side[0]), split_row(a.side[1]);
+  const int64_t kg = groups_of(a.side[0], rows, cache->heads), vg = groups_of(a.side[1], rows, cache->heads);
+  MEGA_CHECK_ARG(kg + vg <= 0x7fffffff, "mega_paged_cache_write: too many rows for one launch");
+  a.key_groups = static_cast<uint32_t>(kg);
+  const bool eight = cache->k_exponents != nullptr;
+  if (dtype == MEGA_BF16)
+    return eight ? launch(paged_write_kernel<MEGA_BF16, true>, a, kg + vg, stream) : launch(paged_write_kernel<MEGA_BF16, false>, a, kg + vg, stream);
+  // (a copy does not look at its elements: one kernel for both types)
+  return eight ? launch(paged_write_kernel<MEGA_F16, true>, a, kg + vg, stream) : launch(paged_write_kernel<MEGA_BF16, false>, a, kg + vg, stream);
+}
+
+extern "C" int mega_paged_cache_read(const mega_paged_cache* cache, int dtype, const int32_t* begins, const int32_t* cu, int64_t rows,
+                                     void* k_out, void* v_out, int clear_rest, void* stream) {
+  if (const int rc = check_paged_cache(cache, dtype, "mega_paged_cache_read"); rc != MEGA_OK) return rc;
+  MEGA_CHECK_ARG(rows >= 0 && rows <= 0x7fffffff, "mega_paged_cache_read: bad number of rows");
+  if (rows == 0) return MEGA_OK;
+  MEGA_CHECK_ARG(cache->batch >= 1, "mega_paged_cache_read: rows of no sequence");
+  MEGA_CHECK_ARG(k_out != nullptr && v_out != nullptr && begins != nullptr && cu != nullptr, "mega_paged_cache_read: null pointer");
+  MEGA_CHECK_ARG(!unaligned(k_out) && !unaligned(v_out), "mega_paged_cache_read: outputs must be 16-byte aligned");
+  const int64_t H = cache->heads;
+  CacheArgs a{paged_view(cache), {{paged_pool(cache, false), k_out, H * cache->k_width, cache->k_width, 0, 0},
+                                  {paged_pool(cache, true), v_out, H * cache->v_width, cache->v_width, 0, 0}},
+              begins, cu, static_cast<int32_t>(rows), static_cast<int32_t>(H), 0, clear_rest != 0};
+  split_row(a.side[0]), split_row(a.side[1]);
+  const int64_t kg = groups_of(a.side[0], rows, H), vg = groups_of(a.side[1], rows, H);
+  MEGA_CHECK_ARG(kg + vg <= 0x7fffffff, "mega_paged_cache_read: too many rows for one launch");
+  a.key_groups = static_cast<uint32_t>(kg);
+  const bool eight = cache->k_exponents != nullptr;
+  if (dtype == MEGA_BF16)
+    return eight ? launch(paged_read_kernel<MEGA_BF16, true>, a, kg + vg, stream) : launch(paged_read_kernel<MEGA_BF16, false>, a, kg + vg, stream);
+  return eight ? launch(paged_read_kernel<MEGA_F16, true>, a, kg + vg, stream) : launch(paged_read_kernel<MEGA_BF16, false>, a, kg + vg, stream);
+}

@@ -20,6 +20,7 @@ from torch import Tensor, nn
 from torch.nn.modules import module as nn_module
 
 from ..fused_ops import memory_efficient_dropout, swift_efficient_attention
+from .paged_cache import PagedCache
 
 _FUSED = {"swift": swift_efficient_attention, "fused": swift_efficient_attention}
 
@@ -111,6 +112,20 @@ class _InnerAttention(nn.Module):
         return out.reshape(batch, new_len, -1), carried
 
     _own_forward = forward
+
+    @torch.no_grad()
+    def forward_paged(self, xq: Tensor, xk: Tensor, xv: Tensor, cache: PagedCache, block_table: Tensor, lengths: Tensor,
+                      cu_new: Tensor) -> Tensor:
+        """The same attention for a ragged batch on a paged cache: rows cu_new[b] .. cu_new[b + 1] of the projections
+        (rows, heads * dim) are the last positions of sequence b, which has lengths[b] of them now.  Their keys and values
+        enter `cache`, then each row attends from the start of its chunk to itself.  Rotary angles, which
+        go by a token's position inside its chunk, have been applied.  Evaluation only."""
+        if self.training and self.dropout > 0.0:
+            raise RuntimeError("forward_paged has no dropout: call it in evaluation mode")
+        cache.write(xk.unflatten(-1, (self.n_heads, self.z_head_dim)), xv.unflatten(-1, (self.n_heads, self.v_head_dim)),
+                    block_table, lengths, cu_new)
+        out = cache.attend(xq.unflatten(-1, (self.n_heads, self.z_head_dim)), block_table, lengths, cu_new, chunk_size=self.chunk_size)
+        return out.flatten(1)
 
     def extra_repr(self) -> str:
         return (f"heads={self.n_heads}, z_head_dim={self.z_head_dim}, v_head_dim={self.v_head_dim}, "
