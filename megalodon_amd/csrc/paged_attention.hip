@@ -22,19 +22,22 @@
 //
 // A page holds 16 keys at least, and key groups are aligned, so a lane group's keys share a page: its base is a scalar.
 //
-// Few rows (single tokens, drafts): bound by the cache's bytes.  The key range of a row block is cut into equal runs
-// until the launch fills the chip; their (o, m, l) go to a workspace in float32 and a second kernel joins them.
-// Many rows: bound by the matrix cores and by what L2 gives for the operands.
+// Few row blocks (single tokens, drafts, one prompt's piece): bound by the cache's bytes.  The blocks' keys, in units of 32,
+// form one line, block after block, which is cut into as many equal parts as workgroups fill the chip, whatever
+// the sequences' lengths: a workgroup goes through the pieces of blocks that its part holds, leaves each one's (o, m, l)
+// in a workspace in float32, and a second kernel joins them.  Many row blocks: a workgroup each, bound by the
+// matrix cores and by what L2 gives for the operands.
 #include "paged.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mega {
 namespace {
 
 constexpr int kMaxWaves = 8;
 constexpr int kMaxKeyWidth = 512;
-constexpr int kMaxRuns = 64;
+constexpr int kCus = 256;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -48,52 +51,119 @@ struct AttnArgs {
   int64_t q_row, q_head;
   const int32_t *lengths, *cu;
   uint16_t* out;
-  float *part, *stats;        // runs > 1: (runs, rows, q_heads, v_width), (runs, rows, q_heads, 2)
-  int32_t rows, heads, shared, chunk, runs, slabs, blocks;
+  float *part, *stats;        // parts > 0: (heads, slots, part_rows, v_width), (heads, slots, part_rows, 2)
+  int32_t rows, heads, shared, chunk, slabs, blocks;
+  int32_t parts, slots, part_rows;  // parts of the line of units for each head and slab; 0: a workgroup a block
   int32_t clear_rest;
   float scale;                // times log2(e)
 };
 
 // A row block of one sequence and the keys that any of its rows sees.
 struct Block {
+  int32_t sequence;
   int32_t start, row0, count;  // first packed row of the sequence; first row (token * shared + head) and their number
   int32_t position0;           // position of the sequence's first new token
   int32_t keys;                // positions that have a place
   int32_t begin, end;          // keys that the block sees, [begin, end)
-  int32_t sequence;
 };
+
+// A load that the scalar unit may make: of what no kernel writes while this one runs, at an address that a wave has in common.
+typedef const int32_t __attribute__((address_space(4))) ConstInt;
+__device__ __forceinline__ int32_t constant_at(const int32_t* p, int64_t i) { return reinterpret_cast<ConstInt*>(reinterpret_cast<uint64_t>(p))[i]; }
 
 __device__ __forceinline__ int chunk_start(int position, int chunk) { return chunk > 0 && position > 0 ? position / chunk * chunk : 0; }
 
-// Row blocks are numbered so that sequence b's begin at cu[b] shared / kRows + b: enough for ceil(n shared / kRows) of them
-// before the next sequence's, whatever the lengths, and the host need not know these.  (`rest`: rows behind the last
-// sequence form one more, which has no keys.)
+// Sequence b (the rows behind the last one are one more, without keys) and its row block `number`; false: it has no such block.
 template <int kRows>
-__device__ __forceinline__ bool find_block(const AttnArgs& a, int number, Block& k) {
-  const int32_t* cu = a.cu;
-  const int sequences = a.view.batch + (a.clear_rest ? 1 : 0);
-  if (sequences == 0) return false;
-  const auto first = [&](int b) { return static_cast<int64_t>(row_bound(cu, b, a.rows)) * a.shared / kRows + b; };
-  const int b = last_not_above(sequences, number, first);
+__device__ __forceinline__ bool block_of(const AttnArgs& a, int b, int64_t number, Block& k) {
   k.sequence = b;
-  k.start = row_bound(cu, b, a.rows);
-  const int n = (b < a.view.batch ? row_bound(cu, b + 1, a.rows) : a.rows) - k.start;
-  const int64_t row0 = (number - first(b)) * kRows;
+  k.start = row_bound(a.cu, b, a.rows);
+  const int n = (b < a.view.batch ? row_bound(a.cu, b + 1, a.rows) : a.rows) - k.start;
+  const int64_t row0 = number * kRows;
   if (row0 < 0 || row0 >= static_cast<int64_t>(n) * a.shared) return false;
   k.row0 = static_cast<int32_t>(row0);
   k.count = static_cast<int32_t>(min(static_cast<int64_t>(kRows), static_cast<int64_t>(n) * a.shared - row0));
   const int length = b < a.view.batch ? max(a.lengths[b], 0) : 0;
-  k.keys = min(static_cast<int64_t>(length), static_cast<int64_t>(a.view.table_width) << a.view.page_shift);
+  k.keys = static_cast<int32_t>(min(static_cast<int64_t>(length), static_cast<int64_t>(a.view.table_width) << a.view.page_shift));
   k.position0 = length - n;
   k.begin = chunk_start(k.position0 + k.row0 / a.shared, a.chunk);
   k.end = min(k.position0 + (k.row0 + k.count - 1) / a.shared + 1, k.keys);
   return true;
 }
 
-// Run `i` of a block's keys: [begin, end), begin a multiple of 32; empty where there are fewer runs.
-__device__ __forceinline__ int run_length(const Block& k, int runs) {
-  const int groups = (k.end - (k.begin & ~31) + 31) >> 5;
-  return max((groups + runs - 1) / runs, 1) * 32;
+// A workgroup a block: blocks are numbered so that sequence b's begin at cu[b] shared / kRows + b, which leaves ceil(n shared / kRows)
+// numbers before the next sequence's whatever the lengths are, and the host need not know these.
+template <int kRows>
+__device__ __forceinline__ bool find_block(const AttnArgs& a, int number, Block& k) {
+  const int sequences = a.view.batch + (a.clear_rest ? 1 : 0);
+  if (sequences == 0) return false;
+  const auto first = [&](int b) { return static_cast<int64_t>(row_bound(a.cu, b, a.rows)) * a.shared / kRows + b; };
+  const int b = last_not_above(sequences, number, first);
+  return block_of<kRows>(a, b, number - first(b), k);
+}
+
+// The line of units.  Every block of a sequence has as many units as its last one sees keys from the first one's first on
+// (all of them in front of a chunk's border alike; the earlier blocks' last units are empty).
+struct Share {
+  int32_t blocks, units;  // of a sequence: row blocks, units of each
+  int32_t from;           // its first unit's first key
+};
+template <int kRows>
+__device__ __forceinline__ Share share_of(const AttnArgs& a, int b) {
+  const int start = row_bound(a.cu, b, a.rows), n = row_bound(a.cu, b + 1, a.rows) - start, length = max(a.lengths[b], 0);
+  if (n <= 0) return {0, 0, 0};
+  const int keys = static_cast<int>(min(static_cast<int64_t>(length), static_cast<int64_t>(a.view.table_width) << a.view.page_shift));
+  const int from = chunk_start(length - n, a.chunk) & ~31;
+  return {static_cast<int32_t>((static_cast<int64_t>(n) * a.shared + kRows - 1) / kRows), max(keys - from + 31, 0) >> 5, from};
+}
+// A place on the line: the sequence, its share, and the blocks and units in front of it.
+struct Mark {
+  int32_t sequence;
+  Share share;
+  int32_t blocks_before, units_before, total;  // total: of the whole line (the host cuts no line of 2^31 units)
+};
+// units of a part; the parts behind the line's end are empty
+__device__ __forceinline__ int part_units(int total, int parts) { return (total + parts - 1) / parts; }
+// The place of `sequence`, or where it is negative of the sequence in which part `part` begins (false: the part is empty); all lanes of a
+// wave together, 64 sequences a round.
+template <int kRows>
+__device__ __forceinline__ bool find_mark(const AttnArgs& a, int sequence, int part, int parts, Mark& mark) {
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  Share s{};
+  int units = 0, blocks = 0;
+  const auto round = [&](int b0) {  // inclusive sums over the lanes' sequences
+    const int b = b0 + lane;
+    s = b < a.view.batch ? share_of<kRows>(a, b) : Share{0, 0, 0};
+    units = s.blocks * s.units, blocks = s.blocks;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int u = __shfl_up(units, off, 64), c = __shfl_up(blocks, off, 64);
+      if (lane >= off) units += u, blocks += c;
+    }
+  };
+  mark.total = 0;
+  for (int b0 = 0; b0 < a.view.batch; b0 += 64) {
+    round(b0);
+    mark.total += __builtin_amdgcn_readlane(units, 63);
+  }
+  const int first = part * part_units(mark.total, parts);
+  if (sequence < 0 && first >= mark.total) return false;
+  int units_before = 0, blocks_before = 0;
+  for (int b0 = 0; b0 < a.view.batch; b0 += 64) {
+    if (a.view.batch > 64) round(b0);
+    const uint64_t which = __ballot(sequence < 0 ? units_before + units > first : b0 + lane >= sequence);
+    if (which != 0) {
+      const int l = __ffsll(static_cast<unsigned long long>(which)) - 1;
+      mark.sequence = b0 + l;
+      mark.share = {__builtin_amdgcn_readlane(s.blocks, l), __builtin_amdgcn_readlane(s.units, l), __builtin_amdgcn_readlane(s.from, l)};
+      mark.units_before = units_before + __builtin_amdgcn_readlane(units, l) - mark.share.blocks * mark.share.units;
+      mark.blocks_before = blocks_before + __builtin_amdgcn_readlane(blocks, l) - mark.share.blocks;
+      return true;
+    }
+    units_before += __builtin_amdgcn_readlane(units, 63);
+    blocks_before += __builtin_amdgcn_readlane(blocks, 63);
+  }
+  return false;
 }
 
 template <int DT>
@@ -116,11 +186,18 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return static_cast<uint32_t>(float_to_f16_bits(lo)) | (static_cast<uint32_t>(float_to_f16_bits(hi)) << 16);
 }
 
-// whether one of a word's two 16-bit numbers is infinite or NaN
+// ones over those halves of a word whose 16-bit numbers are finite
 template <int DT>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   constexpr uint32_t top = DT == MEGA_BF16 ? 0x7f80u : 0x7c00u;
-  return (w & top) == top || ((w >> 16) & top) == top;
+  return ((w & top) == top ? 0u : 0xffffu) | ((w >> 16 & top) == top ? 0u : 0xffff0000u);
+}
+
+// v, of which the compiler knows nothing: what is computed from it is computed where it is used, not once ahead of a loop
+// and kept in registers that the loop has no room for
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 __device__ __forceinline__ float across(float v, int mask) { return __shfl_xor(v, mask, 64); }
@@ -131,20 +208,37 @@ struct Page {
   bool there;
 };
 __device__ __forceinline__ Page page_of(const AttnArgs& a, int sequence, int key) {
-  const uint32_t e = static_cast<uint32_t>(a.view.table[sequence * a.view.table_stride + (key >> a.view.page_shift)]);
+  const uint32_t e = static_cast<uint32_t>(constant_at(a.view.table, sequence * a.view.table_stride + (key >> a.view.page_shift)));
   const bool there = e < static_cast<uint32_t>(a.view.pages);
   return {there ? e : 0, there};
 }
 
+// A lane's values of 32 keys in one group of 16 kCols columns, as they lie in the pool: kCols columns of eight keys.
+template <bool kEight, int kCols>
+struct Values {
+  static constexpr int kWords = kCols * (kEight ? 1 : 2) / 4;
+  typedef uint32_t Piece __attribute__((ext_vector_type(kWords)));
+  Piece x[8];
+};
+
+// Where a workgroup is on the line of units, kept in LDS while it works on a piece.
+struct Progress {
+  Mark mark;
+  int32_t unit, unit_end, per, number;
+  bool alone;
+};
+
 template <int DT, bool kEight, int RT, int CT, int KS>  // KS: 32-wide steps of a key row
 __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnArgs a) {
-  constexpr int kRows = 16 * RT, kGroups = CT / 8;  // column groups of 128
+  // 16-byte loads of values where the registers allow it: eight of a lane's columns at a time, else four
+  constexpr int kRows = 16 * RT, kCols = RT > 1 && !kEight ? 4 : 8, kGroups = CT / kCols;
   extern __shared__ __align__(16) uint4 lds[];
-  const int lane = static_cast<int>(threadIdx.x) & 63, n = lane & 15, h = lane >> 4;
+  __shared__ Progress progress;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), waves = static_cast<int>(blockDim.x) >> 6;
   uint4* const lds_q = lds;                       // [RT][KS][64]
   uint4* const lds_p = lds + RT * KS * 64;        // [waves][RT][64]
   float* const lds_m = reinterpret_cast<float*>(lds_p + waves * RT * 64);  // [kRows][8]
+  int* const lds_pages = reinterpret_cast<int*>(lds_m + kRows * 8);        // [8]: the waves' keys have pages
 
   // column slab and head fastest: workgroups that read the same keys and values share an XCD's L2 (the hardware deals
   // workgroups to the eight XCDs in turn); late row blocks, which see the most keys, first
@@ -153,356 +247,485 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
   id /= a.slabs;
   const int head = id % a.heads;
   id /= a.heads;
-  const int run = id % a.runs;
-  Block k;
-  if (!find_block<kRows>(a, a.blocks - 1 - static_cast<int>(id / a.runs), k)) return;
-  int begin = k.begin & ~31, end = k.end;
-  if (a.runs > 1) {
-    const int length = run_length(k, a.runs);
-    begin += run * length;
-    end = min(end, begin + length);
-    if (begin >= end) return;  // (the join knows as many runs as there are)
-  }
-
-  // rows to LDS, in the order in which the matrix instructions take them
-  for (int c = threadIdx.x; c < kRows * KS * 4; c += blockDim.x) {
-    const int row = c / (KS * 4), d = c % (KS * 4);  // eight elements of a row
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (row < k.count && d * 8 < a.k.width) {
-      const int r = k.row0 + row, t = r / a.shared, g = r - t * a.shared;
-      x = *reinterpret_cast<const uint4*>(a.q + (static_cast<int64_t>(k.start) + t) * a.q_row + (static_cast<int64_t>(head) * a.shared + g) * a.q_head + d * 8);
-    }
-    // (8-bit keys: a lane reads 16 codes at a time, which serve two steps)
-    const int step = kEight ? (d >> 3) * 2 + (d & 1) : d >> 2, quarter = kEight ? (d >> 1) & 3 : d & 3;
-    lds_q[((row >> 4) * KS + step) * 64 + quarter * 16 + (row & 15)] = x;
-  }
-  __syncthreads();
-
-  int low[RT], high[RT];  // the lane's rows see keys low .. high
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int row = rt * 16 + n, position = k.position0 + (k.row0 + row) / a.shared;
-    low[rt] = chunk_start(position, a.chunk);
-    high[rt] = row < k.count ? min(position, k.keys - 1) : -1;
-  }
-  // keys all_low .. all_high are seen by every row of the block
-  const int all_low = chunk_start(k.position0 + (k.row0 + k.count - 1) / a.shared, a.chunk), all_high = min(k.position0 + k.row0 / a.shared, k.keys - 1);
-
-  f32x4 acc[RT][CT];
-  float m[RT], l[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -__builtin_inff(), l[rt] = 0.f;
-#pragma unroll
-    for (int c = 0; c < CT; ++c) acc[rt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
   const int page_mask = (1 << a.view.page_shift) - 1;
-  const int column = (slab * waves + wave) * CT * 16 + n * 8;  // + 128 g
+  const int first_column = (slab * waves + wave) * CT * 16;
 
-  for (int tile = begin; tile < end; tile += 32 * waves) {
-    // ---- scores of the wave's 32 keys
-    const int mine = tile + 32 * wave;
-    f32x4 s[2][RT];
-    if (mine < end) {
-      bool whole = mine >= all_low && mine + 31 <= all_high;
+  Block k;
+  if (a.parts == 0) {
+    if (!find_block<kRows>(a, a.blocks - 1 - static_cast<int>(id), k)) return;
+  } else {
+    Progress at;
+    if (!find_mark<kRows>(a, -1, static_cast<int>(id), a.parts, at.mark)) return;
+    at.per = part_units(at.mark.total, a.parts);
+    at.unit = static_cast<int>(id) * at.per, at.unit_end = min(at.unit + at.per, at.mark.total);
+    if (threadIdx.x == 0) progress = at;
+    __syncthreads();
+  }
+
+  for (;;) {
+    // (anew for each piece and each use: kept out of the registers in between)
+    const int lane = opaque(static_cast<int>(threadIdx.x) & 63), n = lane & 15, h = lane >> 4;
+    int begin, end;
+    if (a.parts == 0) {
+      begin = k.begin & ~31, end = k.end;
+    } else {
+      Progress at = progress;
+      __syncthreads();
+      while (at.unit >= at.mark.units_before + at.mark.share.blocks * at.mark.share.units) {  // (unit < total: there is one)
+        at.mark.units_before += at.mark.share.blocks * at.mark.share.units;
+        at.mark.blocks_before += at.mark.share.blocks;
+        at.mark.share = share_of<kRows>(a, ++at.mark.sequence);
+      }
+      const int units = at.mark.share.units;
+      at.number = (at.unit - at.mark.units_before) / units;
+      const int first = at.mark.units_before + at.number * units, last = min(first + units, at.unit_end);
+      block_of<kRows>(a, __builtin_amdgcn_readfirstlane(at.mark.sequence), __builtin_amdgcn_readfirstlane(at.number), k);
+      begin = __builtin_amdgcn_readfirstlane(max(at.mark.share.from + (at.unit - first) * 32, k.begin & ~31));
+      end = __builtin_amdgcn_readfirstlane(min(at.mark.share.from + (last - first) * 32, k.end));
+      at.alone = first / at.per == (first + units - 1) / at.per;  // the whole block is this workgroup's
+      at.unit = last;
+      if (threadIdx.x == 0) progress = at;
+    }
+
+    // rows to LDS, in the order in which the matrix instructions take them
+    for (int c = threadIdx.x; c < kRows * KS * 4; c += blockDim.x) {
+      const int row = c / (KS * 4), d = c % (KS * 4);  // eight elements of a row
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (row < k.count && d * 8 < a.k.width) {
+        const int r = k.row0 + row, t = r / a.shared, g = r - t * a.shared;
+        x = *reinterpret_cast<const uint4*>(a.q + (static_cast<int64_t>(k.start) + t) * a.q_row + (static_cast<int64_t>(head) * a.shared + g) * a.q_head + d * 8);
+      }
+      // (8-bit keys: a lane reads 16 codes at a time, which serve two steps)
+      const int step = kEight ? (d >> 3) * 2 + (d & 1) : d >> 2, quarter = kEight ? (d >> 1) & 3 : d & 3;
+      lds_q[((row >> 4) * KS + step) * 64 + quarter * 16 + (row & 15)] = x;
+    }
+
+    // the lane's rows see keys low .. low + span of this piece (none: a low that no key reaches)
+    int low[RT];
+    uint32_t span[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int row = rt * 16 + n, position = k.position0 + (k.row0 + row) / a.shared, high = min(position, end - 1);
+      low[rt] = chunk_start(position, a.chunk);
+      const bool none = row >= k.count || high < low[rt];
+      span[rt] = none ? 0u : static_cast<uint32_t>(high - low[rt]);
+      if (none) low[rt] = 0x7fffffff;
+    }
+    const auto sees = [&](int rt, int key) { return static_cast<uint32_t>(key) - static_cast<uint32_t>(low[rt]) <= span[rt]; };
+    // keys all_low .. all_high are seen by every row of the block
+    const int all_low = chunk_start(k.position0 + (k.row0 + k.count - 1) / a.shared, a.chunk), all_high = min(k.position0 + k.row0 / a.shared, end - 1);
+
+    // the two 16-key groups of a step: where this head's first value lies, and whether the group has a page
+    constexpr int kBytes = kEight ? 1 : 2;
+    struct Step {
+      const uint8_t* from[2];
+      const uint8_t* exponents[2];
+      bool there[2];
+    };
+    const auto step_at = [&](int first) {
+      Step t;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int group = mine + 16 * half, held = min(group, (end - 1) & ~15);
+        const int held = min(first + 16 * half, (end - 1) & ~15), place = held & page_mask;
         const Page page = page_of(a, k.sequence, held);
-        whole = whole && page.there;
-        const int place = (held & page_mask) + n;
-        u32x4 kx[KS];
-        if constexpr (kEight) {
-          const uint8_t* from = static_cast<const uint8_t*>(a.k.rows) + page.number * a.k.page + static_cast<int64_t>(head) * a.k.head;
-          const uint32_t at = static_cast<uint32_t>(place) * a.k.slot + h * 16;
-#pragma unroll
-          for (int c = 0; c < KS / 2; ++c) {
-            const int d = c * 64 + h * 16;
-            const u32x4 x = d < a.k.width ? *reinterpret_cast<const u32x4*>(from + at + c * 64) : u32x4{0, 0, 0, 0};
-            kx[2 * c] = u32x4{widen<DT, false>(x[0], 1.f), widen<DT, true>(x[0], 1.f), widen<DT, false>(x[1], 1.f), widen<DT, true>(x[1], 1.f)};
-            kx[2 * c + 1] = u32x4{widen<DT, false>(x[2], 1.f), widen<DT, true>(x[2], 1.f), widen<DT, false>(x[3], 1.f), widen<DT, true>(x[3], 1.f)};
-          }
-        } else {
-          const uint16_t* from = static_cast<const uint16_t*>(a.k.rows) + page.number * a.k.page + static_cast<int64_t>(head) * a.k.head;
-          const uint32_t at = static_cast<uint32_t>(place) * a.k.slot + h * 8;
-#pragma unroll
-          for (int c = 0; c < KS; ++c)
-            kx[c] = c * 32 + h * 8 < a.k.width ? *reinterpret_cast<const u32x4*>(from + at + c * 32) : u32x4{0, 0, 0, 0};
-        }
-        f32x4 factor = {a.scale, a.scale, a.scale, a.scale};
-        if constexpr (kEight) {
-          const uint8_t* e = a.k.exponents + page.number * a.k.ePage + static_cast<int64_t>(head) * a.k.eHead;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) factor[i] *= exponent_value(e[static_cast<uint32_t>((held & page_mask) + 4 * h + i) * a.k.eSlot]);
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[half][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < KS; ++c)
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[half][rt] = mma<DT>(kx[c], __builtin_bit_cast(u32x4, lds_q[(rt * KS + c) * 64 + lane]), s[half][rt]);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[half][rt] *= factor;
-        if (!whole) {
-          const int first = group + 4 * h;
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (!page.there || first + i < low[rt] || first + i > high[rt] || first + i >= end) s[half][rt][i] = -__builtin_inff();
-        }
+        t.there[half] = page.there;
+        t.from[half] = static_cast<const uint8_t*>(a.v.rows) + (page.number * a.v.page + static_cast<int64_t>(head) * a.v.head + static_cast<int64_t>(place) * a.v.slot) * kBytes;
+        if constexpr (kEight) t.exponents[half] = a.v.exponents + (page.number * a.v.ePage + static_cast<int64_t>(head) * a.v.eHead + static_cast<int64_t>(place) * a.v.eSlot);
       }
-    } else {
+      return t;
+    };
+    const auto load_values = [&](const Step& t, int g, Values<kEight, kCols>& x) {
+      // (columns behind the last are computed from others and not written)
+      const int l = opaque(lane);
+      const uint32_t offset = (static_cast<uint32_t>(4 * (l >> 4)) * a.v.slot + min(first_column + g * 16 * kCols + (l & 15) * kCols, a.v.width - kCols)) * kBytes;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) s[0][rt] = s[1][rt] = f32x4{-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
-    }
+      for (int i = 0; i < 8; ++i)
+        x.x[i] = *reinterpret_cast<const typename Values<kEight, kCols>::Piece*>(t.from[i >> 2] + (offset + static_cast<uint32_t>((i & 3) * a.v.slot * kBytes)));
+    };
+    const auto load_exponents = [&](const Step& t, uint32_t* e) {
+      if constexpr (kEight) {
+        const uint32_t offset = static_cast<uint32_t>(4 * (opaque(lane) >> 4)) * a.v.eSlot;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = t.exponents[i >> 2][offset + static_cast<uint32_t>((i & 3) * a.v.eSlot)];
+      }
+    };
 
-    // ---- the rows' new maxima
-    float top[RT];
+    f32x4 acc[RT][CT];
+    float m[RT], l[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float t = fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3]));
-      t = fmaxf(t, fmaxf(fmaxf(s[1][rt][0], s[1][rt][1]), fmaxf(s[1][rt][2], s[1][rt][3])));
-      t = fmaxf(t, across(t, 16));
-      top[rt] = fmaxf(t, across(t, 32));
+      m[rt] = -__builtin_inff(), l[rt] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) acc[rt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (waves > 1) {
-      if (h == 0)
+    // the next 32 keys' values are on their way while these are worked on
+    Values<kEight, kCols> x[kGroups];
+    uint32_t e[8];
+    bool there[2] = {false, false};
+    if (begin < end) {
+      const Step t = step_at(begin);
+      load_exponents(t, e);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * 8 + wave] = top[rt];
-      __syncthreads();
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-        for (int w = 0; w < waves; ++w) top[rt] = fmaxf(top[rt], lds_m[(rt * 16 + n) * 8 + w]);
+      for (int g = 0; g < kGroups; ++g) load_values(t, g, x[g]);
+      there[0] = t.there[0], there[1] = t.there[1];
     }
-
-    // ---- probabilities, in the operand order of the second product
-    bool moved = false;
-    float alpha[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const float now = fmaxf(m[rt], top[rt]), base = now == -__builtin_inff() ? 0.f : now;
-      alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - base);
-      moved = moved || now != m[rt];
-      m[rt] = now;
-      float p[8], sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(s[i >> 2][rt][i & 3] - base);
-        sum += p[i];
-      }
-      l[rt] = l[rt] * alpha[rt] + sum;
-      lds_p[(wave * RT + rt) * 64 + lane] = make_uint4(pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7]));
-    }
-    if (__any(moved))
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int c = 0; c < CT; ++c) acc[rt][c] *= alpha[rt];
+    for (int c = threadIdx.x; c < kRows * 8; c += blockDim.x) lds_m[c] = -__builtin_inff();  // (of waves that there are not, too)
+    if (threadIdx.x < kMaxWaves) lds_pages[threadIdx.x] = 1;
     __syncthreads();
 
-    // ---- values: 32 keys a step
-    for (int step = 0; step < waves; ++step) {
+    // 32 keys' values into the accumulators, those of the 32 after them called for (of these once more at the end: a load that is
+    // always made needs no wait where it might not have been).  kAll: every row sees every one of the keys
+    const auto values_of = [&](int tile, int step, auto all) {
+      constexpr bool kAll = decltype(all)::value;
       const int first = tile + 32 * step;
-      if (first >= end) break;
-      const int held[2] = {first, min(first + 16, (end - 1) & ~15)};
-      const Page page[2] = {page_of(a, k.sequence, held[0]), page_of(a, k.sequence, held[1])};
-      u32x4 vt[CT];
-      const bool inside = first >= k.begin && first + 32 <= end && page[0].there && page[1].there;
+      const Step next = step_at(min(first + 32, (end - 1) & ~31));
+      bool odd = false;
       float unit[8];
       if constexpr (kEight) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint8_t* e = a.v.exponents + page[half].number * a.v.ePage + static_cast<int64_t>(head) * a.v.eHead;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) unit[4 * half + i] = exponent_value(e[static_cast<uint32_t>((held[half] & page_mask) + 4 * h + i) * a.v.eSlot]);
-        }
+        for (int i = 0; i < 8; ++i) unit[i] = exponent_value(e[i]);
+        load_exponents(next, e);
       }
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        const int c0 = min(column + 128 * g, a.v.width - 8);  // (columns behind the last are computed from others and not written)
-        u32x4 x[8];
+        uint32_t w[8][kCols / 2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int64_t base = page[half].number * a.v.page + static_cast<int64_t>(head) * a.v.head;
-          const uint32_t at = static_cast<uint32_t>((held[half] & page_mask) + 4 * h) * a.v.slot + c0;
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if constexpr (kEight) {
-              const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v.rows) + base + (at + static_cast<uint32_t>(i) * a.v.slot));
-              const float u = unit[4 * half + i];
-              x[4 * half + i] = u32x4{widen<DT, false>(c.x, u), widen<DT, true>(c.x, u), widen<DT, false>(c.y, u), widen<DT, true>(c.y, u)};
-            } else {
-              x[4 * half + i] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.v.rows) + base + (at + static_cast<uint32_t>(i) * a.v.slot));
-            }
+          for (int j = 0; j < kCols / 2; ++j) {
+            if constexpr (kEight)
+              w[i][j] = (j & 1) ? widen<DT, true>(x[g].x[i][j >> 1], unit[i]) : widen<DT, false>(x[g].x[i][j >> 1], unit[i]);
+            else
+              w[i][j] = x[g].x[i][j];
           }
-        }
-        if (!inside)  // what is not there, or not this run's, must not meet a probability of zero as NaN
+        // what is not there, or not this workgroup's, must not meet a probability of zero as an infinity or NaN; nor must such a
+        // value of a key that only some rows see, which goes to those alone below
+        if constexpr (!kAll)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int key = first + 16 * (i >> 2) + 4 * h + (i & 3);
-            if (key < k.begin || key >= end || !page[i >> 2].there) x[i] = u32x4{0, 0, 0, 0};
-          }
+            const uint32_t keep = key >= k.begin && key < end && there[i >> 2] ? ~0u : 0u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < kCols / 2; ++j) {
+              const uint32_t finite = finite_halves<DT>(w[i][j]);
+              odd = odd || (~finite & keep) != 0;
+              w[i][j] &= keep & finite;
+            }
+          }
+        u32x4 vt[kCols];
+#pragma unroll
+        for (int j = 0; j < kCols / 2; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            vt[8 * g + 2 * j][i] = __builtin_amdgcn_perm(x[2 * i + 1][j], x[2 * i][j], 0x05040100);
-            vt[8 * g + 2 * j + 1][i] = __builtin_amdgcn_perm(x[2 * i + 1][j], x[2 * i][j], 0x07060302);
+            vt[2 * j][i] = __builtin_amdgcn_perm(w[2 * i + 1][j], w[2 * i][j], 0x05040100);
+            vt[2 * j + 1][i] = __builtin_amdgcn_perm(w[2 * i + 1][j], w[2 * i][j], 0x07060302);
           }
-      }
-      bool plain = first >= all_low && first + 31 <= all_high;
-      if (!plain) {  // some row does not see some of these keys: harmless unless a value is infinite or NaN
-        bool odd = false;
-#pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) odd = odd || not_finite<DT>(vt[c][i]);
-        plain = !__any(odd);
-      }
-      if (plain) {
+        load_values(next, g, x[g]);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           const u32x4 p = __builtin_bit_cast(u32x4, lds_p[(step * RT + rt) * 64 + lane]);
 #pragma unroll
-          for (int c = 0; c < CT; ++c) acc[rt][c] = mma<DT>(vt[c], p, acc[rt][c]);
+          for (int c = 0; c < kCols; ++c) acc[rt][g * kCols + c] = mma<DT>(vt[c], p, acc[rt][g * kCols + c]);
         }
-      } else {  // key by key, each into the rows that see it
+      }
+      if constexpr (!kAll)
+        if (__any(odd)) {  // key by key, its infinities and NaN into the rows that see it
+          const Step t = step_at(first);
+          const int l = opaque(lane), n = l & 15, h = l >> 4;
 #pragma unroll 1
-        for (int slot = 0; slot < 32; ++slot) {
-          const int e = slot & 7, key = first + 16 * (e >> 2) + 4 * (slot >> 3) + (e & 3);
-          u32x4 keep;
+          for (int slot = 0; slot < 32; ++slot) {
+            const int place = slot & 7, half = place >> 2, in_group = 4 * (slot >> 3) + (place & 3), key = first + 16 * half + in_group;
+            if (key < k.begin || key >= end || !(half ? t.there[1] : t.there[0])) continue;
+            const uint8_t* const row = (half ? t.from[1] : t.from[0]) + static_cast<int64_t>(in_group) * a.v.slot * kBytes;
+            float p[RT];
+            bool its[RT];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) keep[i] = h == slot >> 3 && i == e >> 1 ? ((e & 1) ? 0xffff0000u : 0x0000ffffu) : 0u;
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            const u32x4 p = __builtin_bit_cast(u32x4, lds_p[(step * RT + rt) * 64 + lane]);
-            const bool sees = key >= low[rt] && key <= high[rt];
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-              const f32x4 with = mma<DT>(vt[c] & keep, p, acc[rt][c]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) acc[rt][c][i] = sees ? with[i] : acc[rt][c][i];
+            for (int rt = 0; rt < RT; ++rt) {
+              const uint16_t bits = reinterpret_cast<const uint16_t*>(lds_p + (step * RT + rt) * 64 + (slot & ~7) * 2 + n)[place];
+              p[rt] = DT == MEGA_BF16 ? bf16_bits_to_float(bits) : f16_bits_to_float(bits);
+              its[rt] = sees(rt, key);
             }
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int at = min(first_column + 16 * kCols * (c / kCols) + kCols * (4 * h + i) + c % kCols, a.v.width - 1);
+                float v;
+                if constexpr (kEight) {
+                  v = (row[at] & 0x7f) == 0x7f ? __builtin_nanf("") : 0.f;
+                } else {
+                  const uint16_t bits = reinterpret_cast<const uint16_t*>(row)[at];
+                  v = DT == MEGA_BF16 ? bf16_bits_to_float(bits) : f16_bits_to_float(bits);
+                }
+                const bool finite = fabsf(v) < __builtin_inff();
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[rt][c][i] = finite || !its[rt] ? acc[rt][c][i] : fmaf(p[rt], v, acc[rt][c][i]);
+                __builtin_amdgcn_sched_barrier(0);
+              }
           }
         }
-      }
-    }
-  }
+      there[0] = next.there[0], there[1] = next.there[1];
+    };
 
-  // ---- the rows' sums over the lanes and waves that had their keys
+    for (int tile = begin; tile < end; tile += 32 * waves) {
+      // ---- scores of the wave's 32 keys
+      const int mine = tile + 32 * wave;
+      f32x4 s[2][RT];
+      bool pages_there = true;
+      if (mine < end) {
+        bool whole = mine >= all_low && mine + 31 <= all_high;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    l[rt] += across(l[rt], 16);
-    l[rt] += across(l[rt], 32);
-  }
-  if (waves > 1) {
-    __syncthreads();  // (the maxima of the last tile have been read)
-    if (h == 0)
+        for (int half = 0; half < 2; ++half) {
+          const int group = mine + 16 * half, held = min(group, (end - 1) & ~15);
+          const Page page = page_of(a, k.sequence, held);
+          pages_there = pages_there && page.there;
+          const int l = opaque(lane), n = l & 15, h = l >> 4, place = (held & page_mask) + n;
+          constexpr int kLoads = kEight ? KS / 2 : KS, kStep = kEight ? 64 : 32, kPiece = kEight ? 16 : 8;  // of a row; elements of one and of a lane's part
+          u32x4 kx[kLoads];
+          f32x4 factor = {a.scale, a.scale, a.scale, a.scale};
+          const uint8_t* from = static_cast<const uint8_t*>(a.k.rows) + (page.number * a.k.page + static_cast<int64_t>(head) * a.k.head) * kBytes;
+          const uint32_t offset = (static_cast<uint32_t>(place) * a.k.slot + h * kPiece) * kBytes;
+          if (a.k.width == 32 * KS)
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * 8 + wave] = l[rt];
-    __syncthreads();
+            for (int c = 0; c < kLoads; ++c) kx[c] = *reinterpret_cast<const u32x4*>(from + offset + c * kStep * kBytes);
+          else
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      l[rt] = 0.f;
-      for (int w = 0; w < waves; ++w) l[rt] += lds_m[(rt * 16 + n) * 8 + w];
-    }
-  }
+            for (int c = 0; c < kLoads; ++c)
+              kx[c] = c * kStep + h * kPiece < a.k.width ? *reinterpret_cast<const u32x4*>(from + offset + c * kStep * kBytes) : u32x4{0, 0, 0, 0};
+          if constexpr (kEight) {
+            const uint8_t* e = a.k.exponents + page.number * a.k.ePage + static_cast<int64_t>(head) * a.k.eHead;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int row = rt * 16 + n;
-    if (row >= k.count) continue;
-    const int r = k.row0 + row, t = r / a.shared, g = r - t * a.shared;
-    const int64_t at = (static_cast<int64_t>(k.start) + t) * (a.heads * a.shared) + head * a.shared + g;
-    const int64_t all = static_cast<int64_t>(a.rows) * a.heads * a.shared;
-    const float inverse = l[rt] == 0.f ? 0.f : 1.f / l[rt];
-    if (a.runs > 1 && slab == 0 && wave == 0 && h == 0) {
-      a.stats[(run * all + at) * 2] = m[rt];
-      a.stats[(run * all + at) * 2 + 1] = l[rt];
-    }
+            for (int i = 0; i < 4; ++i) factor[i] *= exponent_value(e[static_cast<uint32_t>((held & page_mask) + 4 * h + i) * a.k.eSlot]);
+          }
 #pragma unroll
-    for (int cg = 0; cg < kGroups; ++cg)
+          for (int rt = 0; rt < RT; ++rt) s[half][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // accumulator element i of column operand j is column 8 (4 h + i) + j of the group
-        const int c = (slab * waves + wave) * CT * 16 + 128 * cg + 8 * (4 * h + i);
-        if (c >= a.v.width) continue;
-        float o[8];
+          for (int c = 0; c < KS; ++c) {
+            u32x4 key;
+            if constexpr (kEight) {
+              const u32x4 w = kx[c >> 1];
+              const uint32_t lo = (c & 1) ? w[2] : w[0], hi = (c & 1) ? w[3] : w[1];
+              key = u32x4{widen<DT, false>(lo, 1.f), widen<DT, true>(lo, 1.f), widen<DT, false>(hi, 1.f), widen<DT, true>(hi, 1.f)};
+            } else {
+              key = kx[c];
+            }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = acc[rt][8 * cg + j][i];
-        if (a.runs > 1) {
-          float4* to = reinterpret_cast<float4*>(a.part + (run * all + at) * a.v.width + c);
-          to[0] = make_float4(o[0], o[1], o[2], o[3]);
-          to[1] = make_float4(o[4], o[5], o[6], o[7]);
-        } else {
+            for (int rt = 0; rt < RT; ++rt) s[half][rt] = mma<DT>(key, __builtin_bit_cast(u32x4, lds_q[(rt * KS + c) * 64 + lane]), s[half][rt]);
+            if (RT * (c & 3) == 3 * RT || RT == 4) __builtin_amdgcn_sched_barrier(0);  // (or all of the rows' operands are fetched ahead)
+          }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = l[rt] == 0.f ? 0.f : o[j] * inverse;
-          *reinterpret_cast<uint4*>(a.out + at * a.v.width + c) = pack8<DT>(o);
+          for (int rt = 0; rt < RT; ++rt) s[half][rt] *= factor;
+          if (!whole || !page.there) {
+            const int first = group + 4 * h;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (!page.there || !sees(rt, first + i)) s[half][rt][i] = -__builtin_inff();
+          }
+          __builtin_amdgcn_sched_barrier(0);  // (one half's keys at a time: both do not fit the registers beside four row tiles)
+        }
+      } else {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[0][rt] = s[1][rt] = f32x4{-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
+      }
+
+      // ---- the rows' new maxima
+      float top[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float t = fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3]));
+        t = fmaxf(t, fmaxf(fmaxf(s[1][rt][0], s[1][rt][1]), fmaxf(s[1][rt][2], s[1][rt][3])));
+        t = fmaxf(t, across(t, 16));
+        top[rt] = fmaxf(t, across(t, 32));
+      }
+      if (waves > 1) {
+        if (h == 0)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * 8 + wave] = top[rt];
+        if (lane == 0) lds_pages[wave] = pages_there;
+        __syncthreads();
+        const int4 u = *reinterpret_cast<const int4*>(lds_pages), v = *reinterpret_cast<const int4*>(lds_pages + 4);
+        pages_there = __builtin_amdgcn_readfirstlane(u.x & u.y & u.z & u.w & v.x & v.y & v.z & v.w) != 0;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const float4 u = *reinterpret_cast<const float4*>(lds_m + (rt * 16 + n) * 8), v = *reinterpret_cast<const float4*>(lds_m + (rt * 16 + n) * 8 + 4);
+          top[rt] = fmaxf(fmaxf(fmaxf(u.x, u.y), fmaxf(u.z, u.w)), fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
         }
       }
+
+      // ---- probabilities, in the operand order of the second product
+      bool moved = false;
+      float alpha[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float now = fmaxf(m[rt], top[rt]), base = now == -__builtin_inff() ? 0.f : now;
+        alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - base);
+        moved = moved || now != m[rt];
+        m[rt] = now;
+        float p[8], sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(s[i >> 2][rt][i & 3] - base);
+          sum += p[i];
+        }
+        l[rt] = l[rt] * alpha[rt] + sum;
+        lds_p[(wave * RT + rt) * 64 + lane] = make_uint4(pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7]));
+      }
+      if (__any(moved))
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int c = 0; c < CT; ++c) acc[rt][c] *= alpha[rt];
+      __syncthreads();
+
+      // ---- values: 32 keys a step
+      const int steps = min(waves, (end - tile + 31) >> 5);
+      int step = 0;
+      if (pages_there && tile >= all_low) {
+        const int all = min(steps, (all_high + 1 - tile) >> 5);
+        for (; step < all; ++step) values_of(tile, step, std::true_type());
+      }
+      for (; step < steps; ++step) values_of(tile, step, std::false_type());
+    }
+
+    // ---- the rows' sums over the lanes and waves that had their keys
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      l[rt] += across(l[rt], 16);
+      l[rt] += across(l[rt], 32);
+    }
+    if (waves > 1) {
+      __syncthreads();  // (the maxima of the last tile have been read)
+      if (h == 0)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * 8 + wave] = l[rt];
+      __syncthreads();
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        l[rt] = 0.f;
+        for (int w = 0; w < waves; ++w) l[rt] += lds_m[(rt * 16 + n) * 8 + w];
+      }
+    }
+    const int l_ = opaque(lane), n_ = l_ & 15, h_ = l_ >> 4;
+    bool alone = true, last = true;
+    int64_t slot = 0;
+    if (a.parts > 0) {
+      slot = (static_cast<int64_t>(head) * a.slots + id + progress.mark.blocks_before + progress.number) * a.part_rows;
+      alone = progress.alone, last = progress.unit >= progress.unit_end;
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int row = rt * 16 + n_;
+      if (row >= k.count) continue;
+      const int r = k.row0 + row, t = r / a.shared, g = r - t * a.shared;
+      const int64_t at = (static_cast<int64_t>(k.start) + t) * (a.heads * a.shared) + head * a.shared + g;
+      const float inverse = l[rt] == 0.f ? 0.f : 1.f / l[rt];
+      if (!alone && slab == 0 && wave == 0 && h_ == 0) {
+        a.stats[(slot + row) * 2] = m[rt];
+        a.stats[(slot + row) * 2 + 1] = l[rt];
+      }
+#pragma unroll
+      for (int cg = 0; cg < kGroups; ++cg)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // accumulator element i of column operand j is column kCols (4 h + i) + j of the group
+          const int c = first_column + 16 * kCols * cg + kCols * (4 * h_ + i);
+          if (c >= a.v.width) continue;
+          float o[kCols];
+#pragma unroll
+          for (int j = 0; j < kCols; ++j) o[j] = acc[rt][kCols * cg + j][i];
+          if (!alone) {
+            float4* to = reinterpret_cast<float4*>(a.part + (slot + row) * a.v.width + c);
+#pragma unroll
+            for (int j = 0; j < kCols / 4; ++j) to[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) o[j] = l[rt] == 0.f ? 0.f : o[j] * inverse;
+            uint32_t* to = reinterpret_cast<uint32_t*>(a.out + at * a.v.width + c);
+            if constexpr (kCols == 8)
+              *reinterpret_cast<uint4*>(to) = make_uint4(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]), pack2<DT>(o[4], o[5]), pack2<DT>(o[6], o[7]));
+            else
+              *reinterpret_cast<uint2*>(to) = make_uint2(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]));
+          }
+        }
+    }
+    if (last) break;
+    __syncthreads();  // (the rows, maxima and probabilities of this piece have been read)
   }
 }
 
-// Joins a row's runs: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i with m = max_i m_i.  A thread has eight columns of
-// a row; the runs come in their order, whatever order they were made in.
-constexpr int kJoinThreads = 256;
+// Joins the pieces of the blocks that several workgroups had: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i with
+// m = max_i m_i.  A wave has a row's 32 columns: four lanes of eight columns times sixteen pieces at a time.
+constexpr int kJoinThreads = 256, kJoinColumns = 32;
 template <int DT, int kRows>
 __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(AttnArgs a) {
-  const int pieces = a.v.width / 8, q_heads = a.heads * a.shared;
-  const int64_t all = static_cast<int64_t>(a.rows) * q_heads, items = all * pieces;
-  const int64_t item0 = static_cast<int64_t>(blockIdx.x) * kJoinThreads + (threadIdx.x & ~63u), item = item0 + (threadIdx.x & 63u);
-  if (item0 >= items) return;
-  int b = last_not_above(a.view.batch + 1, item0 / pieces / q_heads, [&](int i) { return static_cast<int64_t>(row_bound(a.cu, i, a.rows)); });
-  if (item >= items) return;
-  const int64_t row = item / pieces;
-  const int token = static_cast<int>(row / q_heads), c = static_cast<int>(item - row * pieces) * 8;
-  while (b < a.view.batch && row_bound(a.cu, b + 1, a.rows) <= token) ++b;
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const uint32_t strips = (a.v.width + kJoinColumns - 1) / kJoinColumns, q_heads = a.heads * a.shared;
+  const uint32_t item = blockIdx.x * (kJoinThreads / kWave) + (threadIdx.x >> 6);
+  if (item >= static_cast<uint64_t>(a.rows) * q_heads * strips) return;
+  const uint32_t row = item / strips;
+  const int c = static_cast<int>(item % strips) * kJoinColumns + (lane & 3) * 8;
+  const int token = static_cast<int>(row / q_heads), q_head = static_cast<int>(row % q_heads), head = q_head / a.shared;
+  const int b = last_not_above(a.view.batch + 1, token, [&](int i) { return static_cast<int64_t>(row_bound(a.cu, i, a.rows)); });
   if (b == a.view.batch && !a.clear_rest) return;
-  int runs = 0;
+  int pieces = 0, piece_row = 0;
+  int64_t slot = 0;
   if (b < a.view.batch) {
-    Block k;
-    k.start = row_bound(a.cu, b, a.rows);
-    if (token < k.start) return;
-    const int n = row_bound(a.cu, b + 1, a.rows) - k.start, length = max(a.lengths[b], 0);
-    const int r = (token - k.start) * a.shared + static_cast<int>(row % q_heads) % a.shared;
-    k.row0 = r / kRows * kRows;
-    k.count = min(static_cast<int64_t>(kRows), static_cast<int64_t>(n) * a.shared - k.row0);
-    k.keys = min(static_cast<int64_t>(length), static_cast<int64_t>(a.view.table_width) << a.view.page_shift);
-    k.position0 = length - n;
-    k.begin = chunk_start(k.position0 + k.row0 / a.shared, a.chunk);
-    k.end = min(k.position0 + (k.row0 + k.count - 1) / a.shared + 1, k.keys);
-    const int from = k.begin & ~31;
-    if (k.end > from) runs = (k.end - from + run_length(k, a.runs) - 1) / run_length(k, a.runs);
+    const int r = (token - row_bound(a.cu, b, a.rows)) * a.shared + q_head % a.shared;
+    if (r < 0) return;
+    Mark mark;
+    if (!find_mark<kRows>(a, b, 0, a.parts, mark)) return;
+    if (mark.share.units > 0) {
+      const int per = part_units(mark.total, a.parts), first = mark.units_before + r / kRows * mark.share.units;
+      const int i0 = first / per, i1 = (first + mark.share.units - 1) / per;
+      if (i0 == i1) return;  // (written by its workgroup)
+      pieces = i1 - i0 + 1;
+      piece_row = r % kRows;
+      slot = static_cast<int64_t>(head) * a.slots + i0 + mark.blocks_before + r / kRows;
+    }
   }
   float m = -__builtin_inff();
-  for (int i = 0; i < runs; ++i) m = fmaxf(m, a.stats[(i * all + row) * 2]);
+  for (int i = lane; i < pieces; i += 64) m = fmaxf(m, a.stats[((slot + i) * a.part_rows + piece_row) * 2]);
+  m = wave_max(m);
   float l = 0.f, o[8] = {};
-  if (m != -__builtin_inff())
-    for (int i = 0; i < runs; ++i) {
-      const float mi = a.stats[(i * all + row) * 2];
+  const bool column = c < a.v.width;
+  if (m != -__builtin_inff()) {
+    for (int i = lane >> 2; i < pieces; i += 16) {
+      const int64_t at = (slot + i) * a.part_rows + piece_row;
+      const float mi = a.stats[at * 2], li = a.stats[at * 2 + 1], w = __builtin_amdgcn_exp2f(mi - m);
       if (mi == -__builtin_inff()) continue;
-      const float w = __builtin_amdgcn_exp2f(mi - m);
-      l += w * a.stats[(i * all + row) * 2 + 1];
-      const float4* from = reinterpret_cast<const float4*>(a.part + (i * all + row) * a.v.width + c);
+      l = fmaf(w, li, l);
+      if (!column) continue;
+      const float4* from = reinterpret_cast<const float4*>(a.part + at * a.v.width + c);
       const float4 x = from[0], y = from[1];
       const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] = fmaf(w, v[j], o[j]);
     }
+#pragma unroll
+    for (int off = 4; off < 64; off <<= 1) {
+      l += across(l, off);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] += across(o[j], off);
+    }
+  }
+  if (lane >= 4 || !column) return;
   const float inverse = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int j = 0; j < 8; ++j) o[j] = l == 0.f ? 0.f : o[j] * inverse;
-  *reinterpret_cast<uint4*>(a.out + row * a.v.width + c) = pack8<DT>(o);
+  *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(row) * a.v.width + c) = pack8<DT>(o);
 }
 
 // How a call is cut.
 struct Plan {
-  int rt, ct, ks, waves, slabs, runs;
-  int64_t blocks;
-  int64_t workgroups(int64_t heads) const { return blocks * runs * heads * slabs; }
+  int rt, ct, ks, waves, slabs;
+  int64_t blocks, parts;  // row blocks at most; parts of the line of units for each head and slab (0: a workgroup a block)
+  int64_t slots, part_rows;
+  int64_t workgroups(int64_t heads) const { return (parts > 0 ? parts : blocks) * heads * slabs; }
 };
 
-Plan plan_of(const mega_paged_cache* c, int64_t rows, int64_t q_heads, int64_t chunk) {
+Plan plan_of(const mega_paged_cache* c, int64_t rows, int64_t q_heads) {
   Plan p{};
   const int64_t shared = q_heads / c->heads, sequences = std::max<int64_t>(c->batch, 1);
   // rows of a sequence, on average: a block's rows pad to the next size
@@ -510,31 +733,34 @@ Plan plan_of(const mega_paged_cache* c, int64_t rows, int64_t q_heads, int64_t c
   p.rt = mean <= 16 ? 1 : mean <= 32 ? 2 : 4;
   p.ks = c->k_width <= 128 ? 4 : c->k_width <= 256 ? 8 : 16;
   p.ct = p.rt == 1 && c->v_width > 1024 ? 16 : 8;
-  const int64_t per_wave = 16 * p.ct;
+  const int64_t per_wave = 16 * p.ct, kRows = 16 * p.rt;
   p.slabs = static_cast<int>((c->v_width + kMaxWaves * per_wave - 1) / (kMaxWaves * per_wave));
   const int64_t slab = (c->v_width + p.slabs - 1) / p.slabs;
   p.waves = static_cast<int>((slab + per_wave - 1) / per_wave);
-  p.blocks = rows * shared / (16 * p.rt) + c->batch + 1;
-  // runs: until the chip has its waves; none shorter than 32 keys
-  const int64_t keys = std::min(c->table_width * c->page_size, chunk > 0 ? chunk : INT64_MAX);
-  const int64_t full = std::max<int64_t>(1, std::max(rows * shared / (16 * p.rt), std::min(c->batch, rows))) * c->heads * p.slabs * p.waves;
-  const int64_t wanted = 2048;  // eight waves to a CU
-  p.runs = static_cast<int>(std::clamp<int64_t>(wanted / full, 1, std::min<int64_t>(kMaxRuns, std::max<int64_t>(1, keys / 32))));
+  p.blocks = rows * shared / kRows + c->batch + 1;
+  // workgroups that the chip holds at a time: eight waves to a CU
+  const int64_t resident = kCus * kMaxWaves / p.waves, pairs = c->heads * p.slabs;
+  const int64_t full = std::max(rows * shared / kRows, std::min(c->batch, rows)) * pairs;
+  if (c->batch > 0 && full < 4 * resident && p.blocks * (c->table_width * c->page_size / 32 + 1) < 0x40000000) {
+    p.parts = std::max<int64_t>(1, resident / pairs);
+    p.part_rows = std::min(kRows, rows * shared);
+    p.slots = p.parts + rows * shared / kRows + c->batch;
+  }
   return p;
 }
 
 template <int DT, bool kEight, int RT, int CT, int KS>
 int launch_attn(const AttnArgs& a, const Plan& p, void* stream) {
   const auto kernel = paged_attn_kernel<DT, kEight, RT, CT, KS>;
-  const size_t bytes = (RT * KS * 64 + p.waves * RT * 64) * sizeof(uint4) + RT * 16 * 8 * sizeof(float);
+  const size_t bytes = (RT * KS * 64 + p.waves * RT * 64) * sizeof(uint4) + RT * 16 * 8 * sizeof(float) + kMaxWaves * sizeof(int);
   if (bytes > 65536)
     MEGA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
   hipStream_t s = static_cast<hipStream_t>(stream);
   kernel<<<dim3(static_cast<uint32_t>(p.workgroups(a.heads))), dim3(p.waves * kWave), bytes, s>>>(a);
   MEGA_CHECK_LAUNCH();
-  if (p.runs > 1) {
-    const int64_t items = static_cast<int64_t>(a.rows) * a.heads * a.shared * (a.v.width / 8);
-    paged_join_kernel<DT, 16 * RT><<<dim3(static_cast<uint32_t>((items + kJoinThreads - 1) / kJoinThreads)), dim3(kJoinThreads), 0, s>>>(a);
+  if (p.parts > 0) {
+    const int64_t waves = static_cast<int64_t>(a.rows) * a.heads * a.shared * ((a.v.width + kJoinColumns - 1) / kJoinColumns);
+    paged_join_kernel<DT, 16 * RT><<<dim3(static_cast<uint32_t>((waves + kJoinThreads / kWave - 1) / (kJoinThreads / kWave))), dim3(kJoinThreads), 0, s>>>(a);
     MEGA_CHECK_LAUNCH();
   }
   return MEGA_OK;
@@ -567,8 +793,8 @@ using namespace mega;
 
 extern "C" int64_t mega_paged_attention_workspace_bytes(const mega_paged_cache* cache, int64_t rows, int64_t q_heads, int64_t chunk) {
   if (!sizes_fit(cache, rows, q_heads, chunk) || rows == 0) return 0;
-  const Plan p = plan_of(cache, rows, q_heads, chunk);
-  return p.runs > 1 ? p.runs * rows * q_heads * (cache->v_width + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+  const Plan p = plan_of(cache, rows, q_heads);
+  return p.parts > 0 ? cache->heads * p.slots * p.part_rows * (cache->v_width + 2) * static_cast<int64_t>(sizeof(float)) : 0;
 }
 
 extern "C" int mega_paged_attention_fwd(const mega_paged_cache* cache, int dtype, const void* q, int64_t q_row, int64_t q_head,
@@ -581,18 +807,19 @@ extern "C" int mega_paged_attention_fwd(const mega_paged_cache* cache, int dtype
   MEGA_CHECK_ARG(q != nullptr && out != nullptr && (lengths != nullptr || cache->batch == 0) && cu != nullptr, "mega_paged_attention_fwd: null pointer");
   MEGA_CHECK_ARG(reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_row % 8 == 0 && q_head % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
                  "mega_paged_attention_fwd: q and out must be 16-byte aligned");
-  const Plan p = plan_of(cache, rows, q_heads, chunk);
+  const Plan p = plan_of(cache, rows, q_heads);
   MEGA_CHECK_ARG(p.workgroups(cache->heads) <= 0x7fffffff && rows * (q_heads / cache->heads) <= 0x7fffffff, "mega_paged_attention_fwd: too many rows for one launch");
-  MEGA_CHECK_ARG(p.runs == 1 || (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+  MEGA_CHECK_ARG(p.parts == 0 || (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                  "mega_paged_attention_fwd: a 16-byte aligned workspace is needed");
   AttnArgs a{};
   a.view = paged_view(cache), a.k = paged_pool(cache, false), a.v = paged_pool(cache, true);
   a.q = static_cast<const uint16_t*>(q), a.q_row = q_row, a.q_head = q_head;
   a.lengths = lengths, a.cu = cu, a.out = static_cast<uint16_t*>(out);
   a.part = static_cast<float*>(workspace);
-  if (p.runs > 1) a.stats = a.part + p.runs * rows * q_heads * cache->v_width;
+  if (p.parts > 0) a.stats = a.part + cache->heads * p.slots * p.part_rows * cache->v_width;
   a.rows = static_cast<int32_t>(rows), a.heads = static_cast<int32_t>(cache->heads), a.shared = static_cast<int32_t>(q_heads / cache->heads);
-  a.chunk = static_cast<int32_t>(chunk), a.runs = p.runs, a.slabs = p.slabs, a.blocks = static_cast<int32_t>(p.blocks);
+  a.chunk = static_cast<int32_t>(chunk), a.slabs = p.slabs, a.blocks = static_cast<int32_t>(p.blocks);
+  a.parts = static_cast<int32_t>(p.parts), a.slots = static_cast<int32_t>(p.slots), a.part_rows = static_cast<int32_t>(p.part_rows);
   a.clear_rest = clear_rest != 0;
   a.scale = static_cast<float>(scale * 1.4426950408889634);
   const bool eight = cache->k_exponents != nullptr;
