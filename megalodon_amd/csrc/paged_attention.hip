@@ -239,6 +239,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
   uint4* const lds_p = lds + RT * KS * 64;        // [waves][RT][64]
   float* const lds_m = reinterpret_cast<float*>(lds_p + waves * RT * 64);  // [kRows][8]
   int* const lds_pages = reinterpret_cast<int*>(lds_m + kRows * 8);        // [8]: the waves' keys have pages
+  int2* const lds_sees = reinterpret_cast<int2*>(lds_pages + kMaxWaves);   // [kRows]: first key and number of further ones that a row sees
 
   // column slab and head fastest: workgroups that read the same keys and values share an XCD's L2 (the hardware deals
   // workgroups to the eight XCDs in turn); late row blocks, which see the most keys, first
@@ -300,18 +301,13 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
       lds_q[((row >> 4) * KS + step) * 64 + quarter * 16 + (row & 15)] = x;
     }
 
-    // the lane's rows see keys low .. low + span of this piece (none: a low that no key reaches)
-    int low[RT];
-    uint32_t span[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int row = rt * 16 + n, position = k.position0 + (k.row0 + row) / a.shared, high = min(position, end - 1);
-      low[rt] = chunk_start(position, a.chunk);
-      const bool none = row >= k.count || high < low[rt];
-      span[rt] = none ? 0u : static_cast<uint32_t>(high - low[rt]);
-      if (none) low[rt] = 0x7fffffff;
+    // the rows' visible keys of this piece to LDS: low .. low + span (none: a low that no key reaches)
+    for (int row = threadIdx.x; row < kRows; row += blockDim.x) {
+      const int position = k.position0 + (k.row0 + row) / a.shared, low = chunk_start(position, a.chunk), high = min(position, end - 1);
+      const bool none = row >= k.count || high < low;
+      lds_sees[row] = none ? make_int2(0x7fffffff, 0) : make_int2(low, high - low);
     }
-    const auto sees = [&](int rt, int key) { return static_cast<uint32_t>(key) - static_cast<uint32_t>(low[rt]) <= span[rt]; };
+    const auto sees = [&](int2 range, int key) { return static_cast<uint32_t>(key) - static_cast<uint32_t>(range.x) <= static_cast<uint32_t>(range.y); };
     // keys all_low .. all_high are seen by every row of the block
     const int all_low = chunk_start(k.position0 + (k.row0 + k.count - 1) / a.shared, a.chunk), all_high = min(k.position0 + k.row0 / a.shared, end - 1);
 
@@ -358,33 +354,78 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
 #pragma unroll
       for (int c = 0; c < CT; ++c) acc[rt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // the next 32 keys' values are on their way while these are worked on
+    // the next 32 keys' values are on their way while these are worked on (four row tiles: within a tile of keys; beside the
+    // scores there is no room for them)
+    constexpr bool kAcross = RT < 4;
     Values<kEight, kCols> x[kGroups];
     uint32_t e[8];
     bool there[2] = {false, false};
-    if (begin < end) {
-      const Step t = step_at(begin);
+    // keys: the wave's first 16 of a tile are on their way before the tile is reached, the second 16 take their registers
+    constexpr int kLoads = kEight ? KS / 2 : KS;  // a lane's 16-byte parts of a row: 8 elements of 32, or 16 of 64
+    struct Keys {
+      const uint8_t* from;
+      const uint8_t* exponents;
+      int place;
+      bool there;
+    };
+    u32x4 kx[kLoads];
+    uint32_t ke[4];
+    const auto keys_at = [&](int group) {
+      Keys t;
+      const int held = min(group, (end - 1) & ~15);
+      const Page page = page_of(a, k.sequence, held);
+      t.there = page.there, t.place = held & page_mask;
+      t.from = static_cast<const uint8_t*>(a.k.rows) + (page.number * a.k.page + static_cast<int64_t>(head) * a.k.head) * kBytes;
+      if constexpr (kEight) t.exponents = a.k.exponents + (page.number * a.k.ePage + static_cast<int64_t>(head) * a.k.eHead + static_cast<int64_t>(t.place) * a.k.eSlot);
+      return t;
+    };
+    const auto load_key = [&](const Keys& t, int c) {
+      const int l = opaque(lane), d = min((kEight ? 64 : 32) * c + (kEight ? 16 : 8) * (l >> 4), a.k.width - (kEight ? 16 : 8));
+      kx[c] = *reinterpret_cast<const u32x4*>(t.from + (static_cast<uint32_t>(t.place + (l & 15)) * a.k.slot + d) * kBytes);
+    };
+    const auto load_key_exponents = [&](const Keys& t) {
+      if constexpr (kEight) {
+        const uint32_t offset = static_cast<uint32_t>(4 * (opaque(lane) >> 4)) * a.k.eSlot;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ke[i] = t.exponents[offset + static_cast<uint32_t>(i * a.k.eSlot)];
+      }
+    };
+    const auto load_first_keys = [&](int tile) {
+      if (tile + 32 * wave >= end) return;
+      const Keys t = keys_at(tile + 32 * wave);
+      load_key_exponents(t);
+#pragma unroll
+      for (int c = 0; c < kLoads; ++c) load_key(t, c);
+    };
+    const auto load_step = [&](int first) {
+      const Step t = step_at(first);
       load_exponents(t, e);
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) load_values(t, g, x[g]);
       there[0] = t.there[0], there[1] = t.there[1];
-    }
+    };
+    if (kAcross) load_first_keys(begin);
+    if (kAcross && begin < end) load_step(begin);
     for (int c = threadIdx.x; c < kRows * 8; c += blockDim.x) lds_m[c] = -__builtin_inff();  // (of waves that there are not, too)
     if (threadIdx.x < kMaxWaves) lds_pages[threadIdx.x] = 1;
     __syncthreads();
 
-    // 32 keys' values into the accumulators, those of the 32 after them called for (of these once more at the end: a load that is
+    // 32 keys' values into the accumulators, those of the 32 after them called for (kNext; of these once more at the end: a load that is
     // always made needs no wait where it might not have been).  kAll: every row sees every one of the keys
-    const auto values_of = [&](int tile, int step, auto all) {
-      constexpr bool kAll = decltype(all)::value;
+    const auto values_of = [&](int tile, int step, auto all, auto call) {
+      constexpr bool kAll = decltype(all)::value, kNext = decltype(call)::value;
       const int first = tile + 32 * step;
-      const Step next = step_at(min(first + 32, (end - 1) & ~31));
+      Step next;
+      if constexpr (kNext) next = step_at(min(first + 32, (end - 1) & ~31));
+      u32x4 p[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) p[rt] = __builtin_bit_cast(u32x4, lds_p[(step * RT + rt) * 64 + lane]);
       bool odd = false;
       float unit[8];
       if constexpr (kEight) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) unit[i] = exponent_value(e[i]);
-        load_exponents(next, e);
+        if constexpr (kNext) load_exponents(next, e);
       }
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
@@ -420,30 +461,29 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
             vt[2 * j][i] = __builtin_amdgcn_perm(w[2 * i + 1][j], w[2 * i][j], 0x05040100);
             vt[2 * j + 1][i] = __builtin_amdgcn_perm(w[2 * i + 1][j], w[2 * i][j], 0x07060302);
           }
-        load_values(next, g, x[g]);
+        if constexpr (kNext) load_values(next, g, x[g]);
+        __builtin_amdgcn_sched_barrier(0);  // (in front of the products, not behind them)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const u32x4 p = __builtin_bit_cast(u32x4, lds_p[(step * RT + rt) * 64 + lane]);
+        for (int c = 0; c < kCols; ++c)
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) acc[rt][g * kCols + c] = mma<DT>(vt[c], p, acc[rt][g * kCols + c]);
-        }
+          for (int rt = 0; rt < RT; ++rt) acc[rt][g * kCols + c] = mma<DT>(vt[c], p[rt], acc[rt][g * kCols + c]);
       }
       if constexpr (!kAll)
         if (__any(odd)) {  // key by key, its infinities and NaN into the rows that see it
           const Step t = step_at(first);
-          const int l = opaque(lane), n = l & 15, h = l >> 4;
 #pragma unroll 1
           for (int slot = 0; slot < 32; ++slot) {
+            const int l = opaque(lane), n = l & 15, h = l >> 4;
             const int place = slot & 7, half = place >> 2, in_group = 4 * (slot >> 3) + (place & 3), key = first + 16 * half + in_group;
             if (key < k.begin || key >= end || !(half ? t.there[1] : t.there[0])) continue;
             const uint8_t* const row = (half ? t.from[1] : t.from[0]) + static_cast<int64_t>(in_group) * a.v.slot * kBytes;
-            float p[RT];
+            float weight[RT];
             bool its[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
               const uint16_t bits = reinterpret_cast<const uint16_t*>(lds_p + (step * RT + rt) * 64 + (slot & ~7) * 2 + n)[place];
-              p[rt] = DT == MEGA_BF16 ? bf16_bits_to_float(bits) : f16_bits_to_float(bits);
-              its[rt] = sees(rt, key);
+              weight[rt] = DT == MEGA_BF16 ? bf16_bits_to_float(bits) : f16_bits_to_float(bits);
+              its[rt] = sees(lds_sees[rt * 16 + n], key);
             }
 #pragma unroll
             for (int c = 0; c < CT; ++c)
@@ -459,48 +499,45 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
                 }
                 const bool finite = fabsf(v) < __builtin_inff();
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[rt][c][i] = finite || !its[rt] ? acc[rt][c][i] : fmaf(p[rt], v, acc[rt][c][i]);
+                for (int rt = 0; rt < RT; ++rt) acc[rt][c][i] = finite || !its[rt] ? acc[rt][c][i] : fmaf(weight[rt], v, acc[rt][c][i]);
                 __builtin_amdgcn_sched_barrier(0);
               }
           }
         }
-      there[0] = next.there[0], there[1] = next.there[1];
+      if constexpr (kNext) there[0] = next.there[0], there[1] = next.there[1];
     };
 
     for (int tile = begin; tile < end; tile += 32 * waves) {
       // ---- scores of the wave's 32 keys
       const int mine = tile + 32 * wave;
+      if (!kAcross) load_first_keys(tile);
       f32x4 s[2][RT];
       bool pages_there = true;
       if (mine < end) {
-        bool whole = mine >= all_low && mine + 31 <= all_high;
+        const bool whole = mine >= all_low && mine + 31 <= all_high;
+        Keys now = keys_at(mine);
+        const Keys second = keys_at(mine + 16);
+        pages_there = now.there && second.there;
+        u32x4 q[RT], q_next[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) q_next[rt] = __builtin_bit_cast(u32x4, lds_q[rt * KS * 64 + lane]);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const int group = mine + 16 * half, held = min(group, (end - 1) & ~15);
-          const Page page = page_of(a, k.sequence, held);
-          pages_there = pages_there && page.there;
-          const int l = opaque(lane), n = l & 15, h = l >> 4, place = (held & page_mask) + n;
-          constexpr int kLoads = kEight ? KS / 2 : KS, kStep = kEight ? 64 : 32, kPiece = kEight ? 16 : 8;  // of a row; elements of one and of a lane's part
-          u32x4 kx[kLoads];
           f32x4 factor = {a.scale, a.scale, a.scale, a.scale};
-          const uint8_t* from = static_cast<const uint8_t*>(a.k.rows) + (page.number * a.k.page + static_cast<int64_t>(head) * a.k.head) * kBytes;
-          const uint32_t offset = (static_cast<uint32_t>(place) * a.k.slot + h * kPiece) * kBytes;
-          if (a.k.width == 32 * KS)
-#pragma unroll
-            for (int c = 0; c < kLoads; ++c) kx[c] = *reinterpret_cast<const u32x4*>(from + offset + c * kStep * kBytes);
-          else
-#pragma unroll
-            for (int c = 0; c < kLoads; ++c)
-              kx[c] = c * kStep + h * kPiece < a.k.width ? *reinterpret_cast<const u32x4*>(from + offset + c * kStep * kBytes) : u32x4{0, 0, 0, 0};
           if constexpr (kEight) {
-            const uint8_t* e = a.k.exponents + page.number * a.k.ePage + static_cast<int64_t>(head) * a.k.eHead;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) factor[i] *= exponent_value(e[static_cast<uint32_t>((held & page_mask) + 4 * h + i) * a.k.eSlot]);
+            for (int i = 0; i < 4; ++i) factor[i] *= exponent_value(ke[i]);
+            if (half == 0) load_key_exponents(second);
           }
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) s[half][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < KS; ++c) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {  // (the rows' operands one step ahead; fences keep it at that)
+              q[rt] = q_next[rt];
+              if (half == 0 || c + 1 < KS) q_next[rt] = __builtin_bit_cast(u32x4, lds_q[(rt * KS + (c + 1) % KS) * 64 + lane]);
+            }
             u32x4 key;
             if constexpr (kEight) {
               const u32x4 w = kx[c >> 1];
@@ -509,26 +546,35 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
             } else {
               key = kx[c];
             }
+            if (a.k.width != 32 * KS) {  // (behind the row's end the rows' operands are zero, and infinity times zero is not)
+              const int d = kEight ? (c >> 1) * 64 + (opaque(lane) >> 4) * 16 : c * 32 + (opaque(lane) >> 4) * 8;
+              if (d >= a.k.width) key = u32x4{0, 0, 0, 0};
+            }
+            if (half == 0 && (!kEight || (c & 1))) load_key(second, kEight ? c >> 1 : c);  // into the registers that have become free
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) s[half][rt] = mma<DT>(key, __builtin_bit_cast(u32x4, lds_q[(rt * KS + c) * 64 + lane]), s[half][rt]);
-            if (RT * (c & 3) == 3 * RT || RT == 4) __builtin_amdgcn_sched_barrier(0);  // (or all of the rows' operands are fetched ahead)
+            for (int rt = 0; rt < RT; ++rt) s[half][rt] = mma<DT>(key, q[rt], s[half][rt]);
+            __builtin_amdgcn_sched_barrier(0);
           }
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) s[half][rt] *= factor;
-          if (!whole || !page.there) {
-            const int first = group + 4 * h;
+          const bool there = half ? second.there : now.there;
+          if (!whole || !there) {
+            const int l = opaque(lane), first = mine + 16 * half + 4 * (l >> 4);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
+            for (int rt = 0; rt < RT; ++rt) {
+              const int2 range = lds_sees[rt * 16 + (l & 15)];
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                if (!page.there || !sees(rt, first + i)) s[half][rt][i] = -__builtin_inff();
+                if (!there || !sees(range, first + i)) s[half][rt][i] = -__builtin_inff();
+            }
           }
-          __builtin_amdgcn_sched_barrier(0);  // (one half's keys at a time: both do not fit the registers beside four row tiles)
         }
       } else {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[0][rt] = s[1][rt] = f32x4{-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
       }
+      if (!kAcross) load_step(tile);
+      if (kAcross) load_first_keys(tile + 32 * waves);
 
       // ---- the rows' new maxima
       float top[RT];
@@ -555,11 +601,13 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
       }
 
       // ---- probabilities, in the operand order of the second product
+      // (m follows the maximum when that is 2^8 above it, not at each step: the factor leaves p, l and o alike, and a probability
+      // of up to 2^8 is as exact as one of up to 1)
       bool moved = false;
       float alpha[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float now = fmaxf(m[rt], top[rt]), base = now == -__builtin_inff() ? 0.f : now;
+        const float now = top[rt] > m[rt] + 8.f ? top[rt] : m[rt], base = now == -__builtin_inff() ? 0.f : now;
         alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - base);
         moved = moved || now != m[rt];
         m[rt] = now;
@@ -571,6 +619,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
         }
         l[rt] = l[rt] * alpha[rt] + sum;
         lds_p[(wave * RT + rt) * 64 + lane] = make_uint4(pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7]));
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (__any(moved))
 #pragma unroll
@@ -582,11 +631,13 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
       // ---- values: 32 keys a step
       const int steps = min(waves, (end - tile + 31) >> 5);
       int step = 0;
-      if (pages_there && tile >= all_low) {
+      const bool some = pages_there && tile >= all_low;
+      if (some) {
         const int all = min(steps, (all_high + 1 - tile) >> 5);
-        for (; step < all; ++step) values_of(tile, step, std::true_type());
+        for (; step < (kAcross ? all : min(all, steps - 1)); ++step) values_of(tile, step, std::true_type(), std::true_type());
+        if (!kAcross && step < all) values_of(tile, step++, std::true_type(), std::false_type());
       }
-      for (; step < steps; ++step) values_of(tile, step, std::false_type());
+      for (; step < steps; ++step) values_of(tile, step, std::false_type(), std::true_type());
     }
 
     // ---- the rows' sums over the lanes and waves that had their keys
@@ -730,8 +781,8 @@ Plan plan_of(const mega_paged_cache* c, int64_t rows, int64_t q_heads) {
   const int64_t shared = q_heads / c->heads, sequences = std::max<int64_t>(c->batch, 1);
   // rows of a sequence, on average: a block's rows pad to the next size
   const int64_t mean = (rows * shared + sequences - 1) / sequences;
-  p.rt = mean <= 16 ? 1 : mean <= 32 ? 2 : 4;
   p.ks = c->k_width <= 128 ? 4 : c->k_width <= 256 ? 8 : 16;
+  p.rt = mean <= 16 ? 1 : mean <= 32 || p.ks == 16 ? 2 : 4;  // (keys of 512 and four row tiles do not fit the registers)
   p.ct = p.rt == 1 && c->v_width > 1024 ? 16 : 8;
   const int64_t per_wave = 16 * p.ct, kRows = 16 * p.rt;
   p.slabs = static_cast<int>((c->v_width + kMaxWaves * per_wave - 1) / (kMaxWaves * per_wave));
@@ -752,7 +803,7 @@ Plan plan_of(const mega_paged_cache* c, int64_t rows, int64_t q_heads) {
 template <int DT, bool kEight, int RT, int CT, int KS>
 int launch_attn(const AttnArgs& a, const Plan& p, void* stream) {
   const auto kernel = paged_attn_kernel<DT, kEight, RT, CT, KS>;
-  const size_t bytes = (RT * KS * 64 + p.waves * RT * 64) * sizeof(uint4) + RT * 16 * 8 * sizeof(float) + kMaxWaves * sizeof(int);
+  const size_t bytes = (RT * KS * 64 + p.waves * RT * 64) * sizeof(uint4) + RT * 16 * 8 * sizeof(float) + kMaxWaves * sizeof(int) + RT * 16 * sizeof(int2);
   if (bytes > 65536)
     MEGA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -770,8 +821,9 @@ template <int DT, bool kEight, int KS>
 int launch_rows(const AttnArgs& a, const Plan& p, void* stream) {
   if (p.rt == 1 && p.ct == 16) return launch_attn<DT, kEight, 1, 16, KS>(a, p, stream);
   if (p.rt == 1) return launch_attn<DT, kEight, 1, 8, KS>(a, p, stream);
-  if (p.rt == 2) return launch_attn<DT, kEight, 2, 8, KS>(a, p, stream);
-  return launch_attn<DT, kEight, 4, 8, KS>(a, p, stream);
+  if constexpr (KS < 16)
+    if (p.rt == 4) return launch_attn<DT, kEight, 4, 8, KS>(a, p, stream);
+  return launch_attn<DT, kEight, 2, 8, KS>(a, p, stream);
 }
 
 template <int DT, bool kEight>
