@@ -52,6 +52,7 @@ struct AttnArgs {
   const int32_t *lengths, *cu;
   uint16_t* out;
   float *part, *stats;        // parts > 0: (heads, slots, part_rows, v_width), (heads, slots, part_rows, 2)
+  int2* joins;                // ... (rows, q_heads): a row's first place in the former and its number of pieces (0: out has it)
   int32_t rows, heads, shared, chunk, slabs, blocks;
   int32_t parts, slots, part_rows;  // parts of the line of units for each head and slab; 0: a workgroup a block
   int32_t clear_rest;
@@ -72,6 +73,9 @@ typedef const int32_t __attribute__((address_space(4))) ConstInt;
 __device__ __forceinline__ int32_t constant_at(const int32_t* p, int64_t i) { return reinterpret_cast<ConstInt*>(reinterpret_cast<uint64_t>(p))[i]; }
 
 __device__ __forceinline__ int chunk_start(int position, int chunk) { return chunk > 0 && position > 0 ? position / chunk * chunk : 0; }
+
+// Sequences, the rows behind the last one counted as one more where they are to be cleared.
+__device__ __forceinline__ int sequences_of(const AttnArgs& a) { return a.view.batch + (a.clear_rest ? 1 : 0); }
 
 // Sequence b (the rows behind the last one are one more, without keys) and its row block `number`; false: it has no such block.
 template <int kRows>
@@ -95,26 +99,26 @@ __device__ __forceinline__ bool block_of(const AttnArgs& a, int b, int64_t numbe
 // numbers before the next sequence's whatever the lengths are, and the host need not know these.
 template <int kRows>
 __device__ __forceinline__ bool find_block(const AttnArgs& a, int number, Block& k) {
-  const int sequences = a.view.batch + (a.clear_rest ? 1 : 0);
-  if (sequences == 0) return false;
+  const int sequences = sequences_of(a);
   const auto first = [&](int b) { return static_cast<int64_t>(row_bound(a.cu, b, a.rows)) * a.shared / kRows + b; };
   const int b = last_not_above(sequences, number, first);
   return block_of<kRows>(a, b, number - first(b), k);
 }
 
 // The line of units.  Every block of a sequence has as many units as its last one sees keys from the first one's first on
-// (all of them in front of a chunk's border alike; the earlier blocks' last units are empty).
+// (all of them in front of a chunk's border alike; the earlier blocks' last units are empty), and one if there are none.
 struct Share {
   int32_t blocks, units;  // of a sequence: row blocks, units of each
   int32_t from;           // its first unit's first key
 };
 template <int kRows>
 __device__ __forceinline__ Share share_of(const AttnArgs& a, int b) {
-  const int start = row_bound(a.cu, b, a.rows), n = row_bound(a.cu, b + 1, a.rows) - start, length = max(a.lengths[b], 0);
+  const bool rest = b >= a.view.batch;
+  const int start = row_bound(a.cu, b, a.rows), n = (rest ? a.rows : row_bound(a.cu, b + 1, a.rows)) - start, length = rest ? 0 : max(a.lengths[b], 0);
   if (n <= 0) return {0, 0, 0};
   const int keys = static_cast<int>(min(static_cast<int64_t>(length), static_cast<int64_t>(a.view.table_width) << a.view.page_shift));
   const int from = chunk_start(length - n, a.chunk) & ~31;
-  return {static_cast<int32_t>((static_cast<int64_t>(n) * a.shared + kRows - 1) / kRows), max(keys - from + 31, 0) >> 5, from};
+  return {static_cast<int32_t>((static_cast<int64_t>(n) * a.shared + kRows - 1) / kRows), max(keys - from + 31, 32) >> 5, from};
 }
 // A place on the line: the sequence, its share, and the blocks and units in front of it.
 struct Mark {
@@ -124,34 +128,32 @@ struct Mark {
 };
 // units of a part; the parts behind the line's end are empty
 __device__ __forceinline__ int part_units(int total, int parts) { return (total + parts - 1) / parts; }
-// The place of `sequence`, or where it is negative of the sequence in which part `part` begins (false: the part is empty); all lanes of a
-// wave together, 64 sequences a round.
+// The sequence in which part `part` begins (false: the part is empty); all lanes of a wave together, 64 sequences a round.
 template <int kRows>
-__device__ __forceinline__ bool find_mark(const AttnArgs& a, int sequence, int part, int parts, Mark& mark) {
-  const int lane = static_cast<int>(threadIdx.x) & 63;
+__device__ __forceinline__ bool find_mark(const AttnArgs& a, int part, Mark& mark) {
+  const int lane = static_cast<int>(threadIdx.x) & 63, sequences = sequences_of(a);
   Share s{};
   int units = 0, blocks = 0;
   const auto round = [&](int b0) {  // inclusive sums over the lanes' sequences
     const int b = b0 + lane;
-    s = b < a.view.batch ? share_of<kRows>(a, b) : Share{0, 0, 0};
+    s = b < sequences ? share_of<kRows>(a, b) : Share{0, 0, 0};
     units = s.blocks * s.units, blocks = s.blocks;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
+    for (int off = 1; off < min(64, sequences); off <<= 1) {
       const int u = __shfl_up(units, off, 64), c = __shfl_up(blocks, off, 64);
       if (lane >= off) units += u, blocks += c;
     }
   };
   mark.total = 0;
-  for (int b0 = 0; b0 < a.view.batch; b0 += 64) {
+  for (int b0 = 0; b0 < sequences; b0 += 64) {
     round(b0);
-    mark.total += __builtin_amdgcn_readlane(units, 63);
+    mark.total += __builtin_amdgcn_readlane(units, min(63, sequences - 1 - b0));
   }
-  const int first = part * part_units(mark.total, parts);
-  if (sequence < 0 && first >= mark.total) return false;
+  const int first = part * part_units(mark.total, a.parts);
+  if (first >= mark.total) return false;
   int units_before = 0, blocks_before = 0;
-  for (int b0 = 0; b0 < a.view.batch; b0 += 64) {
-    if (a.view.batch > 64) round(b0);
-    const uint64_t which = __ballot(sequence < 0 ? units_before + units > first : b0 + lane >= sequence);
+  for (int b0 = 0; b0 < sequences; b0 += 64) {
+    if (sequences > 64) round(b0);
+    const uint64_t which = __ballot(b0 + lane < sequences && units_before + units > first);
     if (which != 0) {
       const int l = __ffsll(static_cast<unsigned long long>(which)) - 1;
       mark.sequence = b0 + l;
@@ -225,7 +227,8 @@ struct Values {
 struct Progress {
   Mark mark;
   int32_t unit, unit_end, per, number;
-  bool alone;
+  int32_t pieces;  // of the block, this one included if it is the first; 0 for the others
+  bool alone;      // the whole block is this workgroup's
 };
 
 template <int DT, bool kEight, int RT, int CT, int KS>  // KS: 32-wide steps of a key row
@@ -256,7 +259,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
     if (!find_block<kRows>(a, a.blocks - 1 - static_cast<int>(id), k)) return;
   } else {
     Progress at;
-    if (!find_mark<kRows>(a, -1, static_cast<int>(id), a.parts, at.mark)) return;
+    if (!find_mark<kRows>(a, static_cast<int>(id), at.mark)) return;
     at.per = part_units(at.mark.total, a.parts);
     at.unit = static_cast<int>(id) * at.per, at.unit_end = min(at.unit + at.per, at.mark.total);
     if (threadIdx.x == 0) progress = at;
@@ -283,7 +286,9 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
       block_of<kRows>(a, __builtin_amdgcn_readfirstlane(at.mark.sequence), __builtin_amdgcn_readfirstlane(at.number), k);
       begin = __builtin_amdgcn_readfirstlane(max(at.mark.share.from + (at.unit - first) * 32, k.begin & ~31));
       end = __builtin_amdgcn_readfirstlane(min(at.mark.share.from + (last - first) * 32, k.end));
-      at.alone = first / at.per == (first + units - 1) / at.per;  // the whole block is this workgroup's
+      const int begins_in = first / at.per, ends_in = (first + units - 1) / at.per;
+      at.alone = begins_in == ends_in;
+      at.pieces = begins_in == static_cast<int>(id) ? ends_in - begins_in + 1 : 0;
       at.unit = last;
       if (threadIdx.x == 0) progress = at;
     }
@@ -661,9 +666,10 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
     const int l_ = opaque(lane), n_ = l_ & 15, h_ = l_ >> 4;
     bool alone = true, last = true;
     int64_t slot = 0;
+    int pieces = 0;
     if (a.parts > 0) {
       slot = (static_cast<int64_t>(head) * a.slots + id + progress.mark.blocks_before + progress.number) * a.part_rows;
-      alone = progress.alone, last = progress.unit >= progress.unit_end;
+      alone = progress.alone, pieces = progress.pieces, last = progress.unit >= progress.unit_end;
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -672,9 +678,10 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
       const int r = k.row0 + row, t = r / a.shared, g = r - t * a.shared;
       const int64_t at = (static_cast<int64_t>(k.start) + t) * (a.heads * a.shared) + head * a.shared + g;
       const float inverse = l[rt] == 0.f ? 0.f : 1.f / l[rt];
-      if (!alone && slab == 0 && wave == 0 && h_ == 0) {
-        a.stats[(slot + row) * 2] = m[rt];
-        a.stats[(slot + row) * 2 + 1] = l[rt];
+      if (a.parts > 0 && slab == 0 && wave == 0 && h_ == 0) {
+        if (!alone) *reinterpret_cast<float2*>(a.stats + (slot + row) * 2) = make_float2(m[rt], l[rt]);
+        // (places are 32-bit numbers: the host sees to that)
+        if (pieces > 0) a.joins[at] = make_int2(static_cast<int>(slot + row), alone ? 0 : pieces);
       }
 #pragma unroll
       for (int cg = 0; cg < kGroups; ++cg)
@@ -707,61 +714,46 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
 }
 
 // Joins the pieces of the blocks that several workgroups had: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i with
-// m = max_i m_i.  A wave has a row's 32 columns: four lanes of eight columns times sixteen pieces at a time.
-constexpr int kJoinThreads = 256, kJoinColumns = 32;
-template <int DT, int kRows>
-__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(AttnArgs a) {
-  const int lane = static_cast<int>(threadIdx.x) & 63;
-  const uint32_t strips = (a.v.width + kJoinColumns - 1) / kJoinColumns, q_heads = a.heads * a.shared;
-  const uint32_t item = blockIdx.x * (kJoinThreads / kWave) + (threadIdx.x >> 6);
-  if (item >= static_cast<uint64_t>(a.rows) * q_heads * strips) return;
-  const uint32_t row = item / strips;
-  const int c = static_cast<int>(item % strips) * kJoinColumns + (lane & 3) * 8;
-  const int token = static_cast<int>(row / q_heads), q_head = static_cast<int>(row % q_heads), head = q_head / a.shared;
-  const int b = last_not_above(a.view.batch + 1, token, [&](int i) { return static_cast<int64_t>(row_bound(a.cu, i, a.rows)); });
-  if (b == a.view.batch && !a.clear_rest) return;
-  int pieces = 0, piece_row = 0;
-  int64_t slot = 0;
-  if (b < a.view.batch) {
-    const int r = (token - row_bound(a.cu, b, a.rows)) * a.shared + q_head % a.shared;
-    if (r < 0) return;
-    Mark mark;
-    if (!find_mark<kRows>(a, b, 0, a.parts, mark)) return;
-    if (mark.share.units > 0) {
-      const int per = part_units(mark.total, a.parts), first = mark.units_before + r / kRows * mark.share.units;
-      const int i0 = first / per, i1 = (first + mark.share.units - 1) / per;
-      if (i0 == i1) return;  // (written by its workgroup)
-      pieces = i1 - i0 + 1;
-      piece_row = r % kRows;
-      slot = static_cast<int64_t>(head) * a.slots + i0 + mark.blocks_before + r / kRows;
-    }
-  }
-  float m = -__builtin_inff();
-  for (int i = lane; i < pieces; i += 64) m = fmaxf(m, a.stats[((slot + i) * a.part_rows + piece_row) * 2]);
-  m = wave_max(m);
-  float l = 0.f, o[8] = {};
+// m = max_i m_i.  A group of 2^lanes_log2 lanes, eight columns each, takes every n-th piece of a row, n groups to a wave, in the
+// pieces' order; the groups meet through the lanes.  Bound by the latency of three dependent loads where there are few rows, by the pieces' bytes else.
+constexpr int kJoinThreads = 256;
+template <int DT>
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(AttnArgs a, int lanes_log2, uint32_t strips) {
+  const int lane = static_cast<int>(threadIdx.x) & 63, lanes = 1 << lanes_log2, groups = 64 >> lanes_log2;
+  const uint32_t item = blockIdx.x * (kJoinThreads / kWave) + (threadIdx.x >> 6), row = item / strips;
+  const int64_t q_heads = a.heads * a.shared, all = a.clear_rest ? a.rows : row_bound(a.cu, a.view.batch, a.rows);
+  if (row >= all * q_heads) return;
+  const int2 join = a.joins[row];
+  const int c = static_cast<int>(item - row * strips) * lanes * 8 + (lane & (lanes - 1)) * 8;
   const bool column = c < a.v.width;
-  if (m != -__builtin_inff()) {
-    for (int i = lane >> 2; i < pieces; i += 16) {
-      const int64_t at = (slot + i) * a.part_rows + piece_row;
-      const float mi = a.stats[at * 2], li = a.stats[at * 2 + 1], w = __builtin_amdgcn_exp2f(mi - m);
-      if (mi == -__builtin_inff()) continue;
-      l = fmaf(w, li, l);
-      if (!column) continue;
-      const float4* from = reinterpret_cast<const float4*>(a.part + at * a.v.width + c);
-      const float4 x = from[0], y = from[1];
-      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  float m = -__builtin_inff(), l = 0.f, o[8] = {};
+#pragma unroll 4
+  for (int i = lane >> lanes_log2; i < join.y; i += groups) {
+    const int64_t at = join.x + static_cast<int64_t>(i) * a.part_rows;
+    const float2 stat = *reinterpret_cast<const float2*>(a.stats + at * 2);
+    const float4* from = reinterpret_cast<const float4*>(a.part + at * a.v.width + (column ? c : 0));
+    const float4 x = from[0], y = from[1];
+    const float now = fmaxf(m, stat.x), base = now == -__builtin_inff() ? 0.f : now;
+    const float before = __builtin_amdgcn_exp2f(m - base), with = __builtin_amdgcn_exp2f(stat.x - base);
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    m = now;
+    l = l * before + stat.y * with;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = fmaf(w, v[j], o[j]);
-    }
-#pragma unroll
-    for (int off = 4; off < 64; off <<= 1) {
-      l += across(l, off);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] += across(o[j], off);
-    }
+    for (int j = 0; j < 8; ++j) o[j] = o[j] * before + v[j] * with;
   }
-  if (lane >= 4 || !column) return;
+  if (join.y <= 0) return;
+  float now = m;
+  for (int off = lanes; off < 64; off <<= 1) now = fmaxf(now, across(now, off));
+  const float with = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.f : now));
+  l *= with;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] *= with;
+  for (int off = lanes; off < 64; off <<= 1) {
+    l += across(l, off);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] += across(o[j], off);
+  }
+  if (lane >= lanes || !column) return;
   const float inverse = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int j = 0; j < 8; ++j) o[j] = l == 0.f ? 0.f : o[j] * inverse;
@@ -773,6 +765,7 @@ struct Plan {
   int rt, ct, ks, waves, slabs;
   int64_t blocks, parts;  // row blocks at most; parts of the line of units for each head and slab (0: a workgroup a block)
   int64_t slots, part_rows;
+  int join_lanes_log2;  // of the join: lanes to a row's strip
   int64_t workgroups(int64_t heads) const { return (parts > 0 ? parts : blocks) * heads * slabs; }
 };
 
@@ -792,10 +785,15 @@ Plan plan_of(const mega_paged_cache* c, int64_t rows, int64_t q_heads) {
   // workgroups that the chip holds at a time: eight waves to a CU
   const int64_t resident = kCus * kMaxWaves / p.waves, pairs = c->heads * p.slabs;
   const int64_t full = std::max(rows * shared / kRows, std::min(c->batch, rows)) * pairs;
-  if (c->batch > 0 && full < 4 * resident && p.blocks * (c->table_width * c->page_size / 32 + 1) < 0x40000000) {
+  if (c->batch > 0 && full < 4 * resident && p.blocks * (c->table_width * c->page_size / 32 + 1) < 0x40000000 &&
+      (resident + p.blocks) * c->heads * kRows < 0x40000000 && rows * q_heads < 0x1000000) {
     p.parts = std::max<int64_t>(1, resident / pairs);
     p.part_rows = std::min(kRows, rows * shared);
-    p.slots = p.parts + rows * shared / kRows + c->batch;
+    p.slots = p.parts + p.blocks;
+    // the join: as many pieces of a row at a time as it has on average
+    const int64_t pieces = p.parts * pairs / std::max<int64_t>(full, 1);
+    p.join_lanes_log2 = pieces > 8 ? 2 : pieces > 4 ? 3 : pieces > 2 ? 4 : 5;
+    while (p.join_lanes_log2 > 1 && (8 << (p.join_lanes_log2 - 1)) >= c->v_width) --p.join_lanes_log2;
   }
   return p;
 }
@@ -810,8 +808,9 @@ int launch_attn(const AttnArgs& a, const Plan& p, void* stream) {
   kernel<<<dim3(static_cast<uint32_t>(p.workgroups(a.heads))), dim3(p.waves * kWave), bytes, s>>>(a);
   MEGA_CHECK_LAUNCH();
   if (p.parts > 0) {
-    const int64_t waves = static_cast<int64_t>(a.rows) * a.heads * a.shared * ((a.v.width + kJoinColumns - 1) / kJoinColumns);
-    paged_join_kernel<DT, 16 * RT><<<dim3(static_cast<uint32_t>((waves + kJoinThreads / kWave - 1) / (kJoinThreads / kWave))), dim3(kJoinThreads), 0, s>>>(a);
+    const int64_t strip = 8 << p.join_lanes_log2, strips = (a.v.width + strip - 1) / strip, waves = static_cast<int64_t>(a.rows) * a.heads * a.shared * strips;
+    paged_join_kernel<DT><<<dim3(static_cast<uint32_t>((waves + kJoinThreads / kWave - 1) / (kJoinThreads / kWave))), dim3(kJoinThreads), 0, s>>>(
+        a, p.join_lanes_log2, static_cast<uint32_t>(strips));
     MEGA_CHECK_LAUNCH();
   }
   return MEGA_OK;
@@ -846,7 +845,7 @@ using namespace mega;
 extern "C" int64_t mega_paged_attention_workspace_bytes(const mega_paged_cache* cache, int64_t rows, int64_t q_heads, int64_t chunk) {
   if (!sizes_fit(cache, rows, q_heads, chunk) || rows == 0) return 0;
   const Plan p = plan_of(cache, rows, q_heads);
-  return p.parts > 0 ? cache->heads * p.slots * p.part_rows * (cache->v_width + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+  return p.parts > 0 ? cache->heads * p.slots * p.part_rows * (cache->v_width + 2) * static_cast<int64_t>(sizeof(float)) + rows * q_heads * static_cast<int64_t>(sizeof(int2)) : 0;
 }
 
 extern "C" int mega_paged_attention_fwd(const mega_paged_cache* cache, int dtype, const void* q, int64_t q_row, int64_t q_head,
@@ -855,7 +854,7 @@ extern "C" int mega_paged_attention_fwd(const mega_paged_cache* cache, int dtype
   if (const int rc = check_paged_cache(cache, dtype, "mega_paged_attention_fwd"); rc != MEGA_OK) return rc;
   MEGA_CHECK_ARG(sizes_fit(cache, rows, q_heads, chunk), "mega_paged_attention_fwd: bad sizes (q_heads has to be a multiple of the cache's heads)");
   MEGA_CHECK_ARG(cache->k_width <= kMaxKeyWidth, "mega_paged_attention_fwd: k_width must be at most 512");
-  if (rows == 0) return MEGA_OK;
+  if (rows == 0 || (cache->batch == 0 && clear_rest == 0)) return MEGA_OK;
   MEGA_CHECK_ARG(q != nullptr && out != nullptr && (lengths != nullptr || cache->batch == 0) && cu != nullptr, "mega_paged_attention_fwd: null pointer");
   MEGA_CHECK_ARG(reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_row % 8 == 0 && q_head % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
                  "mega_paged_attention_fwd: q and out must be 16-byte aligned");
@@ -868,7 +867,10 @@ extern "C" int mega_paged_attention_fwd(const mega_paged_cache* cache, int dtype
   a.q = static_cast<const uint16_t*>(q), a.q_row = q_row, a.q_head = q_head;
   a.lengths = lengths, a.cu = cu, a.out = static_cast<uint16_t*>(out);
   a.part = static_cast<float*>(workspace);
-  if (p.parts > 0) a.stats = a.part + cache->heads * p.slots * p.part_rows * cache->v_width;
+  if (p.parts > 0) {
+    a.stats = a.part + cache->heads * p.slots * p.part_rows * cache->v_width;
+    a.joins = reinterpret_cast<int2*>(a.stats + cache->heads * p.slots * p.part_rows * 2);
+  }
   a.rows = static_cast<int32_t>(rows), a.heads = static_cast<int32_t>(cache->heads), a.shared = static_cast<int32_t>(q_heads / cache->heads);
   a.chunk = static_cast<int32_t>(chunk), a.slabs = p.slabs, a.blocks = static_cast<int32_t>(p.blocks);
   a.parts = static_cast<int32_t>(p.parts), a.slots = static_cast<int32_t>(p.slots), a.part_rows = static_cast<int32_t>(p.part_rows);
