@@ -1,0 +1,356 @@
+// What the kernels of the paged attention share: their arguments, the way from a workgroup to its rows and keys, the rows'
+// way into LDS and the results' way out.
+#pragma once
+
+#include "paged.hpp"
+
+namespace mega {
+
+constexpr int kMaxWaves = 8;
+constexpr int kMaxKeyWidth = 512;
+constexpr int kCus = 256;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct AttnArgs {
+  PagedView view;
+  PagedPool k, v;
+  const uint16_t* q;
+  int64_t q_row, q_head;
+  const int32_t *lengths, *cu;
+  uint16_t* out;
+  float *part, *stats;        // parts > 0: (heads, slots, part_rows, v_width), (heads, slots, part_rows, 2)
+  int2* joins;                // ... (rows, q_heads): a row's first place in the former and its number of pieces (0: out has it)
+  int32_t rows, heads, shared, chunk, slabs, blocks;
+  int32_t parts, slots, part_rows;  // parts of the line of units for each head and slab; 0: a workgroup a block
+  int32_t clear_rest;
+  float scale;                // times log2(e)
+};
+
+// A row block of one sequence and the keys that any of its rows sees.
+struct Block {
+  int32_t sequence;
+  int32_t start, row0, count;  // first packed row of the sequence; first row (token * shared + head) and their number
+  int32_t position0;           // position of the sequence's first new token
+  int32_t keys;                // positions that have a place
+  int32_t begin, end;          // keys that the block sees, [begin, end)
+};
+
+// A load that the scalar unit may make: of what no kernel writes while this one runs, at an address that a wave has in common.
+typedef const int32_t __attribute__((address_space(4))) ConstInt;
+__device__ __forceinline__ int32_t constant_at(const int32_t* p, int64_t i) { return reinterpret_cast<ConstInt*>(reinterpret_cast<uint64_t>(p))[i]; }
+
+__device__ __forceinline__ int chunk_start(int position, int chunk) { return chunk > 0 && position > 0 ? position / chunk * chunk : 0; }
+
+// Sequences, the rows behind the last one counted as one more where they are to be cleared.
+__device__ __forceinline__ int sequences_of(const AttnArgs& a) { return a.view.batch + (a.clear_rest ? 1 : 0); }
+
+// Sequence b (the rows behind the last one are one more, without keys) and its row block `number`; false: it has no such block.
+template <int kRows>
+__device__ __forceinline__ bool block_of(const AttnArgs& a, int b, int64_t number, Block& k) {
+  k.sequence = b;
+  k.start = row_bound(a.cu, b, a.rows);
+  const int n = (b < a.view.batch ? row_bound(a.cu, b + 1, a.rows) : a.rows) - k.start;
+  const int64_t row0 = number * kRows;
+  if (row0 < 0 || row0 >= static_cast<int64_t>(n) * a.shared) return false;
+  k.row0 = static_cast<int32_t>(row0);
+  k.count = static_cast<int32_t>(min(static_cast<int64_t>(kRows), static_cast<int64_t>(n) * a.shared - row0));
+  const int length = b < a.view.batch ? max(a.lengths[b], 0) : 0;
+  k.keys = static_cast<int32_t>(min(static_cast<int64_t>(length), static_cast<int64_t>(a.view.table_width) << a.view.page_shift));
+  k.position0 = length - n;
+  k.begin = chunk_start(k.position0 + k.row0 / a.shared, a.chunk);
+  k.end = min(k.position0 + (k.row0 + k.count - 1) / a.shared + 1, k.keys);
+  return true;
+}
+
+// A workgroup a block: blocks are numbered so that sequence b's begin at cu[b] shared / kRows + b, which leaves ceil(n shared / kRows)
+// numbers before the next sequence's whatever the lengths are, and the host need not know these.
+template <int kRows>
+__device__ __forceinline__ bool find_block(const AttnArgs& a, int number, Block& k) {
+  const int sequences = sequences_of(a);
+  const auto first = [&](int b) { return static_cast<int64_t>(row_bound(a.cu, b, a.rows)) * a.shared / kRows + b; };
+  const int b = last_not_above(sequences, number, first);
+  return block_of<kRows>(a, b, number - first(b), k);
+}
+
+// The line of units: a block has one for every 32 keys that it sees, and one if there are none.
+__device__ __forceinline__ int units_of(const Block& k) { return max(k.end - (k.begin & ~31) + 31, 32) >> 5; }
+template <int kRows>
+__device__ __forceinline__ int blocks_of(const AttnArgs& a, int b) {
+  const int n = (b < a.view.batch ? row_bound(a.cu, b + 1, a.rows) : a.rows) - row_bound(a.cu, b, a.rows);
+  return n > 0 ? static_cast<int>((static_cast<int64_t>(n) * a.shared + kRows - 1) / kRows) : 0;
+}
+// A place on the line: a block (its sequence, its number there), its units, and the blocks and units in front of it.
+struct Mark {
+  int32_t sequence, number, blocks, units;  // blocks: of the sequence
+  int32_t blocks_before, units_before, total;  // total: of the whole line (the host cuts no line of 2^30 units)
+};
+// units of a part; the parts behind the line's end are empty
+__device__ __forceinline__ int part_units(int total, int parts) { return (total + parts - 1) / parts; }
+
+__device__ __forceinline__ int sums_before_and_here(int v) {  // inclusive sums over the lanes
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int u = __shfl_up(v, off, 64);
+    if (lane >= off) v += u;
+  }
+  return v;
+}
+// The units of the 64 blocks of sequence b from `number` on, one to a lane
+template <int kRows>
+__device__ __forceinline__ int lane_units(const AttnArgs& a, int b, int number, int blocks) {
+  Block k;
+  const int i = number + (static_cast<int>(threadIdx.x) & 63);
+  return i < blocks && block_of<kRows>(a, b, i, k) ? units_of(k) : 0;
+}
+
+// The block in which part `part` begins (false: the part is empty); all lanes of a wave together, 64 sequences a round, and 64 blocks of a
+// sequence that has more than one.
+template <int kRows>
+__device__ __forceinline__ bool find_mark(const AttnArgs& a, int part, Mark& mark) {
+  const int lane = static_cast<int>(threadIdx.x) & 63, sequences = sequences_of(a);
+  int blocks = 0, units = 0, units_here = 0, blocks_here = 0;  // of the lane's sequence; inclusive sums
+  const auto round = [&](int b0) {
+    const int b = b0 + lane;
+    blocks = b < sequences ? blocks_of<kRows>(a, b) : 0, units = 0;
+    Block k;
+    if (blocks > 0 && block_of<kRows>(a, b, 0, k)) units = units_of(k);
+    for (uint64_t more = __ballot(blocks > 1); more != 0; more &= more - 1) {
+      const int l = __ffsll(static_cast<unsigned long long>(more)) - 1, count = __builtin_amdgcn_readlane(blocks, l);
+      int sum = 0;
+      for (int i = 0; i < count; i += 64) sum += lane_units<kRows>(a, b0 + l, i, count);
+      sum = __builtin_amdgcn_readlane(sums_before_and_here(sum), 63);
+      if (lane == l) units = sum;
+    }
+    units_here = sums_before_and_here(units), blocks_here = sums_before_and_here(blocks);
+  };
+  mark.total = 0;
+  for (int b0 = 0; b0 < sequences; b0 += 64) {
+    round(b0);
+    mark.total += __builtin_amdgcn_readlane(units_here, 63);
+  }
+  const int first = part * part_units(mark.total, a.parts);
+  if (first >= mark.total) return false;
+  int units_before = 0, blocks_before = 0;
+  for (int b0 = 0; b0 < sequences; b0 += 64) {
+    if (sequences > 64) round(b0);
+    const uint64_t which = __ballot(units_before + units_here > first);
+    if (which != 0) {
+      const int l = __ffsll(static_cast<unsigned long long>(which)) - 1;
+      mark.sequence = b0 + l;
+      mark.blocks = __builtin_amdgcn_readlane(blocks, l);
+      mark.units_before = units_before + __builtin_amdgcn_readlane(units_here - units, l);
+      mark.blocks_before = blocks_before + __builtin_amdgcn_readlane(blocks_here - blocks, l);
+      mark.number = 0, mark.units = __builtin_amdgcn_readlane(units, l);
+      if (mark.blocks == 1) return true;
+      for (int i = 0; i < mark.blocks; i += 64) {
+        const int own = lane_units<kRows>(a, mark.sequence, i, mark.blocks), here = sums_before_and_here(own);
+        const uint64_t found = __ballot(mark.units_before + here > first);
+        if (found != 0) {
+          const int f = __ffsll(static_cast<unsigned long long>(found)) - 1;
+          mark.number = i + f, mark.units = __builtin_amdgcn_readlane(own, f);
+          mark.units_before += __builtin_amdgcn_readlane(here - own, f);
+          mark.blocks_before += mark.number;
+          return true;
+        }
+        mark.units_before += __builtin_amdgcn_readlane(here, 63);
+      }
+    }
+    units_before += __builtin_amdgcn_readlane(units_here, 63);
+    blocks_before += __builtin_amdgcn_readlane(blocks_here, 63);
+  }
+  return false;
+}
+
+template <int DT>
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (DT == MEGA_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <int DT, bool kUpper>
+__device__ __forceinline__ uint32_t widen(uint32_t codes, float scale) {
+  if constexpr (DT == MEGA_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, kUpper));
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, kUpper));
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (DT == MEGA_BF16) return pack_bf16x2(lo, hi);
+  return static_cast<uint32_t>(float_to_f16_bits(lo)) | (static_cast<uint32_t>(float_to_f16_bits(hi)) << 16);
+}
+
+// ones over those halves of a word whose 16-bit numbers are finite
+template <int DT>
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
+  constexpr uint32_t top = DT == MEGA_BF16 ? 0x7f80u : 0x7c00u;
+  return ((w & top) == top ? 0u : 0xffffu) | ((w >> 16 & top) == top ? 0u : 0xffff0000u);
+}
+
+// ones over those bytes of a word whose e4m3 codes are numbers
+__device__ __forceinline__ uint32_t finite_codes(uint32_t w) {
+  uint32_t keep = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) keep |= ((w >> (8 * i)) & 0x7fu) == 0x7fu ? 0u : 0xffu << (8 * i);
+  return keep;
+}
+
+// v, of which the compiler knows nothing: what is computed from it is computed where it is used, not once ahead of a loop
+// and kept in registers that the loop has no room for
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+__device__ __forceinline__ float across(float v, int mask) { return __shfl_xor(v, mask, 64); }
+
+// The page of 16 keys: its number and whether there is one (0 otherwise, so that addresses stay in the pool).
+struct Page {
+  uint32_t number;
+  bool there;
+};
+__device__ __forceinline__ Page page_of(const AttnArgs& a, int sequence, int key) {
+  const uint32_t e = static_cast<uint32_t>(constant_at(a.view.table, sequence * a.view.table_stride + (key >> a.view.page_shift)));
+  const bool there = e < static_cast<uint32_t>(a.view.pages);
+  return {there ? e : 0, there};
+}
+
+// Where a workgroup is on the line of units, kept in LDS while it works on a piece.
+struct Progress {
+  Mark mark;
+  int32_t unit, unit_end, per;
+  int32_t pieces;  // of the block, this one included if it is the first; 0 for the others
+  bool alone;      // the whole block is this workgroup's
+};
+
+// The first row block of a workgroup, or its place on the line of units; false: it has none.
+template <int kRows>
+__device__ __forceinline__ bool first_piece(const AttnArgs& a, int id, Progress& progress, Block& k) {
+  if (a.parts == 0) return find_block<kRows>(a, a.blocks - 1 - id, k);
+  Progress at;
+  if (!find_mark<kRows>(a, id, at.mark)) return false;
+  at.per = part_units(at.mark.total, a.parts);
+  at.unit = id * at.per, at.unit_end = min(at.unit + at.per, at.mark.total);
+  if (threadIdx.x == 0) progress = at;
+  __syncthreads();
+  return true;
+}
+// The workgroup's next piece: a block and which of its keys, [begin, end), begin a multiple of 32.
+template <int kRows>
+__device__ __forceinline__ void take_piece(const AttnArgs& a, int id, Progress& progress, Block& k, int& begin, int& end) {
+  if (a.parts == 0) {
+    begin = k.begin & ~31, end = k.end;
+    return;
+  }
+  Progress at = progress;
+  __syncthreads();
+  if (at.unit == at.mark.units_before + at.mark.units) {  // on to the next block (unit < total: there is one)
+    at.mark.units_before += at.mark.units, ++at.mark.blocks_before;
+    if (++at.mark.number == at.mark.blocks) {
+      do at.mark.blocks = blocks_of<kRows>(a, ++at.mark.sequence);
+      while (at.mark.blocks == 0);
+      at.mark.number = 0;
+    }
+  }
+  block_of<kRows>(a, __builtin_amdgcn_readfirstlane(at.mark.sequence), __builtin_amdgcn_readfirstlane(at.mark.number), k);
+  at.mark.units = units_of(k);
+  const int units = at.mark.units, first = at.mark.units_before, last = min(first + units, at.unit_end);
+  begin = __builtin_amdgcn_readfirstlane((k.begin & ~31) + (at.unit - first) * 32);
+  end = __builtin_amdgcn_readfirstlane(min((k.begin & ~31) + (last - first) * 32, k.end));
+  const int begins_in = first / at.per, ends_in = (first + units - 1) / at.per;
+  at.alone = begins_in == ends_in;
+  at.pieces = begins_in == id ? ends_in - begins_in + 1 : 0;
+  at.unit = last;
+  if (threadIdx.x == 0) progress = at;
+}
+
+// The block's rows of query head `head` ... of the cache head to LDS, [row tile][step][lane]: the order in which the matrix instructions take
+// them, zeros behind the rows' end and in rows that there are not.
+template <bool kEight, int kRows, int KS>
+__device__ __forceinline__ void rows_to_lds(const AttnArgs& a, const Block& k, int head, uint4* lds_q) {
+  for (int c = threadIdx.x; c < kRows * KS * 4; c += blockDim.x) {
+    const int row = c / (KS * 4), d = c % (KS * 4);  // eight elements of a row
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (row < k.count && d * 8 < a.k.width) {
+      const int r = k.row0 + row, t = r / a.shared, g = r - t * a.shared;
+      x = *reinterpret_cast<const uint4*>(a.q + (static_cast<int64_t>(k.start) + t) * a.q_row + (static_cast<int64_t>(head) * a.shared + g) * a.q_head + d * 8);
+    }
+    // (8-bit keys: a lane reads 16 codes at a time, which serve two steps)
+    const int step = kEight ? (d >> 3) * 2 + (d & 1) : d >> 2, quarter = kEight ? (d >> 1) & 3 : d & 3;
+    lds_q[((row >> 4) * KS + step) * 64 + quarter * 16 + (row & 15)] = x;
+  }
+}
+// The rows' visible keys of a piece to LDS: the first one and the number of further ones (none: a first one that no key reaches).
+template <int kRows>
+__device__ __forceinline__ void ranges_to_lds(const AttnArgs& a, const Block& k, int end, int2* lds_sees) {
+  for (int row = threadIdx.x; row < kRows; row += blockDim.x) {
+    const int position = k.position0 + (k.row0 + row) / a.shared, low = chunk_start(position, a.chunk), high = min(position, end - 1);
+    const bool none = row >= k.count || high < low;
+    lds_sees[row] = none ? make_int2(0x7fffffff, 0) : make_int2(low, high - low);
+  }
+}
+__device__ __forceinline__ bool in_range(int2 range, int key) { return static_cast<uint32_t>(key) - static_cast<uint32_t>(range.x) <= static_cast<uint32_t>(range.y); }
+
+// A wave's accumulators to out, or with the rows' m and l to the workspace; true: this was the workgroup's last piece.
+// Accumulator element i of column operand j is column kCols (4 h + i) + j of its group of 16 kCols; eight columns are stored at a time.
+template <int DT, int RT, int CT, int kCols>
+__device__ __forceinline__ bool store_piece(const AttnArgs& a, const Block& k, int id, int head, int slab, int wave, int first_column, const Progress& progress,
+                                            const f32x4 (&acc)[RT][CT], const float (&m)[RT], const float (&l)[RT]) {
+  const int lane = opaque(static_cast<int>(threadIdx.x) & 63), n = lane & 15, h = lane >> 4;
+  bool alone = true, last = true;
+  int64_t slot = 0;
+  int pieces = 0;
+  if (a.parts > 0) {
+    slot = (static_cast<int64_t>(head) * a.slots + id + progress.mark.blocks_before) * a.part_rows;
+    alone = progress.alone, pieces = progress.pieces, last = progress.unit >= progress.unit_end;
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int row = rt * 16 + n;
+    if (row >= k.count) continue;
+    const int r = k.row0 + row, t = r / a.shared, g = r - t * a.shared;
+    const int64_t at = (static_cast<int64_t>(k.start) + t) * (a.heads * a.shared) + head * a.shared + g;
+    const float inverse = l[rt] == 0.f ? 0.f : 1.f / l[rt];
+    if (a.parts > 0 && slab == 0 && wave == 0 && h == 0) {
+      if (!alone) *reinterpret_cast<float2*>(a.stats + (slot + row) * 2) = make_float2(m[rt], l[rt]);
+      // (places are 32-bit numbers: the host sees to that)
+      if (pieces > 0) a.joins[at] = make_int2(static_cast<int>(slot + row), alone ? 0 : pieces);
+    }
+#pragma unroll
+    for (int cg = 0; cg < CT / kCols; ++cg)
+#pragma unroll
+      for (int i = 0; i < 4; i += 8 / kCols) {
+        const int c = first_column + 16 * kCols * cg + kCols * (4 * h + i);
+        if (c >= a.v.width) continue;
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = acc[rt][kCols * cg + j % kCols][i + j / kCols];
+        if (!alone) {
+          float4* to = reinterpret_cast<float4*>(a.part + (slot + row) * a.v.width + c);
+          to[0] = make_float4(o[0], o[1], o[2], o[3]);
+          to[1] = make_float4(o[4], o[5], o[6], o[7]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = l[rt] == 0.f ? 0.f : o[j] * inverse;
+          *reinterpret_cast<uint4*>(a.out + at * a.v.width + c) =
+              make_uint4(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]), pack2<DT>(o[4], o[5]), pack2<DT>(o[6], o[7]));
+        }
+      }
+  }
+  return last;
+}
+
+// Blocks of more than 32 rows (paged_attention_rows.hip).
+struct RowsPlan {
+  int ks, waves;  // 32-wide steps of a key row, waves of a workgroup
+  int64_t workgroups;
+};
+int launch_paged_rows(const AttnArgs& a, const RowsPlan& p, int dtype, bool eight, void* stream);
+
+}  // namespace mega

@@ -1,0 +1,467 @@
+// Paged attention for many rows of a sequence at a time: prompts and their pieces.
+//
+// The mathematics and the lane layout are those of paged_attention.hip; what differs is what bounds it.  With 64 rows a
+// value that has been read serves 64 rows, and the matrix cores are the limit to come near to, so the work of a wave is arranged
+// for them:
+//   - accumulators of 64 rows x 256 columns, the whole accumulation half of a SIMD's registers, one wave to a SIMD, four to a
+//     workgroup: nothing of another wave hides this one's waits, so everything it will need is on its way long before --
+//     the values of the next 32 keys, the keys of the next tile, the next step's probabilities;
+//   - a step's values are turned into operands two columns at a time, while the two columns before them are multiplied;
+//   - a wave's scores are those of 64 keys at a time, so a row operand from LDS serves four key operands.
+// Up to 128 value columns: one wave has all of them, eight workgroups of one wave share a CU (two to a SIMD: the softmax of one beside the
+// products of the other), and probabilities never leave the registers.
+#include "paged_attention.hpp"
+
+namespace mega {
+namespace {
+
+// kSolo: a workgroup is one wave.  KG: 16-key groups of a wave's share of a tile.  kWavesPerSimd: what the registers are cut for; with two, the
+// values of a tile are called for behind its scores, for whose registers they wait.
+template <int DT, bool kEight, int RT, int CT, int KS, int KG, bool kSolo, int kWavesPerSimd>
+__global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPerSimd) void paged_rows_kernel(AttnArgs a) {
+  constexpr int kRows = 16 * RT, kGroups = CT / 8, kBytes = kEight ? 1 : 2, kMostWaves = 4 * kWavesPerSimd, kSteps = KG / 2;
+  constexpr bool kLate = kWavesPerSimd > 1;
+  constexpr int kChunk = KS < 4 ? KS : 4, kLoads = kEight ? kChunk / 2 : kChunk;  // steps of a key row in flight; a lane's 16-byte parts of them
+  extern __shared__ __align__(16) uint4 lds[];
+  __shared__ Progress progress;
+  const int wave = kSolo ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), waves = kSolo ? 1 : static_cast<int>(blockDim.x) >> 6;
+  uint4* const lds_q = lds;                  // [RT][KS][64]
+  uint4* const lds_p = lds + RT * KS * 64;   // [waves * kSteps][RT][64]
+  float* const lds_m = reinterpret_cast<float*>(kSolo ? lds_p : lds_p + waves * kSteps * RT * 64);  // [kRows][kMostWaves]
+  int* const lds_pages = reinterpret_cast<int*>(lds_m + kRows * kMostWaves);                        // [kMostWaves]: the waves' keys have pages
+  int2* const lds_sees = reinterpret_cast<int2*>(lds_pages + kMostWaves);                           // [kRows]
+
+  // (as in paged_attention.hip)
+  uint32_t id = blockIdx.x;
+  const int slab = id % a.slabs;
+  id /= a.slabs;
+  const int head = id % a.heads;
+  id /= a.heads;
+  const int page_mask = (1 << a.view.page_shift) - 1;
+  const int first_column = (slab * waves + wave) * CT * 16;
+  Block k;
+  if (!first_piece<kRows>(a, static_cast<int>(id), progress, k)) return;
+
+  for (;;) {
+    const int lane = opaque(static_cast<int>(threadIdx.x) & 63);
+    int begin, end;
+    take_piece<kRows>(a, static_cast<int>(id), progress, k, begin, end);
+    rows_to_lds<kEight, kRows, KS>(a, k, head, lds_q);
+    ranges_to_lds<kRows>(a, k, end, lds_sees);
+    if constexpr (!kSolo) {
+      for (int c = threadIdx.x; c < kRows * kMostWaves; c += blockDim.x) lds_m[c] = -__builtin_inff();  // (of waves that there are not, too)
+      if (threadIdx.x < kMostWaves) lds_pages[threadIdx.x] = 1;
+    }
+    // keys all_low .. all_high are seen by every row of the block
+    const int all_low = chunk_start(k.position0 + (k.row0 + k.count - 1) / a.shared, a.chunk), all_high = min(k.position0 + k.row0 / a.shared, end - 1);
+
+    // ---- keys: a lane's 16 bytes of key 16 group + (lane & 15)
+    u32x4 kx[KG][kLoads];
+    uint32_t ke[KG][4];
+    struct Keys {
+      const uint8_t* from[KG];
+      const uint8_t* exponents[KG];
+      bool there[KG];
+    };
+    const auto keys_at = [&](int first) {
+      Keys t;
+#pragma unroll
+      for (int g = 0; g < KG; ++g) {
+        const int held = min(first + 16 * g, (end - 1) & ~15), place = held & page_mask;
+        const Page page = page_of(a, k.sequence, held);
+        t.there[g] = page.there;
+        t.from[g] = static_cast<const uint8_t*>(a.k.rows) + (page.number * a.k.page + static_cast<int64_t>(head) * a.k.head + static_cast<int64_t>(place) * a.k.slot) * kBytes;
+        if constexpr (kEight) t.exponents[g] = a.k.exponents + (page.number * a.k.ePage + static_cast<int64_t>(head) * a.k.eHead + static_cast<int64_t>(place) * a.k.eSlot);
+      }
+      return t;
+    };
+    const auto load_key = [&](const Keys& t, int g, int part) {
+      const int l = opaque(lane), d = min((kEight ? 64 : 32) * part + (kEight ? 16 : 8) * (l >> 4), a.k.width - (kEight ? 16 : 8));
+      kx[g][part % kLoads] = *reinterpret_cast<const u32x4*>(t.from[g] + (static_cast<uint32_t>(l & 15) * a.k.slot + d) * kBytes);
+    };
+    const auto load_keys = [&](int tile) {
+      const Keys t = keys_at(min(tile + 16 * KG * wave, (end - 1) & ~31));
+      if constexpr (kEight) {
+        const uint32_t offset = static_cast<uint32_t>(4 * (opaque(lane) >> 4)) * a.k.eSlot;
+#pragma unroll
+        for (int g = 0; g < KG; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ke[g][i] = t.exponents[g][offset + static_cast<uint32_t>(i * a.k.eSlot)];
+      }
+#pragma unroll
+      for (int part = 0; part < kLoads; ++part)
+#pragma unroll
+        for (int g = 0; g < KG; ++g) load_key(t, g, part);
+    };
+
+    // ---- values: eight columns of eight of a step's 32 keys to a lane and column group
+    typedef uint32_t Piece __attribute__((ext_vector_type(kEight ? 2 : 4)));
+    Piece x[kGroups][8];
+    uint32_t e[8];
+    bool there[2] = {false, false};
+    struct Step {
+      const uint8_t* from[2];
+      const uint8_t* exponents[2];
+      bool there[2];
+    };
+    const auto step_at = [&](int first) {
+      Step t;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int held = min(first + 16 * half, (end - 1) & ~15), place = held & page_mask;
+        const Page page = page_of(a, k.sequence, held);
+        t.there[half] = page.there;
+        t.from[half] = static_cast<const uint8_t*>(a.v.rows) + (page.number * a.v.page + static_cast<int64_t>(head) * a.v.head + static_cast<int64_t>(place) * a.v.slot) * kBytes;
+        if constexpr (kEight) t.exponents[half] = a.v.exponents + (page.number * a.v.ePage + static_cast<int64_t>(head) * a.v.eHead + static_cast<int64_t>(place) * a.v.eSlot);
+      }
+      return t;
+    };
+    const auto load_values = [&](const Step& t, int g) {
+      // (columns behind the last are computed from others and not written)
+      const int l = opaque(lane);
+      const uint32_t offset = (static_cast<uint32_t>(4 * (l >> 4)) * a.v.slot + min(first_column + g * 128 + (l & 15) * 8, a.v.width - 8)) * kBytes;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[g][i] = *reinterpret_cast<const Piece*>(t.from[i >> 2] + (offset + static_cast<uint32_t>((i & 3) * a.v.slot * kBytes)));
+    };
+    const auto load_exponents = [&](const Step& t) {
+      if constexpr (kEight) {
+        const uint32_t offset = static_cast<uint32_t>(4 * (opaque(lane) >> 4)) * a.v.eSlot;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = t.exponents[i >> 2][offset + static_cast<uint32_t>((i & 3) * a.v.eSlot)];
+      }
+    };
+    const auto load_step = [&](int first) {
+      const Step t = step_at(first);
+      load_exponents(t);
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) load_values(t, g);
+      there[0] = t.there[0], there[1] = t.there[1];
+    };
+
+    f32x4 acc[RT][CT];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m[rt] = -__builtin_inff(), l[rt] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) acc[rt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (begin < end) {
+      if constexpr (!kLate) load_keys(begin);
+      if constexpr (!kLate) load_step(begin);
+    }
+    __syncthreads();
+
+    for (int tile = begin; tile < end; tile += 16 * KG * waves) {
+      // ---- scores of the wave's keys (a wave behind the end computes others' again: nothing is seen of them)
+      const int mine = tile + 16 * KG * wave;
+      f32x4 s[KG][RT];
+      if constexpr (kLate) load_keys(tile);
+      const Keys keys = keys_at(min(mine, (end - 1) & ~31));
+      bool pages_there = true, whole = mine >= all_low && mine + 16 * KG - 1 <= all_high;
+#pragma unroll
+      for (int g = 0; g < KG; ++g) pages_there = pages_there && keys.there[g];
+      whole = whole && pages_there;
+      {
+        u32x4 q[RT], q_next[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) q_next[rt] = __builtin_bit_cast(u32x4, lds_q[rt * KS * 64 + lane]);
+#pragma unroll
+        for (int g = 0; g < KG; ++g)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) s[g][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KS; ++c) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {  // (the rows' operands one step ahead; the fence keeps it at that)
+            q[rt] = q_next[rt];
+            if (c + 1 < KS) q_next[rt] = __builtin_bit_cast(u32x4, lds_q[(rt * KS + c + 1) * 64 + lane]);
+          }
+#pragma unroll
+          for (int g = 0; g < KG; ++g) {
+            const int part = kEight ? c >> 1 : c;
+            u32x4 key = kx[g][part % kLoads];
+            if constexpr (kEight) {
+              const uint32_t lo = (c & 1) ? key[2] : key[0], hi = (c & 1) ? key[3] : key[1];
+              key = u32x4{widen<DT, false>(lo, 1.f), widen<DT, true>(lo, 1.f), widen<DT, false>(hi, 1.f), widen<DT, true>(hi, 1.f)};
+            }
+            if (a.k.width != 32 * KS) {  // (behind the row's end the rows' operands are zero, and infinity times zero is not)
+              const int d = kEight ? (c >> 1) * 64 + (opaque(lane) >> 4) * 16 : c * 32 + (opaque(lane) >> 4) * 8;
+              if (d >= a.k.width) key = u32x4{0, 0, 0, 0};
+            }
+            if (c + kChunk < KS && (!kEight || (c & 1))) load_key(keys, g, part + kLoads);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) s[g][rt] = mma<DT>(key, q[rt], s[g][rt]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < KG; ++g) {
+        f32x4 factor = {a.scale, a.scale, a.scale, a.scale};
+        if constexpr (kEight)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) factor[i] *= exponent_value(ke[g][i]);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[g][rt] *= factor;
+      }
+      if constexpr (!kLate) load_keys(tile + 16 * KG * waves);
+      if constexpr (kLate) load_step(tile);
+      if (!whole) {
+        const int l = opaque(lane), n = l & 15, first = mine + 4 * (l >> 4);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const int2 range = lds_sees[rt * 16 + n];
+#pragma unroll
+          for (int g = 0; g < KG; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!keys.there[g] || !in_range(range, first + 16 * g + i)) s[g][rt][i] = -__builtin_inff();
+        }
+      }
+
+      // ---- the rows' maxima, probabilities and sums, as in paged_attention.hip
+      float top[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float t = s[0][rt][0];
+#pragma unroll
+        for (int g = 0; g < KG; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t = fmaxf(t, s[g][rt][i]);
+        t = fmaxf(t, across(t, 16));
+        top[rt] = fmaxf(t, across(t, 32));
+      }
+      if constexpr (!kSolo) {
+        const int l = opaque(lane), n = l & 15;
+        if (l < 16)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * kMostWaves + wave] = top[rt];
+        if (l == 0) lds_pages[wave] = pages_there;
+        __syncthreads();
+        int all_there = 1;
+#pragma unroll
+        for (int w = 0; w < kMostWaves; w += 4) {
+          const int4 u = *reinterpret_cast<const int4*>(lds_pages + w);
+          all_there &= u.x & u.y & u.z & u.w;
+        }
+        pages_there = __builtin_amdgcn_readfirstlane(all_there) != 0;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int w = 0; w < kMostWaves; w += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(lds_m + (rt * 16 + n) * kMostWaves + w);
+            top[rt] = fmaxf(top[rt], fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+          }
+      }
+      u32x4 own[kSteps][RT];  // (kSolo: the operands themselves)
+      bool moved = false;
+      float alpha[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float now = top[rt] > m[rt] + 8.f ? top[rt] : m[rt], base = now == -__builtin_inff() ? 0.f : now;
+        alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - base);
+        moved = moved || now != m[rt];
+        m[rt] = now;
+        float sum = 0.f;
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+          float p[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(s[2 * st + (i >> 2)][rt][i & 3] - base);
+            sum += p[i];
+          }
+          own[st][rt] = u32x4{pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
+          if constexpr (!kSolo) lds_p[((wave * kSteps + st) * RT + rt) * 64 + lane] = __builtin_bit_cast(uint4, own[st][rt]);
+        }
+        l[rt] = l[rt] * alpha[rt] + sum;
+      }
+      if (__any(moved))
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int c = 0; c < CT; ++c) acc[rt][c] *= alpha[rt];
+      if constexpr (!kSolo) __syncthreads();
+
+      // ---- values: 32 keys a step
+      const auto operands = [&](int step, u32x4 (&p)[RT]) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) p[rt] = kSolo ? own[step % kSteps][rt] : __builtin_bit_cast(u32x4, lds_p[(step * RT + rt) * 64 + lane]);
+      };
+      const auto step_of = [&](int step, bool more, u32x4 (&p)[RT], u32x4 (&p_next)[RT]) {
+        const int first = tile + 32 * step;
+        const Step next = step_at(min(first + 32, (end - 1) & ~31));
+        bool odd = false;
+        if (first < all_low || first + 31 > all_high || !pages_there) {
+          // what is not there, or not this workgroup's, must not meet a probability of zero as an infinity or NaN; nor must such a
+          // value of a key that only some rows see, which goes to those alone below
+          const int h = opaque(lane) >> 4;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int key = first + 16 * (i >> 2) + 4 * h + (i & 3);
+            const uint32_t keep = key >= k.begin && key < end && there[i >> 2] ? ~0u : 0u;
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+              for (int j = 0; j < (kEight ? 2 : 4); ++j) {
+                const uint32_t finite = kEight ? finite_codes(x[g][i][j]) : finite_halves<DT>(x[g][i][j]);
+                odd = odd || (~finite & keep) != 0;
+                x[g][i][j] &= keep & finite;
+              }
+          }
+        }
+        float unit[8];
+        if constexpr (kEight) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) unit[i] = exponent_value(e[i]);
+          if (more) load_exponents(next);
+        }
+        // columns 2 j, 2 j + 1 of a lane's eight in group g as operands
+        const auto convert = [&](int u, u32x4 (&vt)[2]) {
+          const int g = u >> 2, j = u & 3;
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if constexpr (kEight)
+              w[i] = (j & 1) ? widen<DT, true>(x[g][i][j >> 1], unit[i]) : widen<DT, false>(x[g][i][j >> 1], unit[i]);
+            else
+              w[i] = x[g][i][j];
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            vt[0][i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100);
+            vt[1][i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302);
+          }
+        };
+        u32x4 vt[2][2];
+        convert(0, vt[0]);
+#pragma unroll
+        for (int u = 0; u < 4 * kGroups; ++u) {
+          if (u + 1 < 4 * kGroups) convert(u + 1, vt[(u + 1) & 1]);
+          if ((u & 3) == 2 && more) load_values(next, u >> 2);  // (the group's last columns have just been converted)
+          if (kSolo && u == 0 && more) operands(step + 1, p_next);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) acc[rt][2 * u + j] = mma<DT>(vt[u & 1][j], p[rt], acc[rt][2 * u + j]);
+        }
+        if (__any(odd)) {  // key by key, its infinities and NaN into the rows that see it
+          const Step t = step_at(first);
+#pragma unroll 1
+          for (int slot = 0; slot < 32; ++slot) {
+            const int l = opaque(lane), n = l & 15, h = l >> 4;
+            const int place = slot & 7, half = place >> 2, in_group = 4 * (slot >> 3) + (place & 3), key = first + 16 * half + in_group;
+            if (key < k.begin || key >= end || !(half ? t.there[1] : t.there[0])) continue;
+            const uint8_t* const row = (half ? t.from[1] : t.from[0]) + static_cast<int64_t>(in_group) * a.v.slot * kBytes;
+            float weight[RT];
+            bool its[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              // (the lane of this row and slot has the probability, in its place of eight)
+              uint32_t word = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) word = (place >> 1) == i ? p[rt][i] : word;
+              word = static_cast<uint32_t>(__shfl(static_cast<int>(word), (slot & ~7) * 2 + n, 64));
+              const uint16_t bits = static_cast<uint16_t>((place & 1) ? word >> 16 : word);
+              weight[rt] = DT == MEGA_BF16 ? bf16_bits_to_float(bits) : f16_bits_to_float(bits);
+              its[rt] = in_range(lds_sees[rt * 16 + n], key);
+            }
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int at = min(first_column + 128 * (c / 8) + 8 * (4 * h + i) + c % 8, a.v.width - 1);
+                float v;
+                if constexpr (kEight) {
+                  v = (row[at] & 0x7f) == 0x7f ? __builtin_nanf("") : 0.f;
+                } else {
+                  const uint16_t bits = reinterpret_cast<const uint16_t*>(row)[at];
+                  v = DT == MEGA_BF16 ? bf16_bits_to_float(bits) : f16_bits_to_float(bits);
+                }
+                const bool finite = fabsf(v) < __builtin_inff();
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[rt][c][i] = finite || !its[rt] ? acc[rt][c][i] : fmaf(weight[rt], v, acc[rt][c][i]);
+                __builtin_amdgcn_sched_barrier(0);
+              }
+          }
+        }
+        there[0] = next.there[0], there[1] = next.there[1];
+      };
+      if constexpr (kSolo) {
+        u32x4 p[RT], p_next[RT];
+        if constexpr (kSteps == 1) {
+          operands(0, p);
+          step_of(0, !kLate, p, p_next);
+        } else {
+          const int steps = min(kSteps, (end - tile + 31) >> 5);
+          operands(0, p);
+#pragma unroll 1
+          for (int step = 0; step < steps; ++step) {
+            step_of(step, true, p, p_next);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) p[rt] = p_next[rt];
+          }
+        }
+      } else {
+        const int steps = min(waves * kSteps, (end - tile + 31) >> 5);
+        u32x4 p[RT], p_next[RT];
+#pragma unroll 1
+        for (int step = 0; step < steps; ++step) {
+          operands(step, p);
+          step_of(step, true, p, p_next);
+        }
+      }
+    }
+
+    // ---- the rows' sums over the lanes and waves that had their keys
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      l[rt] += across(l[rt], 16);
+      l[rt] += across(l[rt], 32);
+    }
+    if constexpr (!kSolo) {
+      const int at = opaque(lane), n = at & 15;
+      __syncthreads();  // (the maxima of the last tile have been read)
+      if (at < 16)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * kMostWaves + wave] = l[rt];
+      __syncthreads();
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        l[rt] = 0.f;
+        for (int w = 0; w < waves; ++w) l[rt] += lds_m[(rt * 16 + n) * kMostWaves + w];
+      }
+    }
+    if (store_piece<DT, RT, CT, 8>(a, k, static_cast<int>(id), head, slab, wave, first_column, progress, acc, m, l)) break;
+    __syncthreads();  // (the rows, maxima and probabilities of this piece have been read)
+  }
+}
+
+template <int DT, bool kEight, int RT, int CT, int KS, int KG, bool kSolo, int kWavesPerSimd>
+int launch(const AttnArgs& a, const RowsPlan& p, void* stream) {
+  const auto kernel = paged_rows_kernel<DT, kEight, RT, CT, KS, KG, kSolo, kWavesPerSimd>;
+  // (one step more of probabilities than there are: the operands behind the last step's are fetched too)
+  const size_t bytes = (RT * KS * 64 + (kSolo ? 0 : (p.waves * (KG / 2) + 1) * RT * 64)) * sizeof(uint4) + (RT * 16 * sizeof(float) + sizeof(int)) * 4 * kWavesPerSimd +
+                       RT * 16 * sizeof(int2);
+  if (bytes > 65536)
+    MEGA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+  kernel<<<dim3(static_cast<uint32_t>(p.workgroups)), dim3(p.waves * kWave), bytes, static_cast<hipStream_t>(stream)>>>(a);
+  MEGA_CHECK_LAUNCH();
+  return MEGA_OK;
+}
+
+template <int DT, bool kEight>
+int launch_width(const AttnArgs& a, const RowsPlan& p, void* stream) {
+  if (p.waves == 1) return p.ks == 4 ? launch<DT, kEight, 4, 8, 4, 2, true, 2>(a, p, stream) : launch<DT, kEight, 4, 8, 8, 2, true, 2>(a, p, stream);
+  return p.ks == 4 ? launch<DT, kEight, 4, 8, 4, 2, false, 2>(a, p, stream) : launch<DT, kEight, 4, 8, 8, 2, false, 2>(a, p, stream);
+}
+
+}  // namespace
+
+int launch_paged_rows(const AttnArgs& a, const RowsPlan& p, int dtype, bool eight, void* stream) {
+  if (dtype == MEGA_BF16) return eight ? launch_width<MEGA_BF16, true>(a, p, stream) : launch_width<MEGA_BF16, false>(a, p, stream);
+  return eight ? launch_width<MEGA_F16, true>(a, p, stream) : launch_width<MEGA_F16, false>(a, p, stream);
+}
+
+}  // namespace mega
