@@ -74,10 +74,8 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
     const int lane = opaque(static_cast<int>(threadIdx.x) & 63), n = lane & 15, h = lane >> 4;
     int begin, end;
     take_piece<kRows>(a, static_cast<int>(id), progress, k, begin, end);
-    rows_to_lds<kEight, kRows, KS>(a, k, head, lds_q);
-    ranges_to_lds<kRows>(a, k, end, lds_sees);
     // keys all_low .. all_high are seen by every row of the block
-    const int all_low = chunk_start(k.position0 + (k.row0 + k.count - 1) / a.shared, a.chunk), all_high = min(k.position0 + k.row0 / a.shared, end - 1);
+    const int all_low = chunk_start(a, k.position0 + token_of(a, k.row0 + k.count - 1)), all_high = min(k.position0 + token_of(a, k.row0), end - 1);
 
     // the two 16-key groups of a step: where this head's first value lies, and whether the group has a page
     constexpr int kBytes = kEight ? 1 : 2;
@@ -152,9 +150,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
       const int l = opaque(lane), d = min((kEight ? 64 : 32) * part + (kEight ? 16 : 8) * (l >> 4), a.k.width - (kEight ? 16 : 8));
       kx[half][part % kLoads] = *reinterpret_cast<const u32x4*>(t.from[half] + (static_cast<uint32_t>(t.place[half] + (l & 15)) * a.k.slot + d) * kBytes);
     };
-    const auto load_first_keys = [&](int tile) {
-      if (tile + 32 * wave >= end) return;
-      const Keys t = keys_at(tile + 32 * wave);
+    const auto load_first_keys_at = [&](const Keys& t) {
       if constexpr (kEight) {
         const uint32_t offset = static_cast<uint32_t>(4 * (opaque(lane) >> 4)) * a.k.eSlot;
 #pragma unroll
@@ -167,15 +163,20 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
 #pragma unroll
         for (int half = 0; half < 2; ++half) load_key(t, half, part);
     };
-    const auto load_step = [&](int first) {
-      const Step t = step_at(first);
+    const auto load_first_keys = [&](int tile) {
+      if (tile + 32 * wave < end) load_first_keys_at(keys_at(tile + 32 * wave));
+    };
+    if (begin < end) {  // (all of the pages first: one wait for their numbers)
+      const Keys keys = keys_at(min(begin + 32 * wave, (end - 1) & ~31));
+      const Step t = step_at(begin);
+      if (begin + 32 * wave < end) load_first_keys_at(keys);
       load_exponents(t, e);
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) load_values(t, g, x[g]);
       there[0] = t.there[0], there[1] = t.there[1];
-    };
-    load_first_keys(begin);
-    if (begin < end) load_step(begin);
+    }
+    rows_to_lds<kEight, kRows, KS>(a, k, head, lds_q);
+    ranges_to_lds<kRows>(a, k, end, lds_sees);
     for (int c = threadIdx.x; c < kRows * 8; c += blockDim.x) lds_m[c] = -__builtin_inff();  // (of waves that there are not, too)
     if (threadIdx.x < kMaxWaves) lds_pages[threadIdx.x] = 1;
     __syncthreads();
@@ -549,6 +550,13 @@ int launch_attn(const AttnArgs& a, const Plan& p, bool eight, void* stream) {
   return MEGA_OK;
 }
 
+// the logarithm of a power of two, else -1
+int log2_of(int64_t n) {
+  int l = 0;
+  while ((int64_t{1} << l) < n) ++l;
+  return (int64_t{1} << l) == n ? l : -1;
+}
+
 bool sizes_fit(const mega_paged_cache* c, int64_t rows, int64_t q_heads, int64_t chunk) {
   return c != nullptr && c->heads >= 1 && c->v_width >= 16 && rows >= 0 && rows <= 0x7fffffff && q_heads >= 1 && q_heads <= 65536 &&
          q_heads % c->heads == 0 && chunk >= 0 && chunk <= 0x7fffffff && rows * q_heads <= (int64_t{1} << 40) / c->v_width;
@@ -592,6 +600,8 @@ extern "C" int mega_paged_attention_fwd(const mega_paged_cache* cache, int dtype
   a.chunk = static_cast<int32_t>(chunk), a.slabs = p.slabs, a.blocks = static_cast<int32_t>(p.blocks);
   a.parts = static_cast<int32_t>(p.parts), a.slots = static_cast<int32_t>(p.slots), a.part_rows = static_cast<int32_t>(p.part_rows);
   a.clear_rest = clear_rest != 0;
+  a.chunk_shift = log2_of(a.chunk), a.shared_shift = log2_of(a.shared);
+  a.per_part = p.parts > 0 ? 1.0 / static_cast<double>(p.parts) : 0.0;
   a.scale = static_cast<float>(scale * 1.4426950408889634);
   const bool eight = cache->k_exponents != nullptr;
   return dtype == MEGA_BF16 ? launch_attn<MEGA_BF16>(a, p, eight, stream) : launch_attn<MEGA_F16>(a, p, eight, stream);

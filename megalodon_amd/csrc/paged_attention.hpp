@@ -27,7 +27,9 @@ struct AttnArgs {
   int32_t rows, heads, shared, chunk, slabs, blocks;
   int32_t parts, slots, part_rows;  // parts of the line of units for each head and slab; 0: a workgroup a block
   int32_t clear_rest;
+  int32_t chunk_shift, shared_shift;  // their logarithms where they are powers of two, else -1: a division is thirty instructions in a row
   float scale;                // times log2(e)
+  double per_part;            // 1 / parts
 };
 
 // A row block of one sequence and the keys that any of its rows sees.
@@ -43,26 +45,52 @@ struct Block {
 typedef const int32_t __attribute__((address_space(4))) ConstInt;
 __device__ __forceinline__ int32_t constant_at(const int32_t* p, int64_t i) { return reinterpret_cast<ConstInt*>(reinterpret_cast<uint64_t>(p))[i]; }
 
-__device__ __forceinline__ int chunk_start(int position, int chunk) { return chunk > 0 && position > 0 ? position / chunk * chunk : 0; }
+__device__ __forceinline__ int chunk_start(const AttnArgs& a, int position) {
+  if (a.chunk == 0 || position <= 0) return 0;
+  return a.chunk_shift >= 0 ? position >> a.chunk_shift << a.chunk_shift : position / a.chunk * a.chunk;
+}
+// the new token of row r (token * shared + head)
+__device__ __forceinline__ int token_of(const AttnArgs& a, int r) { return a.shared_shift >= 0 ? r >> a.shared_shift : r / a.shared; }
+
+// A number of `cu` or `lengths`: kUniform: at an index that the wave has in common.
+template <bool kUniform>
+__device__ __forceinline__ int number_at(const int32_t* p, int i) {
+  if constexpr (kUniform) return constant_at(p, i);
+  return p[i];
+}
+template <bool kUniform>
+__device__ __forceinline__ int bound_at(const AttnArgs& a, int i) { return min(max(number_at<kUniform>(a.cu, i), 0), a.rows); }
 
 // Sequences, the rows behind the last one counted as one more where they are to be cleared.
 __device__ __forceinline__ int sequences_of(const AttnArgs& a) { return a.view.batch + (a.clear_rest ? 1 : 0); }
 
-// Sequence b (the rows behind the last one are one more, without keys) and its row block `number`; false: it has no such block.
+// A sequence (the rows behind the last one are one more, without keys): its first packed row, new rows and positions.
+struct Sequence {
+  int32_t start, count, length;
+};
+template <bool kUniform>
+__device__ __forceinline__ Sequence sequence_of(const AttnArgs& a, int b) {
+  const bool rest = b >= a.view.batch;
+  const int start = bound_at<kUniform>(a, b), end = rest ? a.rows : bound_at<kUniform>(a, b + 1);
+  return {start, max(end - start, 0), rest ? 0 : max(number_at<kUniform>(a.lengths, b), 0)};
+}
 template <int kRows>
-__device__ __forceinline__ bool block_of(const AttnArgs& a, int b, int64_t number, Block& k) {
+__device__ __forceinline__ int blocks_of(const AttnArgs& a, const Sequence& s) {
+  return static_cast<int>((static_cast<int64_t>(s.count) * a.shared + kRows - 1) / kRows);
+}
+// Row block `number` of sequence b; false: it has no such block.
+template <int kRows>
+__device__ __forceinline__ bool block_of(const AttnArgs& a, const Sequence& s, int b, int64_t number, Block& k) {
   k.sequence = b;
-  k.start = row_bound(a.cu, b, a.rows);
-  const int n = (b < a.view.batch ? row_bound(a.cu, b + 1, a.rows) : a.rows) - k.start;
-  const int64_t row0 = number * kRows;
-  if (row0 < 0 || row0 >= static_cast<int64_t>(n) * a.shared) return false;
+  k.start = s.start;
+  const int64_t row0 = number * kRows, rows = static_cast<int64_t>(s.count) * a.shared;
+  if (row0 < 0 || row0 >= rows) return false;
   k.row0 = static_cast<int32_t>(row0);
-  k.count = static_cast<int32_t>(min(static_cast<int64_t>(kRows), static_cast<int64_t>(n) * a.shared - row0));
-  const int length = b < a.view.batch ? max(a.lengths[b], 0) : 0;
-  k.keys = static_cast<int32_t>(min(static_cast<int64_t>(length), static_cast<int64_t>(a.view.table_width) << a.view.page_shift));
-  k.position0 = length - n;
-  k.begin = chunk_start(k.position0 + k.row0 / a.shared, a.chunk);
-  k.end = min(k.position0 + (k.row0 + k.count - 1) / a.shared + 1, k.keys);
+  k.count = static_cast<int32_t>(min(static_cast<int64_t>(kRows), rows - row0));
+  k.keys = static_cast<int32_t>(min(static_cast<int64_t>(s.length), static_cast<int64_t>(a.view.table_width) << a.view.page_shift));
+  k.position0 = s.length - s.count;
+  k.begin = chunk_start(a, k.position0 + token_of(a, k.row0));
+  k.end = min(k.position0 + token_of(a, k.row0 + k.count - 1) + 1, k.keys);
   return true;
 }
 
@@ -71,41 +99,39 @@ __device__ __forceinline__ bool block_of(const AttnArgs& a, int b, int64_t numbe
 template <int kRows>
 __device__ __forceinline__ bool find_block(const AttnArgs& a, int number, Block& k) {
   const int sequences = sequences_of(a);
-  const auto first = [&](int b) { return static_cast<int64_t>(row_bound(a.cu, b, a.rows)) * a.shared / kRows + b; };
+  const auto first = [&](int b) { return static_cast<int64_t>(bound_at<false>(a, b)) * a.shared / kRows + b; };
   const int b = last_not_above(sequences, number, first);
-  return block_of<kRows>(a, b, number - first(b), k);
+  return block_of<kRows>(a, sequence_of<true>(a, b), b, number - (static_cast<int64_t>(bound_at<true>(a, b)) * a.shared / kRows + b), k);
 }
 
 // The line of units: a block has one for every 32 keys that it sees, and one if there are none.
 __device__ __forceinline__ int units_of(const Block& k) { return max(k.end - (k.begin & ~31) + 31, 32) >> 5; }
-template <int kRows>
-__device__ __forceinline__ int blocks_of(const AttnArgs& a, int b) {
-  const int n = (b < a.view.batch ? row_bound(a.cu, b + 1, a.rows) : a.rows) - row_bound(a.cu, b, a.rows);
-  return n > 0 ? static_cast<int>((static_cast<int64_t>(n) * a.shared + kRows - 1) / kRows) : 0;
-}
 // A place on the line: a block (its sequence, its number there), its units, and the blocks and units in front of it.
 struct Mark {
   int32_t sequence, number, blocks, units;  // blocks: of the sequence
   int32_t blocks_before, units_before, total;  // total: of the whole line (the host cuts no line of 2^30 units)
 };
-// units of a part; the parts behind the line's end are empty
-__device__ __forceinline__ int part_units(int total, int parts) { return (total + parts - 1) / parts; }
+// units of a part; the parts behind the line's end are empty.  (The quotient in double is right: it is half a part away from the next one.)
+__device__ __forceinline__ int part_units(const AttnArgs& a, int total) { return static_cast<int>((total + a.parts - 0.5) * a.per_part); }
 
-__device__ __forceinline__ int sums_before_and_here(int v) {  // inclusive sums over the lanes
-  const int lane = static_cast<int>(threadIdx.x) & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int u = __shfl_up(v, off, 64);
-    if (lane >= off) v += u;
-  }
-  return v;
+// Inclusive sums over the lanes, in steps that stay in the vector unit (every lane has to be there).
+template <int kControl, int kRowMask>
+__device__ __forceinline__ int plus_moved(int v) { return v + __builtin_amdgcn_update_dpp(0, v, kControl, kRowMask, 0xf, false); }
+__device__ __forceinline__ int sums_before_and_here(int v) {
+  v = plus_moved<0x111, 0xf>(v);  // one, two, four, eight lanes up inside the rows of 16
+  v = plus_moved<0x112, 0xf>(v);
+  v = plus_moved<0x114, 0xf>(v);
+  v = plus_moved<0x118, 0xf>(v);
+  v = plus_moved<0x142, 0xa>(v);  // the last lane of rows 0 and 2 to rows 1 and 3, then lane 31 to rows 2 and 3
+  return plus_moved<0x143, 0xc>(v);
 }
-// The units of the 64 blocks of sequence b from `number` on, one to a lane
+// The units of the 64 blocks of a sequence from `number` on, one to a lane
 template <int kRows>
 __device__ __forceinline__ int lane_units(const AttnArgs& a, int b, int number, int blocks) {
   Block k;
   const int i = number + (static_cast<int>(threadIdx.x) & 63);
-  return i < blocks && block_of<kRows>(a, b, i, k) ? units_of(k) : 0;
+  const bool has = block_of<kRows>(a, sequence_of<true>(a, b), b, i, k);
+  return i < blocks && has ? units_of(k) : 0;
 }
 
 // The block in which part `part` begins (false: the part is empty); all lanes of a wave together, 64 sequences a round, and 64 blocks of a
@@ -115,10 +141,11 @@ __device__ __forceinline__ bool find_mark(const AttnArgs& a, int part, Mark& mar
   const int lane = static_cast<int>(threadIdx.x) & 63, sequences = sequences_of(a);
   int blocks = 0, units = 0, units_here = 0, blocks_here = 0;  // of the lane's sequence; inclusive sums
   const auto round = [&](int b0) {
-    const int b = b0 + lane;
-    blocks = b < sequences ? blocks_of<kRows>(a, b) : 0, units = 0;
+    const int b = min(b0 + lane, sequences - 1);
+    const Sequence q = sequence_of<false>(a, b);
     Block k;
-    if (blocks > 0 && block_of<kRows>(a, b, 0, k)) units = units_of(k);
+    const bool has = block_of<kRows>(a, q, b, 0, k) && b0 + lane < sequences;
+    blocks = has ? blocks_of<kRows>(a, q) : 0, units = has ? units_of(k) : 0;
     for (uint64_t more = __ballot(blocks > 1); more != 0; more &= more - 1) {
       const int l = __ffsll(static_cast<unsigned long long>(more)) - 1, count = __builtin_amdgcn_readlane(blocks, l);
       int sum = 0;
@@ -133,7 +160,7 @@ __device__ __forceinline__ bool find_mark(const AttnArgs& a, int part, Mark& mar
     round(b0);
     mark.total += __builtin_amdgcn_readlane(units_here, 63);
   }
-  const int first = part * part_units(mark.total, a.parts);
+  const int first = part * part_units(a, mark.total);
   if (first >= mark.total) return false;
   int units_before = 0, blocks_before = 0;
   for (int b0 = 0; b0 < sequences; b0 += 64) {
@@ -235,7 +262,7 @@ __device__ __forceinline__ bool first_piece(const AttnArgs& a, int id, Progress&
   if (a.parts == 0) return find_block<kRows>(a, a.blocks - 1 - id, k);
   Progress at;
   if (!find_mark<kRows>(a, id, at.mark)) return false;
-  at.per = part_units(at.mark.total, a.parts);
+  at.per = part_units(a, at.mark.total);
   at.unit = id * at.per, at.unit_end = min(at.unit + at.per, at.mark.total);
   if (threadIdx.x == 0) progress = at;
   __syncthreads();
@@ -253,19 +280,21 @@ __device__ __forceinline__ void take_piece(const AttnArgs& a, int id, Progress& 
   if (at.unit == at.mark.units_before + at.mark.units) {  // on to the next block (unit < total: there is one)
     at.mark.units_before += at.mark.units, ++at.mark.blocks_before;
     if (++at.mark.number == at.mark.blocks) {
-      do at.mark.blocks = blocks_of<kRows>(a, ++at.mark.sequence);
+      do at.mark.blocks = blocks_of<kRows>(a, sequence_of<false>(a, ++at.mark.sequence));
       while (at.mark.blocks == 0);
       at.mark.number = 0;
     }
   }
-  block_of<kRows>(a, __builtin_amdgcn_readfirstlane(at.mark.sequence), __builtin_amdgcn_readfirstlane(at.mark.number), k);
+  const int b = __builtin_amdgcn_readfirstlane(at.mark.sequence);
+  block_of<kRows>(a, sequence_of<true>(a, b), b, __builtin_amdgcn_readfirstlane(at.mark.number), k);
   at.mark.units = units_of(k);
   const int units = at.mark.units, first = at.mark.units_before, last = min(first + units, at.unit_end);
   begin = __builtin_amdgcn_readfirstlane((k.begin & ~31) + (at.unit - first) * 32);
   end = __builtin_amdgcn_readfirstlane(min((k.begin & ~31) + (last - first) * 32, k.end));
-  const int begins_in = first / at.per, ends_in = (first + units - 1) / at.per;
-  at.alone = begins_in == ends_in;
-  at.pieces = begins_in == id ? ends_in - begins_in + 1 : 0;
+  const int part_end = (id + 1) * at.per;
+  const bool begins_here = first >= part_end - at.per;
+  at.alone = begins_here && first + units <= part_end;
+  at.pieces = !begins_here ? 0 : at.alone ? 1 : 1 + (first + units - part_end + at.per - 1) / at.per;
   at.unit = last;
   if (threadIdx.x == 0) progress = at;
 }
@@ -278,7 +307,7 @@ __device__ __forceinline__ void rows_to_lds(const AttnArgs& a, const Block& k, i
     const int row = c / (KS * 4), d = c % (KS * 4);  // eight elements of a row
     uint4 x = make_uint4(0, 0, 0, 0);
     if (row < k.count && d * 8 < a.k.width) {
-      const int r = k.row0 + row, t = r / a.shared, g = r - t * a.shared;
+      const int r = k.row0 + row, t = token_of(a, r), g = r - t * a.shared;
       x = *reinterpret_cast<const uint4*>(a.q + (static_cast<int64_t>(k.start) + t) * a.q_row + (static_cast<int64_t>(head) * a.shared + g) * a.q_head + d * 8);
     }
     // (8-bit keys: a lane reads 16 codes at a time, which serve two steps)
@@ -290,7 +319,7 @@ __device__ __forceinline__ void rows_to_lds(const AttnArgs& a, const Block& k, i
 template <int kRows>
 __device__ __forceinline__ void ranges_to_lds(const AttnArgs& a, const Block& k, int end, int2* lds_sees) {
   for (int row = threadIdx.x; row < kRows; row += blockDim.x) {
-    const int position = k.position0 + (k.row0 + row) / a.shared, low = chunk_start(position, a.chunk), high = min(position, end - 1);
+    const int position = k.position0 + token_of(a, k.row0 + row), low = chunk_start(a, position), high = min(position, end - 1);
     const bool none = row >= k.count || high < low;
     lds_sees[row] = none ? make_int2(0x7fffffff, 0) : make_int2(low, high - low);
   }
@@ -314,7 +343,7 @@ __device__ __forceinline__ bool store_piece(const AttnArgs& a, const Block& k, i
   for (int rt = 0; rt < RT; ++rt) {
     const int row = rt * 16 + n;
     if (row >= k.count) continue;
-    const int r = k.row0 + row, t = r / a.shared, g = r - t * a.shared;
+    const int r = k.row0 + row, t = token_of(a, r), g = r - t * a.shared;
     const int64_t at = (static_cast<int64_t>(k.start) + t) * (a.heads * a.shared) + head * a.shared + g;
     const float inverse = l[rt] == 0.f ? 0.f : 1.f / l[rt];
     if (a.parts > 0 && slab == 0 && wave == 0 && h == 0) {

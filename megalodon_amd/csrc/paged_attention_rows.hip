@@ -15,21 +15,36 @@
 namespace mega {
 namespace {
 
-// kSolo: a workgroup is one wave.  KG: 16-key groups of a wave's share of a tile.  kWavesPerSimd: what the registers are cut for; with two, the
-// values of a tile are called for behind its scores, for whose registers they wait.
-template <int DT, bool kEight, int RT, int CT, int KS, int KG, bool kSolo, int kWavesPerSimd>
-__global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPerSimd) void paged_rows_kernel(AttnArgs a) {
-  constexpr int kRows = 16 * RT, kGroups = CT / 8, kBytes = kEight ? 1 : 2, kMostWaves = 4 * kWavesPerSimd, kSteps = KG / 2;
-  constexpr bool kLate = kWavesPerSimd > 1;
-  constexpr int kChunk = KS < 4 ? KS : 4, kLoads = kEight ? kChunk / 2 : kChunk;  // steps of a key row in flight; a lane's 16-byte parts of them
+// One request: lane l's 16 bytes at base + offset go to LDS bytes lds_dst + 16 l .. + 15 (lds_dst in M0, a wave's own).  Assembly, so that the
+// compiler does not see a vector memory instruction that writes LDS and wait for every request in flight in front of each LDS read; the wait for
+// these requests is explicit, the s_nop the wait state between a scalar write of M0 and a load to LDS.
+__device__ __forceinline__ void load_to_lds16(const void* base, uint32_t offset, uint32_t lds_dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds_dst) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(p)));
+}
+
+constexpr int RT = 4, CT = 8;                        // row and column tiles of a wave
+constexpr int kRows = 16 * RT, kMostWaves = 8;
+// of a key's 16-byte parts to a lane, those that come through LDS: all, or as many as it has room for beside the rows and the probabilities
+constexpr int in_lds(bool solo, int parts) { return solo ? 0 : parts < 5 ? parts : 5; }
+
+// KS: 32-wide steps of a key row; kFull: it has 32 KS elements; kSolo: a workgroup is one wave
+template <int DT, bool kEight, int KS, bool kFull, bool kSolo>
+__global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_rows_kernel(AttnArgs a) {
+  constexpr int kBytes = kEight ? 1 : 2, kParts = kEight ? KS / 2 : KS, kInLds = in_lds(kSolo, kParts);
+  // parts that come through registers, and how many of them are there at a time
+  constexpr int kRest = kParts - kInLds, kHeld = kSolo && kRest > (kEight ? 2 : 4) ? (kEight ? 2 : 4) : kRest;
   extern __shared__ __align__(16) uint4 lds[];
   __shared__ Progress progress;
   const int wave = kSolo ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), waves = kSolo ? 1 : static_cast<int>(blockDim.x) >> 6;
   uint4* const lds_q = lds;                  // [RT][KS][64]
-  uint4* const lds_p = lds + RT * KS * 64;   // [waves * kSteps][RT][64]
-  float* const lds_m = reinterpret_cast<float*>(kSolo ? lds_p : lds_p + waves * kSteps * RT * 64);  // [kRows][kMostWaves]
-  int* const lds_pages = reinterpret_cast<int*>(lds_m + kRows * kMostWaves);                        // [kMostWaves]: the waves' keys have pages
-  int2* const lds_sees = reinterpret_cast<int2*>(lds_pages + kMostWaves);                           // [kRows]
+  uint4* const lds_k = lds + RT * KS * 64;                             // [waves][2][kInLds][64]
+  uint4* const lds_p = lds_k + waves * 2 * kInLds * 64;                // [waves][RT][64]
+  float* const lds_m = reinterpret_cast<float*>(lds_p + (kSolo ? 0 : waves * RT * 64));  // [kRows][kMostWaves]
+  int* const lds_pages = reinterpret_cast<int*>(lds_m + kRows * kMostWaves);             // [kMostWaves]: the waves' keys have pages
+  int2* const lds_sees = reinterpret_cast<int2*>(lds_pages + kMostWaves);                // [kRows]
 
   // (as in paged_attention.hip)
   uint32_t id = blockIdx.x;
@@ -53,50 +68,62 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
       if (threadIdx.x < kMostWaves) lds_pages[threadIdx.x] = 1;
     }
     // keys all_low .. all_high are seen by every row of the block
-    const int all_low = chunk_start(k.position0 + (k.row0 + k.count - 1) / a.shared, a.chunk), all_high = min(k.position0 + k.row0 / a.shared, end - 1);
+    const int all_low = chunk_start(a, k.position0 + token_of(a, k.row0 + k.count - 1)), all_high = min(k.position0 + token_of(a, k.row0), end - 1);
 
-    // ---- keys: a lane's 16 bytes of key 16 group + (lane & 15)
-    u32x4 kx[KG][kLoads];
-    uint32_t ke[KG][4];
+    // ---- keys: part `part` of a lane is 16 bytes of key 16 half + (lane & 15).  Those that come through LDS are asked for a tile ahead, into the
+    // wave's own place and in operand order
+    u32x4 kx[2][kHeld > 0 ? kHeld : 1];
+    uint32_t ke[2][4];
     struct Keys {
-      const uint8_t* from[KG];
-      const uint8_t* exponents[KG];
-      bool there[KG];
+      const uint8_t* from[2];
+      const uint8_t* exponents[2];
+      bool there[2];
     };
     const auto keys_at = [&](int first) {
       Keys t;
 #pragma unroll
-      for (int g = 0; g < KG; ++g) {
-        const int held = min(first + 16 * g, (end - 1) & ~15), place = held & page_mask;
+      for (int half = 0; half < 2; ++half) {
+        const int held = min(first + 16 * half, (end - 1) & ~15), place = held & page_mask;
         const Page page = page_of(a, k.sequence, held);
-        t.there[g] = page.there;
-        t.from[g] = static_cast<const uint8_t*>(a.k.rows) + (page.number * a.k.page + static_cast<int64_t>(head) * a.k.head + static_cast<int64_t>(place) * a.k.slot) * kBytes;
-        if constexpr (kEight) t.exponents[g] = a.k.exponents + (page.number * a.k.ePage + static_cast<int64_t>(head) * a.k.eHead + static_cast<int64_t>(place) * a.k.eSlot);
+        t.there[half] = page.there;
+        t.from[half] = static_cast<const uint8_t*>(a.k.rows) + (page.number * a.k.page + static_cast<int64_t>(head) * a.k.head + static_cast<int64_t>(place) * a.k.slot) * kBytes;
+        if constexpr (kEight) t.exponents[half] = a.k.exponents + (page.number * a.k.ePage + static_cast<int64_t>(head) * a.k.eHead + static_cast<int64_t>(place) * a.k.eSlot);
       }
       return t;
     };
-    const auto load_key = [&](const Keys& t, int g, int part) {
-      const int l = opaque(lane), d = min((kEight ? 64 : 32) * part + (kEight ? 16 : 8) * (l >> 4), a.k.width - (kEight ? 16 : 8));
-      kx[g][part % kLoads] = *reinterpret_cast<const u32x4*>(t.from[g] + (static_cast<uint32_t>(l & 15) * a.k.slot + d) * kBytes);
+    const auto key_offset = [&](int part) {
+      const int l = opaque(lane), d = kFull ? (kEight ? 64 : 32) * part + (kEight ? 16 : 8) * (l >> 4)
+                                           : min((kEight ? 64 : 32) * part + (kEight ? 16 : 8) * (l >> 4), a.k.width - (kEight ? 16 : 8));
+      return (static_cast<uint32_t>(l & 15) * a.k.slot + d) * kBytes;
     };
-    const auto load_keys = [&](int tile) {
-      const Keys t = keys_at(min(tile + 16 * KG * wave, (end - 1) & ~31));
+    const auto load_key = [&](const Keys& t, int half, int part) {
+      kx[half][(part - kInLds) % (kHeld > 0 ? kHeld : 1)] = *reinterpret_cast<const u32x4*>(t.from[half] + key_offset(part));
+    };
+    const auto load_key_exponents = [&](const Keys& t) {
       if constexpr (kEight) {
         const uint32_t offset = static_cast<uint32_t>(4 * (opaque(lane) >> 4)) * a.k.eSlot;
 #pragma unroll
-        for (int g = 0; g < KG; ++g)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) ke[g][i] = t.exponents[g][offset + static_cast<uint32_t>(i * a.k.eSlot)];
+          for (int i = 0; i < 4; ++i) ke[half][i] = t.exponents[half][offset + static_cast<uint32_t>(i * a.k.eSlot)];
       }
+    };
+    const auto ask_for_keys = [&](int tile) {
+      if constexpr (kInLds > 0) {
+        const Keys t = keys_at(min(tile + 32 * wave, (end - 1) & ~31));
+        const uint32_t to = lds_address(lds_k + wave * 2 * kInLds * 64);
 #pragma unroll
-      for (int part = 0; part < kLoads; ++part)
+        for (int part = 0; part < kInLds; ++part) {
+          const uint32_t offset = key_offset(part);
 #pragma unroll
-        for (int g = 0; g < KG; ++g) load_key(t, g, part);
+          for (int half = 0; half < 2; ++half) load_to_lds16(t.from[half], offset, to + (half * kInLds + part) * 1024);
+        }
+      }
     };
 
     // ---- values: eight columns of eight of a step's 32 keys to a lane and column group
     typedef uint32_t Piece __attribute__((ext_vector_type(kEight ? 2 : 4)));
-    Piece x[kGroups][8];
+    Piece x[8];
     uint32_t e[8];
     bool there[2] = {false, false};
     struct Step {
@@ -116,12 +143,12 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
       }
       return t;
     };
-    const auto load_values = [&](const Step& t, int g) {
+    const auto load_values = [&](const Step& t) {
       // (columns behind the last are computed from others and not written)
       const int l = opaque(lane);
-      const uint32_t offset = (static_cast<uint32_t>(4 * (l >> 4)) * a.v.slot + min(first_column + g * 128 + (l & 15) * 8, a.v.width - 8)) * kBytes;
+      const uint32_t offset = (static_cast<uint32_t>(4 * (l >> 4)) * a.v.slot + min(first_column + (l & 15) * 8, a.v.width - 8)) * kBytes;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[g][i] = *reinterpret_cast<const Piece*>(t.from[i >> 2] + (offset + static_cast<uint32_t>((i & 3) * a.v.slot * kBytes)));
+      for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const Piece*>(t.from[i >> 2] + (offset + static_cast<uint32_t>((i & 3) * a.v.slot * kBytes)));
     };
     const auto load_exponents = [&](const Step& t) {
       if constexpr (kEight) {
@@ -133,8 +160,7 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
     const auto load_step = [&](int first) {
       const Step t = step_at(first);
       load_exponents(t);
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) load_values(t, g);
+      load_values(t);
       there[0] = t.there[0], there[1] = t.there[1];
     };
 
@@ -146,77 +172,75 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
 #pragma unroll
       for (int c = 0; c < CT; ++c) acc[rt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (begin < end) {
-      if constexpr (!kLate) load_keys(begin);
-      if constexpr (!kLate) load_step(begin);
-    }
+    if (begin < end) ask_for_keys(begin);
     __syncthreads();
 
-    for (int tile = begin; tile < end; tile += 16 * KG * waves) {
+    for (int tile = begin; tile < end; tile += 32 * waves) {
       // ---- scores of the wave's keys (a wave behind the end computes others' again: nothing is seen of them)
-      const int mine = tile + 16 * KG * wave;
-      f32x4 s[KG][RT];
-      if constexpr (kLate) load_keys(tile);
+      const int mine = tile + 32 * wave;
+      f32x4 s[2][RT];
       const Keys keys = keys_at(min(mine, (end - 1) & ~31));
-      bool pages_there = true, whole = mine >= all_low && mine + 16 * KG - 1 <= all_high;
+      bool pages_there = keys.there[0] && keys.there[1];
+      const bool whole = pages_there && mine >= all_low && mine + 31 <= all_high;
+      if constexpr (kInLds > 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the keys are in LDS)
 #pragma unroll
-      for (int g = 0; g < KG; ++g) pages_there = pages_there && keys.there[g];
-      whole = whole && pages_there;
+      for (int part = kInLds; part < kInLds + kHeld; ++part)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) load_key(keys, half, part);
+      load_key_exponents(keys);
       {
-        u32x4 q[RT], q_next[RT];
+        const auto fetch = [&](int c, u32x4 (&q)[RT]) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) q_next[rt] = __builtin_bit_cast(u32x4, lds_q[rt * KS * 64 + lane]);
+          for (int rt = 0; rt < RT; ++rt) q[rt] = __builtin_bit_cast(u32x4, lds_q[(rt * KS + c) * 64 + lane]);
+        };
+        u32x4 q[2][RT];
+        fetch(0, q[0]);
 #pragma unroll
-        for (int g = 0; g < KG; ++g)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[g][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int rt = 0; rt < RT; ++rt) s[half][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < KS; ++c) {
+        for (int c = 0; c < KS; ++c) {  // (the rows' operands one step ahead; the fence keeps it at that)
+          const int part = kEight ? c >> 1 : c;
+          if (c + 1 < KS) fetch(c + 1, q[(c + 1) & 1]);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {  // (the rows' operands one step ahead; the fence keeps it at that)
-            q[rt] = q_next[rt];
-            if (c + 1 < KS) q_next[rt] = __builtin_bit_cast(u32x4, lds_q[(rt * KS + c + 1) * 64 + lane]);
-          }
-#pragma unroll
-          for (int g = 0; g < KG; ++g) {
-            const int part = kEight ? c >> 1 : c;
-            u32x4 key = kx[g][part % kLoads];
+          for (int half = 0; half < 2; ++half) {
+            u32x4 x = part < kInLds ? __builtin_bit_cast(u32x4, lds_k[((wave * 2 + half) * kInLds + part) * 64 + lane]) : kx[half][(part - kInLds) % (kHeld > 0 ? kHeld : 1)];
             if constexpr (kEight) {
-              const uint32_t lo = (c & 1) ? key[2] : key[0], hi = (c & 1) ? key[3] : key[1];
-              key = u32x4{widen<DT, false>(lo, 1.f), widen<DT, true>(lo, 1.f), widen<DT, false>(hi, 1.f), widen<DT, true>(hi, 1.f)};
+              const uint32_t lo = (c & 1) ? x[2] : x[0], hi = (c & 1) ? x[3] : x[1];
+              x = u32x4{widen<DT, false>(lo, 1.f), widen<DT, true>(lo, 1.f), widen<DT, false>(hi, 1.f), widen<DT, true>(hi, 1.f)};
             }
-            if (a.k.width != 32 * KS) {  // (behind the row's end the rows' operands are zero, and infinity times zero is not)
+            if constexpr (!kFull) {  // (behind the row's end the rows' operands are zero, and infinity times zero is not)
               const int d = kEight ? (c >> 1) * 64 + (opaque(lane) >> 4) * 16 : c * 32 + (opaque(lane) >> 4) * 8;
-              if (d >= a.k.width) key = u32x4{0, 0, 0, 0};
+              if (d >= a.k.width) x = u32x4{0, 0, 0, 0};
             }
-            if (c + kChunk < KS && (!kEight || (c & 1))) load_key(keys, g, part + kLoads);
+            if (part >= kInLds && part + kHeld < kParts && (!kEight || (c & 1))) load_key(keys, half, part + kHeld);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) s[g][rt] = mma<DT>(key, q[rt], s[g][rt]);
+            for (int rt = 0; rt < RT; ++rt) s[half][rt] = mma<DT>(x, q[c & 1][rt], s[half][rt]);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
 #pragma unroll
-      for (int g = 0; g < KG; ++g) {
+      for (int half = 0; half < 2; ++half) {
         f32x4 factor = {a.scale, a.scale, a.scale, a.scale};
         if constexpr (kEight)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) factor[i] *= exponent_value(ke[g][i]);
+          for (int i = 0; i < 4; ++i) factor[i] *= exponent_value(ke[half][i]);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[g][rt] *= factor;
+        for (int rt = 0; rt < RT; ++rt) s[half][rt] *= factor;
       }
-      if constexpr (!kLate) load_keys(tile + 16 * KG * waves);
-      if constexpr (kLate) load_step(tile);
+      load_step(tile);
       if (!whole) {
         const int l = opaque(lane), n = l & 15, first = mine + 4 * (l >> 4);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           const int2 range = lds_sees[rt * 16 + n];
 #pragma unroll
-          for (int g = 0; g < KG; ++g)
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (!keys.there[g] || !in_range(range, first + 16 * g + i)) s[g][rt][i] = -__builtin_inff();
+              if (!keys.there[half] || !in_range(range, first + 16 * half + i)) s[half][rt][i] = -__builtin_inff();
         }
       }
 
@@ -226,9 +250,9 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
       for (int rt = 0; rt < RT; ++rt) {
         float t = s[0][rt][0];
 #pragma unroll
-        for (int g = 0; g < KG; ++g)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) t = fmaxf(t, s[g][rt][i]);
+          for (int i = 0; i < 4; ++i) t = fmaxf(t, s[half][rt][i]);
         t = fmaxf(t, across(t, 16));
         top[rt] = fmaxf(t, across(t, 32));
       }
@@ -254,7 +278,7 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
             top[rt] = fmaxf(top[rt], fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
           }
       }
-      u32x4 own[kSteps][RT];  // (kSolo: the operands themselves)
+      u32x4 own[RT];  // (kSolo: the operands themselves)
       bool moved = false;
       float alpha[RT];
 #pragma unroll
@@ -263,18 +287,14 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
         alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - base);
         moved = moved || now != m[rt];
         m[rt] = now;
-        float sum = 0.f;
+        float p[8], sum = 0.f;
 #pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-          float p[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(s[2 * st + (i >> 2)][rt][i & 3] - base);
-            sum += p[i];
-          }
-          own[st][rt] = u32x4{pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
-          if constexpr (!kSolo) lds_p[((wave * kSteps + st) * RT + rt) * 64 + lane] = __builtin_bit_cast(uint4, own[st][rt]);
+        for (int i = 0; i < 8; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(s[i >> 2][rt][i & 3] - base);
+          sum += p[i];
         }
+        own[rt] = u32x4{pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
+        if constexpr (!kSolo) lds_p[(wave * RT + rt) * 64 + lane] = __builtin_bit_cast(uint4, own[rt]);
         l[rt] = l[rt] * alpha[rt] + sum;
       }
       if (__any(moved))
@@ -285,11 +305,12 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
       if constexpr (!kSolo) __syncthreads();
 
       // ---- values: 32 keys a step
-      const auto operands = [&](int step, u32x4 (&p)[RT]) {
+      const int steps = kSolo ? 1 : min(waves, (end - tile + 31) >> 5);
+#pragma unroll 1
+      for (int step = 0; step < steps; ++step) {
+        u32x4 p[RT];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) p[rt] = kSolo ? own[step % kSteps][rt] : __builtin_bit_cast(u32x4, lds_p[(step * RT + rt) * 64 + lane]);
-      };
-      const auto step_of = [&](int step, bool more, u32x4 (&p)[RT], u32x4 (&p_next)[RT]) {
+        for (int rt = 0; rt < RT; ++rt) p[rt] = kSolo ? own[rt] : __builtin_bit_cast(u32x4, lds_p[(step * RT + rt) * 64 + lane]);
         const int first = tile + 32 * step;
         const Step next = step_at(min(first + 32, (end - 1) & ~31));
         bool odd = false;
@@ -302,31 +323,28 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
             const int key = first + 16 * (i >> 2) + 4 * h + (i & 3);
             const uint32_t keep = key >= k.begin && key < end && there[i >> 2] ? ~0u : 0u;
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-              for (int j = 0; j < (kEight ? 2 : 4); ++j) {
-                const uint32_t finite = kEight ? finite_codes(x[g][i][j]) : finite_halves<DT>(x[g][i][j]);
-                odd = odd || (~finite & keep) != 0;
-                x[g][i][j] &= keep & finite;
-              }
+            for (int j = 0; j < (kEight ? 2 : 4); ++j) {
+              const uint32_t finite = kEight ? finite_codes(x[i][j]) : finite_halves<DT>(x[i][j]);
+              odd = odd || (~finite & keep) != 0;
+              x[i][j] &= keep & finite;
+            }
           }
         }
         float unit[8];
         if constexpr (kEight) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) unit[i] = exponent_value(e[i]);
-          if (more) load_exponents(next);
+          if constexpr (!kSolo) load_exponents(next);
         }
-        // columns 2 j, 2 j + 1 of a lane's eight in group g as operands
-        const auto convert = [&](int u, u32x4 (&vt)[2]) {
-          const int g = u >> 2, j = u & 3;
+        // columns 2 j, 2 j + 1 of a lane's eight as operands
+        const auto convert = [&](int j, u32x4 (&vt)[2]) {
           uint32_t w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             if constexpr (kEight)
-              w[i] = (j & 1) ? widen<DT, true>(x[g][i][j >> 1], unit[i]) : widen<DT, false>(x[g][i][j >> 1], unit[i]);
+              w[i] = (j & 1) ? widen<DT, true>(x[i][j >> 1], unit[i]) : widen<DT, false>(x[i][j >> 1], unit[i]);
             else
-              w[i] = x[g][i][j];
+              w[i] = x[i][j];
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -337,10 +355,15 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
         u32x4 vt[2][2];
         convert(0, vt[0]);
 #pragma unroll
-        for (int u = 0; u < 4 * kGroups; ++u) {
-          if (u + 1 < 4 * kGroups) convert(u + 1, vt[(u + 1) & 1]);
-          if ((u & 3) == 2 && more) load_values(next, u >> 2);  // (the group's last columns have just been converted)
-          if (kSolo && u == 0 && more) operands(step + 1, p_next);
+        for (int u = 0; u < 4; ++u) {
+          if (u + 1 < 4) convert(u + 1, vt[(u + 1) & 1]);
+          // (the last columns have just been converted; the next 32 keys' values, of these once more behind the last)
+          if constexpr (!kSolo)
+            if (u == 2) {
+              // (the next tile's keys in front of them: requests come back in their order, and nobody waits for these alone)
+              if (step == 0 && tile + 32 * waves < end) ask_for_keys(tile + 32 * waves);
+              load_values(next);
+            }
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -371,7 +394,7 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
             for (int c = 0; c < CT; ++c)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const int at = min(first_column + 128 * (c / 8) + 8 * (4 * h + i) + c % 8, a.v.width - 1);
+                const int at = min(first_column + 8 * (4 * h + i) + c, a.v.width - 1);
                 float v;
                 if constexpr (kEight) {
                   v = (row[at] & 0x7f) == 0x7f ? __builtin_nanf("") : 0.f;
@@ -387,30 +410,6 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
           }
         }
         there[0] = next.there[0], there[1] = next.there[1];
-      };
-      if constexpr (kSolo) {
-        u32x4 p[RT], p_next[RT];
-        if constexpr (kSteps == 1) {
-          operands(0, p);
-          step_of(0, !kLate, p, p_next);
-        } else {
-          const int steps = min(kSteps, (end - tile + 31) >> 5);
-          operands(0, p);
-#pragma unroll 1
-          for (int step = 0; step < steps; ++step) {
-            step_of(step, true, p, p_next);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) p[rt] = p_next[rt];
-          }
-        }
-      } else {
-        const int steps = min(waves * kSteps, (end - tile + 31) >> 5);
-        u32x4 p[RT], p_next[RT];
-#pragma unroll 1
-        for (int step = 0; step < steps; ++step) {
-          operands(step, p);
-          step_of(step, true, p, p_next);
-        }
       }
     }
 
@@ -438,12 +437,11 @@ __global__ __launch_bounds__(kSolo ? kWave : 4 * kWavesPerSimd * kWave, kWavesPe
   }
 }
 
-template <int DT, bool kEight, int RT, int CT, int KS, int KG, bool kSolo, int kWavesPerSimd>
+template <int DT, bool kEight, int KS, bool kFull, bool kSolo>
 int launch(const AttnArgs& a, const RowsPlan& p, void* stream) {
-  const auto kernel = paged_rows_kernel<DT, kEight, RT, CT, KS, KG, kSolo, kWavesPerSimd>;
-  // (one step more of probabilities than there are: the operands behind the last step's are fetched too)
-  const size_t bytes = (RT * KS * 64 + (kSolo ? 0 : (p.waves * (KG / 2) + 1) * RT * 64)) * sizeof(uint4) + (RT * 16 * sizeof(float) + sizeof(int)) * 4 * kWavesPerSimd +
-                       RT * 16 * sizeof(int2);
+  const auto kernel = paged_rows_kernel<DT, kEight, KS, kFull, kSolo>;
+  const int parts = kEight ? KS / 2 : KS, kept = p.waves * 2 * in_lds(kSolo, parts) * 64;
+  const size_t bytes = (RT * KS * 64 + kept + (kSolo ? 0 : p.waves * RT * 64)) * sizeof(uint4) + (kRows * sizeof(float) + sizeof(int)) * kMostWaves + kRows * sizeof(int2);
   if (bytes > 65536)
     MEGA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
   kernel<<<dim3(static_cast<uint32_t>(p.workgroups)), dim3(p.waves * kWave), bytes, static_cast<hipStream_t>(stream)>>>(a);
@@ -451,10 +449,16 @@ int launch(const AttnArgs& a, const RowsPlan& p, void* stream) {
   return MEGA_OK;
 }
 
+template <int DT, bool kEight, int KS, bool kFull>
+int launch_columns(const AttnArgs& a, const RowsPlan& p, void* stream) {
+  return p.waves == 1 ? launch<DT, kEight, KS, kFull, true>(a, p, stream) : launch<DT, kEight, KS, kFull, false>(a, p, stream);
+}
+
 template <int DT, bool kEight>
 int launch_width(const AttnArgs& a, const RowsPlan& p, void* stream) {
-  if (p.waves == 1) return p.ks == 4 ? launch<DT, kEight, 4, 8, 4, 2, true, 2>(a, p, stream) : launch<DT, kEight, 4, 8, 8, 2, true, 2>(a, p, stream);
-  return p.ks == 4 ? launch<DT, kEight, 4, 8, 4, 2, false, 2>(a, p, stream) : launch<DT, kEight, 4, 8, 8, 2, false, 2>(a, p, stream);
+  if (a.k.width == 128) return launch_columns<DT, kEight, 4, true>(a, p, stream);
+  if (a.k.width == 256) return launch_columns<DT, kEight, 8, true>(a, p, stream);
+  return p.ks == 4 ? launch_columns<DT, kEight, 4, false>(a, p, stream) : launch_columns<DT, kEight, 8, false>(a, p, stream);
 }
 
 }  // namespace
