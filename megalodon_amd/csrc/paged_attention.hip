@@ -43,6 +43,11 @@ struct Values {
   Piece x[8];
 };
 
+// Whether a tile's keys go through LDS (eight waves' 32 rows each, beside the rows and the probabilities): requests then cover whole rows.  Otherwise
+// they go to registers in operand order, where a request touches 64 bytes of sixteen rows -- one token over 1531 positions: the keys
+// of a run are there 2 us later.
+constexpr bool staged(bool eight, int rt, int ks) { return 8 * 32 * ks * (eight ? 32 : 64) + rt * (ks + 8) * 1024 <= 156 * 1024; }
+
 template <int DT, bool kEight, int RT, int CT, int KS>  // KS: 32-wide steps of a key row
 __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnArgs a) {
   // 16-byte loads of values where the registers allow it: eight of a lane's columns at a time, else four
@@ -51,7 +56,10 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
   __shared__ Progress progress;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), waves = static_cast<int>(blockDim.x) >> 6;
   uint4* const lds_q = lds;                       // [RT][KS][64]
-  uint4* const lds_p = lds + RT * KS * 64;        // [waves][RT][64]
+  constexpr bool kStaged = staged(kEight, RT, KS);
+  constexpr int kPieces = KS * (kEight ? 2 : 4);  // 16-byte pieces of a key row
+  uint4* const lds_k = lds + RT * KS * 64;        // kStaged: [waves][32][kPieces]
+  uint4* const lds_p = lds_k + (kStaged ? waves * 32 * kPieces : 0);  // [waves][RT][64]
   float* const lds_m = reinterpret_cast<float*>(lds_p + waves * RT * 64);  // [kRows][8]
   int* const lds_pages = reinterpret_cast<int*>(lds_m + kRows * 8);        // [8]: the waves' keys have pages
   int2* const lds_sees = reinterpret_cast<int2*>(lds_pages + kMaxWaves);   // [kRows]: first key and number of further ones that a row sees
@@ -67,13 +75,14 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
   const int first_column = (slab * waves + wave) * CT * 16;
 
   Block k;
-  if (!first_piece<kRows>(a, static_cast<int>(id), progress, k)) return;
+  Progress at;
+  if (!first_piece<kRows>(a, static_cast<int>(id), at, k)) return;
 
   for (;;) {
     // (anew for each piece and each use: kept out of the registers in between)
     const int lane = opaque(static_cast<int>(threadIdx.x) & 63), n = lane & 15, h = lane >> 4;
     int begin, end;
-    take_piece<kRows>(a, static_cast<int>(id), progress, k, begin, end);
+    take_piece<kRows>(a, static_cast<int>(id), at, progress, k, begin, end);
     // keys all_low .. all_high are seen by every row of the block
     const int all_low = chunk_start(a, k.position0 + token_of(a, k.row0 + k.count - 1)), all_high = min(k.position0 + token_of(a, k.row0), end - 1);
 
@@ -132,7 +141,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
       int place[2];
       bool there[2];
     };
-    u32x4 kx[2][kLoads];
+    u32x4 kx[2][kStaged ? 1 : kLoads];
     uint32_t ke[2][4];
     const auto keys_at = [&](int group) {
       Keys t;
@@ -158,14 +167,28 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
 #pragma unroll
           for (int i = 0; i < 4; ++i) ke[half][i] = t.exponents[half][offset + static_cast<uint32_t>(i * a.k.eSlot)];
       }
+      if constexpr (kStaged) {
+        // piece p of row r lies at p ^ (r & 15) (& 7 where there are eight): sixteen rows' equal pieces are in different banks
+        constexpr int kRowsAtOnce = 64 / kPieces, kMix = kPieces < 16 ? kPieces - 1 : 15;
+        const int l = opaque(lane), row = l / kPieces, last = a.k.width * kBytes / 16 - 1;
+        const uint32_t to = lds_address(lds_k + wave * 32 * kPieces);
 #pragma unroll
-      for (int part = 0; part < kLoads; ++part)
+        for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
+          const int in_half = (i * kRowsAtOnce & 15) + row, half = i * kRowsAtOnce >> 4;
+          const uint32_t offset = static_cast<uint32_t>(t.place[half] + in_half) * a.k.slot * kBytes + min((l % kPieces) ^ (in_half & kMix), last) * 16;
+          load_to_lds16(t.from[half], offset, to + i * 1024);
+        }
+      } else {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) load_key(t, half, part);
+        for (int part = 0; part < kLoads; ++part)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) load_key(t, half, part);
+      }
     };
     const auto load_first_keys = [&](int tile) {
       if (tile + 32 * wave < end) load_first_keys_at(keys_at(tile + 32 * wave));
     };
+    const uint4 first_rows = static_cast<int>(threadIdx.x) < kRows * KS * 4 ? row_piece<KS>(a, k, head, threadIdx.x) : make_uint4(0, 0, 0, 0);
     if (begin < end) {  // (all of the pages first: one wait for their numbers)
       const Keys keys = keys_at(min(begin + 32 * wave, (end - 1) & ~31));
       const Step t = step_at(begin);
@@ -175,7 +198,8 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
       for (int g = 0; g < kGroups; ++g) load_values(t, g, x[g]);
       there[0] = t.there[0], there[1] = t.there[1];
     }
-    rows_to_lds<kEight, kRows, KS>(a, k, head, lds_q);
+    if (static_cast<int>(threadIdx.x) < kRows * KS * 4) row_piece_to_lds<kEight, KS>(first_rows, threadIdx.x, lds_q);
+    for (int c = threadIdx.x + blockDim.x; c < kRows * KS * 4; c += blockDim.x) row_piece_to_lds<kEight, KS>(row_piece<KS>(a, k, head, c), c, lds_q);
     ranges_to_lds<kRows>(a, k, end, lds_sees);
     for (int c = threadIdx.x; c < kRows * 8; c += blockDim.x) lds_m[c] = -__builtin_inff();  // (of waves that there are not, too)
     if (threadIdx.x < kMaxWaves) lds_pages[threadIdx.x] = 1;
@@ -286,6 +310,8 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
         const bool whole = mine >= all_low && mine + 31 <= all_high;
         const Keys keys = keys_at(mine);
         pages_there = keys.there[0] && keys.there[1];
+        // (younger than the keys: the values of the next step, and their exponents)
+        if constexpr (kStaged) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kGroups * 8 + (kEight ? 8 : 0)) : "memory");
         u32x4 q[RT], q_next[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -302,7 +328,13 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int part = kEight ? c >> 1 : c;
-            u32x4 key = kx[half][part % kLoads];
+            u32x4 key;
+            if constexpr (kStaged) {
+              const int l = opaque(lane), n = l & 15;
+              key = __builtin_bit_cast(u32x4, lds_k[(wave * 32 + 16 * half + n) * kPieces + ((4 * part + (l >> 4)) ^ (n & (kPieces < 16 ? kPieces - 1 : 15)))]);
+            } else {
+              key = kx[half][part % kLoads];
+            }
             if constexpr (kEight) {
               const uint32_t lo = (c & 1) ? key[2] : key[0], hi = (c & 1) ? key[3] : key[1];
               key = u32x4{widen<DT, false>(lo, 1.f), widen<DT, true>(lo, 1.f), widen<DT, false>(hi, 1.f), widen<DT, true>(hi, 1.f)};
@@ -311,7 +343,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
               const int d = kEight ? (c >> 1) * 64 + (opaque(lane) >> 4) * 16 : c * 32 + (opaque(lane) >> 4) * 8;
               if (d >= a.k.width) key = u32x4{0, 0, 0, 0};
             }
-            if (c + kChunk < KS && (!kEight || (c & 1))) load_key(keys, half, part + kLoads);
+            if (!kStaged && c + kChunk < KS && (!kEight || (c & 1))) load_key(keys, half, part + kLoads);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) s[half][rt] = mma<DT>(key, q[rt], s[half][rt]);
           }
@@ -415,13 +447,11 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
         for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * 8 + wave] = l[rt];
       __syncthreads();
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        l[rt] = 0.f;
-        for (int w = 0; w < waves; ++w) l[rt] += lds_m[(rt * 16 + n) * 8 + w];
-      }
+      for (int rt = 0; rt < RT; ++rt) l[rt] = sum_of_waves(lds_m + (rt * 16 + n) * 8, waves);
     }
     if (store_piece<DT, RT, CT, kCols>(a, k, static_cast<int>(id), head, slab, wave, first_column, progress, acc, m, l)) break;
-    __syncthreads();  // (the rows, maxima and probabilities of this piece have been read)
+    at = next_piece<kRows>(a, progress, k);
+    __syncthreads();  // (the rows, maxima, probabilities and progress of this piece have been read)
   }
 }
 
@@ -513,7 +543,7 @@ Plan plan_of(const mega_paged_cache* c, int64_t rows, int64_t q_heads) {
 template <int DT, bool kEight, int RT, int CT, int KS>
 int launch_few(const AttnArgs& a, const Plan& p, void* stream) {
   const auto kernel = paged_attn_kernel<DT, kEight, RT, CT, KS>;
-  const size_t bytes = (RT * KS * 64 + p.waves * RT * 64) * sizeof(uint4) + RT * 16 * 8 * sizeof(float) + kMaxWaves * sizeof(int) + RT * 16 * sizeof(int2);
+  const size_t bytes = (RT * KS * 64 + p.waves * (RT * 64 + (staged(kEight, RT, KS) ? 32 * KS * (kEight ? 2 : 4) : 0))) * sizeof(uint4) + RT * 16 * 8 * sizeof(float) + kMaxWaves * sizeof(int) + RT * 16 * sizeof(int2);
   if (bytes > 65536)
     MEGA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
   hipStream_t s = static_cast<hipStream_t>(stream);

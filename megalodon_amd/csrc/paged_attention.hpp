@@ -137,13 +137,13 @@ __device__ __forceinline__ int lane_units(const AttnArgs& a, int b, int number, 
 // The block in which part `part` begins (false: the part is empty); all lanes of a wave together, 64 sequences a round, and 64 blocks of a
 // sequence that has more than one.
 template <int kRows>
-__device__ __forceinline__ bool find_mark(const AttnArgs& a, int part, Mark& mark) {
+__device__ __forceinline__ bool find_mark(const AttnArgs& a, int part, Mark& mark, Block& block) {
   const int lane = static_cast<int>(threadIdx.x) & 63, sequences = sequences_of(a);
   int blocks = 0, units = 0, units_here = 0, blocks_here = 0;  // of the lane's sequence; inclusive sums
+  Block k;                                                     // its first block
   const auto round = [&](int b0) {
     const int b = min(b0 + lane, sequences - 1);
     const Sequence q = sequence_of<false>(a, b);
-    Block k;
     const bool has = block_of<kRows>(a, q, b, 0, k) && b0 + lane < sequences;
     blocks = has ? blocks_of<kRows>(a, q) : 0, units = has ? units_of(k) : 0;
     for (uint64_t more = __ballot(blocks > 1); more != 0; more &= more - 1) {
@@ -173,7 +173,11 @@ __device__ __forceinline__ bool find_mark(const AttnArgs& a, int part, Mark& mar
       mark.units_before = units_before + __builtin_amdgcn_readlane(units_here - units, l);
       mark.blocks_before = blocks_before + __builtin_amdgcn_readlane(blocks_here - blocks, l);
       mark.number = 0, mark.units = __builtin_amdgcn_readlane(units, l);
-      if (mark.blocks == 1) return true;
+      if (mark.blocks == 1) {
+        block = {mark.sequence, __builtin_amdgcn_readlane(k.start, l), __builtin_amdgcn_readlane(k.row0, l), __builtin_amdgcn_readlane(k.count, l),
+                 __builtin_amdgcn_readlane(k.position0, l), __builtin_amdgcn_readlane(k.keys, l), __builtin_amdgcn_readlane(k.begin, l), __builtin_amdgcn_readlane(k.end, l)};
+        return true;
+      }
       for (int i = 0; i < mark.blocks; i += 64) {
         const int own = lane_units<kRows>(a, mark.sequence, i, mark.blocks), here = sums_before_and_here(own);
         const uint64_t found = __ballot(mark.units_before + here > first);
@@ -182,6 +186,7 @@ __device__ __forceinline__ bool find_mark(const AttnArgs& a, int part, Mark& mar
           mark.number = i + f, mark.units = __builtin_amdgcn_readlane(own, f);
           mark.units_before += __builtin_amdgcn_readlane(here - own, f);
           mark.blocks_before += mark.number;
+          block_of<kRows>(a, sequence_of<true>(a, mark.sequence), mark.sequence, mark.number, block);
           return true;
         }
         mark.units_before += __builtin_amdgcn_readlane(here, 63);
@@ -248,6 +253,16 @@ __device__ __forceinline__ Page page_of(const AttnArgs& a, int sequence, int key
   return {there ? e : 0, there};
 }
 
+// One request: lane l's 16 bytes at base + offset go to LDS bytes lds_dst + 16 l .. + 15 (lds_dst in M0, a wave's own).  Assembly, so that the
+// compiler does not see a vector memory instruction that writes LDS and wait for every request in flight in front of each LDS read; the wait for
+// these requests is explicit, the s_nop the wait state between a scalar write of M0 and a load to LDS.
+__device__ __forceinline__ void load_to_lds16(const void* base, uint32_t offset, uint32_t lds_dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds_dst) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(p)));
+}
+
 // Where a workgroup is on the line of units, kept in LDS while it works on a piece.
 struct Progress {
   Mark mark;
@@ -256,38 +271,22 @@ struct Progress {
   bool alone;      // the whole block is this workgroup's
 };
 
-// The first row block of a workgroup, or its place on the line of units; false: it has none.
+// The first row block of a workgroup, and its place on the line of units; false: it has none.
 template <int kRows>
-__device__ __forceinline__ bool first_piece(const AttnArgs& a, int id, Progress& progress, Block& k) {
+__device__ __forceinline__ bool first_piece(const AttnArgs& a, int id, Progress& at, Block& k) {
   if (a.parts == 0) return find_block<kRows>(a, a.blocks - 1 - id, k);
-  Progress at;
-  if (!find_mark<kRows>(a, id, at.mark)) return false;
+  if (!find_mark<kRows>(a, id, at.mark, k)) return false;
   at.per = part_units(a, at.mark.total);
   at.unit = id * at.per, at.unit_end = min(at.unit + at.per, at.mark.total);
-  if (threadIdx.x == 0) progress = at;
-  __syncthreads();
   return true;
 }
-// The workgroup's next piece: a block and which of its keys, [begin, end), begin a multiple of 32.
+// Which of block k's keys the workgroup has, [begin, end), begin a multiple of 32; its progress goes to LDS.
 template <int kRows>
-__device__ __forceinline__ void take_piece(const AttnArgs& a, int id, Progress& progress, Block& k, int& begin, int& end) {
+__device__ __forceinline__ void take_piece(const AttnArgs& a, int id, Progress at, Progress& progress, const Block& k, int& begin, int& end) {
   if (a.parts == 0) {
     begin = k.begin & ~31, end = k.end;
     return;
   }
-  Progress at = progress;
-  __syncthreads();
-  if (at.unit == at.mark.units_before + at.mark.units) {  // on to the next block (unit < total: there is one)
-    at.mark.units_before += at.mark.units, ++at.mark.blocks_before;
-    if (++at.mark.number == at.mark.blocks) {
-      do at.mark.blocks = blocks_of<kRows>(a, sequence_of<false>(a, ++at.mark.sequence));
-      while (at.mark.blocks == 0);
-      at.mark.number = 0;
-    }
-  }
-  const int b = __builtin_amdgcn_readfirstlane(at.mark.sequence);
-  block_of<kRows>(a, sequence_of<true>(a, b), b, __builtin_amdgcn_readfirstlane(at.mark.number), k);
-  at.mark.units = units_of(k);
   const int units = at.mark.units, first = at.mark.units_before, last = min(first + units, at.unit_end);
   begin = __builtin_amdgcn_readfirstlane((k.begin & ~31) + (at.unit - first) * 32);
   end = __builtin_amdgcn_readfirstlane(min((k.begin & ~31) + (last - first) * 32, k.end));
@@ -298,23 +297,43 @@ __device__ __forceinline__ void take_piece(const AttnArgs& a, int id, Progress& 
   at.unit = last;
   if (threadIdx.x == 0) progress = at;
 }
-
-// The block's rows of query head `head` ... of the cache head to LDS, [row tile][step][lane]: the order in which the matrix instructions take
-// them, zeros behind the rows' end and in rows that there are not.
-template <bool kEight, int kRows, int KS>
-__device__ __forceinline__ void rows_to_lds(const AttnArgs& a, const Block& k, int head, uint4* lds_q) {
-  for (int c = threadIdx.x; c < kRows * KS * 4; c += blockDim.x) {
-    const int row = c / (KS * 4), d = c % (KS * 4);  // eight elements of a row
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (row < k.count && d * 8 < a.k.width) {
-      const int r = k.row0 + row, t = token_of(a, r), g = r - t * a.shared;
-      x = *reinterpret_cast<const uint4*>(a.q + (static_cast<int64_t>(k.start) + t) * a.q_row + (static_cast<int64_t>(head) * a.shared + g) * a.q_head + d * 8);
-    }
-    // (8-bit keys: a lane reads 16 codes at a time, which serve two steps)
-    const int step = kEight ? (d >> 3) * 2 + (d & 1) : d >> 2, quarter = kEight ? (d >> 1) & 3 : d & 3;
-    lds_q[((row >> 4) * KS + step) * 64 + quarter * 16 + (row & 15)] = x;
+// On to the next block (there is one): behind a piece, in front of a barrier.
+template <int kRows>
+__device__ __forceinline__ Progress next_piece(const AttnArgs& a, const Progress& progress, Block& k) {
+  const auto in_common = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  Progress at{};
+  if (a.parts == 0) return at;  // (a workgroup a block: not reached)
+  const Mark& m = progress.mark;
+  at.mark = {in_common(m.sequence), in_common(m.number) + 1, in_common(m.blocks), 0, in_common(m.blocks_before) + 1, in_common(m.units_before) + in_common(m.units), 0};
+  at.unit = in_common(progress.unit), at.unit_end = in_common(progress.unit_end), at.per = in_common(progress.per);
+  Sequence s = sequence_of<true>(a, at.mark.sequence);
+  if (at.mark.number == at.mark.blocks) {
+    do s = sequence_of<true>(a, ++at.mark.sequence);
+    while (s.count == 0);
+    at.mark.blocks = blocks_of<kRows>(a, s), at.mark.number = 0;
   }
+  block_of<kRows>(a, s, at.mark.sequence, at.mark.number, k);
+  at.mark.units = units_of(k);
+  return at;
 }
+
+// The block's rows to LDS, [row tile][step][lane]: the order in which the matrix instructions take them, zeros behind the rows' end and in
+// rows that there are not.  Eight elements at a time: a row's are 4 KS pieces.
+template <int KS>
+__device__ __forceinline__ uint4 row_piece(const AttnArgs& a, const Block& k, int head, int c) {
+  const int row = c / (KS * 4), d = c % (KS * 4);
+  if (row >= k.count || d * 8 >= a.k.width) return make_uint4(0, 0, 0, 0);
+  const int r = k.row0 + row, t = token_of(a, r), g = r - t * a.shared;
+  return *reinterpret_cast<const uint4*>(a.q + (static_cast<int64_t>(k.start) + t) * a.q_row + (static_cast<int64_t>(head) * a.shared + g) * a.q_head + d * 8);
+}
+template <bool kEight, int KS>
+__device__ __forceinline__ void row_piece_to_lds(uint4 x, int c, uint4* lds_q) {
+  // (8-bit keys: a lane reads 16 codes at a time, which serve two steps)
+  const int row = c / (KS * 4), d = c % (KS * 4);
+  const int step = kEight ? (d >> 3) * 2 + (d & 1) : d >> 2, quarter = kEight ? (d >> 1) & 3 : d & 3;
+  lds_q[((row >> 4) * KS + step) * 64 + quarter * 16 + (row & 15)] = x;
+}
+
 // The rows' visible keys of a piece to LDS: the first one and the number of further ones (none: a first one that no key reaches).
 template <int kRows>
 __device__ __forceinline__ void ranges_to_lds(const AttnArgs& a, const Block& k, int end, int2* lds_sees) {
@@ -325,6 +344,16 @@ __device__ __forceinline__ void ranges_to_lds(const AttnArgs& a, const Block& k,
   }
 }
 __device__ __forceinline__ bool in_range(int2 range, int key) { return static_cast<uint32_t>(key) - static_cast<uint32_t>(range.x) <= static_cast<uint32_t>(range.y); }
+
+// The sum of the first `waves` of eight numbers in LDS.
+__device__ __forceinline__ float sum_of_waves(const float* p, int waves) {
+  const float4 u = *reinterpret_cast<const float4*>(p), v = *reinterpret_cast<const float4*>(p + 4);
+  const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+  float sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) sum += w < waves ? x[w] : 0.f;
+  return sum;
+}
 
 // A wave's accumulators to out, or with the rows' m and l to the workspace; true: this was the workgroup's last piece.
 // Accumulator element i of column operand j is column kCols (4 h + i) + j of its group of 16 kCols; eight columns are stored at a time.

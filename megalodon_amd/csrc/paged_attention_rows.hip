@@ -15,16 +15,6 @@
 namespace mega {
 namespace {
 
-// One request: lane l's 16 bytes at base + offset go to LDS bytes lds_dst + 16 l .. + 15 (lds_dst in M0, a wave's own).  Assembly, so that the
-// compiler does not see a vector memory instruction that writes LDS and wait for every request in flight in front of each LDS read; the wait for
-// these requests is explicit, the s_nop the wait state between a scalar write of M0 and a load to LDS.
-__device__ __forceinline__ void load_to_lds16(const void* base, uint32_t offset, uint32_t lds_dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds_dst) : "memory");
-}
-__device__ __forceinline__ uint32_t lds_address(const void* p) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(p)));
-}
-
 constexpr int RT = 4, CT = 8;                        // row and column tiles of a wave
 constexpr int kRows = 16 * RT, kMostWaves = 8;
 // of a key's 16-byte parts to a lane, those that come through LDS: all, or as many as it has room for beside the rows and the probabilities
@@ -55,13 +45,14 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
   const int page_mask = (1 << a.view.page_shift) - 1;
   const int first_column = (slab * waves + wave) * CT * 16;
   Block k;
-  if (!first_piece<kRows>(a, static_cast<int>(id), progress, k)) return;
+  Progress at;
+  if (!first_piece<kRows>(a, static_cast<int>(id), at, k)) return;
 
   for (;;) {
     const int lane = opaque(static_cast<int>(threadIdx.x) & 63);
     int begin, end;
-    take_piece<kRows>(a, static_cast<int>(id), progress, k, begin, end);
-    rows_to_lds<kEight, kRows, KS>(a, k, head, lds_q);
+    take_piece<kRows>(a, static_cast<int>(id), at, progress, k, begin, end);
+    for (int c = threadIdx.x; c < kRows * KS * 4; c += blockDim.x) row_piece_to_lds<kEight, KS>(row_piece<KS>(a, k, head, c), c, lds_q);
     ranges_to_lds<kRows>(a, k, end, lds_sees);
     if constexpr (!kSolo) {
       for (int c = threadIdx.x; c < kRows * kMostWaves; c += blockDim.x) lds_m[c] = -__builtin_inff();  // (of waves that there are not, too)
@@ -427,13 +418,11 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
         for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * kMostWaves + wave] = l[rt];
       __syncthreads();
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        l[rt] = 0.f;
-        for (int w = 0; w < waves; ++w) l[rt] += lds_m[(rt * 16 + n) * kMostWaves + w];
-      }
+      for (int rt = 0; rt < RT; ++rt) l[rt] = sum_of_waves(lds_m + (rt * 16 + n) * kMostWaves, waves);
     }
     if (store_piece<DT, RT, CT, 8>(a, k, static_cast<int>(id), head, slab, wave, first_column, progress, acc, m, l)) break;
-    __syncthreads();  // (the rows, maxima and probabilities of this piece have been read)
+    at = next_piece<kRows>(a, progress, k);
+    __syncthreads();  // (the rows, maxima, probabilities and progress of this piece have been read)
   }
 }
 
