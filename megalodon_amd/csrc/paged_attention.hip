@@ -30,6 +30,8 @@
 #include "paged_attention.hpp"
 
 #include <algorithm>
+#include <cfloat>
+#include <cmath>
 #include <type_traits>
 
 namespace mega {
@@ -82,7 +84,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
     // (anew for each piece and each use: kept out of the registers in between)
     const int lane = opaque(static_cast<int>(threadIdx.x) & 63), n = lane & 15, h = lane >> 4;
     int begin, end;
-    take_piece<kRows>(a, static_cast<int>(id), at, progress, k, begin, end);
+    take_piece<kRows>(a, at, progress, k, begin, end);
     // keys all_low .. all_high are seen by every row of the block
     const int all_low = chunk_start(a, k.position0 + token_of(a, k.row0 + k.count - 1)), all_high = min(k.position0 + token_of(a, k.row0), end - 1);
 
@@ -380,8 +382,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
       for (int rt = 0; rt < RT; ++rt) {
         float t = fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3]));
         t = fmaxf(t, fmaxf(fmaxf(s[1][rt][0], s[1][rt][1]), fmaxf(s[1][rt][2], s[1][rt][3])));
-        t = fmaxf(t, across(t, 16));
-        top[rt] = fmaxf(t, across(t, 32));
+        top[rt] = four_max(t);
       }
       if (waves > 1) {
         if (h == 0)
@@ -436,10 +437,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
 
     // ---- the rows' sums over the lanes and waves that had their keys
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      l[rt] += across(l[rt], 16);
-      l[rt] += across(l[rt], 32);
-    }
+    for (int rt = 0; rt < RT; ++rt) l[rt] = four_sum(l[rt]);
     if (waves > 1) {
       __syncthreads();  // (the maxima of the last tile have been read)
       if (h == 0)
@@ -632,7 +630,9 @@ extern "C" int mega_paged_attention_fwd(const mega_paged_cache* cache, int dtype
   a.clear_rest = clear_rest != 0;
   a.chunk_shift = log2_of(a.chunk), a.shared_shift = log2_of(a.shared);
   a.per_part = p.parts > 0 ? 1.0 / static_cast<double>(p.parts) : 0.0;
-  a.scale = static_cast<float>(scale * 1.4426950408889634);
+  a.scale = static_cast<float>(std::fabs(scale) * 1.4426950408889634);
+  if (a.scale < FLT_MIN) a.scale = FLT_MIN;  // (a scale of zero: every score is zero, and a masked one's infinity stays one)
+  a.sign = scale < 0.0 ? 0x80008000u : 0u;
   const bool eight = cache->k_exponents != nullptr;
   return dtype == MEGA_BF16 ? launch_attn<MEGA_BF16>(a, p, eight, stream) : launch_attn<MEGA_F16>(a, p, eight, stream);
 }

@@ -28,7 +28,8 @@ struct AttnArgs {
   int32_t parts, slots, part_rows;  // parts of the line of units for each head and slab; 0: a workgroup a block
   int32_t clear_rest;
   int32_t chunk_shift, shared_shift;  // their logarithms where they are powers of two, else -1: a division is thirty instructions in a row
-  float scale;                // times log2(e)
+  float scale;                // |scale| log2(e), above zero: a negative scale turns the rows' signs (sign: their bits)
+  uint32_t sign;
   double per_part;            // 1 / parts
 };
 
@@ -241,6 +242,19 @@ __device__ __forceinline__ int opaque(int v) {
 }
 
 __device__ __forceinline__ float across(float v, int mask) { return __shfl_xor(v, mask, 64); }
+// v's maximum and sum over the four lanes n, n + 16, n + 32, n + 48, in all of them: the swapping moves leave both halves in each place
+__device__ __forceinline__ float four_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+__device__ __forceinline__ float four_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+}
 
 // The page of 16 keys: its number and whether there is one (0 otherwise, so that addresses stay in the pool).
 struct Page {
@@ -266,7 +280,7 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 // Where a workgroup is on the line of units, kept in LDS while it works on a piece.
 struct Progress {
   Mark mark;
-  int32_t unit, unit_end, per;
+  int32_t unit, unit_end, per, part;
   int32_t pieces;  // of the block, this one included if it is the first; 0 for the others
   bool alone;      // the whole block is this workgroup's
 };
@@ -275,14 +289,35 @@ struct Progress {
 template <int kRows>
 __device__ __forceinline__ bool first_piece(const AttnArgs& a, int id, Progress& at, Block& k) {
   if (a.parts == 0) return find_block<kRows>(a, a.blocks - 1 - id, k);
+  // One sequence whose blocks see much the same number of keys: as many equal pieces of each block as there are parts for, so that nobody
+  // has two (a piece of 512 tokens behind 1531: 95 us on the line)
+  if (a.view.batch == 1) {
+    const Sequence s = sequence_of<true>(a, 0);
+    const int blocks = blocks_of<kRows>(a, s);
+    if (s.start == 0 && (s.count == a.rows || !a.clear_rest) && blocks > 0 && blocks <= a.parts) {
+      Block first;
+      block_of<kRows>(a, s, 0, 0, first);
+      block_of<kRows>(a, s, 0, blocks - 1, k);
+      if (units_of(first) * 4 >= units_of(k) * 3) {
+        const int each = a.parts / blocks, number = id / each, piece = id - number * each;
+        if (!block_of<kRows>(a, s, 0, number, k)) return false;
+        const int units = units_of(k);
+        at.per = (units + each - 1) / each, at.part = piece;
+        at.unit = piece * at.per, at.unit_end = min(at.unit + at.per, units);
+        at.mark = {0, number, blocks, units, 0, 0, units};
+        return at.unit < units;
+      }
+    }
+  }
   if (!find_mark<kRows>(a, id, at.mark, k)) return false;
+  at.part = id;
   at.per = part_units(a, at.mark.total);
   at.unit = id * at.per, at.unit_end = min(at.unit + at.per, at.mark.total);
   return true;
 }
 // Which of block k's keys the workgroup has, [begin, end), begin a multiple of 32; its progress goes to LDS.
 template <int kRows>
-__device__ __forceinline__ void take_piece(const AttnArgs& a, int id, Progress at, Progress& progress, const Block& k, int& begin, int& end) {
+__device__ __forceinline__ void take_piece(const AttnArgs& a, Progress at, Progress& progress, const Block& k, int& begin, int& end) {
   if (a.parts == 0) {
     begin = k.begin & ~31, end = k.end;
     return;
@@ -290,7 +325,7 @@ __device__ __forceinline__ void take_piece(const AttnArgs& a, int id, Progress a
   const int units = at.mark.units, first = at.mark.units_before, last = min(first + units, at.unit_end);
   begin = __builtin_amdgcn_readfirstlane((k.begin & ~31) + (at.unit - first) * 32);
   end = __builtin_amdgcn_readfirstlane(min((k.begin & ~31) + (last - first) * 32, k.end));
-  const int part_end = (id + 1) * at.per;
+  const int part_end = (at.part + 1) * at.per;
   const bool begins_here = first >= part_end - at.per;
   at.alone = begins_here && first + units <= part_end;
   at.pieces = !begins_here ? 0 : at.alone ? 1 : 1 + (first + units - part_end + at.per - 1) / at.per;
@@ -305,7 +340,7 @@ __device__ __forceinline__ Progress next_piece(const AttnArgs& a, const Progress
   if (a.parts == 0) return at;  // (a workgroup a block: not reached)
   const Mark& m = progress.mark;
   at.mark = {in_common(m.sequence), in_common(m.number) + 1, in_common(m.blocks), 0, in_common(m.blocks_before) + 1, in_common(m.units_before) + in_common(m.units), 0};
-  at.unit = in_common(progress.unit), at.unit_end = in_common(progress.unit_end), at.per = in_common(progress.per);
+  at.unit = in_common(progress.unit), at.unit_end = in_common(progress.unit_end), at.per = in_common(progress.per), at.part = in_common(progress.part);
   Sequence s = sequence_of<true>(a, at.mark.sequence);
   if (at.mark.number == at.mark.blocks) {
     do s = sequence_of<true>(a, ++at.mark.sequence);
@@ -324,7 +359,9 @@ __device__ __forceinline__ uint4 row_piece(const AttnArgs& a, const Block& k, in
   const int row = c / (KS * 4), d = c % (KS * 4);
   if (row >= k.count || d * 8 >= a.k.width) return make_uint4(0, 0, 0, 0);
   const int r = k.row0 + row, t = token_of(a, r), g = r - t * a.shared;
-  return *reinterpret_cast<const uint4*>(a.q + (static_cast<int64_t>(k.start) + t) * a.q_row + (static_cast<int64_t>(head) * a.shared + g) * a.q_head + d * 8);
+  uint4 x = *reinterpret_cast<const uint4*>(a.q + (static_cast<int64_t>(k.start) + t) * a.q_row + (static_cast<int64_t>(head) * a.shared + g) * a.q_head + d * 8);
+  x.x ^= a.sign, x.y ^= a.sign, x.z ^= a.sign, x.w ^= a.sign;
+  return x;
 }
 template <bool kEight, int KS>
 __device__ __forceinline__ void row_piece_to_lds(uint4 x, int c, uint4* lds_q) {

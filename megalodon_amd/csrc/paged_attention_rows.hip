@@ -51,7 +51,7 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
   for (;;) {
     const int lane = opaque(static_cast<int>(threadIdx.x) & 63);
     int begin, end;
-    take_piece<kRows>(a, static_cast<int>(id), at, progress, k, begin, end);
+    take_piece<kRows>(a, at, progress, k, begin, end);
     for (int c = threadIdx.x; c < kRows * KS * 4; c += blockDim.x) row_piece_to_lds<kEight, KS>(row_piece<KS>(a, k, head, c), c, lds_q);
     ranges_to_lds<kRows>(a, k, end, lds_sees);
     if constexpr (!kSolo) {
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
     // ---- keys: part `part` of a lane is 16 bytes of key 16 half + (lane & 15).  Those that come through LDS are asked for a tile ahead, into the
     // wave's own place and in operand order
     u32x4 kx[2][kHeld > 0 ? kHeld : 1];
-    uint32_t ke[2][4];
+    float unit[2];  // of the lane's keys (8 bits)
     struct Keys {
       const uint8_t* from[2];
       const uint8_t* exponents[2];
@@ -92,11 +92,8 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
     };
     const auto load_key_exponents = [&](const Keys& t) {
       if constexpr (kEight) {
-        const uint32_t offset = static_cast<uint32_t>(4 * (opaque(lane) >> 4)) * a.k.eSlot;
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) ke[half][i] = t.exponents[half][offset + static_cast<uint32_t>(i * a.k.eSlot)];
+        for (int half = 0; half < 2; ++half) unit[half] = exponent_value(t.exponents[half][static_cast<uint32_t>(opaque(lane) & 15) * a.k.eSlot]);
       }
     };
     const auto ask_for_keys = [&](int tile) {
@@ -199,7 +196,7 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
             u32x4 x = part < kInLds ? __builtin_bit_cast(u32x4, lds_k[((wave * 2 + half) * kInLds + part) * 64 + lane]) : kx[half][(part - kInLds) % (kHeld > 0 ? kHeld : 1)];
             if constexpr (kEight) {
               const uint32_t lo = (c & 1) ? x[2] : x[0], hi = (c & 1) ? x[3] : x[1];
-              x = u32x4{widen<DT, false>(lo, 1.f), widen<DT, true>(lo, 1.f), widen<DT, false>(hi, 1.f), widen<DT, true>(hi, 1.f)};
+              x = u32x4{widen<DT, false>(lo, unit[half]), widen<DT, true>(lo, unit[half]), widen<DT, false>(hi, unit[half]), widen<DT, true>(hi, unit[half])};
             }
             if constexpr (!kFull) {  // (behind the row's end the rows' operands are zero, and infinity times zero is not)
               const int d = kEight ? (c >> 1) * 64 + (opaque(lane) >> 4) * 16 : c * 32 + (opaque(lane) >> 4) * 8;
@@ -211,15 +208,6 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
           }
           __builtin_amdgcn_sched_barrier(0);
         }
-      }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        f32x4 factor = {a.scale, a.scale, a.scale, a.scale};
-        if constexpr (kEight)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) factor[i] *= exponent_value(ke[half][i]);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[half][rt] *= factor;
       }
       load_step(tile);
       if (!whole) {
@@ -244,8 +232,7 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
         for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int i = 0; i < 4; ++i) t = fmaxf(t, s[half][rt][i]);
-        t = fmaxf(t, across(t, 16));
-        top[rt] = fmaxf(t, across(t, 32));
+        top[rt] = four_max(t);
       }
       if constexpr (!kSolo) {
         const int l = opaque(lane), n = l & 15;
@@ -274,14 +261,14 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
       float alpha[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float now = top[rt] > m[rt] + 8.f ? top[rt] : m[rt], base = now == -__builtin_inff() ? 0.f : now;
+        const float seen = top[rt] * a.scale, now = seen > m[rt] + 8.f ? seen : m[rt], base = now == -__builtin_inff() ? 0.f : now;
         alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - base);
         moved = moved || now != m[rt];
         m[rt] = now;
         float p[8], sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(s[i >> 2][rt][i & 3] - base);
+          p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][rt][i & 3], a.scale, -base));
           sum += p[i];
         }
         own[rt] = u32x4{pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
@@ -406,10 +393,7 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
 
     // ---- the rows' sums over the lanes and waves that had their keys
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      l[rt] += across(l[rt], 16);
-      l[rt] += across(l[rt], 32);
-    }
+    for (int rt = 0; rt < RT; ++rt) l[rt] = four_sum(l[rt]);
     if constexpr (!kSolo) {
       const int at = opaque(lane), n = at & 15;
       __syncthreads();  // (the maxima of the last tile have been read)
