@@ -525,7 +525,7 @@ Plan plan_of(const mega_paged_cache* c, int64_t rows, int64_t q_heads) {
   // workgroups that the chip holds at a time: eight waves to a CU
   const int64_t resident = kCus * kMaxWaves / p.waves, pairs = c->heads * p.slabs;
   const int64_t full = std::max(rows * shared / kRows, std::min(c->batch, rows)) * pairs;
-  if (c->batch > 0 && full < 4 * resident && p.blocks * (c->table_width * c->page_size / 32 + 1) < 0x40000000 &&
+  if (c->batch > 0 && full < 4 * resident && p.blocks * (c->table_width * c->page_size / 32 + 9) < 0x40000000 &&
       (resident + p.blocks) * c->heads * kRows < 0x40000000 && rows * q_heads < 0x1000000) {
     p.parts = std::max<int64_t>(1, resident / pairs);
     p.part_rows = std::min(kRows, rows * shared);
@@ -629,6 +629,7 @@ extern "C" int mega_paged_attention_fwd(const mega_paged_cache* cache, int dtype
   a.parts = static_cast<int32_t>(p.parts), a.slots = static_cast<int32_t>(p.slots), a.part_rows = static_cast<int32_t>(p.part_rows);
   a.clear_rest = clear_rest != 0;
   a.chunk_shift = log2_of(a.chunk), a.shared_shift = log2_of(a.shared);
+  a.lead = p.rt == 4 ? 8 : 1;
   a.per_part = p.parts > 0 ? 1.0 / static_cast<double>(p.parts) : 0.0;
   a.scale = static_cast<float>(std::fabs(scale) * 1.4426950408889634);
   if (a.scale < FLT_MIN) a.scale = FLT_MIN;  // (a scale of zero: every score is zero, and a masked one's infinity stays one)

@@ -26,6 +26,7 @@ struct AttnArgs {
   int2* joins;                // ... (rows, q_heads): a row's first place in the former and its number of pieces (0: out has it)
   int32_t rows, heads, shared, chunk, slabs, blocks;
   int32_t parts, slots, part_rows;  // parts of the line of units for each head and slab; 0: a workgroup a block
+  int32_t lead;               // units in front of a block's own on the line
   int32_t clear_rest;
   int32_t chunk_shift, shared_shift;  // their logarithms where they are powers of two, else -1: a division is thirty instructions in a row
   float scale;                // |scale| log2(e), above zero: a negative scale turns the rows' signs (sign: their bits)
@@ -105,11 +106,13 @@ __device__ __forceinline__ bool find_block(const AttnArgs& a, int number, Block&
   return block_of<kRows>(a, sequence_of<true>(a, b), b, number - (static_cast<int64_t>(bound_at<true>(a, b)) * a.shared / kRows + b), k);
 }
 
-// The line of units: a block has one for every 32 keys that it sees, and one if there are none.
+// The line of units: a block has one for every 32 keys that it sees, and one if there are none, behind a.lead units for what a piece costs
+// whatever its length (its rows' way in, its results' way out).  Only the units behind these are anybody's: a part that ends in a block's
+// lead has nothing of the block, one that begins there has it from its first key.
 __device__ __forceinline__ int units_of(const Block& k) { return max(k.end - (k.begin & ~31) + 31, 32) >> 5; }
 // A place on the line: a block (its sequence, its number there), its units, and the blocks and units in front of it.
 struct Mark {
-  int32_t sequence, number, blocks, units;  // blocks: of the sequence
+  int32_t sequence, number, blocks, units;  // blocks: of the sequence; units: with the lead
   int32_t blocks_before, units_before, total;  // total: of the whole line (the host cuts no line of 2^30 units)
 };
 // units of a part; the parts behind the line's end are empty.  (The quotient in double is right: it is half a part away from the next one.)
@@ -132,7 +135,7 @@ __device__ __forceinline__ int lane_units(const AttnArgs& a, int b, int number, 
   Block k;
   const int i = number + (static_cast<int>(threadIdx.x) & 63);
   const bool has = block_of<kRows>(a, sequence_of<true>(a, b), b, i, k);
-  return i < blocks && has ? units_of(k) : 0;
+  return i < blocks && has ? units_of(k) + a.lead : 0;
 }
 
 // The block in which part `part` begins (false: the part is empty); all lanes of a wave together, 64 sequences a round, and 64 blocks of a
@@ -146,7 +149,7 @@ __device__ __forceinline__ bool find_mark(const AttnArgs& a, int part, Mark& mar
     const int b = min(b0 + lane, sequences - 1);
     const Sequence q = sequence_of<false>(a, b);
     const bool has = block_of<kRows>(a, q, b, 0, k) && b0 + lane < sequences;
-    blocks = has ? blocks_of<kRows>(a, q) : 0, units = has ? units_of(k) : 0;
+    blocks = has ? blocks_of<kRows>(a, q) : 0, units = has ? units_of(k) + a.lead : 0;
     for (uint64_t more = __ballot(blocks > 1); more != 0; more &= more - 1) {
       const int l = __ffsll(static_cast<unsigned long long>(more)) - 1, count = __builtin_amdgcn_readlane(blocks, l);
       int sum = 0;
@@ -304,7 +307,7 @@ __device__ __forceinline__ bool first_piece(const AttnArgs& a, int id, Progress&
         const int units = units_of(k);
         at.per = (units + each - 1) / each, at.part = piece;
         at.unit = piece * at.per, at.unit_end = min(at.unit + at.per, units);
-        at.mark = {0, number, blocks, units, 0, 0, units};
+        at.mark = {0, number, blocks, units + a.lead, 0, -a.lead, units};
         return at.unit < units;
       }
     }
@@ -313,7 +316,8 @@ __device__ __forceinline__ bool first_piece(const AttnArgs& a, int id, Progress&
   at.part = id;
   at.per = part_units(a, at.mark.total);
   at.unit = id * at.per, at.unit_end = min(at.unit + at.per, at.mark.total);
-  return true;
+  // (the part's first block may be one that it has nothing of)
+  return at.unit_end > at.mark.units_before + a.lead;
 }
 // Which of block k's keys the workgroup has, [begin, end), begin a multiple of 32; its progress goes to LDS.
 template <int kRows>
@@ -322,11 +326,12 @@ __device__ __forceinline__ void take_piece(const AttnArgs& a, Progress at, Progr
     begin = k.begin & ~31, end = k.end;
     return;
   }
-  const int units = at.mark.units, first = at.mark.units_before, last = min(first + units, at.unit_end);
+  const int units = at.mark.units - a.lead, first = at.mark.units_before + a.lead, last = min(first + units, at.unit_end);
+  at.unit = max(at.unit, first);
   begin = __builtin_amdgcn_readfirstlane((k.begin & ~31) + (at.unit - first) * 32);
   end = __builtin_amdgcn_readfirstlane(min((k.begin & ~31) + (last - first) * 32, k.end));
   const int part_end = (at.part + 1) * at.per;
-  const bool begins_here = first >= part_end - at.per;
+  const bool begins_here = first >= part_end - at.per;  // (and in front of the part's end)
   at.alone = begins_here && first + units <= part_end;
   at.pieces = !begins_here ? 0 : at.alone ? 1 : 1 + (first + units - part_end + at.per - 1) / at.per;
   at.unit = last;
@@ -348,7 +353,7 @@ __device__ __forceinline__ Progress next_piece(const AttnArgs& a, const Progress
     at.mark.blocks = blocks_of<kRows>(a, s), at.mark.number = 0;
   }
   block_of<kRows>(a, s, at.mark.sequence, at.mark.number, k);
-  at.mark.units = units_of(k);
+  at.mark.units = units_of(k) + a.lead;
   return at;
 }
 
@@ -403,7 +408,7 @@ __device__ __forceinline__ bool store_piece(const AttnArgs& a, const Block& k, i
   int pieces = 0;
   if (a.parts > 0) {
     slot = (static_cast<int64_t>(head) * a.slots + id + progress.mark.blocks_before) * a.part_rows;
-    alone = progress.alone, pieces = progress.pieces, last = progress.unit >= progress.unit_end;
+    alone = progress.alone, pieces = progress.pieces, last = progress.unit + a.lead >= progress.unit_end;
   }
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
