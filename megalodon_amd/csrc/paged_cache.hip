@@ -6,10 +6,13 @@
 // ties to even.  A power of two costs an e4m3 number nothing (its relative step is the same at every scale short of
 // its subnormals), makes both the division and the way back exact, and takes one byte a row.
 //
-// Bound by HBM: a row is read once and written once.  A group of 16, 32 or 64 lanes takes a row, each lane
-// pieces of eight elements (one 16-byte access of 16-bit ones), which it keeps in registers between the maximum
-// and the codes.  Keys and values are rows of the same launch: the first workgroups take keys, the others values.
+// Bound by HBM: a row is read once and written once.  A wave has a token, all of its heads or some of them: where the token lies is looked up
+// once (four loads that wait for each other), then its values go by, then its keys.  16, 32 or 64 lanes take a row, each lane pieces of eight
+// elements (one 16-byte access of 16-bit ones), which it keeps in registers between the maximum and the codes; lanes that a narrow row leaves
+// take the next heads.
 #include "paged.hpp"
+
+#include <algorithm>
 
 namespace mega {
 namespace {
@@ -25,119 +28,145 @@ struct Side {
 };
 struct CacheArgs {
   PagedView view;
-  Side side[2];
+  Side side[2];               // keys, values
   const int32_t *first, *cu;  // first: lengths (write), begins (read)
   int32_t rows, heads;
-  uint32_t key_groups;        // workgroups that take keys
+  int32_t at_once, shares;    // heads of a wave; waves of a token (twice that where `apart`: keys and values have waves of their own)
+  int32_t apart;
   int clear_rest;
 };
 
-// Where a lane's row is.
+// Where a token is, the same for a wave.
 struct Place {
-  int64_t slot, eslot;  // element offsets of the position's row in the pool, -1: nowhere
-  int64_t packed;       // ... and in the packed operand
-  bool row, owned;      // there is such a row; a sequence has it
+  int32_t token, head, end;  // heads head .. end - 1 are the wave's
+  uint32_t page, slot;       // in the pool
+  bool there, owned;         // it has a place; a sequence has it
+  bool keys, values;         // what the wave moves
 };
 
+// false: the wave has nothing to do
 template <bool kWrite>
-__device__ __forceinline__ Place find_place(const CacheArgs& a, const Side& s, uint32_t group) {
-  const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
-  const int per_wave = kWave >> s.lanes_log2;
-  const int64_t items = static_cast<int64_t>(a.rows) * a.heads;
-  const int64_t item0 = (static_cast<int64_t>(group) * kWaves + wave) * per_wave, item = item0 + (lane >> s.lanes_log2);
-  Place p{-1, -1, 0, item < items, false};
-  if (item0 >= items) return p;  // (the whole wave)
-  const int32_t* cu = a.cu;
-  const int t0 = static_cast<int>(item0 / a.heads);
-  int b = last_not_above(a.view.batch, t0, [&](int i) { return static_cast<int64_t>(cu[i]); });
-  if (!p.row) return p;
-  const int t = static_cast<int>(item / a.heads), h = static_cast<int>(item - static_cast<int64_t>(t) * a.heads);
-  p.packed = t * s.row + h * s.head;
-  while (b + 1 < a.view.batch && cu[b + 1] <= t) ++b;  // (a wave's rows may be of several sequences)
-  const int start = row_bound(cu, b, a.rows), end = row_bound(cu, b + 1, a.rows);
-  if (t < start || t >= end) return p;
-  p.owned = true;
-  const int64_t position = kWrite ? static_cast<int64_t>(a.first[b]) - (end - t) : static_cast<int64_t>(a.first[b]) + (t - start);
-  if (position < 0 || (position >> a.view.page_shift) >= a.view.table_width) return p;
-  const uint32_t page = static_cast<uint32_t>(a.view.table[b * a.view.table_stride + (position >> a.view.page_shift)]);
-  if (page >= static_cast<uint32_t>(a.view.pages)) return p;
-  const int64_t in_page = position & ((int64_t{1} << a.view.page_shift) - 1);
-  p.slot = page * s.pool.page + in_page * s.pool.slot + static_cast<int64_t>(h) * s.pool.head;
-  p.eslot = page * s.pool.ePage + in_page * s.pool.eSlot + static_cast<int64_t>(h) * s.pool.eHead;
-  return p;
+__device__ __forceinline__ bool find_place(const CacheArgs& a, Place& p) {
+  int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  p.keys = !a.apart || (item & 1) != 0, p.values = !a.apart || (item & 1) == 0;
+  item >>= a.apart;
+  if (item >= static_cast<int64_t>(a.rows) * a.shares) return false;
+  p.token = static_cast<int32_t>(item / a.shares);
+  p.head = static_cast<int32_t>(item - static_cast<int64_t>(p.token) * a.shares) * a.at_once, p.end = min(p.head + a.at_once, a.heads);
+  p.there = p.owned = false, p.page = p.slot = 0;
+  const int b = last_not_above(a.view.batch, p.token, [&](int i) { return static_cast<int64_t>(a.cu[i]); });
+  const int start = row_bound(a.cu, b, a.rows), end = row_bound(a.cu, b + 1, a.rows);
+  p.owned = p.token >= start && p.token < end;
+  if (!p.owned) return !kWrite && a.clear_rest;
+  const int64_t position = static_cast<int64_t>(a.first[b]) + (kWrite ? p.token - end : p.token - start);
+  if (position >= 0 && (position >> a.view.page_shift) < a.view.table_width) {
+    p.page = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(a.view.table[b * a.view.table_stride + (position >> a.view.page_shift)]));
+    p.slot = static_cast<uint32_t>(position) & ((1u << a.view.page_shift) - 1);
+    p.there = p.page < static_cast<uint32_t>(a.view.pages);
+  }
+  return !kWrite || p.there;
 }
 
-// |x| of a 16-bit pattern, 0 where it is not finite
-template <int DT>
-__device__ __forceinline__ uint32_t finite_magnitude(uint32_t bits) {
-  const uint32_t top = DT == MEGA_BF16 ? 0x7f80u : 0x7c00u, m = bits & 0x7fffu;
-  return m < top ? m : 0;
+// The rows of one side, a few heads at a time: `row(head, active)` for this lane's.
+template <typename F>
+__device__ __forceinline__ void each_row(const Side& s, const Place& p, F row) {
+  const int lane = static_cast<int>(threadIdx.x) & 63, heads = kWave >> s.lanes_log2;
+  for (int h = p.head; h < p.end; h += heads) row(h + (lane >> s.lanes_log2), h + (lane >> s.lanes_log2) < p.end);
+}
+__device__ __forceinline__ int64_t pool_offset(const PagedPool& pool, const Place& p, int head) {
+  return p.page * pool.page + static_cast<int64_t>(p.slot) * pool.slot + static_cast<int64_t>(head) * pool.head;
+}
+__device__ __forceinline__ int64_t exponent_offset(const PagedPool& pool, const Place& p, int head) {
+  return p.page * pool.ePage + static_cast<int64_t>(p.slot) * pool.eSlot + static_cast<int64_t>(head) * pool.eHead;
+}
+
+// the greater of each half's 16-bit magnitudes; with kFinite those of infinities and NaN count as zero
+template <int DT, bool kFinite>
+__device__ __forceinline__ uint32_t greater_magnitudes(uint32_t a, uint32_t w) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  w &= 0x7fff7fffu;
+  if constexpr (kFinite) {
+    constexpr uint32_t top = DT == MEGA_BF16 ? 0x7f80u : 0x7c00u;
+    w = ((w & 0xffffu) >= top ? 0u : w & 0xffffu) | ((w >> 16) >= top ? 0u : w & 0xffff0000u);
+  }
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, w)));
+}
+// a row's greatest magnitude, in all of its lanes (bit patterns of non-negative numbers are ordered as the numbers are)
+template <int DT, bool kFinite>
+__device__ __forceinline__ uint32_t row_top(const uint4 (&x)[kPieces], int lanes) {
+  uint32_t both = 0;
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    both = greater_magnitudes<DT, kFinite>(greater_magnitudes<DT, kFinite>(both, x[i].x), x[i].y);
+    both = greater_magnitudes<DT, kFinite>(greater_magnitudes<DT, kFinite>(both, x[i].z), x[i].w);
+  }
+  uint32_t top = max(both & 0xffffu, both >> 16);
+  for (int off = 1; off < lanes; off <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
+  return top;
 }
 
 template <int DT, bool kEight>
-__global__ __launch_bounds__(kThreads) void paged_write_kernel(CacheArgs a) {
-  const bool values = blockIdx.x >= a.key_groups;
-  const Side& s = a.side[values];
-  const Place p = find_place<true>(a, s, blockIdx.x - (values ? a.key_groups : 0));
+__device__ __forceinline__ void write_rows(const Side& s, const Place& p) {
   const int l = (static_cast<int>(threadIdx.x) & (s.lanes - 1)) * 8, stride = s.lanes * 8, width = s.pool.width;
-  const uint16_t* from = static_cast<const uint16_t*>(s.rows) + p.packed;
-  if (!kEight) {
-    if (p.slot < 0) return;
-    uint16_t* to = static_cast<uint16_t*>(s.pool.rows) + p.slot;
+  each_row(s, p, [&](int head, bool active) {
+    const uint16_t* from = static_cast<const uint16_t*>(s.rows) + p.token * s.row + head * s.head;
+    const int mine = active ? width : 0;
     uint4 x[kPieces];
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       x[i] = make_uint4(0, 0, 0, 0);
-      if (l + i * stride < width) x[i] = *reinterpret_cast<const uint4*>(from + l + i * stride);
+      if (l + i * stride < mine) x[i] = *reinterpret_cast<const uint4*>(from + l + i * stride);
     }
+    if constexpr (!kEight) {
+      uint16_t* to = static_cast<uint16_t*>(s.pool.rows) + pool_offset(s.pool, p, head);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i)
-      if (l + i * stride < width) *reinterpret_cast<uint4*>(to + l + i * stride) = x[i];
-    return;
-  }
-  uint4 x[kPieces];
-  uint32_t top = 0;  // (bit patterns of non-negative numbers are ordered as the numbers are)
-  if (p.slot >= 0) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i)
-      if (l + i * stride < width) {
-        x[i] = *reinterpret_cast<const uint4*>(from + l + i * stride);
-        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) top = max(top, max(finite_magnitude<DT>(w[j] & 0xffffu), finite_magnitude<DT>(w[j] >> 16)));
+      for (int i = 0; i < kPieces; ++i)
+        if (l + i * stride < mine) *reinterpret_cast<uint4*>(to + l + i * stride) = x[i];
+    } else {
+      uint32_t top = row_top<DT, false>(x, s.lanes);
+      const bool odd = __any(top >= (DT == MEGA_BF16 ? 0x7f80u : 0x7c00u));  // (some row has an infinity or NaN)
+      if (odd) top = row_top<DT, true>(x, s.lanes);
+      int e = 0;
+      if (top != 0) {
+        int power;
+        const float fraction = frexpf(DT == MEGA_BF16 ? bf16_bits_to_float(top) : f16_bits_to_float(top), &power);
+        e = max(fraction > 0.875f ? power - 8 : power - 9, -126);
       }
-  }
-  for (int off = 1; off < s.lanes; off <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
-  if (p.slot < 0) return;
-  int e = 0;
-  if (top != 0) {
-    int power;
-    const float fraction = frexpf(DT == MEGA_BF16 ? bf16_bits_to_float(top) : f16_bits_to_float(top), &power);
-    e = max(fraction > 0.875f ? power - 8 : power - 9, -126);
-  }
-  const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-  // 256 2^e is twice the type's greatest power of two: a magnitude that would round to it stays at 240
-  const float limit = e == (DT == MEGA_BF16 ? 120 : 8) ? 240.f : 448.f;
-  uint8_t* to = static_cast<uint8_t*>(s.pool.rows) + p.slot;
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      // 256 2^e is twice the type's greatest power of two: a magnitude that would round to it stays at 240
+      const bool edge = e == (DT == MEGA_BF16 ? 120 : 8);
+      const float limit = edge ? 240.f : 448.f;
+      const bool plain = !odd && !__any(edge);
+      uint8_t* to = static_cast<uint8_t*>(s.pool.rows) + pool_offset(s.pool, p, head);
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i)
-    if (l + i * stride < width) {
-      float v[8];
-      unpack8<DT>(x[i], v);
-      int code[2] = {0, 0};
+      for (int i = 0; i < kPieces; ++i)
+        if (l + i * stride < mine) {
+          float v[8];
+          unpack8<DT>(x[i], v);
+          int code[2] = {0, 0};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float y = v[j] * down;
-        v[j] = fabsf(v[j]) < __builtin_inff() ? fminf(fmaxf(y, -limit), limit) : __builtin_nanf("");
-      }
+          for (int j = 0; j < 8; ++j) {
+            const float y = v[j] * down;
+            v[j] = plain ? y : fabsf(v[j]) < __builtin_inff() ? fminf(fmaxf(y, -limit), limit) : __builtin_nanf("");
+          }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        code[j] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j], v[4 * j + 1], 0, false);
-        code[j] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j + 2], v[4 * j + 3], code[j], true);
-      }
-      *reinterpret_cast<uint2*>(to + l + i * stride) = make_uint2(static_cast<uint32_t>(code[0]), static_cast<uint32_t>(code[1]));
+          for (int j = 0; j < 2; ++j) {
+            code[j] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j], v[4 * j + 1], 0, false);
+            code[j] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j + 2], v[4 * j + 3], code[j], true);
+          }
+          *reinterpret_cast<uint2*>(to + l + i * stride) = make_uint2(static_cast<uint32_t>(code[0]), static_cast<uint32_t>(code[1]));
+        }
+      if (l == 0 && active) s.pool.exponents[exponent_offset(s.pool, p, head)] = static_cast<uint8_t>(e + 127);
     }
-  if (l == 0) s.pool.exponents[p.eslot] = static_cast<uint8_t>(e + 127);
+  });
+}
+
+template <int DT, bool kEight>
+__global__ __launch_bounds__(kThreads) void paged_write_kernel(CacheArgs a) {
+  Place p;
+  if (!find_place<true>(a, p)) return;
+  if (p.values) write_rows<DT, kEight>(a.side[1], p);
+  if (p.keys) write_rows<DT, kEight>(a.side[0], p);
 }
 
 // two e4m3 codes of a word's lower or upper half times a power of two, as 16-bit numbers
@@ -148,36 +177,44 @@ __device__ __forceinline__ uint32_t widen(uint32_t codes, float scale) {
 }
 
 template <int DT, bool kEight>
-__global__ __launch_bounds__(kThreads) void paged_read_kernel(CacheArgs a) {
-  const bool values = blockIdx.x >= a.key_groups;
-  const Side& s = a.side[values];
-  const Place p = find_place<false>(a, s, blockIdx.x - (values ? a.key_groups : 0));
-  if (!p.row || !(p.owned || a.clear_rest)) return;
+__device__ __forceinline__ void read_rows(const Side& s, const Place& p) {
   const int l = (static_cast<int>(threadIdx.x) & (s.lanes - 1)) * 8, stride = s.lanes * 8, width = s.pool.width;
-  uint16_t* to = static_cast<uint16_t*>(s.rows) + p.packed;
-  uint4 x[kPieces];
-  float scale = 0.f;
-  if (kEight && p.slot >= 0) scale = exponent_value(s.pool.exponents[p.eslot]);
+  each_row(s, p, [&](int head, bool active) {
+    uint16_t* to = static_cast<uint16_t*>(s.rows) + p.token * s.row + head * s.head;
+    const int mine = active ? width : 0, stored = p.there ? mine : 0;
+    float scale = 0.f;
+    if (kEight && stored > 0) scale = exponent_value(s.pool.exponents[exponent_offset(s.pool, p, head)]);
+    uint4 x[kPieces];
+    const int64_t from = pool_offset(s.pool, p, head);
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i)
-    if (l + i * stride < width) {
+    for (int i = 0; i < kPieces; ++i) {
       x[i] = make_uint4(0, 0, 0, 0);
-      if (p.slot < 0) continue;
-      if (kEight) {
-        const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.pool.rows) + p.slot + l + i * stride);
-        x[i].x = c.x, x[i].y = c.y;
-      } else {
-        x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(s.pool.rows) + p.slot + l + i * stride);
+      if (l + i * stride < stored) {
+        if (kEight) {
+          const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.pool.rows) + from + l + i * stride);
+          x[i].x = c.x, x[i].y = c.y;
+        } else {
+          x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(s.pool.rows) + from + l + i * stride);
+        }
       }
     }
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i)
-    if (l + i * stride < width) {
-      if (kEight)
-        x[i] = make_uint4(widen<DT, false>(x[i].x, scale), widen<DT, true>(x[i].x, scale), widen<DT, false>(x[i].y, scale),
-                          widen<DT, true>(x[i].y, scale));
-      *reinterpret_cast<uint4*>(to + l + i * stride) = x[i];
-    }
+    for (int i = 0; i < kPieces; ++i)
+      if (l + i * stride < mine) {
+        if (kEight)
+          x[i] = make_uint4(widen<DT, false>(x[i].x, scale), widen<DT, true>(x[i].x, scale), widen<DT, false>(x[i].y, scale),
+                            widen<DT, true>(x[i].y, scale));
+        *reinterpret_cast<uint4*>(to + l + i * stride) = x[i];
+      }
+  });
+}
+
+template <int DT, bool kEight>
+__global__ __launch_bounds__(kThreads) void paged_read_kernel(CacheArgs a) {
+  Place p;
+  if (!find_place<false>(a, p)) return;
+  if (p.values) read_rows<DT, kEight>(a.side[1], p);
+  if (p.keys) read_rows<DT, kEight>(a.side[0], p);
 }
 
 // lanes to a row: as few as take it in one piece each, 16 at the least
@@ -185,13 +222,21 @@ void split_row(Side& s) {
   s.lanes = 16, s.lanes_log2 = 4;
   while (s.lanes < kWave && s.lanes * 8 < s.pool.width) s.lanes *= 2, ++s.lanes_log2;
 }
-int64_t groups_of(const Side& s, int64_t rows, int64_t heads) {
-  const int64_t per_group = static_cast<int64_t>(kWaves) * (kWave / s.lanes);
-  return (rows * heads + per_group - 1) / per_group;
+// all heads of a token to a wave where that leaves waves enough (sixteen to a CU), fewer where it does not
+void split_heads(CacheArgs& a) {
+  constexpr int64_t kEnough = 256 * 16;
+  a.shares = static_cast<int32_t>(std::clamp<int64_t>(kEnough / a.rows, 1, a.heads));
+  a.at_once = (a.heads + a.shares - 1) / a.shares;
+  a.shares = (a.heads + a.at_once - 1) / a.at_once;
+  a.apart = static_cast<int64_t>(a.rows) * a.shares < kEnough;
 }
 
 template <typename K>
-int launch(K kernel, const CacheArgs& a, int64_t groups, void* stream) {
+int launch(K kernel, CacheArgs& a, const char* who, void* stream) {
+  split_row(a.side[0]), split_row(a.side[1]);
+  split_heads(a);
+  const int64_t groups = ((static_cast<int64_t>(a.rows) * a.shares << a.apart) + kWaves - 1) / kWaves;
+  MEGA_CHECK_ARG(groups <= 0x7fffffff, "%s: too many rows for one launch", who);
   kernel<<<dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, static_cast<hipStream_t>(stream)>>>(a);
   MEGA_CHECK_LAUNCH();
   return MEGA_OK;
@@ -255,16 +300,12 @@ extern "C" int mega_paged_cache_write(const mega_paged_cache* cache, int dtype, 
                  "mega_paged_cache_write: new rows must be 16-byte aligned");
   CacheArgs a{paged_view(cache), {{paged_pool(cache, false), const_cast<void*>(k_new), k_row, k_head, 0, 0},
                                   {paged_pool(cache, true), const_cast<void*>(v_new), v_row, v_head, 0, 0}},
-              lengths, cu, static_cast<int32_t>(rows), static_cast<int32_t>(cache->heads), 0, 0};
-  split_row(a.side[0]), split_row(a.side[1]);
-  const int64_t kg = groups_of(a.side[0], rows, cache->heads), vg = groups_of(a.side[1], rows, cache->heads);
-  MEGA_CHECK_ARG(kg + vg <= 0x7fffffff, "mega_paged_cache_write: too many rows for one launch");
-  a.key_groups = static_cast<uint32_t>(kg);
+              lengths, cu, static_cast<int32_t>(rows), static_cast<int32_t>(cache->heads), 0, 0, 0, 0};
   const bool eight = cache->k_exponents != nullptr;
   if (dtype == MEGA_BF16)
-    return eight ? launch(paged_write_kernel<MEGA_BF16, true>, a, kg + vg, stream) : launch(paged_write_kernel<MEGA_BF16, false>, a, kg + vg, stream);
+    return eight ? launch(paged_write_kernel<MEGA_BF16, true>, a, "mega_paged_cache_write", stream) : launch(paged_write_kernel<MEGA_BF16, false>, a, "mega_paged_cache_write", stream);
   // (a copy does not look at its elements: one kernel for both types)
-  return eight ? launch(paged_write_kernel<MEGA_F16, true>, a, kg + vg, stream) : launch(paged_write_kernel<MEGA_BF16, false>, a, kg + vg, stream);
+  return eight ? launch(paged_write_kernel<MEGA_F16, true>, a, "mega_paged_cache_write", stream) : launch(paged_write_kernel<MEGA_BF16, false>, a, "mega_paged_cache_write", stream);
 }
 
 extern "C" int mega_paged_cache_read(const mega_paged_cache* cache, int dtype, const int32_t* begins, const int32_t* cu, int64_t rows,
@@ -278,13 +319,9 @@ extern "C" int mega_paged_cache_read(const mega_paged_cache* cache, int dtype, c
   const int64_t H = cache->heads;
   CacheArgs a{paged_view(cache), {{paged_pool(cache, false), k_out, H * cache->k_width, cache->k_width, 0, 0},
                                   {paged_pool(cache, true), v_out, H * cache->v_width, cache->v_width, 0, 0}},
-              begins, cu, static_cast<int32_t>(rows), static_cast<int32_t>(H), 0, clear_rest != 0};
-  split_row(a.side[0]), split_row(a.side[1]);
-  const int64_t kg = groups_of(a.side[0], rows, H), vg = groups_of(a.side[1], rows, H);
-  MEGA_CHECK_ARG(kg + vg <= 0x7fffffff, "mega_paged_cache_read: too many rows for one launch");
-  a.key_groups = static_cast<uint32_t>(kg);
+              begins, cu, static_cast<int32_t>(rows), static_cast<int32_t>(H), 0, 0, 0, clear_rest != 0};
   const bool eight = cache->k_exponents != nullptr;
   if (dtype == MEGA_BF16)
-    return eight ? launch(paged_read_kernel<MEGA_BF16, true>, a, kg + vg, stream) : launch(paged_read_kernel<MEGA_BF16, false>, a, kg + vg, stream);
-  return eight ? launch(paged_read_kernel<MEGA_F16, true>, a, kg + vg, stream) : launch(paged_read_kernel<MEGA_BF16, false>, a, kg + vg, stream);
+    return eight ? launch(paged_read_kernel<MEGA_BF16, true>, a, "mega_paged_cache_read", stream) : launch(paged_read_kernel<MEGA_BF16, false>, a, "mega_paged_cache_read", stream);
+  return eight ? launch(paged_read_kernel<MEGA_F16, true>, a, "mega_paged_cache_read", stream) : launch(paged_read_kernel<MEGA_BF16, false>, a, "mega_paged_cache_read", stream);
 }
