@@ -50,6 +50,41 @@ struct Values {
 // of a run are there 2 us later.
 constexpr bool staged(bool eight, int rt, int ks) { return 8 * 32 * ks * (eight ? 32 : 64) + rt * (ks + 8) * 1024 <= 156 * 1024; }
 
+// A wave's accumulators to out or to the workspace.  Accumulator element i of column operand j is column kCols (4 h + i) + j of its group of
+// 16 kCols; eight columns are stored at a time.
+template <int DT, int RT, int CT, int kCols>
+__device__ __forceinline__ void store_piece(const AttnArgs& a, const Block& k, const Destination& to, int head, bool notes, int first_column,
+                                            const f32x4 (&acc)[RT][CT], const float (&m)[RT], const float (&l)[RT]) {
+  const int lane = opaque(static_cast<int>(threadIdx.x) & 63), n = lane & 15, h = lane >> 4;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int row = rt * 16 + n;
+    if (row >= k.count) continue;
+    const int64_t at = place_of_row(a, k, to, head, row, notes && h == 0, m[rt], l[rt]);
+    const float inverse = l[rt] == 0.f ? 0.f : 1.f / l[rt];
+#pragma unroll
+    for (int cg = 0; cg < CT / kCols; ++cg)
+#pragma unroll
+      for (int i = 0; i < 4; i += 8 / kCols) {
+        const int c = first_column + 16 * kCols * cg + kCols * (4 * h + i);
+        if (c >= a.v.width) continue;
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = acc[rt][kCols * cg + j % kCols][i + j / kCols];
+        if (!to.alone) {
+          float4* part = reinterpret_cast<float4*>(a.part + (to.slot + row) * a.v.width + c);
+          part[0] = make_float4(o[0], o[1], o[2], o[3]);
+          part[1] = make_float4(o[4], o[5], o[6], o[7]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = l[rt] == 0.f ? 0.f : o[j] * inverse;
+          *reinterpret_cast<uint4*>(a.out + at * a.v.width + c) =
+              make_uint4(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]), pack2<DT>(o[4], o[5]), pack2<DT>(o[6], o[7]));
+        }
+      }
+  }
+}
+
 template <int DT, bool kEight, int RT, int CT, int KS>  // KS: 32-wide steps of a key row
 __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnArgs a) {
   // 16-byte loads of values where the registers allow it: eight of a lane's columns at a time, else four
@@ -400,14 +435,12 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
       }
 
       // ---- probabilities, in the operand order of the second product
-      // (m follows the maximum when that is 2^8 above it, not at each step: the factor leaves p, l and o alike, and a probability
-      // of up to 2^8 is as exact as one of up to 1)
       bool moved = false;
       float alpha[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float now = top[rt] > m[rt] + 8.f ? top[rt] : m[rt], base = now == -__builtin_inff() ? 0.f : now;
-        alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - base);
+        const float now = top[rt] > m[rt] + kSlack ? top[rt] : m[rt], held = now == -__builtin_inff() ? 0.f : now, base = held - kLift<DT>;
+        alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - held);
         moved = moved || now != m[rt];
         m[rt] = now;
         float p[8], sum = 0.f;
@@ -447,7 +480,9 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) l[rt] = sum_of_waves(lds_m + (rt * 16 + n) * 8, waves);
     }
-    if (store_piece<DT, RT, CT, kCols>(a, k, static_cast<int>(id), head, slab, wave, first_column, progress, acc, m, l)) break;
+    const Destination to = destination_of(a, progress, static_cast<int>(id), head);
+    if (to.fits) store_piece<DT, RT, CT, kCols>(a, k, to, head, slab == 0 && wave == 0, first_column, acc, m, l);
+    if (to.last) break;
     at = next_piece<kRows>(a, progress, k);
     __syncthreads();  // (the rows, maxima, probabilities and progress of this piece have been read)
   }
@@ -464,6 +499,8 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(AttnArgs a, in
   const int64_t q_heads = a.heads * a.shared, all = a.clear_rest ? a.rows : row_bound(a.cu, a.view.batch, a.rows);
   if (row >= all * q_heads) return;
   const int2 join = a.joins[row];
+  // (a row of no sequence, cu does not begin with zero, has none)
+  if (join.x < 0 || join.y <= 0 || join.x + (join.y - 1) * static_cast<int64_t>(a.part_rows) >= static_cast<int64_t>(a.heads) * a.slots * a.part_rows) return;
   const int c = static_cast<int>(item - row * strips) * lanes * 8 + (lane & (lanes - 1)) * 8;
   const bool column = c < a.v.width;
   float m = -__builtin_inff(), l = 0.f, o[8] = {};
@@ -481,7 +518,6 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(AttnArgs a, in
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[j] = o[j] * before + v[j] * with;
   }
-  if (join.y <= 0) return;
   float now = m;
   for (int off = lanes; off < 64; off <<= 1) now = fmaxf(now, across(now, off));
   const float with = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.f : now));

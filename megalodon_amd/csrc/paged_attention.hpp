@@ -9,6 +9,12 @@ namespace mega {
 constexpr int kMaxWaves = 8;
 constexpr int kMaxKeyWidth = 512;
 constexpr int kCus = 256;
+// A row's m stays until a score is more than 2^kSlack times above it: probabilities up to 2^kSlack are as exact as those up to 1, and the
+// factor leaves p, l and o alike.  In float16 they are lifted further, to 2^15 at the most: below 2^-14 its numbers thin out, and many
+// small probabilities of a long sequence weigh as much as a large one.
+constexpr float kSlack = 8.f;
+template <int DT>
+constexpr float kLift = DT == MEGA_F16 ? 7.f : 0.f;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -349,7 +355,7 @@ __device__ __forceinline__ Progress next_piece(const AttnArgs& a, const Progress
   Sequence s = sequence_of<true>(a, at.mark.sequence);
   if (at.mark.number == at.mark.blocks) {
     do s = sequence_of<true>(a, ++at.mark.sequence);
-    while (s.count == 0);
+    while (s.count == 0 && at.mark.sequence + 1 < sequences_of(a));
     at.mark.blocks = blocks_of<kRows>(a, s), at.mark.number = 0;
   }
   block_of<kRows>(a, s, at.mark.sequence, at.mark.number, k);
@@ -397,53 +403,29 @@ __device__ __forceinline__ float sum_of_waves(const float* p, int waves) {
   return sum;
 }
 
-// A wave's accumulators to out, or with the rows' m and l to the workspace; true: this was the workgroup's last piece.
-// Accumulator element i of column operand j is column kCols (4 h + i) + j of its group of 16 kCols; eight columns are stored at a time.
-template <int DT, int RT, int CT, int kCols>
-__device__ __forceinline__ bool store_piece(const AttnArgs& a, const Block& k, int id, int head, int slab, int wave, int first_column, const Progress& progress,
-                                            const f32x4 (&acc)[RT][CT], const float (&m)[RT], const float (&l)[RT]) {
-  const int lane = opaque(static_cast<int>(threadIdx.x) & 63), n = lane & 15, h = lane >> 4;
-  bool alone = true, last = true;
-  int64_t slot = 0;
-  int pieces = 0;
-  if (a.parts > 0) {
-    slot = (static_cast<int64_t>(head) * a.slots + id + progress.mark.blocks_before) * a.part_rows;
-    alone = progress.alone, pieces = progress.pieces, last = progress.unit + a.lead >= progress.unit_end;
+// Where a piece's results go.
+struct Destination {
+  bool alone, last;  // to out, the block is this workgroup's; this was its last piece
+  bool fits;
+  int32_t pieces;
+  int64_t slot;      // else: its first row in the workspace
+};
+__device__ __forceinline__ Destination destination_of(const AttnArgs& a, const Progress& progress, int id, int head) {
+  if (a.parts == 0) return {true, true, true, 0, 0};
+  const int number = id + progress.mark.blocks_before;  // (more blocks than there are rows for: cu decreases somewhere)
+  return {progress.alone, progress.unit + a.lead >= progress.unit_end, number < a.slots, progress.pieces,
+          (static_cast<int64_t>(head) * a.slots + number) * a.part_rows};
+}
+// A row's number in out and, with `note`, its m and l to the workspace and the number of its pieces.
+__device__ __forceinline__ int64_t place_of_row(const AttnArgs& a, const Block& k, const Destination& to, int head, int row, bool note, float m, float l) {
+  const int r = k.row0 + row, t = token_of(a, r), g = r - t * a.shared;
+  const int64_t at = (static_cast<int64_t>(k.start) + t) * (a.heads * a.shared) + head * a.shared + g;
+  if (note && a.parts > 0 && row < k.count) {
+    if (!to.alone) *reinterpret_cast<float2*>(a.stats + (to.slot + row) * 2) = make_float2(m, l);
+    // (places are 32-bit numbers: the host sees to that)
+    if (to.pieces > 0) a.joins[at] = make_int2(static_cast<int>(to.slot + row), to.alone ? 0 : to.pieces);
   }
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int row = rt * 16 + n;
-    if (row >= k.count) continue;
-    const int r = k.row0 + row, t = token_of(a, r), g = r - t * a.shared;
-    const int64_t at = (static_cast<int64_t>(k.start) + t) * (a.heads * a.shared) + head * a.shared + g;
-    const float inverse = l[rt] == 0.f ? 0.f : 1.f / l[rt];
-    if (a.parts > 0 && slab == 0 && wave == 0 && h == 0) {
-      if (!alone) *reinterpret_cast<float2*>(a.stats + (slot + row) * 2) = make_float2(m[rt], l[rt]);
-      // (places are 32-bit numbers: the host sees to that)
-      if (pieces > 0) a.joins[at] = make_int2(static_cast<int>(slot + row), alone ? 0 : pieces);
-    }
-#pragma unroll
-    for (int cg = 0; cg < CT / kCols; ++cg)
-#pragma unroll
-      for (int i = 0; i < 4; i += 8 / kCols) {
-        const int c = first_column + 16 * kCols * cg + kCols * (4 * h + i);
-        if (c >= a.v.width) continue;
-        float o[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = acc[rt][kCols * cg + j % kCols][i + j / kCols];
-        if (!alone) {
-          float4* to = reinterpret_cast<float4*>(a.part + (slot + row) * a.v.width + c);
-          to[0] = make_float4(o[0], o[1], o[2], o[3]);
-          to[1] = make_float4(o[4], o[5], o[6], o[7]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = l[rt] == 0.f ? 0.f : o[j] * inverse;
-          *reinterpret_cast<uint4*>(a.out + at * a.v.width + c) =
-              make_uint4(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]), pack2<DT>(o[4], o[5]), pack2<DT>(o[6], o[7]));
-        }
-      }
-  }
-  return last;
+  return at;
 }
 
 // Blocks of more than 32 rows (paged_attention_rows.hip).

@@ -20,6 +20,54 @@ constexpr int kRows = 16 * RT, kMostWaves = 8;
 // of a key's 16-byte parts to a lane, those that come through LDS: all, or as many as it has room for beside the rows and the probabilities
 constexpr int in_lds(bool solo, int parts) { return solo ? 0 : parts < 5 ? parts : 5; }
 
+// A wave's accumulators to out, or to the workspace: there sixteen rows at a time through the wave's own LDS (free behind the last keys), as an
+// instruction would write 16 bytes of 64 lines from the registers -- 512 tokens behind 1531: 25 us more.  Out has half the bytes,
+// and one write of them for many keys: a prompt takes the same time either way.
+constexpr int kTurned = 16 * CT + 4;  // floats of a row there: sixteen rows' equal columns are in different banks
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+template <int DT>
+__device__ __forceinline__ void store_piece(const AttnArgs& a, const Block& k, const Destination& to, int head, bool notes, int first_column, float* turned,
+                                            const f32x4 (&acc)[RT][CT], const float (&m)[RT], const float (&l)[RT]) {
+  const int lane = opaque(static_cast<int>(threadIdx.x) & 63), n = lane & 15, h = lane >> 4;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int64_t at = place_of_row(a, k, to, head, rt * 16 + n, notes && h == 0, m[rt], l[rt]);
+    if (to.alone) {
+      if (rt * 16 + n >= k.count) continue;
+      const float inverse = l[rt] == 0.f ? 0.f : 1.f / l[rt];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = first_column + CT * (4 * h + i);
+        if (c >= a.v.width) continue;
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = l[rt] == 0.f ? 0.f : acc[rt][j][i] * inverse;
+        *reinterpret_cast<uint4*>(a.out + at * a.v.width + c) =
+            make_uint4(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]), pack2<DT>(o[4], o[5]), pack2<DT>(o[6], o[7]));
+      }
+    } else {
+      wave_lds_fence();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; j += 4)
+          *reinterpret_cast<float4*>(turned + n * kTurned + CT * (4 * h + i) + j) = make_float4(acc[rt][j][i], acc[rt][j + 1][i], acc[rt][j + 2][i], acc[rt][j + 3][i]);
+      wave_lds_fence();
+      const int c = (lane & 31) * 4, row = rt * 16 + (lane >> 5);
+      float* const part = a.part + (to.slot + row) * a.v.width + first_column + c;
+      if (first_column + c < a.v.width)
+#pragma unroll
+        for (int pair = 0; pair < 16; pair += 2)
+          if (row + pair < k.count)
+            *reinterpret_cast<float4*>(part + static_cast<int64_t>(pair) * a.v.width) = *reinterpret_cast<const float4*>(turned + (pair + (lane >> 5)) * kTurned + c);
+    }
+  }
+}
+
 // KS: 32-wide steps of a key row; kFull: it has 32 KS elements; kSolo: a workgroup is one wave
 template <int DT, bool kEight, int KS, bool kFull, bool kSolo>
 __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_rows_kernel(AttnArgs a) {
@@ -261,8 +309,8 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
       float alpha[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float seen = top[rt] * a.scale, now = seen > m[rt] + 8.f ? seen : m[rt], base = now == -__builtin_inff() ? 0.f : now;
-        alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - base);
+        const float seen = top[rt] * a.scale, now = seen > m[rt] + kSlack ? seen : m[rt], held = now == -__builtin_inff() ? 0.f : now, base = held - kLift<DT>;
+        alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - held);
         moved = moved || now != m[rt];
         m[rt] = now;
         float p[8], sum = 0.f;
@@ -283,6 +331,9 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
       if constexpr (!kSolo) __syncthreads();
 
       // ---- values: 32 keys a step
+      // (kSolo: in front of the other wave, whose scores and exponentials fill the gaps; the older of two equals has them all, and the younger ends
+      // alone -- four pieces of prompts on shared heads: 300 us without)
+      if constexpr (kSolo) __builtin_amdgcn_s_setprio(1);
       const int steps = kSolo ? 1 : min(waves, (end - tile + 31) >> 5);
 #pragma unroll 1
       for (int step = 0; step < steps; ++step) {
@@ -389,6 +440,7 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
         }
         there[0] = next.there[0], there[1] = next.there[1];
       }
+      if constexpr (kSolo) __builtin_amdgcn_s_setprio(0);
     }
 
     // ---- the rows' sums over the lanes and waves that had their keys
@@ -404,7 +456,9 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) l[rt] = sum_of_waves(lds_m + (rt * 16 + n) * kMostWaves, waves);
     }
-    if (store_piece<DT, RT, CT, 8>(a, k, static_cast<int>(id), head, slab, wave, first_column, progress, acc, m, l)) break;
+    const Destination to = destination_of(a, progress, static_cast<int>(id), head);
+    if (to.fits) store_piece<DT>(a, k, to, head, slab == 0 && wave == 0, first_column, reinterpret_cast<float*>(lds) + wave * 16 * kTurned, acc, m, l);
+    if (to.last) break;
     at = next_piece<kRows>(a, progress, k);
     __syncthreads();  // (the rows, maxima, probabilities and progress of this piece have been read)
   }

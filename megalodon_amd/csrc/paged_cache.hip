@@ -253,8 +253,8 @@ int check_paged_cache(const mega_paged_cache* c, int dtype, const char* who) {
   MEGA_CHECK_ARG(c->page_size >= kMinPage && c->page_size <= kMaxPage && (c->page_size & (c->page_size - 1)) == 0,
                  "%s: page_size must be a power of two, 16 .. 65536", who);
   MEGA_CHECK_ARG(c->pages >= 1 && c->pages <= 0x7fffffff, "%s: bad number of pages", who);
-  MEGA_CHECK_ARG(c->table_width >= 0 && c->table_width * c->page_size <= 0x7fffffff && c->table_stride >= 0,
-                 "%s: a row of the table holds up to 2^31 - 1 positions", who);
+  MEGA_CHECK_ARG(c->table_width >= 0 && c->table_width * c->page_size <= 0x40000000 && c->table_stride >= 0,
+                 "%s: a row of the table holds up to 2^30 positions", who);
   for (const int64_t w : {c->k_width, c->v_width})
     MEGA_CHECK_ARG(w >= 16 && w <= kMaxCacheWidth && w % 16 == 0, "%s: widths must be multiples of 16, 16 .. 4096", who);
   MEGA_CHECK_ARG(c->k != nullptr && c->v != nullptr && (c->table != nullptr || c->batch == 0 || c->table_width == 0), "%s: null pointer", who);
