@@ -865,7 +865,8 @@ int mega_block_decode(const mega_block_decode_args* args, void* stream);
  * Strides are in elements (of the pool's type; bytes for the exponents), the
  * last axis is contiguous.  page_size is a power of two, 16 .. 65536; widths are
  * multiples of 16, at most 4096 (k_width of an attention call: 512); pools are
- * 16-byte aligned and their strides multiples of 16 elements.
+ * 16-byte aligned and their strides multiples of 16 elements; table_width *
+ * page_size is at most 2^30.
  *
  * Metadata lies on the device and is not checked by the host.  Every kernel
  * stays inside the pool and the table whatever it says: a table entry that names
@@ -910,8 +911,10 @@ int mega_paged_cache_read(const mega_paged_cache* cache, int dtype, const int32_
  * q_heads is a multiple of the cache's heads; query head h reads head
  * h / (q_heads / heads).  A row that sees nothing, or whose scores are all -inf,
  * becomes zeros.  What a row does not see cannot reach it, NaN and infinities
- * included.  float32 scores, softmax and sums; probabilities are rounded to
- * dtype for the matrix cores.
+ * included.  float32 scores, softmax and sums; probabilities, and the numbers
+ * that 8-bit codes and exponents stand for, are rounded to dtype for the matrix
+ * cores (the latter as mega_paged_cache_read does; float16 holds no number
+ * above 65504, so that rows written from bfloat16 are best read in it).
  * out (rows, q_heads, v_width) contiguous; clear_rest as above.  workspace:
  * mega_paged_attention_workspace_bytes(...) bytes (0: none is needed), used by
  * this call alone while it runs. */

@@ -497,9 +497,9 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(AttnArgs a, in
   const int lane = static_cast<int>(threadIdx.x) & 63, lanes = 1 << lanes_log2, groups = 64 >> lanes_log2;
   const uint32_t item = blockIdx.x * (kJoinThreads / kWave) + (threadIdx.x >> 6), row = item / strips;
   const int64_t q_heads = a.heads * a.shared, all = a.clear_rest ? a.rows : row_bound(a.cu, a.view.batch, a.rows);
-  if (row >= all * q_heads) return;
+  if (row >= all * q_heads || row < row_bound(a.cu, 0, a.rows) * q_heads) return;
   const int2 join = a.joins[row];
-  // (a row of no sequence, cu does not begin with zero, has none)
+  // (nor has every row one where cu decreases)
   if (join.x < 0 || join.y <= 0 || join.x + (join.y - 1) * static_cast<int64_t>(a.part_rows) >= static_cast<int64_t>(a.heads) * a.slots * a.part_rows) return;
   const int c = static_cast<int>(item - row * strips) * lanes * 8 + (lane & (lanes - 1)) * 8;
   const bool column = c < a.v.width;

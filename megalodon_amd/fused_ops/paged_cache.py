@@ -15,7 +15,8 @@ has one length for a whole batch.  Here sequences of any lengths share pools of 
 * ``lengths`` (sequences) int32: positions of each sequence, its new ones included, so that new row i of n is
   position lengths[b] - n + i.
 
-page_size is a power of two from 16 on; widths are multiples of 16, up to 4096 (keys under attention: 512).
+page_size is a power of two from 16 on; widths are multiples of 16, up to 4096 (keys under attention: 512);
+a row of block_table holds up to 2 ** 30 positions.
 All metadata stays on the device: the calls do not synchronise and may be captured into a graph whose
 replays follow new lengths and tables.  Pages may belong to several sequences as long as only one writes.
 Inference only: a gradient that is asked for raises."""
@@ -52,6 +53,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Te
 
     The token at position p sees positions from the start of its chunk of `chunk_size` (0: from the first) to p; its own key
     and value have been written before.  The number of query heads is a multiple of the cache's: h reads head
-    h // (query heads // heads).  A token that sees no key, or whose scores are all -inf, gets zeros.  Returns
+    h // (query heads // heads).  A token that sees no key, or whose scores are all -inf, gets zeros.  What 8-bit rows stand
+    for is rounded to q's dtype as paged_cache_read does.  Returns
     (rows, query heads, v_width): rows behind the last sequence are zeros, or left as they are in a given `out`."""
     return _lib.host().paged_attention(q, k_pages, v_pages, block_table, lengths, cu_new, scale, chunk_size, k_exponents, v_exponents, out)

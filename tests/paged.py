@@ -86,8 +86,8 @@ class Batch:
             out.append(x if e is None else x * powers(e[page, slot])[..., None])
         return out
 
-    def attention(self, scale, chunk):
-        """(out, bound): float64, and what 16-bit probabilities and results and 32-bit arithmetic may be off by.
+    def attention(self, scale, chunk, heads=None):
+        """(out, bound) of the query heads in `heads` (None: all): float64, and what 16-bit probabilities and results and 32-bit arithmetic may be off by.
 
         With u half a step of the type, A = sum_j p_j |v_j|, N keys of width W: rounding the result costs u |o|, rounding
         the probabilities u A (below float16's normal numbers 2^-25 sum |v| instead), the float32 sums (N + 8) 2^-23 A.
@@ -104,7 +104,7 @@ class Batch:
             for t in range(n):
                 p = self.olds[b] + t
                 low = p // chunk * chunk if chunk else 0
-                for g in range(self.heads * self.shared):
+                for g in heads or range(self.heads * self.shared):
                     kh, vh, q = k[low:p + 1, g // self.shared], v[low:p + 1, g // self.shared], self.q[self.cu[b] + t, g].double()
                     w = torch.softmax(kh @ q * scale, 0)
                     o, A = w @ vh, w @ vh.abs()

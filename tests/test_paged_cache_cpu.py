@@ -93,6 +93,12 @@ def test_calls_of_nothing_launch_nothing():
     assert attend(cache(), rows=0) == 0 and write(cache(), rows=0) == 0 and read(cache(), rows=0) == 0 and write(cache(batch=0)) == 0
 
 
+def test_a_table_row_holds_up_to_two_to_the_30_positions():
+    c = cache(table_width=(1 << 26) + 1)
+    assert attend(c) == 1 and b"2^30" in _lib.load().mega_last_error()
+    assert write(c) == 1 and read(c) == 1
+
+
 def test_questions_leave_the_last_error():
     lib = _lib.load()
     assert attend(cache(), dtype=7) == 1
