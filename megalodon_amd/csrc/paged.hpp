@@ -44,6 +44,12 @@ __device__ __forceinline__ int row_bound(const int32_t* cu, int i, int rows) { r
 
 // 2^(e - 127) of an exponent byte 1 .. 254
 __device__ __forceinline__ float exponent_value(uint32_t e) { return __uint_as_float(e << 23); }
+// two e4m3 codes of a word's lower or upper half times a power of two, as 16-bit numbers
+template <int DT, bool kUpper>
+__device__ __forceinline__ uint32_t widen(uint32_t codes, float scale) {
+  if constexpr (DT == MEGA_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, kUpper));
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, kUpper));
+}
 
 // The host's half: MEGA_OK, or the error with its message.
 int check_paged_cache(const mega_paged_cache* c, int dtype, const char* who);

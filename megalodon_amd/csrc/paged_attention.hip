@@ -4,14 +4,14 @@
 //   s_j = scale q . k_j,  m = max_j s_j,  l = sum_j e^(s_j - m),  o = sum_j e^(s_j - m) v_j / l,
 // in one pass over the keys with the running m and l; accumulators follow a rising m by the factor
 // e^(m_old - m_new).  Scores, m, l and o are float32; the probabilities that go into the second product are
-// rounded to the operands' type, which is what the matrix cores take (each is off by 2^-9 or 2^-12 of itself at most,
-// below the rounding of the result); l sums them unrounded.
+// rounded to the operands' type, which is what the matrix cores take (each is off by 2^-8 or 2^-11 of itself at most,
+// as the result is by its own rounding); l sums them unrounded.
 //
 // Layout.  A workgroup has kRows = 16 RT rows (new tokens of one sequence, and the query heads that share a key /
 // value head, side by side) of one cache head, and W waves; wave w has 16 CT of its value columns.  A tile is
 // 32 W keys:
-//   scores   wave w takes 32 of them, all rows: S^T = K Q^T with K straight from the pool into registers (its rows
-//            are the instruction's k-contiguous operand) and Q from LDS in operand order;
+//   scores   wave w takes 32 of them, all rows: S^T = K Q^T with K by whole rows through the wave's own LDS (rows too wide for that: in
+//            operand order into registers, as keys are the instruction's k-contiguous operand) and Q from LDS in operand order;
 //   softmax  a row's keys lie in four lanes of a wave and in W waves: maxima meet in LDS, P^T goes there;
 //   values   every wave takes all 32 W keys for its own columns: O^T = V^T P^T.  No value is read twice in a
 //            workgroup, so values pass through registers only: a lane reads eight columns of eight keys, and a byte
@@ -20,13 +20,19 @@
 // leaves the first product in the very registers that the second one takes: which of the 32 keys sits in which k slot is
 // free as long as V agrees, and slot (8 h + i) is key 4 h + i of the first 16 for i < 4, of the second 16 above.
 //
-// A page holds 16 keys at least, and key groups are aligned, so a lane group's keys share a page: its base is a scalar.
+// A page holds 16 keys at least, and key groups are aligned, so a lane group's keys share a page: its base is a scalar, its number a
+// load of the scalar unit (a vector load would be waited for in turn with the keys and values in flight).
 //
-// Few row blocks (single tokens, drafts, one prompt's piece): bound by the cache's bytes.  The blocks' keys, in units of 32,
-// form one line, block after block, which is cut into as many equal parts as workgroups fill the chip, whatever
-// the sequences' lengths: a workgroup goes through the pieces of blocks that its part holds, leaves each one's (o, m, l)
-// in a workspace in float32, and a second kernel joins them.  Many row blocks: a workgroup each, bound by the
-// matrix cores and by what L2 gives for the operands.
+// Few row blocks (single tokens, drafts, a prompt's piece).  The blocks' keys, in units of 32, form one line, block after block, which is
+// cut into as many equal parts as workgroups fill the chip, whatever the sequences' lengths: a workgroup goes through the
+// pieces of blocks that its part holds, leaves each one's (o, m, l) in a workspace in float32, and a second kernel joins them.
+// Many row blocks: a workgroup each.
+//
+// This file: up to 32 rows of a sequence on average.  Bound by the cache's bytes: 32 tokens on shared heads over 16-bit caches of up to 16000
+// positions, 205 us, 5.3 TB/s (a large read reaches 6.0); sixteen tokens over 8-bit ones of up to 4000, 80 us, 4.7 TB/s; drafts of eight
+// sequences, 76 us, 4.2 TB/s.  Short of that by what comes before the first and behind the last key of a workgroup, some 8 us: chains of
+// dependent loads (bounds, lengths, page numbers, keys; 4 us), the results' way out, the join (4 us); one token over 1531 positions
+// takes 21 us, of them 5 on the cache.  A third wave on a SIMD for narrow heads: 229 us against 205, the registers of the values in flight.
 #include "paged_attention.hpp"
 
 #include <algorithm>
@@ -489,13 +495,14 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
 }
 
 // Joins the pieces of the blocks that several workgroups had: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i with
-// m = max_i m_i.  A group of 2^lanes_log2 lanes, eight columns each, takes every n-th piece of a row, n groups to a wave, in the
-// pieces' order; the groups meet through the lanes.  Bound by the latency of three dependent loads where there are few rows, by the pieces' bytes else.
+// m = max_i m_i.  2^span_log2 lanes have a row: a group of 2^lanes_log2 of them, eight columns each, takes every n-th piece, n groups, in the
+// pieces' order; the groups meet through the lanes.  Bound by the latency of three dependent loads where there are few rows (4 us), by the pieces' bytes
+// else (100 MB read, 18 written: 21 us, 5.6 TB/s).
 constexpr int kJoinThreads = 256;
 template <int DT>
-__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(AttnArgs a, int lanes_log2, uint32_t strips) {
-  const int lane = static_cast<int>(threadIdx.x) & 63, lanes = 1 << lanes_log2, groups = 64 >> lanes_log2;
-  const uint32_t item = blockIdx.x * (kJoinThreads / kWave) + (threadIdx.x >> 6), row = item / strips;
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(AttnArgs a, int lanes_log2, int span_log2, uint32_t strips) {
+  const int span = 1 << span_log2, lane = static_cast<int>(threadIdx.x) & (span - 1), lanes = 1 << lanes_log2, groups = span >> lanes_log2;
+  const uint32_t item = blockIdx.x * (kJoinThreads >> span_log2) + (threadIdx.x >> span_log2), row = item / strips;
   const int64_t q_heads = a.heads * a.shared, all = a.clear_rest ? a.rows : row_bound(a.cu, a.view.batch, a.rows);
   if (row >= all * q_heads || row < row_bound(a.cu, 0, a.rows) * q_heads) return;
   const int2 join = a.joins[row];
@@ -519,12 +526,12 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(AttnArgs a, in
     for (int j = 0; j < 8; ++j) o[j] = o[j] * before + v[j] * with;
   }
   float now = m;
-  for (int off = lanes; off < 64; off <<= 1) now = fmaxf(now, across(now, off));
+  for (int off = lanes; off < span; off <<= 1) now = fmaxf(now, across(now, off));
   const float with = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.f : now));
   l *= with;
 #pragma unroll
   for (int j = 0; j < 8; ++j) o[j] *= with;
-  for (int off = lanes; off < 64; off <<= 1) {
+  for (int off = lanes; off < span; off <<= 1) {
     l += across(l, off);
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[j] += across(o[j], off);
@@ -541,7 +548,7 @@ struct Plan {
   int rt, ct, ks, waves, slabs;
   int64_t blocks, parts;  // row blocks at most; parts of the line of units for each head and slab (0: a workgroup a block)
   int64_t slots, part_rows;
-  int join_lanes_log2;  // of the join: lanes to a row's strip
+  int join_lanes_log2, join_span_log2;  // of the join: lanes to a row's strip in a piece, in all pieces
   int64_t workgroups(int64_t heads) const { return (parts > 0 ? parts : blocks) * heads * slabs; }
 };
 
@@ -570,6 +577,9 @@ Plan plan_of(const mega_paged_cache* c, int64_t rows, int64_t q_heads) {
     const int64_t pieces = p.parts * pairs / std::max<int64_t>(full, 1);
     p.join_lanes_log2 = pieces > 8 ? 2 : pieces > 4 ? 3 : pieces > 2 ? 4 : 5;
     while (p.join_lanes_log2 > 1 && (8 << (p.join_lanes_log2 - 1)) >= c->v_width) --p.join_lanes_log2;
+    // (lanes for no more pieces than twice that, the rest have other rows: 1.6 pieces of 128 columns, 28 us with a wave a row)
+    p.join_span_log2 = p.join_lanes_log2;
+    while (p.join_span_log2 < 6 && (int64_t{1} << (p.join_span_log2 - p.join_lanes_log2)) < 2 * pieces) ++p.join_span_log2;
   }
   return p;
 }
@@ -607,9 +617,10 @@ int launch_attn(const AttnArgs& a, const Plan& p, bool eight, void* stream) {
   else
     rc = eight ? launch_width<DT, true>(a, p, stream) : launch_width<DT, false>(a, p, stream);
   if (rc != MEGA_OK || p.parts == 0) return rc;
-  const int64_t strip = 8 << p.join_lanes_log2, strips = (a.v.width + strip - 1) / strip, waves = static_cast<int64_t>(a.rows) * a.heads * a.shared * strips;
-  paged_join_kernel<DT><<<dim3(static_cast<uint32_t>((waves + kJoinThreads / kWave - 1) / (kJoinThreads / kWave))), dim3(kJoinThreads), 0,
-                          static_cast<hipStream_t>(stream)>>>(a, p.join_lanes_log2, static_cast<uint32_t>(strips));
+  const int64_t strip = 8 << p.join_lanes_log2, strips = (a.v.width + strip - 1) / strip, items = static_cast<int64_t>(a.rows) * a.heads * a.shared * strips;
+  const int64_t at_once = kJoinThreads >> p.join_span_log2;
+  paged_join_kernel<DT><<<dim3(static_cast<uint32_t>((items + at_once - 1) / at_once)), dim3(kJoinThreads), 0, static_cast<hipStream_t>(stream)>>>(
+      a, p.join_lanes_log2, p.join_span_log2, static_cast<uint32_t>(strips));
   MEGA_CHECK_LAUNCH();
   return MEGA_OK;
 }

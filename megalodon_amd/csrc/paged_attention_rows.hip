@@ -1,22 +1,25 @@
-// Paged attention for many rows of a sequence at a time: prompts and their pieces.
+// Paged attention for many rows of a sequence at a time (more than 32 on average): prompts and their pieces.
 //
-// The mathematics and the lane layout are those of paged_attention.hip; what differs is what bounds it.  With 64 rows a
-// value that has been read serves 64 rows, and the matrix cores are the limit to come near to, so the work of a wave is arranged
-// for them:
-//   - accumulators of 64 rows x 256 columns, the whole accumulation half of a SIMD's registers, one wave to a SIMD, four to a
-//     workgroup: nothing of another wave hides this one's waits, so everything it will need is on its way long before --
-//     the values of the next 32 keys, the keys of the next tile, the next step's probabilities;
-//   - a step's values are turned into operands two columns at a time, while the two columns before them are multiplied;
-//   - a wave's scores are those of 64 keys at a time, so a row operand from LDS serves four key operands.
-// Up to 128 value columns: one wave has all of them, eight workgroups of one wave share a CU (two to a SIMD: the softmax of one beside the
-// products of the other), and probabilities never leave the registers.
+// The mathematics and the lane layout are those of paged_attention.hip; what differs is what bounds it.  A value that has been read serves 64
+// rows; a wave has 64 rows x 128 columns of accumulators, half of its registers, and two waves share a SIMD: one's products beside the
+// other's scores and exponentials.
+//   - More than 128 value columns: up to eight waves with their columns and 32 keys of a tile each, as there.  A tile's keys are asked for a
+//     tile ahead, into LDS and in operand order, the next step's values while the last two columns of this one's are multiplied.
+//     Bound by what a CU is given of L2, 41 bytes a cycle: the values of 256 keys take 17000 cycles, their products 8200; the
+//     scores of the tile 2200, the softmax 1600, the waves' meeting at the maxima 5500.  A prompt of 8192 tokens in chunks of 4096, four heads of
+//     256 / 2048: 485 us, 640 TFLOP/s.  One wave to a SIMD with 64 x 256 spilled 1.5 KB a lane; four-wave workgroups of 64 x 512, whose
+//     scores are made twice: 549 us; two-wave ones: 910.  Blocks in other orders over the XCDs: 501, 673.
+//   - Up to 128: a workgroup is one wave, eight to a CU, and probabilities never leave the registers.  Bound by the issue of vector
+//     instructions (conversions, exponentials, maxima: 1750 cycles for 32 keys) beside 1000 of products: 255 to 1023 tokens behind up to
+//     7001 in 8 bits, 265 us, 650 TFLOP/s.  32 rows a wave: 589 us; its keys ahead in registers: 469 us (spills).
+// A piece leaves 64 rows in float32: 512 tokens behind 1531 write and read 67 MB beside a cache of 38, 58 us.
 #include "paged_attention.hpp"
 
 namespace mega {
 namespace {
 
 constexpr int RT = 4, CT = 8;                        // row and column tiles of a wave
-constexpr int kRows = 16 * RT, kMostWaves = 8;
+constexpr int kRows = 16 * RT;
 // of a key's 16-byte parts to a lane, those that come through LDS: all, or as many as it has room for beside the rows and the probabilities
 constexpr int in_lds(bool solo, int parts) { return solo ? 0 : parts < 5 ? parts : 5; }
 
@@ -70,7 +73,7 @@ __device__ __forceinline__ void store_piece(const AttnArgs& a, const Block& k, c
 
 // KS: 32-wide steps of a key row; kFull: it has 32 KS elements; kSolo: a workgroup is one wave
 template <int DT, bool kEight, int KS, bool kFull, bool kSolo>
-__global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_rows_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_rows_kernel(AttnArgs a) {
   constexpr int kBytes = kEight ? 1 : 2, kParts = kEight ? KS / 2 : KS, kInLds = in_lds(kSolo, kParts);
   // parts that come through registers, and how many of them are there at a time
   constexpr int kRest = kParts - kInLds, kHeld = kSolo && kRest > (kEight ? 2 : 4) ? (kEight ? 2 : 4) : kRest;
@@ -80,9 +83,9 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
   uint4* const lds_q = lds;                  // [RT][KS][64]
   uint4* const lds_k = lds + RT * KS * 64;                             // [waves][2][kInLds][64]
   uint4* const lds_p = lds_k + waves * 2 * kInLds * 64;                // [waves][RT][64]
-  float* const lds_m = reinterpret_cast<float*>(lds_p + (kSolo ? 0 : waves * RT * 64));  // [kRows][kMostWaves]
-  int* const lds_pages = reinterpret_cast<int*>(lds_m + kRows * kMostWaves);             // [kMostWaves]: the waves' keys have pages
-  int2* const lds_sees = reinterpret_cast<int2*>(lds_pages + kMostWaves);                // [kRows]
+  float* const lds_m = reinterpret_cast<float*>(lds_p + (kSolo ? 0 : waves * RT * 64));  // [kRows][kMaxWaves]
+  int* const lds_pages = reinterpret_cast<int*>(lds_m + kRows * kMaxWaves);             // [kMaxWaves]: the waves' keys have pages
+  int2* const lds_sees = reinterpret_cast<int2*>(lds_pages + kMaxWaves);                // [kRows]
 
   // (as in paged_attention.hip)
   uint32_t id = blockIdx.x;
@@ -103,8 +106,8 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
     for (int c = threadIdx.x; c < kRows * KS * 4; c += blockDim.x) row_piece_to_lds<kEight, KS>(row_piece<KS>(a, k, head, c), c, lds_q);
     ranges_to_lds<kRows>(a, k, end, lds_sees);
     if constexpr (!kSolo) {
-      for (int c = threadIdx.x; c < kRows * kMostWaves; c += blockDim.x) lds_m[c] = -__builtin_inff();  // (of waves that there are not, too)
-      if (threadIdx.x < kMostWaves) lds_pages[threadIdx.x] = 1;
+      for (int c = threadIdx.x; c < kRows * kMaxWaves; c += blockDim.x) lds_m[c] = -__builtin_inff();  // (of waves that there are not, too)
+      if (threadIdx.x < kMaxWaves) lds_pages[threadIdx.x] = 1;
     }
     // keys all_low .. all_high are seen by every row of the block
     const int all_low = chunk_start(a, k.position0 + token_of(a, k.row0 + k.count - 1)), all_high = min(k.position0 + token_of(a, k.row0), end - 1);
@@ -286,12 +289,12 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
         const int l = opaque(lane), n = l & 15;
         if (l < 16)
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * kMostWaves + wave] = top[rt];
+          for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * kMaxWaves + wave] = top[rt];
         if (l == 0) lds_pages[wave] = pages_there;
         __syncthreads();
         int all_there = 1;
 #pragma unroll
-        for (int w = 0; w < kMostWaves; w += 4) {
+        for (int w = 0; w < kMaxWaves; w += 4) {
           const int4 u = *reinterpret_cast<const int4*>(lds_pages + w);
           all_there &= u.x & u.y & u.z & u.w;
         }
@@ -299,8 +302,8 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int w = 0; w < kMostWaves; w += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(lds_m + (rt * 16 + n) * kMostWaves + w);
+          for (int w = 0; w < kMaxWaves; w += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(lds_m + (rt * 16 + n) * kMaxWaves + w);
             top[rt] = fmaxf(top[rt], fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
           }
       }
@@ -451,10 +454,10 @@ __global__ __launch_bounds__(kSolo ? kWave : kMostWaves * kWave, 2) void paged_r
       __syncthreads();  // (the maxima of the last tile have been read)
       if (at < 16)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * kMostWaves + wave] = l[rt];
+        for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * kMaxWaves + wave] = l[rt];
       __syncthreads();
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) l[rt] = sum_of_waves(lds_m + (rt * 16 + n) * kMostWaves, waves);
+      for (int rt = 0; rt < RT; ++rt) l[rt] = sum_of_waves(lds_m + (rt * 16 + n) * kMaxWaves, waves);
     }
     const Destination to = destination_of(a, progress, static_cast<int>(id), head);
     if (to.fits) store_piece<DT>(a, k, to, head, slab == 0 && wave == 0, first_column, reinterpret_cast<float*>(lds) + wave * 16 * kTurned, acc, m, l);
@@ -468,7 +471,7 @@ template <int DT, bool kEight, int KS, bool kFull, bool kSolo>
 int launch(const AttnArgs& a, const RowsPlan& p, void* stream) {
   const auto kernel = paged_rows_kernel<DT, kEight, KS, kFull, kSolo>;
   const int parts = kEight ? KS / 2 : KS, kept = p.waves * 2 * in_lds(kSolo, parts) * 64;
-  const size_t bytes = (RT * KS * 64 + kept + (kSolo ? 0 : p.waves * RT * 64)) * sizeof(uint4) + (kRows * sizeof(float) + sizeof(int)) * kMostWaves + kRows * sizeof(int2);
+  const size_t bytes = (RT * KS * 64 + kept + (kSolo ? 0 : p.waves * RT * 64)) * sizeof(uint4) + (kRows * sizeof(float) + sizeof(int)) * kMaxWaves + kRows * sizeof(int2);
   if (bytes > 65536)
     MEGA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
   kernel<<<dim3(static_cast<uint32_t>(p.workgroups)), dim3(p.waves * kWave), bytes, static_cast<hipStream_t>(stream)>>>(a);

@@ -9,7 +9,8 @@
 // Bound by HBM: a row is read once and written once.  A wave has a token, all of its heads or some of them: where the token lies is looked up
 // once (four loads that wait for each other), then its values go by, then its keys.  16, 32 or 64 lanes take a row, each lane pieces of eight
 // elements (one 16-byte access of 16-bit ones), which it keeps in registers between the maximum and the codes; lanes that a narrow row leaves
-// take the next heads.
+// take the next heads.  Measured: 8-bit rows of 32000 positions back to 16 bits, 886 MB: 185 us, 4.8 TB/s (a large copy: 5.2); 4096 positions
+// into 8 bits, 113 MB: 24 us, 4.7 TB/s; one token a sequence: a launch (4 - 5 us).  A wave a row instead: 215 us, the look-up in front of each.
 #include "paged.hpp"
 
 #include <algorithm>
@@ -167,13 +168,6 @@ __global__ __launch_bounds__(kThreads) void paged_write_kernel(CacheArgs a) {
   if (!find_place<true>(a, p)) return;
   if (p.values) write_rows<DT, kEight>(a.side[1], p);
   if (p.keys) write_rows<DT, kEight>(a.side[0], p);
-}
-
-// two e4m3 codes of a word's lower or upper half times a power of two, as 16-bit numbers
-template <int DT, bool kUpper>
-__device__ __forceinline__ uint32_t widen(uint32_t codes, float scale) {
-  if (DT == MEGA_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, kUpper));
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, kUpper));
 }
 
 template <int DT, bool kEight>
