@@ -21,7 +21,7 @@ namespace {
 constexpr int RT = 4, CT = 8;                        // row and column tiles of a wave
 constexpr int kRows = 16 * RT;
 // of a key's 16-byte parts to a lane, those that come through LDS: all, or as many as it has room for beside the rows and the probabilities
-constexpr int in_lds(bool solo, int parts) { return solo ? 0 : parts < 5 ? parts : 5; }
+constexpr int in_lds(bool solo, int parts) { return solo ? 0 : parts < 3 ? parts : 3; }
 
 // A wave's accumulators to out, or to the workspace: there sixteen rows at a time through the wave's own LDS (free behind the last keys), as an
 // instruction would write 16 bytes of 64 lines from the registers -- 512 tokens behind 1531: 25 us more.  Out has half the bytes,
@@ -76,16 +76,16 @@ template <int DT, bool kEight, int KS, bool kFull, bool kSolo>
 __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_rows_kernel(AttnArgs a) {
   constexpr int kBytes = kEight ? 1 : 2, kParts = kEight ? KS / 2 : KS, kInLds = in_lds(kSolo, kParts);
   // parts that come through registers, and how many of them are there at a time
-  constexpr int kRest = kParts - kInLds, kHeld = kSolo && kRest > (kEight ? 2 : 4) ? (kEight ? 2 : 4) : kRest;
+  constexpr int kRest = kParts - kInLds, kMost = kSolo && !kEight ? 4 : 2, kHeld = kRest < kMost ? kRest : kMost;
   extern __shared__ __align__(16) uint4 lds[];
   __shared__ Progress progress;
   const int wave = kSolo ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), waves = kSolo ? 1 : static_cast<int>(blockDim.x) >> 6;
   uint4* const lds_q = lds;                  // [RT][KS][64]
   uint4* const lds_k = lds + RT * KS * 64;                             // [waves][2][kInLds][64]
-  uint4* const lds_p = lds_k + waves * 2 * kInLds * 64;                // [waves][RT][64]
-  float* const lds_m = reinterpret_cast<float*>(lds_p + (kSolo ? 0 : waves * RT * 64));  // [kRows][kMaxWaves]
-  int* const lds_pages = reinterpret_cast<int*>(lds_m + kRows * kMaxWaves);             // [kMaxWaves]: the waves' keys have pages
-  int2* const lds_sees = reinterpret_cast<int2*>(lds_pages + kMaxWaves);                // [kRows]
+  uint4* const lds_p = lds_k + waves * 2 * kInLds * 64;                // [2][waves][RT][64]: a tile's and the next one's
+  float* const lds_m = reinterpret_cast<float*>(lds_p + (kSolo ? 0 : 2 * waves * RT * 64));  // [kRows][kMaxWaves]
+  int* const lds_says = reinterpret_cast<int*>(lds_m + kRows * kMaxWaves);              // [2][kMaxWaves]: the waves' keys have pages (1), and no score above the slack (2)
+  int2* const lds_sees = reinterpret_cast<int2*>(lds_says + 2 * kMaxWaves);                // [kRows]
 
   // (as in paged_attention.hip)
   uint32_t id = blockIdx.x;
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_ro
     ranges_to_lds<kRows>(a, k, end, lds_sees);
     if constexpr (!kSolo) {
       for (int c = threadIdx.x; c < kRows * kMaxWaves; c += blockDim.x) lds_m[c] = -__builtin_inff();  // (of waves that there are not, too)
-      if (threadIdx.x < kMaxWaves) lds_pages[threadIdx.x] = 1;
+      if (threadIdx.x < 2 * kMaxWaves) lds_says[threadIdx.x] = 3;
     }
     // keys all_low .. all_high are seen by every row of the block
     const int all_low = chunk_start(a, k.position0 + token_of(a, k.row0 + k.count - 1)), all_high = min(k.position0 + token_of(a, k.row0), end - 1);
@@ -214,7 +214,8 @@ __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_ro
     if (begin < end) ask_for_keys(begin);
     __syncthreads();
 
-    for (int tile = begin; tile < end; tile += 32 * waves) {
+    int side = 0;  // of the probabilities: a wave that is done with its values goes on while others read theirs, so that the waves meet once a tile
+    for (int tile = begin; tile < end; tile += 32 * waves, side ^= 1) {
       // ---- scores of the wave's keys (a wave behind the end computes others' again: nothing is seen of them)
       const int mine = tile + 32 * wave;
       f32x4 s[2][RT];
@@ -274,8 +275,9 @@ __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_ro
         }
       }
 
-      // ---- the rows' maxima, probabilities and sums, as in paged_attention.hip
-      float top[RT];
+      // ---- probabilities and sums.  A tile whose scores are all within the rows' slack above m, as nearly all are behind the first, needs no maxima
+      float top[RT];  // of the lane's scores
+      bool over = false;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         float t = s[0][rt][0];
@@ -283,55 +285,78 @@ __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_ro
         for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int i = 0; i < 4; ++i) t = fmaxf(t, s[half][rt][i]);
-        top[rt] = four_max(t);
-      }
-      if constexpr (!kSolo) {
-        const int l = opaque(lane), n = l & 15;
-        if (l < 16)
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) lds_m[(rt * 16 + n) * kMaxWaves + wave] = top[rt];
-        if (l == 0) lds_pages[wave] = pages_there;
-        __syncthreads();
-        int all_there = 1;
-#pragma unroll
-        for (int w = 0; w < kMaxWaves; w += 4) {
-          const int4 u = *reinterpret_cast<const int4*>(lds_pages + w);
-          all_there &= u.x & u.y & u.z & u.w;
-        }
-        pages_there = __builtin_amdgcn_readfirstlane(all_there) != 0;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int w = 0; w < kMaxWaves; w += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(lds_m + (rt * 16 + n) * kMaxWaves + w);
-            top[rt] = fmaxf(top[rt], fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
-          }
+        top[rt] = t * a.scale;
+        over = over || top[rt] > m[rt] + kSlack;
       }
       u32x4 own[RT];  // (kSolo: the operands themselves)
-      bool moved = false;
-      float alpha[RT];
+      float sum[RT];
+      const auto weigh = [&] {
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const float seen = top[rt] * a.scale, now = seen > m[rt] + kSlack ? seen : m[rt], held = now == -__builtin_inff() ? 0.f : now, base = held - kLift<DT>;
-        alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - held);
-        moved = moved || now != m[rt];
-        m[rt] = now;
-        float p[8], sum = 0.f;
+        for (int rt = 0; rt < RT; ++rt) {
+          const float base = (m[rt] == -__builtin_inff() ? 0.f : m[rt]) - kLift<DT>;
+          float p[8];
+          sum[rt] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][rt][i & 3], a.scale, -base));
-          sum += p[i];
+          for (int i = 0; i < 8; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][rt][i & 3], a.scale, -base));
+            sum[rt] += p[i];
+          }
+          own[rt] = u32x4{pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
+          if constexpr (!kSolo) lds_p[((side * waves + wave) * RT + rt) * 64 + lane] = __builtin_bit_cast(uint4, own[rt]);
         }
-        own[rt] = u32x4{pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
-        if constexpr (!kSolo) lds_p[(wave * RT + rt) * 64 + lane] = __builtin_bit_cast(uint4, own[rt]);
-        l[rt] = l[rt] * alpha[rt] + sum;
+      };
+      // (top: of the whole rows)
+      const auto follow = [&] {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const float now = top[rt] > m[rt] + kSlack ? top[rt] : m[rt], alpha = __builtin_amdgcn_exp2f(m[rt] - (now == -__builtin_inff() ? 0.f : now));
+          m[rt] = now, l[rt] *= alpha;
+#pragma unroll
+          for (int c = 0; c < CT; ++c) acc[rt][c] *= alpha;
+        }
+      };
+      if constexpr (kSolo) {
+        if (__any(over)) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) top[rt] = four_max(top[rt]);
+          follow();
+        }
+        weigh();
+      } else {
+        over = __any(over);
+        if (!over) weigh();
+        if (opaque(lane) == 0) lds_says[side * kMaxWaves + wave] = (pages_there ? 1 : 0) | (over ? 0 : 2);
+        __syncthreads();
+        int says = 3;
+#pragma unroll
+        for (int w = 0; w < kMaxWaves; w += 4) {
+          const int4 u = *reinterpret_cast<const int4*>(lds_says + side * kMaxWaves + w);
+          says &= u.x & u.y & u.z & u.w;
+        }
+        says = __builtin_amdgcn_readfirstlane(says);
+        pages_there = (says & 1) != 0;
+        if ((says & 2) == 0) {
+          const int l = opaque(lane), n = l & 15;
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            top[rt] = four_max(top[rt]);
+            if (l < 16) lds_m[(rt * 16 + n) * kMaxWaves + wave] = top[rt];
+          }
+          __syncthreads();
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int w = 0; w < kMaxWaves; w += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(lds_m + (rt * 16 + n) * kMaxWaves + w);
+              top[rt] = fmaxf(top[rt], fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+            }
+          follow();
+          weigh();
+          __syncthreads();
+        }
       }
-      if (__any(moved))
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int c = 0; c < CT; ++c) acc[rt][c] *= alpha[rt];
-      if constexpr (!kSolo) __syncthreads();
+      for (int rt = 0; rt < RT; ++rt) l[rt] += sum[rt];
 
       // ---- values: 32 keys a step
       // (kSolo: in front of the other wave, whose scores and exponentials fill the gaps; the older of two equals has them all, and the younger ends
@@ -342,7 +367,7 @@ __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_ro
       for (int step = 0; step < steps; ++step) {
         u32x4 p[RT];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) p[rt] = kSolo ? own[rt] : __builtin_bit_cast(u32x4, lds_p[(step * RT + rt) * 64 + lane]);
+        for (int rt = 0; rt < RT; ++rt) p[rt] = kSolo ? own[rt] : __builtin_bit_cast(u32x4, lds_p[((side * waves + step) * RT + rt) * 64 + lane]);
         const int first = tile + 32 * step;
         const Step next = step_at(min(first + 32, (end - 1) & ~31));
         bool odd = false;
@@ -471,7 +496,7 @@ template <int DT, bool kEight, int KS, bool kFull, bool kSolo>
 int launch(const AttnArgs& a, const RowsPlan& p, void* stream) {
   const auto kernel = paged_rows_kernel<DT, kEight, KS, kFull, kSolo>;
   const int parts = kEight ? KS / 2 : KS, kept = p.waves * 2 * in_lds(kSolo, parts) * 64;
-  const size_t bytes = (RT * KS * 64 + kept + (kSolo ? 0 : p.waves * RT * 64)) * sizeof(uint4) + (kRows * sizeof(float) + sizeof(int)) * kMaxWaves + kRows * sizeof(int2);
+  const size_t bytes = (RT * KS * 64 + kept + (kSolo ? 0 : 2 * p.waves * RT * 64)) * sizeof(uint4) + (kRows * sizeof(float) + 2 * sizeof(int)) * kMaxWaves + kRows * sizeof(int2);
   if (bytes > 65536)
     MEGA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
   kernel<<<dim3(static_cast<uint32_t>(p.workgroups)), dim3(p.waves * kWave), bytes, static_cast<hipStream_t>(stream)>>>(a);
