@@ -5,14 +5,15 @@
 // other's scores and exponentials.
 //   - More than 128 value columns: up to eight waves with their columns and 32 keys of a tile each, as there.  A tile's keys are asked for a
 //     tile ahead, into LDS and in operand order, the next step's values while the last two columns of this one's are multiplied.
-//     Bound by what a CU is given of L2, 41 bytes a cycle: the values of 256 keys take 17000 cycles, their products 8200; the
-//     scores of the tile 2200, the softmax 1600, the waves' meeting at the maxima 5500.  A prompt of 8192 tokens in chunks of 4096, four heads of
-//     256 / 2048: 485 us, 640 TFLOP/s.  One wave to a SIMD with 64 x 256 spilled 1.5 KB a lane; four-wave workgroups of 64 x 512, whose
-//     scores are made twice: 549 us; two-wave ones: 910.  Blocks in other orders over the XCDs: 501, 673.
+//     Bound by what a CU is given of L2, 41 bytes a cycle while values are read: those of 256 keys take 17000 cycles, their products 8200,
+//     the tile's scores and softmax 4000 more.  The waves meet once a tile (twice, at the maxima and at the probabilities: 489 us).  A prompt
+//     of 8192 tokens in chunks of 4096, four heads of 256 / 2048: 465 us, 665 TFLOP/s.  One wave to a SIMD with 64 x 256 spilled 1.5 KB a lane;
+//     four-wave workgroups of 64 x 512, whose scores are made twice, took a fifth longer, two-wave ones twice as long; blocks in other orders over
+//     the XCDs 5 and 40 % longer; the first values of a tile on their way during its scores do not fit the registers.
 //   - Up to 128: a workgroup is one wave, eight to a CU, and probabilities never leave the registers.  Bound by the issue of vector
 //     instructions (conversions, exponentials, maxima: 1750 cycles for 32 keys) beside 1000 of products: 255 to 1023 tokens behind up to
-//     7001 in 8 bits, 265 us, 650 TFLOP/s.  32 rows a wave: 589 us; its keys ahead in registers: 469 us (spills).
-// A piece leaves 64 rows in float32: 512 tokens behind 1531 write and read 67 MB beside a cache of 38, 58 us.
+//     7001 in 8 bits, 260 us, 663 TFLOP/s.  32 rows a wave: 589 us; its keys ahead in registers: 469 us (spills).
+// A piece leaves 64 rows in float32: 512 tokens behind 1531 write and read 67 MB beside a cache of 38, 57 us.
 #include "paged_attention.hpp"
 
 namespace mega {
@@ -360,7 +361,7 @@ __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_ro
 
       // ---- values: 32 keys a step
       // (kSolo: in front of the other wave, whose scores and exponentials fill the gaps; the older of two equals has them all, and the younger ends
-      // alone -- four pieces of prompts on shared heads: 300 us without)
+      // alone -- four pieces of prompts on shared heads: 289 us without, 272 with)
       if constexpr (kSolo) __builtin_amdgcn_s_setprio(1);
       const int steps = kSolo ? 1 : min(waves, (end - tile + 31) >> 5);
 #pragma unroll 1
