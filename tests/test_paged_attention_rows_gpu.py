@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from megalodon_amd import fused_ops
-from paged import Batch
+from paged import Batch, to_8_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -199,3 +199,24 @@ def test_bounds_that_make_no_sense_stay_inside(cu):
     torch.cuda.synchronize()
     assert bool((room[:10] == 7).all()) and bool((room[160:] == 7).all())
     assert torch.equal(attend(x, 0.2, 0), want)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("dv", [128, 272, 1040])
+@pytest.mark.parametrize("news,olds", [([1], [900]), ([100], [900]), ([70, 40], [300, 650])])
+@pytest.mark.parametrize("rising", [True, False])
+def test_maxima_that_rise_all_the_way_or_never(news, olds, dv, bits, rising):
+    """Keys along one direction whose scores rise by some 2^9 a tile of 32 keys, or fall by that: m follows at every tile, or never."""
+    x = Batch(news, olds, 1, 1, 64, dv, 16, BF16, 16, seed=17)
+    x.q[..., 0] = 8.0
+    for b in range(len(news)):
+        for p in range(x.lengths[b]):
+            x.k[int(x.table[b, p // 16]), p % 16, 0, 0] = (p if rising else -p) / 32
+    if bits == 8:
+        whole = x
+        x = Batch(news, olds, 1, 1, 64, dv, 16, BF16, 8, seed=17)
+        x.q = whole.q
+        codes, e = to_8_bits(whole.k)
+        x.k, x.ke = codes.to(torch.float8_e4m3fn), e
+    want, bound = x.attention(0.8, 0)
+    check(attend(x, 0.8, 0), want, bound)
