@@ -306,41 +306,10 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
           for (int rt = 0; rt < RT; ++rt) acc[rt][g * kCols + c] = mma<DT>(vt[c], p[rt], acc[rt][g * kCols + c]);
       }
       if constexpr (!kAll)
-        if (__any(odd)) {  // key by key, its infinities and NaN into the rows that see it
-          const Step t = step_at(first);
-#pragma unroll 1
-          for (int slot = 0; slot < 32; ++slot) {
-            const int l = opaque(lane), n = l & 15, h = l >> 4;
-            const int place = slot & 7, half = place >> 2, in_group = 4 * (slot >> 3) + (place & 3), key = first + 16 * half + in_group;
-            if (key < k.begin || key >= end || !(half ? t.there[1] : t.there[0])) continue;
-            const uint8_t* const row = (half ? t.from[1] : t.from[0]) + static_cast<int64_t>(in_group) * a.v.slot * kBytes;
-            float weight[RT];
-            bool its[RT];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-              const uint16_t bits = reinterpret_cast<const uint16_t*>(lds_p + (step * RT + rt) * 64 + (slot & ~7) * 2 + n)[place];
-              weight[rt] = DT == MEGA_BF16 ? bf16_bits_to_float(bits) : f16_bits_to_float(bits);
-              its[rt] = in_range(lds_sees[rt * 16 + n], key);
-            }
-#pragma unroll
-            for (int c = 0; c < CT; ++c)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int at = min(first_column + 16 * kCols * (c / kCols) + kCols * (4 * h + i) + c % kCols, a.v.width - 1);
-                float v;
-                if constexpr (kEight) {
-                  v = (row[at] & 0x7f) == 0x7f ? __builtin_nanf("") : 0.f;
-                } else {
-                  const uint16_t bits = reinterpret_cast<const uint16_t*>(row)[at];
-                  v = DT == MEGA_BF16 ? bf16_bits_to_float(bits) : f16_bits_to_float(bits);
-                }
-                const bool finite = fabsf(v) < __builtin_inff();
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[rt][c][i] = finite || !its[rt] ? acc[rt][c][i] : fmaf(weight[rt], v, acc[rt][c][i]);
-                __builtin_amdgcn_sched_barrier(0);
-              }
-          }
-        }
+        if (__any(odd))
+          add_odd_values<DT, kEight, kCols>(a, k, end, first, first_column, step_at(first), lds_sees, [&](int rt, int slot) -> uint32_t {
+            return reinterpret_cast<const uint16_t*>(lds_p + (step * RT + rt) * 64 + (slot & ~7) * 2 + (opaque(lane) & 15))[slot & 7];
+          }, acc);
       there[0] = next.there[0], there[1] = next.there[1];
     };
 

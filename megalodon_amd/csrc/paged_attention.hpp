@@ -387,6 +387,46 @@ __device__ __forceinline__ void ranges_to_lds(const AttnArgs& a, const Block& k,
 }
 __device__ __forceinline__ bool in_range(int2 range, int key) { return static_cast<uint32_t>(key) - static_cast<uint32_t>(range.x) <= static_cast<uint32_t>(range.y); }
 
+// Key by key, the infinities and NaN among 32 keys' values (from `first` on, slot 8 h + i as in paged_attention.hip) into the rows that see them; the
+// product had zeros in their places.  An 8-bit value is what its code and exponent stand for in the rows' type, which may not hold it.
+// weight(rt, slot): the bits of the probability of row rt * 16 + (lane & 15).
+template <int DT, bool kEight, int kCols, int RT, int CT, typename Step, typename Weight>
+__device__ __forceinline__ void add_odd_values(const AttnArgs& a, const Block& k, int end, int first, int first_column, const Step& t, const int2* lds_sees,
+                                               Weight weight, f32x4 (&acc)[RT][CT]) {
+  const auto number = [](uint32_t bits) { return DT == MEGA_BF16 ? bf16_bits_to_float(static_cast<uint16_t>(bits)) : f16_bits_to_float(static_cast<uint16_t>(bits)); };
+#pragma unroll 1
+  for (int slot = 0; slot < 32; ++slot) {
+    const int l = opaque(static_cast<int>(threadIdx.x) & 63), n = l & 15, h = l >> 4;
+    const int place = slot & 7, half = place >> 2, in_group = 4 * (slot >> 3) + (place & 3), key = first + 16 * half + in_group;
+    if (key < k.begin || key >= end || !(half ? t.there[1] : t.there[0])) continue;
+    const uint8_t* const row = (half ? t.from[1] : t.from[0]) + static_cast<int64_t>(in_group) * a.v.slot * (kEight ? 1 : 2);
+    float unit = 0.f;
+    if constexpr (kEight) unit = exponent_value((half ? t.exponents[1] : t.exponents[0])[static_cast<int64_t>(in_group) * a.v.eSlot]);
+    float p[RT];
+    bool its[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      p[rt] = number(weight(rt, slot));
+      its[rt] = in_range(lds_sees[rt * 16 + n], key);
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = min(first_column + 16 * kCols * (c / kCols) + kCols * (4 * h + i) + c % kCols, a.v.width - 1);
+        float v;
+        if constexpr (kEight)
+          v = number(widen<DT, false>(row[at], unit));
+        else
+          v = number(reinterpret_cast<const uint16_t*>(row)[at]);
+        const bool finite = fabsf(v) < __builtin_inff();
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt][c][i] = finite || !its[rt] ? acc[rt][c][i] : fmaf(p[rt], v, acc[rt][c][i]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  }
+}
+
 // The sum of the first `waves` of eight numbers in LDS.
 __device__ __forceinline__ float sum_of_waves(const float* p, int waves) {
   const float4 u = *reinterpret_cast<const float4*>(p), v = *reinterpret_cast<const float4*>(p + 4);

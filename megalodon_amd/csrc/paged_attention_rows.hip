@@ -427,46 +427,16 @@ __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_ro
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) acc[rt][2 * u + j] = mma<DT>(vt[u & 1][j], p[rt], acc[rt][2 * u + j]);
         }
-        if (__any(odd)) {  // key by key, its infinities and NaN into the rows that see it
-          const Step t = step_at(first);
-#pragma unroll 1
-          for (int slot = 0; slot < 32; ++slot) {
-            const int l = opaque(lane), n = l & 15, h = l >> 4;
-            const int place = slot & 7, half = place >> 2, in_group = 4 * (slot >> 3) + (place & 3), key = first + 16 * half + in_group;
-            if (key < k.begin || key >= end || !(half ? t.there[1] : t.there[0])) continue;
-            const uint8_t* const row = (half ? t.from[1] : t.from[0]) + static_cast<int64_t>(in_group) * a.v.slot * kBytes;
-            float weight[RT];
-            bool its[RT];
+        if (__any(odd))
+          add_odd_values<DT, kEight, 8>(a, k, end, first, first_column, step_at(first), lds_sees, [&](int rt, int slot) -> uint32_t {
+            // (the lane of this row and slot has the probability, in its place of eight)
+            const int place = slot & 7;
+            uint32_t word = 0;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-              // (the lane of this row and slot has the probability, in its place of eight)
-              uint32_t word = 0;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) word = (place >> 1) == i ? p[rt][i] : word;
-              word = static_cast<uint32_t>(__shfl(static_cast<int>(word), (slot & ~7) * 2 + n, 64));
-              const uint16_t bits = static_cast<uint16_t>((place & 1) ? word >> 16 : word);
-              weight[rt] = DT == MEGA_BF16 ? bf16_bits_to_float(bits) : f16_bits_to_float(bits);
-              its[rt] = in_range(lds_sees[rt * 16 + n], key);
-            }
-#pragma unroll
-            for (int c = 0; c < CT; ++c)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int at = min(first_column + 8 * (4 * h + i) + c, a.v.width - 1);
-                float v;
-                if constexpr (kEight) {
-                  v = (row[at] & 0x7f) == 0x7f ? __builtin_nanf("") : 0.f;
-                } else {
-                  const uint16_t bits = reinterpret_cast<const uint16_t*>(row)[at];
-                  v = DT == MEGA_BF16 ? bf16_bits_to_float(bits) : f16_bits_to_float(bits);
-                }
-                const bool finite = fabsf(v) < __builtin_inff();
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[rt][c][i] = finite || !its[rt] ? acc[rt][c][i] : fmaf(weight[rt], v, acc[rt][c][i]);
-                __builtin_amdgcn_sched_barrier(0);
-              }
-          }
-        }
+            for (int i = 0; i < 4; ++i) word = (place >> 1) == i ? p[rt][i] : word;
+            word = static_cast<uint32_t>(__shfl(static_cast<int>(word), (slot & ~7) * 2 + (opaque(lane) & 15), 64));
+            return (place & 1) ? word >> 16 : word;
+          }, acc);
         there[0] = next.there[0], there[1] = next.there[1];
       }
       if constexpr (kSolo) __builtin_amdgcn_s_setprio(0);

@@ -1,0 +1,75 @@
+"""Paged attention over 8-bit rows whose numbers the call's type does not hold."""
+import math
+
+import pytest
+import torch
+
+from megalodon_amd import fused_ops
+from paged import SMALL, UNIT, Batch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def attend(x, scale, chunk):
+    return fused_ops.paged_attention(x.q.cuda(), *x.pools(), x.ints(x.lengths), x.ints(x.cu), scale, chunk, **x.exponents()).cpu()
+
+
+def definition(x, scale, chunk):
+    """As Batch.attention, over the stored numbers rounded to the rows' type (infinite where that does not hold them)."""
+    out = torch.zeros(x.rows, x.heads * x.shared, x.v.shape[3], dtype=torch.float64)
+    bound = torch.zeros_like(out)
+    u, small = UNIT[x.dtype], SMALL[x.dtype]
+    for b, n in enumerate(x.news):
+        k, v = (t.to(x.dtype).double() for t in x.stored(b, 0, x.lengths[b]))
+        for t in range(n):
+            p = x.olds[b] + t
+            low = p // chunk * chunk if chunk else 0
+            for g in range(x.heads * x.shared):
+                kh, vh, q = k[low:p + 1, g // x.shared], v[low:p + 1, g // x.shared], x.q[x.cu[b] + t, g].double()
+                w = torch.softmax((kh * q).sum(-1) * scale, 0)
+                o, A = (w[:, None] * vh).sum(0), (w[:, None] * vh.abs()).sum(0)
+                sizes = (kh.abs() * q.abs()).sum(-1)
+                d = (len(q) + 4) * 2.0 ** -23 * scale * sizes[sizes < math.inf].max()
+                out[x.cu[b] + t, g] = o
+                bound[x.cu[b] + t, g] = 1.01 * u * (o.abs() + A) + (2 * d + 2.0 ** -20 + (p + 9 - low) * 2.0 ** -23) * A + small * (1 + vh.abs().sum(0))
+    return out, bound
+
+
+def check(got, want, bound):
+    finite = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), finite)
+    assert torch.equal(got[~finite].double().nan_to_num(nan=7.0), want[~finite].nan_to_num(nan=7.0))  # (infinities of their sign)
+    assert bool(((got.double() - want)[finite].abs() <= bound[finite]).all())
+
+
+def place(x, position):
+    return int(x.table[0, position // x.page]), position % x.page
+
+
+# few rows of a sequence; the position in keys that all rows see (whole groups of 32, or the last few), that later rows see, of
+# the chunk before
+WHERE = [([1], [40], 10, 0), ([1], [40], 35, 0), ([1], [40], 40, 0), ([5], [300], 5, 0), ([5], [300], 299, 0), ([5], [300], 302, 0), ([5], [62], 63, 64)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dv", [64, 1040])
+@pytest.mark.parametrize("where", WHERE, ids=lambda w: f"{w[0][0]}-{w[1][0]}-{w[2]}-{w[3]}")
+def test_values_past_the_type_are_infinite_to_the_rows_that_see_them(where, dv, dtype):
+    """A stored value of 448 2^9 (2^127) is an infinity in float16 (bfloat16), as it is where the cache is read; small codes beside
+    it are numbers."""
+    news, olds, bad, chunk = where
+    x = Batch(news, olds, 1, 1, 64, dv, 16, dtype, 8, seed=21)
+    clean = attend(x, 0.1, chunk)
+    codes = torch.full((dv,), 2.0 ** -6)
+    codes[1::3], codes[2::7] = 448.0, -448.0
+    x.v[place(x, bad)] = codes.to(x.v.dtype)
+    x.ve[place(x, bad)] = 136 if dtype == F16 else 254
+    want, bound = definition(x, 0.1, chunk)
+    got = attend(x, 0.1, chunk)
+    check(got, want, bound)
+    position = torch.tensor([o + i for n, o in zip(news, olds) for i in range(n)])
+    blind = (position < bad) | (position // (chunk or 10 ** 9) != bad // (chunk or 10 ** 9))
+    blind[news[0]:] = True  # (other sequences)
+    assert torch.equal(got[blind], clean[blind]) and not bool(torch.isfinite(got[~blind]).all(-1).any())
