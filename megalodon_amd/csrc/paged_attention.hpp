@@ -229,12 +229,11 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   return ((w & top) == top ? 0u : 0xffffu) | ((w >> 16 & top) == top ? 0u : 0xffff0000u);
 }
 
-// ones over those bytes of a word whose e4m3 codes are numbers
-__device__ __forceinline__ uint32_t finite_codes(uint32_t w) {
-  uint32_t keep = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) keep |= ((w >> (8 * i)) & 0x7fu) == 0x7fu ? 0u : 0xffu << (8 * i);
-  return keep;
+// ones over those bytes of a word whose e4m3 codes times `unit` are finite numbers of the type
+template <int DT>
+__device__ __forceinline__ uint32_t finite_codes(uint32_t w, float unit) {
+  const uint32_t low = finite_halves<DT>(widen<DT, false>(w, unit)), high = finite_halves<DT>(widen<DT, true>(w, unit));
+  return __builtin_amdgcn_perm(high, low, 0x06040200);
 }
 
 // v, of which the compiler knows nothing: what is computed from it is computed where it is used, not once ahead of a loop

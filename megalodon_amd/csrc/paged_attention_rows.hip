@@ -371,6 +371,10 @@ __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_ro
         for (int rt = 0; rt < RT; ++rt) p[rt] = kSolo ? own[rt] : __builtin_bit_cast(u32x4, lds_p[((side * waves + step) * RT + rt) * 64 + lane]);
         const int first = tile + 32 * step;
         const Step next = step_at(min(first + 32, (end - 1) & ~31));
+        float unit[8];
+        if constexpr (kEight)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) unit[i] = exponent_value(e[i]);
         bool odd = false;
         if (first < all_low || first + 31 > all_high || !pages_there) {
           // what is not there, or not this workgroup's, must not meet a probability of zero as an infinity or NaN; nor must such a
@@ -382,18 +386,17 @@ __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_ro
             const uint32_t keep = key >= k.begin && key < end && there[i >> 2] ? ~0u : 0u;
 #pragma unroll
             for (int j = 0; j < (kEight ? 2 : 4); ++j) {
-              const uint32_t finite = kEight ? finite_codes(x[i][j]) : finite_halves<DT>(x[i][j]);
+              uint32_t finite;
+              if constexpr (kEight)
+                finite = finite_codes<DT>(x[i][j], unit[i]);
+              else
+                finite = finite_halves<DT>(x[i][j]);
               odd = odd || (~finite & keep) != 0;
               x[i][j] &= keep & finite;
             }
           }
         }
-        float unit[8];
-        if constexpr (kEight) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) unit[i] = exponent_value(e[i]);
-          if constexpr (!kSolo) load_exponents(next);
-        }
+        if constexpr (kEight && !kSolo) load_exponents(next);
         // columns 2 j, 2 j + 1 of a lane's eight as operands
         const auto convert = [&](int j, u32x4 (&vt)[2]) {
           uint32_t w[8];

@@ -48,9 +48,10 @@ def place(x, position):
     return int(x.table[0, position // x.page]), position % x.page
 
 
-# few rows of a sequence; the position in keys that all rows see (whole groups of 32, or the last few), that later rows see, of
+# few rows of a sequence and many; the position in keys that all rows see (whole groups of 32, or the last few), that later rows see, of
 # the chunk before
-WHERE = [([1], [40], 10, 0), ([1], [40], 35, 0), ([1], [40], 40, 0), ([5], [300], 5, 0), ([5], [300], 299, 0), ([5], [300], 302, 0), ([5], [62], 63, 64)]
+WHERE = [([1], [40], 10, 0), ([1], [40], 35, 0), ([1], [40], 40, 0), ([5], [300], 5, 0), ([5], [300], 299, 0), ([5], [300], 302, 0), ([5], [62], 63, 64),
+         ([100], [20], 5, 0), ([100], [20], 70, 0), ([100], [20], 63, 64), ([80, 40], [300, 7], 340, 0)]
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
