@@ -394,6 +394,8 @@ __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_ro
               odd = odd || (~finite & keep) != 0;
               x[i][j] &= keep & finite;
             }
+            // (nor their exponents, which nobody need have written: a byte of 255 makes NaN of a zero)
+            if constexpr (kEight) unit[i] = keep != 0 && unit[i] < __builtin_inff() ? unit[i] : 1.f;
           }
         }
         if constexpr (kEight && !kSolo) load_exponents(next);

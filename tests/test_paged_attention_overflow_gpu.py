@@ -1,4 +1,4 @@
-"""Paged attention over 8-bit rows whose numbers the call's type does not hold."""
+"""Paged attention over 8-bit rows whose numbers the call's type does not hold, and behind exponents that nobody wrote."""
 import math
 
 import pytest
@@ -74,3 +74,37 @@ def test_values_past_the_type_are_infinite_to_the_rows_that_see_them(where, dv, 
     blind = (position < bad) | (position // (chunk or 10 ** 9) != bad // (chunk or 10 ** 9))
     blind[news[0]:] = True  # (other sequences)
     assert torch.equal(got[blind], clean[blind]) and not bool(torch.isfinite(got[~blind]).all(-1).any())
+
+
+@pytest.mark.parametrize("dv", [64, 1040])
+@pytest.mark.parametrize("byte", [255, 254, 0])
+@pytest.mark.parametrize("news,olds", [([1], [40]), ([5, 1], [300, 7]), ([100], [20]), ([80, 40], [300, 7])])
+def test_exponents_that_nobody_wrote_do_not_matter(news, olds, byte, dv):
+    """Behind a sequence's end, on pages of nobody, and on the page whose numbers stand in for those of a number that is no page."""
+    for dtype in (BF16, F16):
+        x = Batch(news, olds, 1, 1, 64, dv, 16, dtype, 8, seed=23)
+        pages = x.k.shape[0]
+        spare = next(i for i in range(pages) if i not in x.table.flatten().tolist())
+        turn = [(i + spare) % pages for i in range(pages)]  # the spare page is number 0
+        x.k, x.v, x.ke, x.ve = x.k[turn], x.v[turn], x.ke[turn], x.ve[turn]
+        x.table = torch.where(x.table >= 0, (x.table - spare) % pages, x.table)
+        x.table[0, 1] = -1
+        clean = attend(x, 0.2, 0)
+        owned = torch.zeros(x.ke.shape, dtype=torch.bool)
+        for b, length in enumerate(x.lengths):
+            for p in range(length):
+                if x.table[b, p // 16] >= 0:
+                    owned[x.table[b, p // 16], p % 16] = True
+        x.ke[~owned], x.ve[~owned] = byte, byte
+        assert bool(torch.isfinite(clean).all()) and torch.equal(attend(x, 0.2, 0), clean)
+
+
+@pytest.mark.parametrize("dv", [64, 1040])
+@pytest.mark.parametrize("news,olds", [([6], [300]), ([100], [20])])
+def test_an_exponent_that_is_none_stays_with_the_rows_that_see_it(news, olds, dv):
+    """Byte 255 stands for no number; the rows in front of it are as without."""
+    x = Batch(news, olds, 1, 1, 64, dv, 16, BF16, 8, seed=24)
+    clean = attend(x, 0.2, 0)
+    bad = olds[0] + news[0] // 2
+    x.ve[place(x, bad)] = 255
+    assert torch.equal(attend(x, 0.2, 0)[:news[0] // 2], clean[:news[0] // 2])
