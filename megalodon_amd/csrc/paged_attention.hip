@@ -185,7 +185,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
       bool there[2];
     };
     u32x4 kx[2][kStaged ? 1 : kLoads];
-    uint32_t ke[2][4];
+    uint32_t ke[2];
     const auto keys_at = [&](int group) {
       Keys t;
 #pragma unroll
@@ -204,11 +204,9 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
     };
     const auto load_first_keys_at = [&](const Keys& t) {
       if constexpr (kEight) {
-        const uint32_t offset = static_cast<uint32_t>(4 * (opaque(lane) >> 4)) * a.k.eSlot;
+        const uint32_t offset = static_cast<uint32_t>(opaque(lane) & 15) * a.k.eSlot;
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) ke[half][i] = t.exponents[half][offset + static_cast<uint32_t>(i * a.k.eSlot)];
+        for (int half = 0; half < 2; ++half) ke[half] = t.exponents[half][offset];
       }
       if constexpr (kStaged) {
         // piece p of row r lies at p ^ (r & 15) (& 7 where there are eight): sixteen rows' equal pieces are in different banks
@@ -349,7 +347,8 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
             }
             if constexpr (kEight) {
               const uint32_t lo = (c & 1) ? key[2] : key[0], hi = (c & 1) ? key[3] : key[1];
-              key = u32x4{widen<DT, false>(lo, 1.f), widen<DT, true>(lo, 1.f), widen<DT, false>(hi, 1.f), widen<DT, true>(hi, 1.f)};
+              const float unit = exponent_value(ke[half]);
+              key = u32x4{widen<DT, false>(lo, unit), widen<DT, true>(lo, unit), widen<DT, false>(hi, unit), widen<DT, true>(hi, unit)};
             }
             if (a.k.width != 32 * KS) {  // (behind the row's end the rows' operands are zero, and infinity times zero is not)
               const int d = kEight ? (c >> 1) * 64 + (opaque(lane) >> 4) * 16 : c * 32 + (opaque(lane) >> 4) * 8;
@@ -363,12 +362,8 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          f32x4 factor = {a.scale, a.scale, a.scale, a.scale};
-          if constexpr (kEight)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) factor[i] *= exponent_value(ke[half][i]);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[half][rt] *= factor;
+          for (int rt = 0; rt < RT; ++rt) s[half][rt] *= a.scale;
           if (!whole || !keys.there[half]) {
             const int l = opaque(lane), first = mine + 16 * half + 4 * (l >> 4);
 #pragma unroll

@@ -76,6 +76,21 @@ def test_values_past_the_type_are_infinite_to_the_rows_that_see_them(where, dv, 
     assert torch.equal(got[blind], clean[blind]) and not bool(torch.isfinite(got[~blind]).all(-1).any())
 
 
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("where", WHERE, ids=lambda w: f"{w[0][0]}-{w[1][0]}-{w[2]}-{w[3]}")
+def test_keys_past_the_type_are_infinite(where, sign):
+    """A score of infinity makes a row NaN, one of minus infinity takes the key out, in few rows as in many."""
+    news, olds, bad, chunk = where
+    x = Batch(news, olds, 1, 1, 64, 64, 16, F16, 8, seed=22)
+    x.q[..., 0] = sign
+    codes = torch.zeros(64)
+    codes[0] = 448.0
+    x.k[place(x, bad)] = codes.to(x.k.dtype)
+    x.ke[place(x, bad)] = 136
+    want, bound = definition(x, 0.1, chunk)
+    check(attend(x, 0.1, chunk), want, bound)
+
+
 @pytest.mark.parametrize("dv", [64, 1040])
 @pytest.mark.parametrize("byte", [255, 254, 0])
 @pytest.mark.parametrize("news,olds", [([1], [40]), ([5, 1], [300, 7]), ([100], [20]), ([80, 40], [300, 7])])
