@@ -17,6 +17,7 @@ from typing import Optional, Tuple
 import torch
 import torch.nn.functional as F
 from torch import Tensor, nn
+from torch.autograd import forward_ad
 from torch.nn.modules import module as nn_module
 
 from ..fused_ops import memory_efficient_dropout, swift_efficient_attention
@@ -113,15 +114,17 @@ class _InnerAttention(nn.Module):
 
     _own_forward = forward
 
-    @torch.no_grad()
     def forward_paged(self, xq: Tensor, xk: Tensor, xv: Tensor, cache: PagedCache, block_table: Tensor, lengths: Tensor,
                       cu_new: Tensor) -> Tensor:
         """The same attention for a ragged batch on a paged cache: rows cu_new[b] .. cu_new[b + 1] of the projections
         (rows, heads * dim) are the last positions of sequence b, which has lengths[b] of them now.  Their keys and values
         enter `cache`, then each row attends from the start of its chunk to itself.  Rotary angles, which
-        go by a token's position inside its chunk, have been applied.  Evaluation only."""
+        go by a token's position inside its chunk, have been applied.  Evaluation only: dropout, or a gradient that is
+        asked for, raises before anything is written."""
         if self.training and self.dropout > 0.0:
             raise RuntimeError("forward_paged has no dropout: call it in evaluation mode")
+        if any((torch.is_grad_enabled() and t.requires_grad) or forward_ad.unpack_dual(t).tangent is not None for t in (xq, xk, xv)):
+            raise RuntimeError("forward_paged has no gradient: call it under torch.no_grad()")
         cache.write(xk.unflatten(-1, (self.n_heads, self.z_head_dim)), xv.unflatten(-1, (self.n_heads, self.v_head_dim)),
                     block_table, lengths, cu_new)
         out = cache.attend(xq.unflatten(-1, (self.n_heads, self.z_head_dim)), block_table, lengths, cu_new, chunk_size=self.chunk_size)
