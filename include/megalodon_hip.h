@@ -890,7 +890,9 @@ typedef struct mega_paged_cache {
  * positions lengths[b] - n .. lengths[b] - 1 (a negative one has no place).
  * k_new (rows, heads, k_width), v_new (rows, heads, v_width) of dtype MEGA_BF16 /
  * MEGA_F16 with the given strides (multiples of 8 elements; 16-byte aligned).
- * No place may be written twice in one call. */
+ * No place may be written twice in one call.  Pools and exponents must not share
+ * memory place by place (they may lie between each other, as halves of a row, a
+ * position or a page; refused where strides that differ leave it open). */
 int mega_paged_cache_write(const mega_paged_cache* cache, int dtype, const void* k_new, int64_t k_row, int64_t k_head,
                            const void* v_new, int64_t v_row, int64_t v_head, const int32_t* lengths, const int32_t* cu,
                            int64_t rows, void* stream);

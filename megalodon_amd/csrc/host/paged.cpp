@@ -117,8 +117,8 @@ void paged_cache_write(const Tensor& k, const Tensor& v, const Tensor& k_pages, 
   require(kr.size(1) == c.heads && vr.size(1) == c.heads && kr.size(2) == c.k_width && vr.size(2) == c.v_width,
           "paged_cache_write: k and v must have the pools' heads and widths");
   for (const Tensor* from : {&kr, &vr})
-    for (const Tensor* to : {&k_pages, &v_pages}) require(!overlap(*from, *to), "paged_cache_write: new rows must not lie in the pools");
-  require(!overlap(k_pages, v_pages) || k_pages.storage().data() == v_pages.storage().data(), "paged cache: the pools overlap");
+    for (const Tensor* to : {&k_pages, &v_pages, ke.has_value() ? &*ke : &k_pages, ve.has_value() ? &*ve : &v_pages})
+      require(!overlap(*from, *to), "paged_cache_write: new rows must not lie in the pools");
   const int32_t *n = counts(lengths, cache, c.batch, kPerSequence), *bounds = counts(cu, cache, c.batch + 1, kBounds);
   check(mega_paged_cache_write(&c, code_of(kr.scalar_type()), kr.data_ptr(), step_of(kr, 0), step_of(kr, 1), vr.data_ptr(), step_of(vr, 0), step_of(vr, 1),
                                n, bounds, kr.size(0), stream_of(k_pages)), "mega_paged_cache_write");
@@ -164,7 +164,8 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
     require(y.is_cuda() && y.device() == qr.device() && y.scalar_type() == qr.scalar_type() && y.is_contiguous() && !lazy(y) &&
                 y.sizes() == at::IntArrayRef({rows, heads, c.v_width}),
             "paged_attention: out must be contiguous (rows, query heads, v width) of q's dtype and device");
-    for (const Tensor* t : {&qr, &k_pages, &v_pages}) require(!overlap(y, *t), "paged_attention: out must not overlap q or the pools");
+    for (const Tensor* t : {&qr, &k_pages, &v_pages, ke.has_value() ? &*ke : &k_pages, ve.has_value() ? &*ve : &v_pages})
+      require(!overlap(y, *t), "paged_attention: out must not overlap q or the pools");
   } else {
     y = at::empty({rows, heads, c.v_width}, qr.options());
   }

@@ -236,6 +236,61 @@ int launch(K kernel, CacheArgs& a, const char* who, void* stream) {
   return MEGA_OK;
 }
 
+// A pool's places, in bytes: rows of `width` at base + i stride[0] + j stride[1] + ..., axes of one entry left out, the largest stride first.
+struct Places {
+  uintptr_t base;
+  int64_t stride[3], count[3], width;
+  int axes;
+  // bytes from the first row's begin to the last one's end, over the axes behind the first `from`
+  int64_t span(int from) const {
+    int64_t n = width;
+    for (int i = from; i < axes; ++i) n += (count[i] - 1) * stride[i];
+    return n;
+  }
+};
+Places places_of(const mega_paged_cache* c, const void* base, const int64_t* stride, int64_t width, int64_t bytes) {
+  Places p{reinterpret_cast<uintptr_t>(base), {}, {}, width * bytes, 0};
+  const int64_t count[3] = {c->pages, c->page_size, c->heads};
+  for (int i = 0; i < 3; ++i) {
+    if (count[i] == 1) continue;
+    int at = p.axes++;
+    for (; at > 0 && p.stride[at - 1] < stride[i] * bytes; --at) p.stride[at] = p.stride[at - 1], p.count[at] = p.count[at - 1];
+    p.stride[at] = stride[i] * bytes, p.count[at] = count[i];
+  }
+  return p;
+}
+// Whether two rows of a pool may share memory: an axis steps over all that lies behind it, or they may.
+bool rows_meet(const Places& p) {
+  for (int i = 0; i < p.axes; ++i)
+    if (p.stride[i] < p.span(i + 1)) return true;
+  return false;
+}
+// Whether a row of a and one of b, which begins `ahead` bytes behind a, may share memory: axis by axis, as long as their strides agree.
+bool places_meet(const Places& a, const Places& b, int64_t ahead, int axis = 0) {
+  if (ahead >= a.span(axis) || ahead + b.span(axis) <= 0) return false;
+  if (axis == a.axes || axis == b.axes || a.stride[axis] != b.stride[axis]) return true;
+  const int64_t stride = a.stride[axis], inner_a = a.span(axis + 1), inner_b = b.span(axis + 1);
+  if (inner_a > stride || inner_b > stride) return true;
+  // steps d with -inner_b < ahead + d stride < inner_a, three at the most
+  const auto floor_div = [&](int64_t n) { return n / stride - (n % stride < 0); };
+  const int64_t low = std::max(floor_div(-inner_b - ahead) + 1, 1 - a.count[axis]), high = std::min(floor_div(inner_a - ahead - 1), b.count[axis] - 1);
+  for (int64_t d = low; d <= high; ++d)
+    if (places_meet(a, b, ahead + d * stride, axis + 1)) return true;
+  return false;
+}
+// Rows that are written at once must not share memory: not two of a pool, nor one of a pool with one of another.
+bool pools_meet(const mega_paged_cache* c) {
+  const bool eight = c->k_exponents != nullptr;
+  const Places p[4] = {places_of(c, c->k, c->k_stride, c->k_width, eight ? 1 : 2), places_of(c, c->v, c->v_stride, c->v_width, eight ? 1 : 2),
+                       places_of(c, c->k_exponents, c->ke_stride, 1, 1), places_of(c, c->v_exponents, c->ve_stride, 1, 1)};
+  for (int i = 0; i < (eight ? 4 : 2); ++i) {
+    if (rows_meet(p[i])) return true;
+    for (int j = 0; j < i; ++j)
+      if (places_meet(p[i], p[j], static_cast<int64_t>(p[j].base) - static_cast<int64_t>(p[i].base))) return true;
+  }
+  return false;
+}
+
 bool unaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
 
 }  // namespace
@@ -288,6 +343,7 @@ extern "C" int mega_paged_cache_write(const mega_paged_cache* cache, int dtype, 
                                       int64_t rows, void* stream) {
   if (const int rc = check_paged_cache(cache, dtype, "mega_paged_cache_write"); rc != MEGA_OK) return rc;
   MEGA_CHECK_ARG(rows >= 0 && rows <= 0x7fffffff, "mega_paged_cache_write: bad number of rows");
+  MEGA_CHECK_ARG(!pools_meet(cache), "mega_paged_cache_write: the places of the pools must not share memory");
   if (rows == 0 || cache->batch == 0) return MEGA_OK;
   MEGA_CHECK_ARG(k_new != nullptr && v_new != nullptr && lengths != nullptr && cu != nullptr, "mega_paged_cache_write: null pointer");
   MEGA_CHECK_ARG(!unaligned(k_new) && !unaligned(v_new) && k_row % 8 == 0 && k_head % 8 == 0 && v_row % 8 == 0 && v_head % 8 == 0,

@@ -34,7 +34,7 @@ def paged_cache_write(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, bl
 
     8 bits: a row's exponent is the smallest that keeps its largest finite magnitude at or below 448 codes;
     codes are rounded to nearest, ties to even; infinities and NaN become NaN.  Two new rows of one call
-    must not have one place."""
+    must not have one place.  Pools and exponents may be slices of one tensor, but not of the same memory."""
     _lib.host().paged_cache_write(k, v, k_pages, v_pages, block_table, lengths, cu_new, k_exponents, v_exponents)
 
 
