@@ -39,6 +39,12 @@ __device__ __forceinline__ int last_not_above(int n, int64_t x, F f) {
   return __builtin_amdgcn_readfirstlane(low);
 }
 
+// A launch has fewer than 2^32 threads along an axis (of more, those past a multiple of 2^32 run and no error says so): groups in lines of 2^22,
+// of up to 512 threads each.  The last line has numbers behind the last group's.
+constexpr int64_t kLine = 1 << 22;
+inline dim3 grid_of(int64_t groups) { return dim3(static_cast<uint32_t>(groups < kLine ? groups : kLine), static_cast<uint32_t>((groups + kLine - 1) / kLine)); }
+__device__ __forceinline__ uint32_t group_number() { return blockIdx.y * static_cast<uint32_t>(kLine) + blockIdx.x; }
+
 // row numbers that `cu` gives, kept inside the operand whatever it holds
 __device__ __forceinline__ int row_bound(const int32_t* cu, int i, int rows) { return min(max(cu[i], 0), rows); }
 

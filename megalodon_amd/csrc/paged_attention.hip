@@ -109,7 +109,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave, 2) void paged_attn_kernel(AttnAr
 
   // column slab and head fastest: workgroups that read the same keys and values share an XCD's L2 (the hardware deals
   // workgroups to the eight XCDs in turn); late row blocks, which see the most keys, first
-  uint32_t id = blockIdx.x;
+  uint32_t id = group_number();
   const int slab = id % a.slabs;
   id /= a.slabs;
   const int head = id % a.heads;
@@ -555,7 +555,7 @@ int launch_few(const AttnArgs& a, const Plan& p, void* stream) {
   if (bytes > 65536)
     MEGA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  kernel<<<dim3(static_cast<uint32_t>(p.workgroups(a.heads))), dim3(p.waves * kWave), bytes, s>>>(a);
+  kernel<<<grid_of(p.workgroups(a.heads)), dim3(p.waves * kWave), bytes, s>>>(a);
   MEGA_CHECK_LAUNCH();
   return MEGA_OK;
 }

@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_ro
   int2* const lds_sees = reinterpret_cast<int2*>(lds_says + 2 * kMaxWaves);                // [kRows]
 
   // (as in paged_attention.hip)
-  uint32_t id = blockIdx.x;
+  uint32_t id = group_number();
   const int slab = id % a.slabs;
   id /= a.slabs;
   const int head = id % a.heads;
@@ -475,7 +475,7 @@ int launch(const AttnArgs& a, const RowsPlan& p, void* stream) {
   const size_t bytes = (RT * KS * 64 + kept + (kSolo ? 0 : 2 * p.waves * RT * 64)) * sizeof(uint4) + (kRows * sizeof(float) + 2 * sizeof(int)) * kMaxWaves + kRows * sizeof(int2);
   if (bytes > 65536)
     MEGA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
-  kernel<<<dim3(static_cast<uint32_t>(p.workgroups)), dim3(p.waves * kWave), bytes, static_cast<hipStream_t>(stream)>>>(a);
+  kernel<<<grid_of(p.workgroups), dim3(p.waves * kWave), bytes, static_cast<hipStream_t>(stream)>>>(a);
   MEGA_CHECK_LAUNCH();
   return MEGA_OK;
 }

@@ -48,7 +48,7 @@ struct Place {
 // false: the wave has nothing to do
 template <bool kWrite>
 __device__ __forceinline__ bool find_place(const CacheArgs& a, Place& p) {
-  int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  int64_t item = static_cast<int64_t>(group_number()) * kWaves + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   p.keys = !a.apart || (item & 1) != 0, p.values = !a.apart || (item & 1) == 0;
   item >>= a.apart;
   if (item >= static_cast<int64_t>(a.rows) * a.shares) return false;
@@ -226,12 +226,11 @@ void split_heads(CacheArgs& a) {
 }
 
 template <typename K>
-int launch(K kernel, CacheArgs& a, const char* who, void* stream) {
+int launch(K kernel, CacheArgs& a, void* stream) {
   split_row(a.side[0]), split_row(a.side[1]);
   split_heads(a);
   const int64_t groups = ((static_cast<int64_t>(a.rows) * a.shares << a.apart) + kWaves - 1) / kWaves;
-  MEGA_CHECK_ARG(groups <= 0x7fffffff, "%s: too many rows for one launch", who);
-  kernel<<<dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, static_cast<hipStream_t>(stream)>>>(a);
+  kernel<<<grid_of(groups), dim3(kThreads), 0, static_cast<hipStream_t>(stream)>>>(a);
   MEGA_CHECK_LAUNCH();
   return MEGA_OK;
 }
@@ -243,8 +242,11 @@ struct Places {
   int axes;
   // bytes from the first row's begin to the last one's end, over the axes behind the first `from`
   int64_t span(int from) const {
-    int64_t n = width;
-    for (int i = from; i < axes; ++i) n += (count[i] - 1) * stride[i];
+    constexpr int64_t kAll = int64_t{1} << 60;  // (more than there are addresses)
+    int64_t n = width, step;
+    for (int i = from; i < axes; ++i)
+      if (__builtin_mul_overflow(count[i] - 1, stride[i], &step) || step >= kAll - n) return kAll;
+      else n += step;
     return n;
   }
 };
@@ -353,9 +355,9 @@ extern "C" int mega_paged_cache_write(const mega_paged_cache* cache, int dtype, 
               lengths, cu, static_cast<int32_t>(rows), static_cast<int32_t>(cache->heads), 0, 0, 0, 0};
   const bool eight = cache->k_exponents != nullptr;
   if (dtype == MEGA_BF16)
-    return eight ? launch(paged_write_kernel<MEGA_BF16, true>, a, "mega_paged_cache_write", stream) : launch(paged_write_kernel<MEGA_BF16, false>, a, "mega_paged_cache_write", stream);
+    return eight ? launch(paged_write_kernel<MEGA_BF16, true>, a, stream) : launch(paged_write_kernel<MEGA_BF16, false>, a, stream);
   // (a copy does not look at its elements: one kernel for both types)
-  return eight ? launch(paged_write_kernel<MEGA_F16, true>, a, "mega_paged_cache_write", stream) : launch(paged_write_kernel<MEGA_BF16, false>, a, "mega_paged_cache_write", stream);
+  return eight ? launch(paged_write_kernel<MEGA_F16, true>, a, stream) : launch(paged_write_kernel<MEGA_BF16, false>, a, stream);
 }
 
 extern "C" int mega_paged_cache_read(const mega_paged_cache* cache, int dtype, const int32_t* begins, const int32_t* cu, int64_t rows,
@@ -372,6 +374,6 @@ extern "C" int mega_paged_cache_read(const mega_paged_cache* cache, int dtype, c
               begins, cu, static_cast<int32_t>(rows), static_cast<int32_t>(H), 0, 0, 0, clear_rest != 0};
   const bool eight = cache->k_exponents != nullptr;
   if (dtype == MEGA_BF16)
-    return eight ? launch(paged_read_kernel<MEGA_BF16, true>, a, "mega_paged_cache_read", stream) : launch(paged_read_kernel<MEGA_BF16, false>, a, "mega_paged_cache_read", stream);
-  return eight ? launch(paged_read_kernel<MEGA_F16, true>, a, "mega_paged_cache_read", stream) : launch(paged_read_kernel<MEGA_BF16, false>, a, "mega_paged_cache_read", stream);
+    return eight ? launch(paged_read_kernel<MEGA_BF16, true>, a, stream) : launch(paged_read_kernel<MEGA_BF16, false>, a, stream);
+  return eight ? launch(paged_read_kernel<MEGA_F16, true>, a, stream) : launch(paged_read_kernel<MEGA_BF16, false>, a, stream);
 }
