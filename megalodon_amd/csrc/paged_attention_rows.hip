@@ -311,7 +311,9 @@ __global__ __launch_bounds__(kSolo ? kWave : kMaxWaves * kWave, 2) void paged_ro
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           const float now = top[rt] > m[rt] + kSlack ? top[rt] : m[rt], alpha = __builtin_amdgcn_exp2f(m[rt] - (now == -__builtin_inff() ? 0.f : now));
-          m[rt] = now, l[rt] *= alpha;
+          m[rt] = now;
+          // (a score that only the scale makes infinite is finite in the fused product below, which would give it no weight instead of NaN)
+          l[rt] = now == __builtin_inff() ? __builtin_nanf("") : l[rt] * alpha;
 #pragma unroll
           for (int c = 0; c < CT; ++c) acc[rt][c] *= alpha;
         }
