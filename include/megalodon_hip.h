@@ -916,7 +916,9 @@ int mega_paged_cache_read(const mega_paged_cache* cache, int dtype, const int32_
  * included.  float32 scores, softmax and sums; probabilities, and the numbers
  * that 8-bit codes and exponents stand for, are rounded to dtype for the matrix
  * cores (the latter as mega_paged_cache_read does; float16 holds no number
- * above 65504, so that rows written from bfloat16 are best read in it).
+ * above 65504, so that rows written from bfloat16 are best read in it: what is
+ * past it is an infinity to the rows that see it).  A score past float32's
+ * largest number is infinite; a row with one of plus infinity becomes NaN.
  * out (rows, q_heads, v_width) contiguous; clear_rest as above.  workspace:
  * mega_paged_attention_workspace_bytes(...) bytes (0: none is needed), used by
  * this call alone while it runs. */

@@ -29,7 +29,7 @@
 // Many row blocks: a workgroup each.
 //
 // This file: up to 32 rows of a sequence on average.  Bound by the cache's bytes: 32 tokens on shared heads over 16-bit caches of up to 16000
-// positions, 205 us, 5.3 TB/s (a large read reaches 6.0); sixteen tokens over 8-bit ones of up to 4000, 80 us, 4.7 TB/s; drafts of eight
+// positions, 205 us, 5.3 TB/s (a large read reaches 6.0); sixteen tokens over 8-bit ones of up to 4000, 79 us, 4.7 TB/s; drafts of eight
 // sequences, 76 us, 4.2 TB/s.  Short of that by what comes before the first and behind the last key of a workgroup, some 8 us: chains of
 // dependent loads (bounds, lengths, page numbers, keys; 4 us), the results' way out, the join (4 us); one token over 1531 positions
 // takes 21 us, of them 5 on the cache.  A third wave on a SIMD for narrow heads: 229 us against 205, the registers of the values in flight.
@@ -532,6 +532,9 @@ Plan plan_of(const mega_paged_cache* c, int64_t rows, int64_t q_heads) {
   // workgroups that the chip holds at a time: eight waves to a CU
   const int64_t resident = kCus * kMaxWaves / p.waves, pairs = c->heads * p.slabs;
   const int64_t full = std::max(rows * shared / kRows, std::min(c->batch, rows)) * pairs;
+  // A line of units up to four times that many blocks, a workgroup a block above.  Two to four times: 128 single tokens behind 100 - 4000, wide heads,
+  // 854 us on the line against 988, 256 on shared heads 414 against 484; prompts the other way, 4096 tokens 265 against 210, as their pieces' rows are more
+  // bytes than their keys.  Behind four times: 8192 tokens 614 against 431, 512 single tokens on shared heads the same.
   if (c->batch > 0 && full < 4 * resident && p.blocks * (c->table_width * c->page_size / 32 + 9) < 0x40000000 &&
       (resident + p.blocks) * c->heads * kRows < 0x40000000 && rows * q_heads < 0x1000000) {
     p.parts = std::max<int64_t>(1, resident / pairs);
@@ -640,6 +643,8 @@ extern "C" int mega_paged_attention_fwd(const mega_paged_cache* cache, int dtype
   a.parts = static_cast<int32_t>(p.parts), a.slots = static_cast<int32_t>(p.slots), a.part_rows = static_cast<int32_t>(p.part_rows);
   a.clear_rest = clear_rest != 0;
   a.chunk_shift = log2_of(a.chunk), a.shared_shift = log2_of(a.shared);
+  // (0, 1, 8, 16 units: few rows, 16 tokens behind 10 - 400 29, 24, 24, 27 us, 128 on shared heads behind 500 - 16000 778, 775, 782, 792; many rows, eight pieces
+  // on shared heads in 8 bits 654, 606, 506, 526, a prompt of 2048 156, 140, 99, 104)
   a.lead = p.rt == 4 ? 8 : 1;
   a.per_part = p.parts > 0 ? 1.0 / static_cast<double>(p.parts) : 0.0;
   a.scale = static_cast<float>(std::fabs(scale) * 1.4426950408889634);

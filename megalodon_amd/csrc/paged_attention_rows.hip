@@ -7,7 +7,7 @@
 //     tile ahead, into LDS and in operand order, the next step's values while the last two columns of this one's are multiplied.
 //     Bound by what a CU is given of L2, 41 bytes a cycle while values are read: those of 256 keys take 17000 cycles, their products 8200,
 //     the tile's scores and softmax 4000 more.  The waves meet once a tile (twice, at the maxima and at the probabilities: 489 us).  A prompt
-//     of 8192 tokens in chunks of 4096, four heads of 256 / 2048: 465 us, 665 TFLOP/s.  One wave to a SIMD with 64 x 256 spilled 1.5 KB a lane;
+//     of 8192 tokens in chunks of 4096, four heads of 256 / 2048: 463 us, 668 TFLOP/s.  One wave to a SIMD with 64 x 256 spilled 1.5 KB a lane;
 //     four-wave workgroups of 64 x 512, whose scores are made twice, took a fifth longer, two-wave ones twice as long; blocks in other orders over
 //     the XCDs 5 and 40 % longer; the first values of a tile on their way during its scores do not fit the registers.
 //   - Up to 128: a workgroup is one wave, eight to a CU, and probabilities never leave the registers.  Bound by the issue of vector

@@ -9,7 +9,7 @@
 // Bound by HBM: a row is read once and written once.  A wave has a token, all of its heads or some of them: where the token lies is looked up
 // once (four loads that wait for each other), then its values go by, then its keys.  16, 32 or 64 lanes take a row, each lane pieces of eight
 // elements (one 16-byte access of 16-bit ones), which it keeps in registers between the maximum and the codes; lanes that a narrow row leaves
-// take the next heads.  Measured: 8-bit rows of 32000 positions back to 16 bits, 886 MB: 185 us, 4.8 TB/s (a large copy: 5.2); 4096 positions
+// take the next heads.  Measured: 8-bit rows of 32000 positions back to 16 bits, 885 MB: 185 us, 4.8 TB/s (the streaming copy: 5.9); 4096 positions
 // into 8 bits, 113 MB: 24 us, 4.7 TB/s; one token a sequence: a launch (4 - 5 us).  A wave a row instead: 215 us, the look-up in front of each.
 #include "paged.hpp"
 

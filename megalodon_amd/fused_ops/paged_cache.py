@@ -54,6 +54,6 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Te
     The token at position p sees positions from the start of its chunk of `chunk_size` (0: from the first) to p; its own key
     and value have been written before.  The number of query heads is a multiple of the cache's: h reads head
     h // (query heads // heads).  A token that sees no key, or whose scores are all -inf, gets zeros.  What 8-bit rows stand
-    for is rounded to q's dtype as paged_cache_read does.  Returns
+    for is rounded to q's dtype as paged_cache_read does (infinite past its largest number).  Returns
     (rows, query heads, v_width): rows behind the last sequence are zeros, or left as they are in a given `out`."""
     return _lib.host().paged_attention(q, k_pages, v_pages, block_table, lengths, cu_new, scale, chunk_size, k_exponents, v_exponents, out)
