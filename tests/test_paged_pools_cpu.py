@@ -10,7 +10,7 @@ from test_paged_cache_cpu import Cache, i64
 BF16, E4M3 = torch.bfloat16, torch.float8_e4m3fn
 
 
-def verdict(k, v, ke=None, ve=None):
+def answer(k, v, ke=None, ve=None):
     """The C entry's answer to a write of no rows: 0 or a refusal.  The tensors lend their addresses and strides."""
     fields = {"k_stride": k.stride()[:3], "v_stride": v.stride()[:3]}
     if ke is not None:
@@ -70,25 +70,25 @@ def layouts():
 
 @pytest.mark.parametrize("name,k,v", list(layouts()), ids=lambda x: x if isinstance(x, str) else "")
 def test_layouts(name, k, v):
-    assert verdict(k, v) == verdict(v, k) == int(share(k, v))
+    assert answer(k, v) == answer(v, k) == int(share(k, v))
 
 
 def test_rows_of_a_pool_that_share_memory():
     flat, v = torch.empty(4096, dtype=BF16), torch.empty(3, 16, 2, 32, dtype=BF16)
     for stride, meets in (((1024, 64, 32, 1), False), ((1024, 32, 512, 1), False), ((512, 64, 32, 1), True), ((1024, 48, 32, 1), True), ((1024, 64, 16, 1), True)):
         k = flat.as_strided((3, 16, 2, 32), stride)
-        assert verdict(k, v) == int(meets) and verdict(v, k) == int(meets)
+        assert answer(k, v) == int(meets) and answer(v, k) == int(meets)
 
 
 def test_exponents():
     k, v = (torch.empty(3, 16, 2, w, dtype=E4M3) for w in (32, 48))
     both = torch.empty(3, 16, 2, 2, dtype=torch.uint8)
-    assert verdict(k, v, both[..., 0], both[..., 1]) == 0
-    assert verdict(k, v, both[..., 0], both[..., 0]) == 1
+    assert answer(k, v, both[..., 0], both[..., 1]) == 0
+    assert answer(k, v, both[..., 0], both[..., 0]) == 1
     # exponents behind the codes of a row, and on them
     rows = torch.empty(3, 16, 2, 48, dtype=torch.uint8)
-    assert verdict(rows[..., :32].view(E4M3), v, rows[..., 32], both[..., 1]) == 0
-    assert verdict(rows[..., :32].view(E4M3), v, rows[..., 31], both[..., 1]) == 1
+    assert answer(rows[..., :32].view(E4M3), v, rows[..., 32], both[..., 1]) == 0
+    assert answer(rows[..., :32].view(E4M3), v, rows[..., 31], both[..., 1]) == 1
 
 
 def test_random_layouts_are_never_taken_for_apart():
@@ -110,7 +110,7 @@ def test_random_layouts_are_never_taken_for_apart():
             continue
         meets = share(k, v)
         met, apart = met + meets, apart + (not meets)
-        assert verdict(k, v) >= int(meets)
+        assert answer(k, v) >= int(meets)
         if k.stride() == v.stride():
-            assert verdict(k, v) == int(meets)
+            assert answer(k, v) == int(meets)
     assert met > 20 and apart > 20
