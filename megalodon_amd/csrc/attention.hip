@@ -22,6 +22,7 @@
 // diagonal by L2 - L1 columns in every one of these rules.
 #include "common.hpp"
 #include "dropkey.hpp"
+#include "gated.hpp"
 #include "linear_plan.hpp"
 
 #include <algorithm>
@@ -529,6 +530,57 @@ __device__ __forceinline__ void store_tile(const floatx16 (&acc)[IT][2], const G
   }
 }
 
+// silu(a) b and two of them in 16 bits.  (The quotient is IEEE's: exp(-a) may be infinite, then the result is 0 times b.)
+__device__ __forceinline__ float gated(float a, float b) { return a / (1.f + __expf(-a)) * b; }
+template <int DT>
+__device__ __forceinline__ uint2 pack4(const float* v) {
+  if (DT == MEGA_BF16) return uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+  return uint2{static_cast<uint32_t>(float_to_f16_bits(v[0])) | (static_cast<uint32_t>(float_to_f16_bits(v[1])) << 16),
+               static_cast<uint32_t>(float_to_f16_bits(v[2])) | (static_cast<uint32_t>(float_to_f16_bits(v[3])) << 16)};
+}
+// Epilogue of a workgroup of NW waves in two columns' groups ... whose accumulators [.][0] are columns of A B^T and [.][1] the same
+// columns of A B2^T: h = silu(a) b from float32, and where they are kept a and b, rounded once each.  `rows` x `cols` elements of the
+// workgroup's part at row0, col0 of the outputs go through `stage` ([row][cols + 8], shared by the waves), since a wave has 64-byte pieces of
+// rows and half lines are written slowly.  wrow, wcol: the wave's place in the part.
+template <int DT, int IT, int ROWS, int COLS, int THREADS>
+__device__ __forceinline__ void store_gate(const floatx16 (&acc)[IT][2], const GemmParams& p, int row0, int col0, int wrow, int wcol, int lane,
+                                           int thread, uint16_t* stage) {
+  constexpr int EP = COLS + 8, kPieces = COLS / 8;
+  const int n_out = p.Ca != nullptr ? 3 : 1;
+  const bool vec_ok = p.gate_n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.C) | reinterpret_cast<uintptr_t>(p.Ca) | reinterpret_cast<uintptr_t>(p.Cb)) % 16 == 0;
+  for (int what = 0; what < n_out; ++what) {
+    if (what > 0) lds_barrier();  // the output before has been read
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float a = acc[i][0][4 * q4 + e], b = acc[i][1][4 * q4 + e];
+          v[e] = what == 0 ? gated(a, b) : what == 1 ? a : b;
+        }
+        *reinterpret_cast<uint2*>(stage + (wrow + i * 32 + (lane & 31)) * EP + wcol + 8 * q4 + 4 * (lane >> 5)) = pack4<DT>(v);
+      }
+    lds_barrier();
+    uint16_t* const out = what == 0 ? p.C : what == 1 ? p.Ca : p.Cb;
+#pragma unroll 4
+    for (int c = thread; c < ROWS * kPieces; c += THREADS) {
+      const int row = c / kPieces, kc = c % kPieces * 8, grow = row0 + row, gcol = col0 + kc;
+      if (grow >= p.M || gcol >= p.gate_n) continue;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(stage + row * EP + kc);
+      uint16_t* dst = out + static_cast<int64_t>(grow) * p.gate_n + gcol;
+      if (vec_ok) {
+        *reinterpret_cast<u32x4*>(dst) = v;
+      } else {
+        const uint16_t* e = reinterpret_cast<const uint16_t*>(&v);
+        for (int q = 0; q < 8; ++q)
+          if (gcol + q < p.gate_n) dst[q] = e[q];
+      }
+    }
+  }
+}
+
 // CUT: a workgroup's part of an item, neighbours on an XCD; false where there is none.
 __device__ __forceinline__ bool cut_item(const GemmParams& p, int* item, int* part) {
   const int G = static_cast<int>(gridDim.x), lin = static_cast<int>(blockIdx.x);
@@ -604,7 +656,7 @@ __device__ __forceinline__ void load_to_lds16(u32x4 buffer, uint32_t offset, uin
 // T: the workgroup's tile, 256 (2 x 4 waves of 128 x 64) or 128 (2 x 2 waves of 64 x 64, two workgroups per CU).
 // RAG: p.kvb and p.ms are set (B k-major).  SEG: p.seg_start and the operands behind it are (apart, since the choice of the
 // operands with every request costs a product of one pair 10 %: 4096 x 1024 -> 2752 21.3 us, 23.6 so)
-template <int DT, bool TA, bool TB, bool RAG = false, int T = kTile, bool LIN = false, bool SEG = false, bool CUT = false>
+template <int DT, bool TA, bool TB, bool RAG = false, int T = kTile, bool LIN = false, bool SEG = false, bool CUT = false, bool GATE = false>
 __global__ __launch_bounds__(2 * T) void gemm_dma_kernel(const GemmParams p) {
   extern __shared__ __align__(16) uint16_t smem[];
   constexpr int JN = 2, NL = 2;
@@ -720,8 +772,13 @@ __global__ __launch_bounds__(2 * T) void gemm_dma_kernel(const GemmParams p) {
     else offa[i] = static_cast<uint32_t>((SEG ? 0 : static_cast<int64_t>(min(m0 + row, t.M - 1)) * t.lda + kb + ck * 8) * 2);
     if constexpr (SEG) row_a[i] = static_cast<uint32_t>(min(m0 + row, t.M - 1)), offa[i] = static_cast<uint32_t>(ck * 16);
     if (TB) offb[i] = static_cast<uint32_t>(((kb + krow) * p.ldb + min(n0 + cm * 8, t.N - 8)) * 2);
+    else if (GATE) offb[i] = static_cast<uint32_t>((static_cast<int64_t>(min(n0 / 2 + (pc >> 2) * 32 + (row & 31), p.gate_n - 1)) * p.ldb + kb + ck * 8) * 2);
     else offb[i] = static_cast<uint32_t>((static_cast<int64_t>(min(n0 + row, t.N - 1)) * p.ldb + kb + ck * 8) * 2);
   }
+  // GATE: pieces of 16 rows, two of one matrix and two of the other (all of a wave's are of one: NW is a multiple of 4)
+  static_assert(!GATE || (!TA && !TB && !RAG && !SEG), "two k-contiguous operands");
+  if constexpr (GATE)
+    if (__builtin_amdgcn_readfirstlane(wave) & 2) B = p.B2;
   const uint32_t stepa = static_cast<uint32_t>((TA ? t.lda : 1) * kSlab * 2);
   const uint32_t stepb = static_cast<uint32_t>((TB ? p.ldb : 1) * kSlab * 2);
   const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(
@@ -864,6 +921,7 @@ __global__ __launch_bounds__(2 * T) void gemm_dma_kernel(const GemmParams p) {
 #undef MEGA_SGB
 
   if constexpr (CUT) store_part<IT, NW>(acc, p, item, part, wave, lane, t.M - m0 - wm * 32 * IT);
+  else if constexpr (GATE) store_gate<DT, IT, T, T / 2, 2 * T>(acc, p, m0, n0 / 2, wm * 32 * IT, wn * 32, lane, tid, smem);
   else store_tile<DT, IT, LIN>(acc, p, t, RAG && !LIN ? p.ms : t.M, m0 + wm * 32 * IT, n0 + wn * 64, lane, smem + wave * 32 * IT * (64 + 8));
   // the output regions overlap the slab buffers: every read of this tile's epilogue
   // retires before the next tile's first slab is requested
@@ -889,7 +947,7 @@ constexpr int kDma64Operand = kTile * kSlab64;  // elements of an operand slab (
 constexpr int kDma64Stage = 2 * kDma64Operand;
 static_assert(sizeof(uint16_t) * 2 * kDma64Stage <= kDmaLds, "two slab buffers fit");
 
-template <int DT, bool TA, bool TB, int T = kTile, bool LIN = false, bool CUT = false>
+template <int DT, bool TA, bool TB, int T = kTile, bool LIN = false, bool CUT = false, bool GATE = false>
 __global__ __launch_bounds__(2 * T) void gemm_dma64_kernel(const GemmParams p) {
   extern __shared__ __align__(16) uint16_t smem[];
   constexpr int JN = 2, NL = 4;
@@ -972,8 +1030,13 @@ __global__ __launch_bounds__(2 * T) void gemm_dma64_kernel(const GemmParams p) {
     if (TA) offa[i] = static_cast<uint32_t>(((kb + krow) * t.lda + min(m0 + cm * 8, t.M - 8)) * 2);
     else offa[i] = static_cast<uint32_t>((static_cast<int64_t>(min(m0 + row, t.M - 1)) * t.lda + kb + ck * 8) * 2);
     if (TB) offb[i] = static_cast<uint32_t>(((kb + krow) * p.ldb + min(n0 + cm * 8, t.N - 8)) * 2);
+    else if (GATE) offb[i] = static_cast<uint32_t>((static_cast<int64_t>(min(n0 / 2 + (pc >> 3) * 32 + (row & 31), p.gate_n - 1)) * p.ldb + kb + ck * 8) * 2);
     else offb[i] = static_cast<uint32_t>((static_cast<int64_t>(min(n0 + row, t.N - 1)) * p.ldb + kb + ck * 8) * 2);
   }
+  // GATE: pieces of 8 rows, four of one matrix and four of the other: eight waves have one matrix each, four waves send them in turn
+  static_assert(!GATE || (!TA && !TB), "two k-contiguous operands");
+  const uint16_t* const b_odd = !GATE ? nullptr : NW == 8 && (__builtin_amdgcn_readfirstlane(wave) & 4) == 0 ? p.B : p.B2;
+  if constexpr (GATE && NW == 8) B = b_odd;
   const uint32_t stepa = static_cast<uint32_t>((TA ? t.lda : 1) * kSlab64 * 2);
   const uint32_t stepb = static_cast<uint32_t>((TB ? p.ldb : 1) * kSlab64 * 2);
   const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(
@@ -982,7 +1045,7 @@ __global__ __launch_bounds__(2 * T) void gemm_dma64_kernel(const GemmParams p) {
   auto request_one = [&](int s, int stage, int n) {
     const uint32_t sc = static_cast<uint32_t>(min(s, nslab - 1));
     const uint32_t dst = lds_wave + static_cast<uint32_t>(stage * kStage + (n >> 1) * NW * 512 + (n & 1) * kOperand) * 2;
-    if (n & 1) load_to_lds16(B, offb[n >> 1] + sc * stepb, dst);
+    if (n & 1) load_to_lds16(GATE && NW == 4 && (n >> 1) % 2 == 1 ? b_odd : B, offb[n >> 1] + sc * stepb, dst);
     else load_to_lds16(A, offa[n >> 1] + sc * stepa, dst);
   };
   auto request = [&](int s, int stage) {
@@ -1088,6 +1151,8 @@ __global__ __launch_bounds__(2 * T) void gemm_dma64_kernel(const GemmParams p) {
 
   if constexpr (CUT) {
     store_part<IT, NW>(acc, p, item, part, wave, lane, t.M - m0 - wm * 32 * IT);
+  } else if constexpr (GATE) {
+    store_gate<DT, IT, T, T / 2, 2 * T>(acc, p, m0, n0 / 2, wm * 32 * IT, wn * 32, lane, tid, smem);
   } else {
     store_tile<DT, IT, LIN>(acc, p, t, t.M, m0 + wm * 32 * IT, n0 + wn * 64, lane, smem + wave * 32 * IT * (64 + 8));
   }
@@ -1098,7 +1163,7 @@ __global__ __launch_bounds__(2 * T) void gemm_dma64_kernel(const GemmParams p) {
 
 // The parts of cut tiles added up, in order: 32 x 64 values of a wave of the product per workgroup, one wave, so that the parts
 // of few tiles are read by many CUs.
-template <int DT, int T, bool TA, bool TB>
+template <int DT, int T, bool TA, bool TB, bool GATE = false>
 __global__ __launch_bounds__(kWave) void linear_parts_kernel(const GemmParams p) {
   __shared__ __align__(16) uint16_t stage[32 * (64 + 8)];
   constexpr int IT = T / 64, NW = T / 32, kPart = 32 * IT * 64;  // blocks of 32 rows of a wave, waves, values of a wave
@@ -1126,7 +1191,8 @@ __global__ __launch_bounds__(kWave) void linear_parts_kernel(const GemmParams p)
         acc[0][j][4 * q4 + 2] += v.z;
         acc[0][j][4 * q4 + 3] += v.w;
       }
-  store_tile<DT, 1, true>(acc, p, t, t.M, t.mt * T + wm * 32 * IT + 32 * i, t.nt * T + wn * 64, lane, stage);
+  if constexpr (GATE) store_gate<DT, 1, 32, 32, kWave>(acc, p, t.mt * T + wm * 32 * IT + 32 * i, t.nt * (T / 2) + wn * 32, 0, 0, lane, lane, stage);
+  else store_tile<DT, 1, true>(acc, p, t, t.M, t.mt * T + wm * 32 * IT + 32 * i, t.nt * T + wn * 64, lane, stage);
 }
 
 // ---- one k-contiguous and one k-major operand: A in slabs of 64 k, B in slabs of 32 k ------
@@ -2049,7 +2115,68 @@ int launch_linear(GemmParams q, int kind, int count, const int64_t* sizes, hipSt
   return launch_tiles<gemm_dma_kernel<DT, true, true, false, kSmall, true>>(q, grid, threads, lds, s);
 }
 
+// Forward products of two layers that meet in silu(a) b: planned as one layer of 2 n_out features.
+template <int DT>
+int launch_gated(GemmParams q, int cus, hipStream_t s) {
+  q.nh = 1; q.alpha = 1.f; q.n_group = 8;
+  const int64_t both = q.N;
+  bool small = false;
+  plan(q, kForward, 1, &both, cus, &small);
+  const size_t lds = small ? sizeof(uint16_t) * kStages * 2 * kSmall * kSlab : kDmaLds;
+  const int threads = small ? 2 * kSmall : 2 * kTile;
+  int grid = (q.items + kXcds - 1) / kXcds * kXcds;
+  if (!small) grid = std::min(grid, std::max(cus / kXcds, 1) * kXcds);
+  if (!small && q.cut > 0) {
+    const int left = q.items - q.full;
+    GemmParams whole = q;
+    whole.items = q.full;
+    if (q.full > 0)
+      if (const int rc = launch_tiles<gemm_dma64_kernel<DT, false, false, kTile, false, false, true>>(whole, grid, threads, lds, s); rc != MEGA_OK) return rc;
+    grid = (left * q.cut + kXcds - 1) / kXcds * kXcds;
+    if (const int rc = launch_tiles<gemm_dma64_kernel<DT, false, false, kTile, false, true, true>>(q, grid, threads, lds, s); rc != MEGA_OK) return rc;
+    return launch_tiles<linear_parts_kernel<DT, kTile, false, false, true>>(q, left * 32, kWave, 0, s);
+  }
+  if (!small) return launch_tiles<gemm_dma64_kernel<DT, false, false, kTile, false, false, true>>(q, grid, threads, lds, s);
+  if (q.cut > 0) {
+    grid = (q.items * q.cut + kXcds - 1) / kXcds * kXcds;
+    if (const int rc = launch_tiles<gemm_dma_kernel<DT, false, false, false, kSmall, false, false, true, true>>(q, grid, threads, lds, s); rc != MEGA_OK) return rc;
+    return launch_tiles<linear_parts_kernel<DT, kSmall, false, false, true>>(q, q.items * 8, kWave, 0, s);
+  }
+  if (q.items <= cus) return launch_tiles<gemm_dma_kernel<DT, false, false, false, kSmall, false, false, false, true>>(q, grid, threads, lds, s);
+  return launch_tiles<gemm_dma64_kernel<DT, false, false, kSmall, false, false, true>>(q, grid, threads, lds, s);
+}
+
 }  // namespace
+
+int64_t gated_parts_bytes(int64_t tokens, int64_t n_in, int64_t n_out) {
+  int cus = 0;
+  if (compute_units(&cus) != MEGA_OK) return 0;
+  const int64_t both = 2 * n_out;
+  return linear_workspace_bytes(kForward, tokens, n_in, 1, &both, cus);
+}
+
+int weight_grad_onto(int dtype, const uint16_t* dy, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, const uint16_t* add,
+                     uint16_t* dw, float* parts, hipStream_t s) {
+  GemmParams g{};
+  g.A = dy; g.B = x; g.C = dw; g.add = add;
+  g.M = (int)n_out; g.N = (int)n_in; g.K = (int)tokens;
+  g.lda = n_out; g.ldb = n_in; g.ldc = n_in; g.ta = 1; g.tb = 1;
+  g.parts = parts; g.split_ok = parts != nullptr;
+  return dtype == MEGA_BF16 ? launch_linear<MEGA_BF16>(g, kWeightGrad, 1, &n_out, s) : launch_linear<MEGA_F16>(g, kWeightGrad, 1, &n_out, s);
+}
+
+int gated_product(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
+                  uint16_t* h, uint16_t* a, uint16_t* b, float* parts, hipStream_t s) {
+  GemmParams g{};
+  g.A = x; g.B = w1; g.B2 = w3; g.C = h; g.Ca = a; g.Cb = b;
+  g.M = (int)tokens; g.N = (int)(2 * n_out); g.K = (int)n_in; g.gate_n = (int)n_out;
+  g.lda = g.ldb = n_in; g.ldc = n_out;
+  g.parts = parts; g.split_ok = parts != nullptr;
+  int cus = 0;
+  if (const int rc = compute_units(&cus); rc != MEGA_OK) return rc;
+  return dtype == MEGA_BF16 ? launch_gated<MEGA_BF16>(g, cus, s) : launch_gated<MEGA_F16>(g, cus, s);
+}
+
 }  // namespace mega
 
 static int check_linear(const char* who, int kind, int dtype, int64_t tokens, int64_t n_in, int count, const int64_t* n_out) {
