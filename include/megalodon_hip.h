@@ -523,6 +523,49 @@ int mega_silu_mul_bwd(const void* dout, const void* a, const void* b, int dtype,
                       void* da, void* db, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Embedding (the reference's ParallelEmbedding at model-parallel world size 1,
+ * megalodon/modules/model_parallel/layers.py).
+ *
+ *   y[r] = scale * table[tokens[r]]; dw[v] = scale * sum over r with tokens[r] = v, v != padding, of dy[r]
+ *
+ * tokens: n numbers of token_bits (32 or 64) bits; table (vocab, width), rows ld elements apart; out, dy (n, width) and dw
+ * (vocab, width) contiguous, of `dtype` (MEGA_F32, MEGA_BF16, MEGA_F16), on any element's boundary.  n and vocab below 2^31,
+ * width up to 2^20.  A token that is no row of the table gives zeros and has no gradient; padding: a row without a gradient, or -1.
+ * Float32 inside, one rounding; sums run in an order that the sizes alone set, without atomics.
+ * bwd writes every row of dw and uses mega_embedding_workspace_bytes(...) bytes on a 16-byte boundary. */
+int mega_embedding_fwd(const void* tokens, int token_bits, const void* table, int dtype, int64_t n, int64_t vocab, int64_t width,
+                       int64_t ld, double scale, void* out, void* stream);
+int64_t mega_embedding_workspace_bytes(int dtype, int64_t n, int64_t vocab, int64_t width);
+int mega_embedding_bwd(const void* dy, int dtype, const void* tokens, int token_bits, int64_t n, int64_t vocab, int64_t width,
+                       double scale, int64_t padding, void* dw, void* workspace, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The norm of many tensors together, and clipping by it (the clip_grad_norm_ of the reference's training loop,
+ * megalodon/distributed/fairscale_fsdp.py, on one device).
+ *
+ *   norm = sqrt(sum of all squares), or the largest magnitude (MEGA_NORM_MAX); NaN where an element is NaN
+ *   to[i] = from[i] * min(1, max_norm / (norm + 1e-6))
+ *
+ * `count` tensors of size[i] elements of dtype[i] (MEGA_F32, MEGA_BF16, MEGA_F16), dense, on any element's boundary; `tensors` and the
+ * arrays in it are HOST memory, read before the call returns.  Squares and their sums in float64, so that no square overflows or
+ * vanishes; the order of summation is set by the sizes alone.  out_norm: one float32.
+ * scale: to[i] (of dtype[i]) may be from[i]; where nothing is to be scaled such a tensor is not read again.  No other
+ * overlap.  `workspace`: mega_tensors_workspace_bytes(...) bytes on a 16-byte boundary, for mega_tensors_clip the one that
+ * mega_tensors_norm of the same tensors left. */
+#define MEGA_NORM_2 0
+#define MEGA_NORM_MAX 1
+typedef struct mega_tensors {
+  int64_t count;
+  const void* const* from;
+  void* const* to;      /* mega_tensors_clip only */
+  const int64_t* size;
+  const int32_t* dtype;
+} mega_tensors;
+int64_t mega_tensors_workspace_bytes(const mega_tensors* tensors);
+int mega_tensors_norm(const mega_tensors* tensors, int kind, float* out_norm, void* workspace, void* stream);
+int mega_tensors_clip(const mega_tensors* tensors, double max_norm, const void* workspace, void* stream);
+
+/* ------------------------------------------------------------------------
  * The gated half of a feed-forward network, in one product kernel.
  *
  *   h = silu(x w1^T) * (x w3^T);  x (tokens, n_in), w1 and w3 (n_out, n_in), h (tokens, n_out)

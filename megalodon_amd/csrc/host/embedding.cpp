@@ -1,0 +1,77 @@
+// Embedding as a C++ autograd node (csrc/embedding.hip).
+#include "host.hpp"
+
+#include <torch/csrc/autograd/custom_function.h>
+
+namespace mega_host {
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+Tensor gather(const Tensor& tokens, const Tensor& table, double scale) {
+  const int64_t n = tokens.numel(), width = table.size(1);
+  auto shape = tokens.sizes().vec();
+  shape.push_back(width);
+  Tensor out = at::empty(shape, table.options());
+  const Tensor rows = width <= 1 || table.stride(1) == 1 ? table : table.contiguous();
+  check(mega_embedding_fwd(tokens.data_ptr(), tokens.scalar_type() == at::kLong ? 64 : 32, rows.data_ptr(), code_of(table.scalar_type()), n, table.size(0), width,
+                           rows.size(0) > 1 ? rows.stride(0) : width, scale, out.data_ptr(), stream_of(table)), "mega_embedding_fwd");
+  return out;
+}
+
+struct EmbeddingFn : Function<EmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& tokens, double scale, int64_t padding) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    ctx->saved_data["vocab"] = table.size(0);
+    return gather(tokens, table, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const Tensor tokens = ctx->get_saved_variables()[0].contiguous();  // (saved-tensor hooks may hand back any layout)
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const int64_t padding = ctx->saved_data["padding"].toInt(), vocab = ctx->saved_data["vocab"].toInt();
+    c10::DeviceGuard guard(g[0].device());
+    const int64_t width = g[0].size(-1), n = tokens.numel();
+    if (at::GradMode::is_enabled()) {  // differentiated again: recorded operations
+      const Tensor t = tokens.reshape({-1}).to(at::kLong), kept = at::logical_and(at::logical_and(t.ge(0), t.lt(vocab)), t.ne(padding));
+      const Tensor rows = at::where(kept.unsqueeze(1), g[0].reshape({-1, width}) * scale, 0);
+      return {at::zeros({vocab, width}, g[0].options()).index_add(0, t.clamp(0, vocab - 1), rows), Tensor(), Tensor(), Tensor()};
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor dy = stored(g[0]).contiguous();
+    const int code = code_of(dy.scalar_type());
+    Tensor dw = at::empty({vocab, width}, dy.options());
+    const Tensor ws = at::empty({mega_embedding_workspace_bytes(code, n, vocab, width)}, dy.options().dtype(at::kByte));
+    check(mega_embedding_bwd(dy.data_ptr(), code, tokens.data_ptr(), tokens.scalar_type() == at::kLong ? 64 : 32, n, vocab, width, scale, padding, dw.data_ptr(),
+                             n > 0 ? ws.data_ptr() : nullptr, stream_of(dy)), "mega_embedding_bwd");
+    return {dw, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor embedding(const Tensor& tokens_, const Tensor& table_, double scale, std::optional<int64_t> padding_) {
+  require(tokens_.is_cuda() && table_.is_cuda(), "megalodon_amd ops need GPU (HIP) tensors; there is no CPU fallback");
+  require(tokens_.device() == table_.device(), "all tensors must be on the same device");
+  require(tokens_.scalar_type() == at::kLong || tokens_.scalar_type() == at::kInt, "embedding: tokens must be int64 or int32");
+  require(table_.dim() == 2 && code_of(table_.scalar_type()) >= 0, "embedding: weight must be (vocabulary, width), float32, bfloat16 or float16");
+  const int64_t vocab = table_.size(0);
+  require(vocab >= 1 && table_.size(1) >= 1, "embedding: weight must not be empty");
+  int64_t padding = -1;
+  if (padding_.has_value()) {
+    require(*padding_ >= -vocab && *padding_ < vocab, "embedding: padding_idx must be a row of weight");
+    padding = *padding_ < 0 ? *padding_ + vocab : *padding_;
+  }
+  c10::DeviceGuard guard(table_.device());
+  const Tensor tokens = tokens_.contiguous(), table = stored(table_);
+  if ((at::GradMode::is_enabled() && table.requires_grad()) || has_tangent(table)) return EmbeddingFn::apply(table, tokens, scale, padding);
+  return gather(tokens, table, scale);
+}
+
+}  // namespace
+
+void bind_embedding(py::module_& m) { m.def("embedding", &embedding, py::call_guard<py::gil_scoped_release>()); }
+
+}  // namespace mega_host

@@ -49,7 +49,9 @@ inline Tensor stored(const Tensor& t) { return lazy(t) ? t.resolve_conj().resolv
 // whether a forward-mode derivative travels with the tensor
 inline bool has_tangent(const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
 
+void bind_clip(py::module_& m);
 void bind_decode(py::module_& m);
+void bind_embedding(py::module_& m);
 void bind_ops(py::module_& m);
 void bind_paged(py::module_& m);
 
