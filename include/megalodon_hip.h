@@ -573,7 +573,7 @@ int mega_tensors_clip(const mega_tensors* tensors, double max_norm, const void* 
  * (`F.silu(self.fc1(x)) * self.fc3(x)`, megalodon/modules/normalized_feedforward_network.py:82, with both projections.)
  * Tensors of `dtype` (MEGA_BF16 / MEGA_F16), contiguous, of any sizes from 1 (n_in and n_out up to 2^20, the two matrices
  * together, n_in rounded up to 64, below 2^30 elements, tokens below 2^31); x, the matrices and what is written for them on 16-byte boundaries.  Products and gate in float32, h rounded once from them.
- *   fwd: a = x w1^T and b = x w3^T (tokens, n_out) as well, or null for both; they are what bwd wants.
+ *   fwd: a = x w1^T and b = x w3^T (tokens, n_out) as well, in `kept` (`dtype` or MEGA_F32), or null for both; they are what bwd wants.
  *   bwd: dx (tokens, n_in) or null; dw (2, n_out, n_in), the gradients of w1 and w3, or null.  The gradients of a and b are
  *        rounded to `dtype`, operands of the matrix cores as they are; sums are float32 and rounded once (dw of more than
  *        2^30 / (2 n_out) tokens: once for each 2^30 / (2 n_out) of them).
@@ -581,8 +581,8 @@ int mega_tensors_clip(const mega_tensors* tensors, double max_norm, const void* 
  * (backward = 0, or bits: 1 for dx, 2 for dw) bytes that the call wants, on a 16-byte boundary. */
 int64_t mega_gated_linear_workspace_bytes(int64_t tokens, int64_t n_in, int64_t n_out, int backward);
 int mega_gated_linear_fwd(const void* x, const void* w1, const void* w3, int dtype, int64_t tokens, int64_t n_in, int64_t n_out,
-                          void* h, void* a, void* b, void* workspace, void* stream);
-int mega_gated_linear_bwd(const void* dh, const void* x, const void* w1, const void* w3, const void* a, const void* b, int dtype,
+                          void* h, void* a, void* b, int kept, void* workspace, void* stream);
+int mega_gated_linear_bwd(const void* dh, const void* x, const void* w1, const void* w3, const void* a, const void* b, int kept, int dtype,
                           int64_t tokens, int64_t n_in, int64_t n_out, void* dx, void* dw, void* workspace, void* stream);
 
 /* ------------------------------------------------------------------------

@@ -538,46 +538,50 @@ __device__ __forceinline__ uint2 pack4(const float* v) {
   return uint2{static_cast<uint32_t>(float_to_f16_bits(v[0])) | (static_cast<uint32_t>(float_to_f16_bits(v[1])) << 16),
                static_cast<uint32_t>(float_to_f16_bits(v[2])) | (static_cast<uint32_t>(float_to_f16_bits(v[3])) << 16)};
 }
-// Epilogue of a workgroup of NW waves in two columns' groups ... whose accumulators [.][0] are columns of A B^T and [.][1] the same
-// columns of A B2^T: h = silu(a) b from float32, and where they are kept a and b, rounded once each.  `rows` x `cols` elements of the
-// workgroup's part at row0, col0 of the outputs go through `stage` ([row][cols + 8], shared by the waves), since a wave has 64-byte pieces of
-// rows and half lines are written slowly.  wrow, wcol: the wave's place in the part.
+// Epilogue of waves whose accumulators [.][0] are 32 columns of A B^T and [.][1] the same columns of A B2^T: h = silu(a) b from float32,
+// and where they are kept a and b.  The ROWS x COLS elements at row0, col0 of the outputs go through `stage` ([row][.]), which all of
+// the workgroup's waves share, since a wave has 64-byte pieces of rows and half lines are written slowly.  wrow, wcol: the wave's
+// place among them.
 template <int DT, int IT, int ROWS, int COLS, int THREADS>
 __device__ __forceinline__ void store_gate(const floatx16 (&acc)[IT][2], const GemmParams& p, int row0, int col0, int wrow, int wcol, int lane,
-                                           int thread, uint16_t* stage) {
-  constexpr int EP = COLS + 8, kPieces = COLS / 8;
-  const int n_out = p.Ca != nullptr ? 3 : 1;
-  const bool vec_ok = p.gate_n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.C) | reinterpret_cast<uintptr_t>(p.Ca) | reinterpret_cast<uintptr_t>(p.Cb)) % 16 == 0;
-  for (int what = 0; what < n_out; ++what) {
-    if (what > 0) lds_barrier();  // the output before has been read
+                                           int thread, void* stage) {
+  const auto out = [&](auto zero, void* to, auto value) {
+    using T = decltype(zero);
+    constexpr int kPer = 16 / sizeof(T), EP = COLS + kPer, kPieces = COLS / kPer;
+    T* const st = static_cast<T*>(stage);
 #pragma unroll
     for (int i = 0; i < IT; ++i)
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
+        T* const at = st + (wrow + i * 32 + (lane & 31)) * EP + wcol + 8 * q4 + 4 * (lane >> 5);
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float a = acc[i][0][4 * q4 + e], b = acc[i][1][4 * q4 + e];
-          v[e] = what == 0 ? gated(a, b) : what == 1 ? a : b;
-        }
-        *reinterpret_cast<uint2*>(stage + (wrow + i * 32 + (lane & 31)) * EP + wcol + 8 * q4 + 4 * (lane >> 5)) = pack4<DT>(v);
+        for (int e = 0; e < 4; ++e) v[e] = value(acc[i][0][4 * q4 + e], acc[i][1][4 * q4 + e]);
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(at) = pack4<DT>(v);
+        else *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
       }
     lds_barrier();
-    uint16_t* const out = what == 0 ? p.C : what == 1 ? p.Ca : p.Cb;
+    const bool vec_ok = p.gate_n % kPer == 0 && reinterpret_cast<uintptr_t>(to) % 16 == 0;
 #pragma unroll 4
     for (int c = thread; c < ROWS * kPieces; c += THREADS) {
-      const int row = c / kPieces, kc = c % kPieces * 8, grow = row0 + row, gcol = col0 + kc;
+      const int row = c / kPieces, kc = c % kPieces * kPer, grow = row0 + row, gcol = col0 + kc;
       if (grow >= p.M || gcol >= p.gate_n) continue;
-      const u32x4 v = *reinterpret_cast<const u32x4*>(stage + row * EP + kc);
-      uint16_t* dst = out + static_cast<int64_t>(grow) * p.gate_n + gcol;
+      T* const dst = static_cast<T*>(to) + static_cast<int64_t>(grow) * p.gate_n + gcol;
       if (vec_ok) {
-        *reinterpret_cast<u32x4*>(dst) = v;
+        *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(st + row * EP + kc);
       } else {
-        const uint16_t* e = reinterpret_cast<const uint16_t*>(&v);
-        for (int q = 0; q < 8; ++q)
-          if (gcol + q < p.gate_n) dst[q] = e[q];
+        for (int q = 0; q < kPer; ++q)
+          if (gcol + q < p.gate_n) dst[q] = st[row * EP + kc + q];
       }
     }
+  };
+  out(uint16_t(), p.C, [](float a, float b) { return gated(a, b); });
+  if (p.Ca == nullptr) return;
+  for (int j = 0; j < 2; ++j) {
+    lds_barrier();  // the output before has been read
+    const auto one = [j](float a, float b) { return j == 0 ? a : b; };
+    if (p.wide) out(float(), j == 0 ? p.Ca : p.Cb, one);
+    else out(uint16_t(), j == 0 ? p.Ca : p.Cb, one);
   }
 }
 
@@ -2122,28 +2126,24 @@ int launch_gated(GemmParams q, int cus, hipStream_t s) {
   const int64_t both = q.N;
   bool small = false;
   plan(q, kForward, 1, &both, cus, &small);
-  const size_t lds = small ? sizeof(uint16_t) * kStages * 2 * kSmall * kSlab : kDmaLds;
-  const int threads = small ? 2 * kSmall : 2 * kTile;
-  int grid = (q.items + kXcds - 1) / kXcds * kXcds;
-  if (!small) grid = std::min(grid, std::max(cus / kXcds, 1) * kXcds);
-  if (!small && q.cut > 0) {
-    const int left = q.items - q.full;
-    GemmParams whole = q;
-    whole.items = q.full;
-    if (q.full > 0)
-      if (const int rc = launch_tiles<gemm_dma64_kernel<DT, false, false, kTile, false, false, true>>(whole, grid, threads, lds, s); rc != MEGA_OK) return rc;
-    grid = (left * q.cut + kXcds - 1) / kXcds * kXcds;
-    if (const int rc = launch_tiles<gemm_dma64_kernel<DT, false, false, kTile, false, true, true>>(q, grid, threads, lds, s); rc != MEGA_OK) return rc;
+  if (!small) {
+    const int whole = q.cut > 0 ? q.full : q.items, most = std::max(cus / kXcds, 1) * kXcds;
+    const GatedTiles t{q.A, q.B, q.B2, q.C, q.Ca, q.Cb, q.M, q.K, q.gate_n, q.mt_count, q.nt_count, whole};
+    if (whole > 0)
+      if (const int rc = gated_tiles(DT, q.Ca == nullptr ? 0 : q.wide ? 2 : 1, t, std::min((whole + kXcds - 1) / kXcds * kXcds, most), s); rc != MEGA_OK) return rc;
+    if (q.cut == 0) return MEGA_OK;
+    const int left = q.items - q.full, grid = (left * q.cut + kXcds - 1) / kXcds * kXcds;
+    if (const int rc = launch_tiles<gemm_dma64_kernel<DT, false, false, kTile, false, true, true>>(q, grid, 2 * kTile, kDmaLds, s); rc != MEGA_OK) return rc;
     return launch_tiles<linear_parts_kernel<DT, kTile, false, false, true>>(q, left * 32, kWave, 0, s);
   }
-  if (!small) return launch_tiles<gemm_dma64_kernel<DT, false, false, kTile, false, false, true>>(q, grid, threads, lds, s);
+  const size_t lds = sizeof(uint16_t) * kStages * 2 * kSmall * kSlab;
+  const int grid = (q.items * std::max(q.cut, 1) + kXcds - 1) / kXcds * kXcds;
   if (q.cut > 0) {
-    grid = (q.items * q.cut + kXcds - 1) / kXcds * kXcds;
-    if (const int rc = launch_tiles<gemm_dma_kernel<DT, false, false, false, kSmall, false, false, true, true>>(q, grid, threads, lds, s); rc != MEGA_OK) return rc;
+    if (const int rc = launch_tiles<gemm_dma_kernel<DT, false, false, false, kSmall, false, false, true, true>>(q, grid, 2 * kSmall, lds, s); rc != MEGA_OK) return rc;
     return launch_tiles<linear_parts_kernel<DT, kSmall, false, false, true>>(q, q.items * 8, kWave, 0, s);
   }
-  if (q.items <= cus) return launch_tiles<gemm_dma_kernel<DT, false, false, false, kSmall, false, false, false, true>>(q, grid, threads, lds, s);
-  return launch_tiles<gemm_dma64_kernel<DT, false, false, kSmall, false, false, true>>(q, grid, threads, lds, s);
+  if (q.items <= cus) return launch_tiles<gemm_dma_kernel<DT, false, false, false, kSmall, false, false, false, true>>(q, grid, 2 * kSmall, lds, s);
+  return launch_tiles<gemm_dma64_kernel<DT, false, false, kSmall, false, false, true>>(q, grid, 2 * kSmall, lds, s);
 }
 
 }  // namespace
@@ -2166,9 +2166,9 @@ int weight_grad_onto(int dtype, const uint16_t* dy, const uint16_t* x, int64_t t
 }
 
 int gated_product(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
-                  uint16_t* h, uint16_t* a, uint16_t* b, float* parts, hipStream_t s) {
+                  uint16_t* h, void* a, void* b, bool wide, float* parts, hipStream_t s) {
   GemmParams g{};
-  g.A = x; g.B = w1; g.B2 = w3; g.C = h; g.Ca = a; g.Cb = b;
+  g.A = x; g.B = w1; g.B2 = w3; g.C = h; g.Ca = a; g.Cb = b; g.wide = wide;
   g.M = (int)tokens; g.N = (int)(2 * n_out); g.K = (int)n_in; g.gate_n = (int)n_out;
   g.lda = g.ldb = n_in; g.ldc = n_out;
   g.parts = parts; g.split_ok = parts != nullptr;

@@ -2,7 +2,7 @@
 //   norm = sqrt(sum g^2) or max |g|; to = g min(1, max_norm / (norm + 1e-6))
 // Bound by the bytes: all tensors once for the norm, once more and a write for the scaling.  The tensors' addresses and sizes
 // are kernel arguments (a graph that is replayed has them with it; nothing is copied to the device), as many to a launch as
-// 4 KB of arguments hold.  A launch's tensors are cut into chunks of 64 KB, walked by a grid that fills the device; every
+// 4 KB of arguments hold.  A launch's tensors are cut into chunks, walked by a grid that fills the device; every
 // workgroup leaves one number, a second kernel adds them up in their order: no atomics, the same bits from call to call.
 // Squares and sums are float64 (a product of two floats is exact there, and neither 1e30 nor 1e-30 is lost); the vector units have
 // room for it, 4.5 elements a clock and CU at the memory's rate for 16 bits.
@@ -15,7 +15,6 @@ namespace mega {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunkBytes = 65536;
 constexpr int kGroups = 2048;  // workgroups of a launch: eight of four waves for each CU
 constexpr int kPerLaunch = 160;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -28,7 +27,7 @@ struct Tensors {
   uint32_t start[kPerLaunch + 1];
   uint16_t last[kPerLaunch];  // less one
   uint8_t dtype[kPerLaunch];
-  int count;
+  int count, chunk_bytes;
 };
 static_assert(sizeof(Tensors) <= 4000, "kernel arguments have 4 KB");
 
@@ -37,17 +36,21 @@ struct Chunk {
   void* to;
   int n, dtype;
 };
+// (The lanes look at all of the starts at once: a search by halves is a chain of up to eight loads of the arguments, each
+// waited for.)
 __device__ __forceinline__ Chunk chunk_of(const Tensors& t, uint32_t c) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (t.start[mid] <= c) lo = mid;
-    else hi = mid - 1;
+  const int lane = threadIdx.x % kWave;
+  int at = -1;
+#pragma unroll
+  for (int q = 0; q < (kPerLaunch + kWave - 1) / kWave; ++q) {
+    const int i = min(q * kWave + lane, kPerLaunch - 1);
+    at += __popcll(__ballot(q * kWave + lane < t.count && t.start[i] <= c));
   }
-  const int dtype = t.dtype[lo], size = dtype == MEGA_F32 ? 4 : 2;
-  const int64_t at = static_cast<int64_t>(c - t.start[lo]) * kChunkBytes;
-  const int n = c + 1 == t.start[lo + 1] ? t.last[lo] + 1 : kChunkBytes / size;
-  return {static_cast<const char*>(t.from[lo]) + at, static_cast<char*>(t.to[lo]) + at, n, dtype};
+  at = __builtin_amdgcn_readfirstlane(at);
+  const int dtype = t.dtype[at], size = dtype == MEGA_F32 ? 4 : 2;
+  const int64_t offset = static_cast<int64_t>(c - t.start[at]) * t.chunk_bytes;
+  const int n = c + 1 == t.start[at + 1] ? t.last[at] + 1 : t.chunk_bytes / size;
+  return {static_cast<const char*>(t.from[at]) + offset, static_cast<char*>(t.to[at]) + offset, n, dtype};
 }
 
 template <int DT>
@@ -96,9 +99,9 @@ __device__ __forceinline__ void norm_chunk(const Chunk& c, double& sum, uint32_t
 }
 
 // sum over the workgroup, in an order of its own, for thread 0
-template <bool MAX>
+template <bool MAX, int THREADS>
 __device__ __forceinline__ double workgroup_total(double sum, uint32_t most) {
-  __shared__ double sums[kThreads / kWave];
+  __shared__ double sums[THREADS / kWave];
   if constexpr (MAX) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), off)));
@@ -110,7 +113,8 @@ __device__ __forceinline__ double workgroup_total(double sum, uint32_t most) {
   if (threadIdx.x % kWave == 0) sums[threadIdx.x / kWave] = sum;
   __syncthreads();
   if (threadIdx.x != 0) return 0.0;
-  for (int w = 1; w < kThreads / kWave; ++w) {
+#pragma unroll
+  for (int w = 1; w < THREADS / kWave; ++w) {
     if constexpr (MAX) sum = sums[w] > sum || sums[w] != sums[w] ? sums[w] : sum;
     else sum += sums[w];
   }
@@ -128,26 +132,35 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const Tensors t, double*
     else if (k.dtype == MEGA_BF16) norm_chunk<MEGA_BF16, MAX>(k, sum, most);
     else norm_chunk<MEGA_F16, MAX>(k, sum, most);
   }
-  sum = workgroup_total<MAX>(sum, most);
+  sum = workgroup_total<MAX, kThreads>(sum, most);
   if (threadIdx.x == 0) totals[blockIdx.x] = sum;
 }
 
+// the workgroups' numbers: eight loads of a thread in flight
+constexpr int kTotalThreads = 512;
 template <bool MAX>
-__global__ __launch_bounds__(kThreads) void total_kernel(const double* totals, int64_t n, double* norm, float* out) {
+__global__ __launch_bounds__(kTotalThreads) void total_kernel(const double* totals, int64_t n, double* norm, float* out) {
   double sum = 0;
   uint32_t most = 0;
-  for (int64_t i = threadIdx.x; i < n; i += kThreads) {
-    if constexpr (MAX) most = max(most, magnitude(static_cast<float>(totals[i])));
-    else sum += totals[i];
+  for (int64_t i = threadIdx.x; i < n; i += 8 * kTotalThreads) {
+    double v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = totals[min(i + q * kTotalThreads, n - 1)];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if (i + q * kTotalThreads >= n) break;
+      if constexpr (MAX) most = max(most, magnitude(static_cast<float>(v[q])));
+      else sum += v[q];
+    }
   }
-  sum = workgroup_total<MAX>(sum, most);
+  sum = workgroup_total<MAX, kTotalThreads>(sum, most);
   if (threadIdx.x != 0) return;
   if constexpr (!MAX) sum = sqrt(sum);
   *norm = sum;
   *out = static_cast<float>(sum);
 }
 
-template <int DT>
+template <int DT, bool APART>
 __device__ __forceinline__ void scale_chunk(const Chunk& c, float factor) {
   using T = typename Elem<DT>::type;
   constexpr int kPer = DT == MEGA_F32 ? 4 : 8, kAhead = 4;
@@ -162,7 +175,9 @@ __device__ __forceinline__ void scale_chunk(const Chunk& c, float factor) {
     uint4 w;
     if constexpr (DT == MEGA_F32) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
     else w = pack8<DT>(v);
-    *reinterpret_cast<u32x4_any*>(to + static_cast<int64_t>(i) * kPer) = __builtin_bit_cast(u32x4_any, w);
+    u32x4_any* const at = reinterpret_cast<u32x4_any*>(to + static_cast<int64_t>(i) * kPer);
+    if constexpr (APART) __builtin_nontemporal_store(__builtin_bit_cast(u32x4_any, w), at);
+    else *at = __builtin_bit_cast(u32x4_any, w);
   };
   int i = threadIdx.x;
   for (; i + (kAhead - 1) * kThreads < whole; i += kAhead * kThreads) {
@@ -180,12 +195,15 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(const Tensors t, const 
   const double ratio = max_norm / (*norm + 1e-6);
   const float factor = ratio >= 1 ? 1.f : static_cast<float>(ratio);  // (NaN stays NaN)
   const uint32_t chunks = t.start[t.count];
-  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const Chunk k = chunk_of(t, c);
-    if (factor == 1.f && k.from == k.to) continue;
-    if (k.dtype == MEGA_F32) scale_chunk<MEGA_F32>(k, factor);
-    else if (k.dtype == MEGA_BF16) scale_chunk<MEGA_BF16>(k, factor);
-    else scale_chunk<MEGA_F16>(k, factor);
+  for (uint32_t i = blockIdx.x; i < chunks; i += gridDim.x) {
+    // (from the end: what the norm read last is the likeliest to be in the memory-side cache)
+    const Chunk k = chunk_of(t, chunks - 1 - i);
+    const bool apart = k.from != k.to;
+    if (factor == 1.f && !apart) continue;
+    const auto run = [&](auto together, auto streaming) { apart ? streaming(k, factor) : together(k, factor); };
+    if (k.dtype == MEGA_F32) run(scale_chunk<MEGA_F32, false>, scale_chunk<MEGA_F32, true>);
+    else if (k.dtype == MEGA_BF16) run(scale_chunk<MEGA_BF16, false>, scale_chunk<MEGA_BF16, true>);
+    else run(scale_chunk<MEGA_F16, false>, scale_chunk<MEGA_F16, true>);
   }
 }
 
@@ -199,13 +217,19 @@ int check_tensors(const char* who, const mega_tensors* t, bool to) {
   }
   return MEGA_OK;
 }
-int64_t chunks_of(const mega_tensors& t, int64_t i) { return (t.size[i] * elem_size(t.dtype[i]) + kChunkBytes - 1) / kChunkBytes; }
+// Chunks of 64 KB, or of 16 KB (four pieces a thread, all in flight at once) where 64 KB would leave the device part empty.
+int chunk_bytes_of(const mega_tensors& t) {
+  int64_t bytes = 0;
+  for (int64_t i = 0; i < t.count; ++i) bytes += t.size[i] * elem_size(t.dtype[i]);
+  return bytes < (int64_t{kGroups} << 16) ? 1 << 14 : 1 << 16;
+}
 constexpr int64_t kMostChunks = 1ll << 31;  // of a launch
 
 // The launches of a call, one after the other: f(tensors, workgroups).
 template <typename F>
 int each_launch(const mega_tensors& t, bool to, F f) {
   Tensors a{};
+  a.chunk_bytes = chunk_bytes_of(t);
   const auto flush = [&]() {
     if (a.count == 0) return static_cast<int>(MEGA_OK);
     const int rc = f(a, static_cast<unsigned>(std::min<int64_t>(a.start[a.count], kGroups)));
@@ -213,7 +237,7 @@ int each_launch(const mega_tensors& t, bool to, F f) {
     return rc;
   };
   for (int64_t i = 0; i < t.count; ++i) {
-    const int64_t chunks = chunks_of(t, i), size = elem_size(t.dtype[i]);
+    const int64_t size = elem_size(t.dtype[i]), chunks = (t.size[i] * size + a.chunk_bytes - 1) / a.chunk_bytes;
     if (chunks == 0) continue;
     if (a.count == kPerLaunch || (a.count > 0 && a.start[a.count] + chunks > kMostChunks))
       if (const int rc = flush(); rc != MEGA_OK) return rc;
@@ -221,7 +245,7 @@ int each_launch(const mega_tensors& t, bool to, F f) {
     a.from[k] = t.from[i];
     a.to[k] = to ? t.to[i] : nullptr;
     a.start[k + 1] = a.start[k] + static_cast<uint32_t>(chunks);
-    a.last[k] = static_cast<uint16_t>(t.size[i] - (chunks - 1) * (kChunkBytes / size) - 1);
+    a.last[k] = static_cast<uint16_t>(t.size[i] - (chunks - 1) * (a.chunk_bytes / size) - 1);
     a.dtype[k] = static_cast<uint8_t>(t.dtype[i]);
   }
   return flush();
@@ -258,8 +282,8 @@ extern "C" int mega_tensors_norm(const mega_tensors* tensors, int kind, float* o
     return static_cast<int>(MEGA_OK);
   });
   if (rc != MEGA_OK) return rc;
-  if (kind == MEGA_NORM_2) total_kernel<false><<<1, kThreads, 0, s>>>(totals, n, norm, out_norm);
-  else total_kernel<true><<<1, kThreads, 0, s>>>(totals, n, norm, out_norm);
+  if (kind == MEGA_NORM_2) total_kernel<false><<<1, kTotalThreads, 0, s>>>(totals, n, norm, out_norm);
+  else total_kernel<true><<<1, kTotalThreads, 0, s>>>(totals, n, norm, out_norm);
   MEGA_CHECK_LAUNCH();
   return MEGA_OK;
 }

@@ -39,12 +39,19 @@ template <int DT> struct Row {
       unpack8<DT>(q, v);
     }
   }
-  static __device__ __forceinline__ void store(T* p, int left, const float* v) {
+  // (a whole piece of what is read once)
+  static __device__ __forceinline__ void load_once(const T* p, int left, float* v) {
+    if (left >= kPer) unpack(__builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const Any*>(p))), v);
+    else load(p, left, v);
+  }
+  // (streaming: whole cache lines that nobody reads here; half lines are written slowly with the hint)
+  static __device__ __forceinline__ void store(T* p, int left, const float* v, bool streaming) {
     if (left >= kPer) {
       uint4 q;
       if constexpr (DT == MEGA_F32) q = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
       else q = pack8<DT>(v);
-      *reinterpret_cast<Any*>(p) = __builtin_bit_cast(Any, q);
+      if (streaming) __builtin_nontemporal_store(__builtin_bit_cast(Any, q), reinterpret_cast<Any*>(p));
+      else *reinterpret_cast<Any*>(p) = __builtin_bit_cast(Any, q);
     } else {
 #pragma unroll
       for (int e = 0; e < kPer; ++e)
@@ -57,7 +64,7 @@ template <int DT> struct Row {
 // A thread has one 16-byte piece of ROWS rows, so that as many table rows are in flight behind their tokens.
 template <int DT, typename Token, int ROWS>
 __global__ __launch_bounds__(kThreads) void gather_kernel(const Token* tokens, const typename Elem<DT>::type* table, typename Elem<DT>::type* out,
-                                                         int64_t n, int64_t vocab, int width, int64_t ld, float scale) {
+                                                         int64_t n, int64_t vocab, int width, int64_t ld, float scale, bool streaming) {
   constexpr int kPer = Row<DT>::kPer;
   const int pieces = (width + kPer - 1) / kPer;
   const int64_t groups = (n + ROWS - 1) / ROWS;
@@ -81,7 +88,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(const Token* tokens, c
       if (r0 + q >= n) break;
 #pragma unroll
       for (int e = 0; e < kPer; ++e) v[q][e] *= scale;
-      Row<DT>::store(out + (r0 + q) * width + k, width - k, v[q]);
+      Row<DT>::store(out + (r0 + q) * width + k, width - k, v[q], streaming);
     }
   }
 }
@@ -95,43 +102,47 @@ __device__ __forceinline__ uint32_t key_of(Token t, int64_t vocab, int64_t paddi
 }
 
 // Up to kRankTokens positions: the place of a position is the number of keys below its own and of equal ones in front of it, n^2 comparisons
-// with keys in LDS.  A workgroup has 64 positions, its waves a part of the keys each.
-constexpr int kRankTokens = 8192, kRankWaves = 16;
+// with keys in LDS.  A workgroup has 16 positions; sixteen lanes at a time have a 64th of the keys each.
+constexpr int kRankTokens = 8192, kRankWaves = 16, kRankEach = 16, kRankParts = kRankWaves * kWave / kRankEach;
 
 template <typename Token>
 __global__ __launch_bounds__(kRankWaves * kWave) void rank_kernel(const Token* tokens, int n, int64_t vocab, int64_t padding, uint32_t* keys, uint32_t* order) {
   __shared__ __align__(16) uint32_t all[kRankTokens + 4];
-  __shared__ uint32_t counts[kRankWaves][kWave];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  for (int j = threadIdx.x; j < (n + 3) / 4 * 4; j += kRankWaves * kWave) all[j] = j < n ? key_of(tokens[j], vocab, padding) : 0xffffffffu;
-  __syncthreads();
-  const int i = blockIdx.x * kWave + lane, first = blockIdx.x * kWave;
-  const uint32_t mine = i < n ? all[i] : 0xffffffffu;
+  __shared__ uint32_t counts[kRankParts][kRankEach];
   const int quads = (n + 3) / 4;
-  const int lo = quads * wave / kRankWaves * 4, hi = quads * (wave + 1) / kRankWaves * 4;
-  uint32_t count = 0;
-  // keys in front of the workgroup's positions (equal ones count), its own, and those behind (equal ones do not)
-  int j = lo;
-  for (; j < min(hi, first); j += 4) {
-    const uint4 q = *reinterpret_cast<const uint4*>(all + j);
-    count += (q.x <= mine) + (q.y <= mine) + (q.z <= mine) + (q.w <= mine);
-  }
-  for (; j < min(hi, first + kWave); ++j) count += all[j] < mine || (all[j] == mine && j < i);
-  for (; j < hi; j += 4) {
-    const uint4 q = *reinterpret_cast<const uint4*>(all + j);
-    count += (q.x < mine) + (q.y < mine) + (q.z < mine) + (q.w < mine);
-  }
-  counts[wave][lane] = count;
+  for (int j = threadIdx.x; j < quads * 4; j += kRankWaves * kWave) all[j] = j < n ? key_of(tokens[j], vocab, padding) : 0xffffffffu;
   __syncthreads();
-  if (wave > 0 || i >= n) return;
+  const int own = threadIdx.x % kRankEach, part = threadIdx.x / kRankEach, first = blockIdx.x * kRankEach, i = first + own;
+  const uint32_t mine = i < n ? all[i] : 0xffffffffu;
+  // quads of keys in front of the workgroup's positions (equal ones count), its own, and those behind (equal ones do not)
+  uint32_t count = 0;
+  const int own_quad = first / 4;
+  int q = part;
+#pragma unroll 4
+  for (; q < own_quad; q += kRankParts) {
+    const uint4 k = *reinterpret_cast<const uint4*>(all + 4 * q);
+    count += (k.x <= mine) + (k.y <= mine) + (k.z <= mine) + (k.w <= mine);
+  }
+  if (q < min(own_quad + kRankEach / 4, quads)) {
+    for (int j = 4 * q; j < 4 * q + 4; ++j) count += all[j] < mine || (all[j] == mine && j < i);
+    q += kRankParts;
+  }
+#pragma unroll 4
+  for (; q < quads; q += kRankParts) {
+    const uint4 k = *reinterpret_cast<const uint4*>(all + 4 * q);
+    count += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
+  }
+  counts[part][own] = count;
+  __syncthreads();
+  if (part > 0 || i >= n) return;
 #pragma unroll
-  for (int w = 1; w < kRankWaves; ++w) count += counts[w][lane];
+  for (int p = 1; p < kRankParts; ++p) count += counts[p][own];
   keys[count] = mine;
   order[count] = static_cast<uint32_t>(i);
 }
 
 // More: digits from the lowest up, each a stable move of all positions; a workgroup has kSortBlock of them.
-constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave, kSortEach = 4, kSortBlock = kSortThreads * kSortEach, kMostDigits = 2048;
+constexpr int kSortThreads = 512, kSortWaves = kSortThreads / kWave, kSortEach = 4, kSortBlock = kSortThreads * kSortEach, kMostDigits = 2048;
 
 // what the passes move: in the first, the tokens themselves
 template <typename Token>
@@ -167,11 +178,12 @@ __global__ __launch_bounds__(kSortThreads) void move_kernel(const Positions<Toke
   uint32_t* const seen = lds + digits;           // [wave][digits]
   __shared__ uint32_t wave_sums[kSortWaves];
   for (int d = threadIdx.x; d < digits * kSortWaves; d += kSortThreads) seen[d] = 0;
-  // two neighbouring digits a thread: their totals and those in front
-  uint32_t total[2] = {0, 0}, before[2] = {0, 0};
+  // neighbouring digits a thread: their totals and those in front
+  constexpr int kEach = kMostDigits / kSortThreads;
+  uint32_t total[kEach] = {}, before[kEach] = {}, sum = 0;
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int d = 2 * threadIdx.x + q;
+  for (int q = 0; q < kEach; ++q) {
+    const int d = kEach * threadIdx.x + q;
     if (d < digits) {
 #pragma unroll 8
       for (unsigned b = 0; b < gridDim.x; ++b) {
@@ -180,8 +192,9 @@ __global__ __launch_bounds__(kSortThreads) void move_kernel(const Positions<Toke
         total[q] += c;
       }
     }
+    sum += total[q];
   }
-  uint32_t sum = total[0] + total[1];
+  const uint32_t own = sum;
 #pragma unroll
   for (int step = 1; step < kWave; step *= 2) {
     const uint32_t up = __shfl_up(sum, step);
@@ -189,11 +202,12 @@ __global__ __launch_bounds__(kSortThreads) void move_kernel(const Positions<Toke
   }
   if (lane == kWave - 1) wave_sums[wave] = sum;
   __syncthreads();
-  uint32_t at = sum - total[0] - total[1];
+  uint32_t at = sum - own;
   for (int w = 0; w < wave; ++w) at += wave_sums[w];
-  if (2 * static_cast<int>(threadIdx.x) < digits) {
-    begins[2 * threadIdx.x] = at + before[0];
-    begins[2 * threadIdx.x + 1] = at + total[0] + before[1];
+#pragma unroll
+  for (int q = 0; q < kEach; ++q) {
+    if (kEach * static_cast<int>(threadIdx.x) + q < digits) begins[kEach * threadIdx.x + q] = at + before[q];
+    at += total[q];
   }
   __syncthreads();
   uint32_t key[kSortEach], rank[kSortEach];
@@ -249,6 +263,7 @@ struct SumParams {
   int width, per_piece, slices;
   int64_t pieces;
   float scale;
+  bool streaming;
 };
 constexpr int kZeroRows = 16;  // rows of dW that a workgroup looks at
 constexpr int kMostPiece = 1024;
@@ -283,7 +298,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
     const float zeros[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (uint32_t m = empty; m != 0; m &= m - 1) {
       T* const row = static_cast<T*>(p.dw) + (v0 + __builtin_ctz(m)) * p.width;
-      for (int k = tid * kPer; k < p.width; k += kThreads * kPer) R::store(row + k, p.width - k, zeros);
+      for (int k = tid * kPer; k < p.width; k += kThreads * kPer) R::store(row + k, p.width - k, zeros, p.streaming);
     }
     __syncthreads();
     }
@@ -310,7 +325,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
   for (int i = 0; i < count; i += kAhead) {
     float v[kAhead][kPer];
 #pragma unroll
-    for (int q = 0; q < kAhead; ++q) R::load(dy + static_cast<int64_t>(order[min(i + q, count - 1)]) * p.width, left, v[q]);
+    for (int q = 0; q < kAhead; ++q) R::load_once(dy + static_cast<int64_t>(order[min(i + q, count - 1)]) * p.width, left, v[q]);
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
       if (i + q >= count) break;
@@ -323,7 +338,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
       if (begun && ends) {
 #pragma unroll
         for (int e = 0; e < kPer; ++e) sum[e] *= p.scale;
-        R::store(dw + static_cast<int64_t>(key) * p.width, left, sum);
+        R::store(dw + static_cast<int64_t>(key) * p.width, left, sum, p.streaming);
       } else {
         // (a piece inside a run: its sum counts as that of the run's part from in front)
         float* const to = open + (begun ? p.width : 0);
@@ -341,31 +356,41 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
 // Runs over the end of the piece that they begin in: the parts of it and of the pieces behind, in their order.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void join_kernel(const SumParams p) {
-  const int64_t slices = (p.width + kThreads - 1) / kThreads, piece = blockIdx.x / slices;
+  const unsigned slices = (p.width + kThreads - 1) / kThreads, piece = blockIdx.x / slices;
   const int k = static_cast<int>(blockIdx.x % slices) * kThreads + threadIdx.x;
-  const int64_t first = piece * p.per_piece, behind = first + p.per_piece;
+  const int64_t first = static_cast<int64_t>(piece) * p.per_piece, behind = first + p.per_piece;
   if (behind >= p.n) return;
-  const uint32_t key = p.keys[behind];
-  if (key >= p.vocab || p.keys[behind - 1] != key) return;
-  if (p.keys[first] == key && first > 0 && p.keys[first - 1] == key) return;  // begins further in front
+  const uint32_t key = p.keys[behind], last = p.keys[behind - 1], head = p.keys[first], ahead = first > 0 ? p.keys[first - 1] : 0xffffffffu;
+  if (key >= p.vocab || last != key) return;
+  if (head == key && ahead == key) return;  // begins further in front
   // pieces behind whose first position is of the run
-  int64_t parts = 0;
+  int parts = 0;
   for (bool more = true; more; ) {
-    const int64_t at = behind + (parts + threadIdx.x % kWave) * p.per_piece;
+    const int64_t at = behind + static_cast<int64_t>(parts + threadIdx.x % kWave) * p.per_piece;
     const uint64_t in = __ballot(at < p.n && p.keys[min(at, p.n - 1)] == key);
     const int run = in == ~0ull ? kWave : __builtin_ctzll(~in);
     parts += run;
     more = run == kWave;
   }
   if (k >= p.width) return;
-  const float* const open = p.open + piece * 2 * p.width + k;
+  const int64_t step = 2 * static_cast<int64_t>(p.width);
+  const float* open = p.open + piece * step + k;
   float sum = open[p.width];
-#pragma unroll 8
-  for (int64_t q = 1; q <= parts; ++q) sum += open[q * 2 * p.width];
+  constexpr int kAhead = 16;  // parts in flight
+  for (; parts >= kAhead; parts -= kAhead) {
+    float v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) v[i] = *(open += step);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) sum += v[i];
+  }
+  for (; parts > 0; --parts) sum += *(open += step);
   Elem<DT>::store(static_cast<typename Elem<DT>::type*>(p.dw) + static_cast<int64_t>(key) * p.width + k, sum * p.scale);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------
+// rows of whole cache lines
+bool whole_lines(const void* p, int64_t width, int dtype) { return reinterpret_cast<uintptr_t>(p) % 128 == 0 && width * elem_size(dtype) % 128 == 0; }
 int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct Sizes {
@@ -380,8 +405,8 @@ struct Sizes {
     blocks = (n + kSortBlock - 1) / kSortBlock;
     const int per = kThreads * (dtype == MEGA_F32 ? 4 : 8);
     slices = static_cast<int>((width + per - 1) / per);
-    per_piece = 4;
-    while (per_piece < kMostPiece && per_piece * 2048ll < n * slices) per_piece *= 2;
+    per_piece = 16;
+    while (per_piece < kMostPiece && per_piece * 1024ll < n * slices) per_piece *= 2;
     pieces = (n + per_piece - 1) / per_piece;
     const bool sorts = n > kRankTokens;
     bytes = 0;
@@ -403,11 +428,12 @@ template <int DT, typename Token>
 int gather(const Token* tokens, const void* table, int64_t n, int64_t vocab, int64_t width, int64_t ld, float scale, void* out, hipStream_t s) {
   using T = typename Elem<DT>::type;
   const int64_t pieces = (width + Row<DT>::kPer - 1) / Row<DT>::kPer;
+  const bool streaming = whole_lines(out, width, DT);
   const auto grid = [&](int64_t rows) { return static_cast<unsigned>(std::min<int64_t>(((n + rows - 1) / rows * pieces + kThreads - 1) / kThreads, 1 << 20)); };
   if (n * pieces <= (1 << 18))
-    gather_kernel<DT, Token, 1><<<grid(1), kThreads, 0, s>>>(tokens, static_cast<const T*>(table), static_cast<T*>(out), n, vocab, static_cast<int>(width), ld, scale);
+    gather_kernel<DT, Token, 1><<<grid(1), kThreads, 0, s>>>(tokens, static_cast<const T*>(table), static_cast<T*>(out), n, vocab, static_cast<int>(width), ld, scale, streaming);
   else
-    gather_kernel<DT, Token, 4><<<grid(4), kThreads, 0, s>>>(tokens, static_cast<const T*>(table), static_cast<T*>(out), n, vocab, static_cast<int>(width), ld, scale);
+    gather_kernel<DT, Token, 4><<<grid(4), kThreads, 0, s>>>(tokens, static_cast<const T*>(table), static_cast<T*>(out), n, vocab, static_cast<int>(width), ld, scale, streaming);
   MEGA_CHECK_LAUNCH();
   return MEGA_OK;
 }
@@ -416,7 +442,7 @@ template <typename Token>
 int sort_positions(const Token* tokens, int64_t n, int64_t vocab, int64_t padding, const Sizes& z, char* ws, const uint32_t** keys, const uint32_t** order, hipStream_t s) {
   const auto at = [&](int64_t offset) { return reinterpret_cast<uint32_t*>(ws + offset); };
   if (n <= kRankTokens) {
-    rank_kernel<Token><<<static_cast<unsigned>((n + kWave - 1) / kWave), kRankWaves * kWave, 0, s>>>(tokens, static_cast<int>(n), vocab, padding, at(z.keys[0]), at(z.order[0]));
+    rank_kernel<Token><<<static_cast<unsigned>((n + kRankEach - 1) / kRankEach), kRankWaves * kWave, 0, s>>>(tokens, static_cast<int>(n), vocab, padding, at(z.keys[0]), at(z.order[0]));
     MEGA_CHECK_LAUNCH();
     *keys = at(z.keys[0]), *order = at(z.order[0]);
     return MEGA_OK;
@@ -441,7 +467,7 @@ int table_grad(const void* dy, const void* tokens, int token_bits, int64_t n, in
   const Sizes z(DT, n, vocab, width);
   SumParams p{};
   p.dy = dy, p.dw = dw, p.open = reinterpret_cast<float*>(ws + z.open);
-  p.n = n, p.vocab = vocab, p.width = static_cast<int>(width), p.per_piece = z.per_piece, p.slices = z.slices, p.pieces = z.pieces, p.scale = scale;
+  p.n = n, p.vocab = vocab, p.width = static_cast<int>(width), p.per_piece = z.per_piece, p.slices = z.slices, p.pieces = z.pieces, p.scale = scale, p.streaming = whole_lines(dw, width, DT);
   if (n > 0) {
     const int rc = token_bits == 64 ? sort_positions(static_cast<const int64_t*>(tokens), n, vocab, padding, z, ws, &p.keys, &p.order, s)
                                     : sort_positions(static_cast<const int32_t*>(tokens), n, vocab, padding, z, ws, &p.keys, &p.order, s);

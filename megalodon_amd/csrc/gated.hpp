@@ -1,4 +1,4 @@
-// The gated product between its entry points (gated_linear.hip) and the tiles that it runs in (attention.hip).
+// The gated product between its entry points (gated_linear.hip) and the tiles that it runs in (gated_tiles.hip, attention.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -6,10 +6,20 @@
 
 namespace mega {
 
-// h = silu(x w1^T) o (x w3^T) in tiles, and the two products where a and b are given; tokens * n_in and n_out * n_in below 2^30, n_in a
-// multiple of 64, rows of x, w1 and w3 on 16-byte boundaries.  parts: gated_parts_bytes, or null
+// h = silu(x w1^T) o (x w3^T), and the two products where they are kept (a and b; null: they are not); tokens * n_in and n_out * n_in
+// below 2^30, n_in a multiple of 64, rows of x, w1 and w3 on 16-byte boundaries.
+// Tiles 0 .. tiles - 1 of 256 tokens x 128 features, in bands of eight columns of tiles, row by row in each.
+struct GatedTiles {
+  const uint16_t *x, *w1, *w3;
+  uint16_t* h;
+  void *a, *b;
+  int tokens, n_in, n_out, row_tiles, col_tiles, tiles;
+};
+int gated_tiles(int dtype, int keep, const GatedTiles& p, int grid, hipStream_t s);
+
+// parts: gated_parts_bytes, or null; wide: a and b in float32
 int gated_product(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
-                  uint16_t* h, uint16_t* a, uint16_t* b, float* parts, hipStream_t s);
+                  uint16_t* h, void* a, void* b, bool wide, float* parts, hipStream_t s);
 int64_t gated_parts_bytes(int64_t tokens, int64_t n_in, int64_t n_out);
 
 }  // namespace mega

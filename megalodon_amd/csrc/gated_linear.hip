@@ -3,8 +3,9 @@
 //   da = dh b sigma(a) (1 + a (1 - sigma(a))), db = dh a sigma(a)
 //   dx = da w1 + db w3, dw1 = da^T x, dw3 = db^T x
 // One kernel has both projections: a wave's accumulators hold a and b of the same elements, and the gate is taken from them
-// in float32, so that neither product goes through memory (training keeps both, rounded, for the backward: 4 bytes an element
-// where float32 would be 8; the gradients that come of them are rounded to 16 bits for the matrix cores anyway).
+// in float32, so that neither product goes through memory.  Training keeps both for the backward, in float32 or rounded to the
+// operands' type: half the memory, and a third rounding of the gradients besides those of da and db (operands of the matrix
+// cores) and of the results.  KEEPMEASURE
 //
 // Many tokens: the product kernels of attention.hip with a gate for an epilogue (gated_product).  Few: the weights' stream from memory is all
 // the time there is, and the kernel below reads them once, straight into the operand registers of the matrix cores.
@@ -37,17 +38,27 @@ __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
 __device__ __forceinline__ float sigmoidf(float a) { return 1.f / (1.f + __expf(-a)); }
 
 // ---- few tokens -------------------------------------------------------------------------------------
-// A workgroup has 16 features of both matrices and all of the tokens (NT blocks of 16); its waves have equal runs of k and meet in
-// LDS, in their order.  A product of 16 features x 16 tokens x 32 k: lane l holds 8 k of feature l % 16 and 8 k of token l % 16,
-// k = 32 step + 8 (l / 16), so that both come from memory as they are, 64 bytes of a row to four lanes.  It gives lane l
-// token l % 16 of features 4 (l / 16) .. + 3.
+// A workgroup has FT groups of 8 features and all of the tokens (NT blocks of 16); its waves take turns along k and meet in LDS, in
+// their order.  A product of 16 rows (8 features of w1, the same 8 of w3) x 16 tokens x 32 k: lane l holds 8 k of row l % 16 and
+// 8 k of token l % 16, k = 32 step + 8 (l / 16), so that both come from memory as they are, 64 bytes of a row to four lanes, and what a workgroup has
+// in flight are whole pieces of rows.  It gives lane l token l % 16 of rows 4 (l / 16) .. + 3.
 // Rows behind the last feature or token are the last one again, never stored.  WHOLE: rows are whole 16-byte pieces.
-constexpr int kFewTokens = 64, kFewWaves = 8;
+constexpr int kFewWaves = 8;
+
+// Which calls go here: up to 16 tokens all; then the tokens, read again for every few features, cost more than the tiles' second launch
+// the more the larger the weights are (us, here / tiles: 4096 -> 11008 16 tokens 47 / 50, 24 53 / 51, 64 80 / 54; 2048 -> 5504
+// 16 15 / 19, 48 20.2 / 20.7, 64 21.9 / 20.8; 1024 -> 2752 64 8.4 / 12.7).  Rows that the tiles need laid out anew: up to 64.
+bool few(int64_t tokens, int64_t n_in, int64_t n_out) {
+  if (tokens <= 16 || tokens > 64) return tokens <= 16;
+  return n_in % 64 != 0 || static_cast<double>(tokens - 16) * n_in * n_out <= 4e8;
+}
+
 
 struct FewParams {
   const uint16_t *x, *w1, *w3;
-  uint16_t *h, *a, *b;
-  int tokens, n_in, n_out;
+  uint16_t* h;
+  void *a, *b;
+  int tokens, n_in, n_out, wide;
 };
 
 template <bool WHOLE>
@@ -62,80 +73,107 @@ __device__ __forceinline__ u32x4 eight(const uint16_t* row, int k, int n) {
   return u32x4{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
 }
 
-template <int DT, int NT, bool WHOLE>
+template <int DT, int NT, int FT, bool WHOLE>
 __global__ __launch_bounds__(kFewWaves * kWave) void gated_few_kernel(const FewParams p) {
-  __shared__ f32x4 sums[kFewWaves][2 * NT][kWave];
+  __shared__ f32x4 sums[kFewWaves][FT * NT][kWave];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r = lane % 16, g = lane / 16;
-  const int f0 = blockIdx.x * 16;
-  const int64_t feature = static_cast<int64_t>(min(f0 + r, p.n_out - 1)) * p.n_in;
-  const uint16_t *w1 = p.w1 + feature, *w3 = p.w3 + feature;
-  const uint16_t* x[NT];
+  const int f0 = blockIdx.x * (8 * FT);
+  const uint16_t *w[FT], *x[NT];
+#pragma unroll
+  for (int f = 0; f < FT; ++f) w[f] = (r < 8 ? p.w1 : p.w3) + static_cast<int64_t>(min(f0 + 8 * f + r % 8, p.n_out - 1)) * p.n_in;
 #pragma unroll
   for (int t = 0; t < NT; ++t) x[t] = p.x + static_cast<int64_t>(min(16 * t + r, p.tokens - 1)) * p.n_in;
-  f32x4 acc[2][NT];
+  f32x4 acc[FT][NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) acc[0][t] = acc[1][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int steps = (p.n_in + 31) / 32, lo = steps * wave / kFewWaves, hi = steps * (wave + 1) / kFewWaves;
-  constexpr int U = NT > 2 ? 2 : 4;  // steps whose operands are asked for together
-  int s = lo;
-  for (; s + U <= hi && 32 * (s + U) <= p.n_in; s += U) {
-    u32x4 a[U], b[U], v[U][NT];
+  for (int f = 0; f < FT; ++f)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[f][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int steps = p.n_in / 32;  // (whole ones)
+  constexpr int U = FT * NT > 1 && FT * NT <= 4 ? 4 : 1;  // steps whose operands are asked for together (measured)
+  // Every workgroup begins somewhere else along k: in step with each other they would all ask the same channels of L2 and memory.
+  const int rounds = steps / (U * kFewWaves);
+  int at = rounds > 0 ? static_cast<int>(blockIdx.x % rounds) : 0;
+  for (int i = 0; i < rounds; ++i) {
+    const int s = at * (U * kFewWaves) + wave;
+    if (++at == rounds) at = 0;
+    u32x4 a[U][FT], v[U][NT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = 32 * (s + u) + 8 * g;
-      a[u] = eight<WHOLE>(w1, k, 0x7fffffff);
-      b[u] = eight<WHOLE>(w3, k, 0x7fffffff);
+      const int k = 32 * (s + u * kFewWaves) + 8 * g;
+#pragma unroll
+      for (int f = 0; f < FT; ++f) a[u][f] = eight<WHOLE>(w[f], k, 0x7fffffff);
 #pragma unroll
       for (int t = 0; t < NT; ++t) v[u][t] = eight<WHOLE>(x[t], k, 0x7fffffff);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        acc[0][t] = mma16<DT>(a[u], v[u][t], acc[0][t]);
-        acc[1][t] = mma16<DT>(b[u], v[u][t], acc[1][t]);
-      }
+      for (int f = 0; f < FT; ++f)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[f][t] = mma16<DT>(a[u][f], v[u][t], acc[f][t]);
   }
-  for (; s < hi; ++s) {
+  for (int s = rounds * (U * kFewWaves) + wave; 32 * s < p.n_in; s += kFewWaves) {
     const int k = 32 * s + 8 * g;
-    const u32x4 a = eight<WHOLE>(w1, k, p.n_in), b = eight<WHOLE>(w3, k, p.n_in);
+    u32x4 a[FT], v[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const u32x4 v = eight<WHOLE>(x[t], k, p.n_in);
-      acc[0][t] = mma16<DT>(a, v, acc[0][t]);
-      acc[1][t] = mma16<DT>(b, v, acc[1][t]);
-    }
+    for (int f = 0; f < FT; ++f) a[f] = eight<WHOLE>(w[f], k, p.n_in);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) v[t] = eight<WHOLE>(x[t], k, p.n_in);
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[f][t] = mma16<DT>(a[f], v[t], acc[f][t]);
   }
 #pragma unroll
-  for (int t = 0; t < NT; ++t) sums[wave][t][lane] = acc[0][t], sums[wave][NT + t][lane] = acc[1][t];
+  for (int f = 0; f < FT; ++f)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) sums[wave][f * NT + t][lane] = acc[f][t];
   __syncthreads();
-  if (wave >= NT) return;
-  const int token = 16 * wave + r, f = f0 + 4 * g;
-  f32x4 a = sums[0][wave][lane], b = sums[0][NT + wave][lane];
+  // a wave adds up half a block: features 4 half .. + 3 of 16 tokens are lanes 16 half .. of a and 32 lanes on of b
+  for (int i = threadIdx.x / 16; i < FT * NT * 2; i += kFewWaves * kWave / 16) {
+    const int block = i / 2, half = i % 2, at = 16 * half + r;
+    f32x4 a = sums[0][block][at], b = sums[0][block][at + 32];
 #pragma unroll
-  for (int w = 1; w < kFewWaves; ++w) a += sums[w][wave][lane], b += sums[w][NT + wave][lane];
-  if (token >= p.tokens) return;
-  const int64_t at = static_cast<int64_t>(token) * p.n_out + f;
+    for (int q = 1; q < kFewWaves; ++q) a += sums[q][block][at], b += sums[q][block][at + 32];
+    const int token = 16 * (block % NT) + r, f = f0 + 8 * (block / NT) + 4 * half;
+    if (token >= p.tokens) continue;
+    const int64_t to = static_cast<int64_t>(token) * p.n_out + f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (f + e >= p.n_out) break;
-    Elem<DT>::store(p.h + at + e, a[e] * sigmoidf(a[e]) * b[e]);
-    if (p.a != nullptr) Elem<DT>::store(p.a + at + e, a[e]), Elem<DT>::store(p.b + at + e, b[e]);
+    for (int e = 0; e < 4; ++e) {
+      if (f + e >= p.n_out) break;
+      Elem<DT>::store(p.h + to + e, a[e] * sigmoidf(a[e]) * b[e]);
+      if (p.a == nullptr) continue;
+      if (p.wide) static_cast<float*>(p.a)[to + e] = a[e], static_cast<float*>(p.b)[to + e] = b[e];
+      else Elem<DT>::store(static_cast<uint16_t*>(p.a) + to + e, a[e]), Elem<DT>::store(static_cast<uint16_t*>(p.b) + to + e, b[e]);
+    }
   }
 }
 
-template <int DT>
+template <int DT, int NT, int FT>
 int launch_few(const FewParams& p, hipStream_t s) {
-  const dim3 grid((p.n_out + 15) / 16), block(kFewWaves * kWave);
-  const bool whole = p.n_in % 8 == 0;
-#define MEGA_FEW(NT)                                                              \
-  (whole ? gated_few_kernel<DT, NT, true><<<grid, block, 0, s>>>(p) : gated_few_kernel<DT, NT, false><<<grid, block, 0, s>>>(p))
-  if (p.tokens <= 16) MEGA_FEW(1);
-  else if (p.tokens <= 32) MEGA_FEW(2);
-  else MEGA_FEW(4);
-#undef MEGA_FEW
+  const dim3 grid((p.n_out + 8 * FT - 1) / (8 * FT)), block(kFewWaves * kWave);
+  if (p.n_in % 8 == 0) gated_few_kernel<DT, NT, FT, true><<<grid, block, 0, s>>>(p);
+  else gated_few_kernel<DT, NT, FT, false><<<grid, block, 0, s>>>(p);
   MEGA_CHECK_LAUNCH();
   return MEGA_OK;
+}
+// Groups of 8 features of a workgroup: the fewer, the more workgroups; the more, the fewer times the tokens are read.  Whatever leaves the
+// CU with the most features the fewest of them, and of equals the larger: us, one / two groups, 1 and 16 tokens: 4096 -> 11008 (6 / 6
+// groups a CU) 36.7 / 36.2 and 57.8 / 46.5, 2048 -> 5504 (3 / 4) 10.4 / 12.5 and 14.1 / 16.8, 1024 -> 2752 (2 / 2) 4.9 / 4.7 and 6.2 / 5.3; two / four
+// groups, 32 tokens 60 / 62, 18.8 / 16.7, 6.4 / 8.3.
+template <int DT, int NT, int FT>
+int few_of(const FewParams& p, int cus, hipStream_t s) {
+  const auto most = [&](int groups) { return ((p.n_out + 8 * groups - 1) / (8 * groups) + cus - 1) / cus * groups; };
+  return most(2 * FT) <= most(FT) ? launch_few<DT, NT, 2 * FT>(p, s) : launch_few<DT, NT, FT>(p, s);
+}
+template <int DT>
+int few_tokens(const FewParams& p, hipStream_t s) {
+  int dev = 0, cus = 0;
+  MEGA_CHECK_HIP(hipGetDevice(&dev));
+  MEGA_CHECK_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+  if (p.tokens <= 16) return few_of<DT, 1, 1>(p, cus, s);
+  if (p.tokens <= 32) return few_of<DT, 2, 2>(p, cus, s);
+  return few_of<DT, 4, 2>(p, cus, s);
 }
 
 // ---- rows of whole 16-byte pieces, and back -----------------------------------------------------------
@@ -180,9 +218,26 @@ int narrow(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t from, int64
 }
 
 // ---- the gate's backward --------------------------------------------------------------------------------
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+template <int DT, bool WIDE>
+__device__ __forceinline__ void kept_eight(const void* row, int k, int n, float* v) {
+  if constexpr (!WIDE) {
+    unpack8<DT>(__builtin_bit_cast(uint4, eight<false>(static_cast<const uint16_t*>(row), k, n)), v);
+  } else {
+    const float* const p = static_cast<const float*>(row) + k;
+    if (k + 8 <= n) {
+      const f32x4_any lo = *reinterpret_cast<const f32x4_any*>(p), hi = *reinterpret_cast<const f32x4_any*>(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = k + e < n ? p[e] : 0.f;
+    }
+  }
+}
 // da, db (tokens, ld) from dh, a, b (tokens, n): 8 elements a thread, zeros from column n to `to`
-template <int DT>
-__global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh, const uint16_t* a, const uint16_t* b, uint16_t* da, uint16_t* db,
+template <int DT, bool WIDE>
+__global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh, const void* a, const void* b, uint16_t* da, uint16_t* db,
                                                             int64_t tokens, int n, int to, int64_t ld) {
   const int64_t pieces = tokens * (to / 8);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < pieces; i += static_cast<int64_t>(gridDim.x) * kThreads) {
@@ -190,8 +245,8 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh,
     const int k = static_cast<int>(i % (to / 8)) * 8;
     float g[8], u[8], v[8], du[8], dv[8];
     unpack8<DT>(__builtin_bit_cast(uint4, eight<false>(dh + row * n, k, n)), g);
-    unpack8<DT>(__builtin_bit_cast(uint4, eight<false>(a + row * n, k, n)), u);
-    unpack8<DT>(__builtin_bit_cast(uint4, eight<false>(b + row * n, k, n)), v);
+    kept_eight<DT, WIDE>(static_cast<const char*>(a) + row * n * (WIDE ? 4 : 2), k, n, u);
+    kept_eight<DT, WIDE>(static_cast<const char*>(b) + row * n * (WIDE ? 4 : 2), k, n, v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float s = sigmoidf(u[e]);
@@ -222,7 +277,7 @@ struct Forward {
   Forward(int64_t tokens, int64_t n_in, int64_t n_out) {
     Room room;
     k = n_in, rows = tokens, x = w1 = w3 = parts = 0;
-    if (tokens > kFewTokens) {
+    if (!few(tokens, n_in, n_out)) {
       k = up(n_in, 64);
       rows = std::min(tokens, std::max<int64_t>((kMost - 1) / k / 256 * 256, 256));
       if (k != n_in) {
@@ -281,16 +336,18 @@ extern "C" int64_t mega_gated_linear_workspace_bytes(int64_t tokens, int64_t n_i
 }
 
 extern "C" int mega_gated_linear_fwd(const void* x_, const void* w1_, const void* w3_, int dtype, int64_t tokens, int64_t n_in, int64_t n_out,
-                                     void* h_, void* a_, void* b_, void* workspace, void* stream) {
+                                     void* h_, void* a, void* b, int kept, void* workspace, void* stream) {
   if (const int rc = check("mega_gated_linear_fwd", dtype, tokens, n_in, n_out); rc != MEGA_OK) return rc;
-  MEGA_CHECK_ARG(x_ && w1_ && w3_ && h_ && (a_ == nullptr) == (b_ == nullptr), "mega_gated_linear_fwd: null pointer");
+  MEGA_CHECK_ARG(x_ && w1_ && w3_ && h_ && (a == nullptr) == (b == nullptr), "mega_gated_linear_fwd: null pointer");
+  MEGA_CHECK_ARG(kept == dtype || kept == MEGA_F32, "mega_gated_linear_fwd: the products are kept in the operands' type or in float32");
   for (const void* q : {x_, w1_, w3_, static_cast<const void*>(workspace)}) MEGA_CHECK_ARG(aligned16(q), "mega_gated_linear_fwd: misaligned pointer");
   const uint16_t *x = static_cast<const uint16_t*>(x_), *w1 = static_cast<const uint16_t*>(w1_), *w3 = static_cast<const uint16_t*>(w3_);
-  uint16_t *h = static_cast<uint16_t*>(h_), *a = static_cast<uint16_t*>(a_), *b = static_cast<uint16_t*>(b_);
+  uint16_t* h = static_cast<uint16_t*>(h_);
+  const bool wide = kept == MEGA_F32;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (tokens <= kFewTokens) {
-    const FewParams p{x, w1, w3, h, a, b, static_cast<int>(tokens), static_cast<int>(n_in), static_cast<int>(n_out)};
-    return dtype == MEGA_BF16 ? launch_few<MEGA_BF16>(p, s) : launch_few<MEGA_F16>(p, s);
+  if (few(tokens, n_in, n_out)) {
+    const FewParams p{x, w1, w3, h, a, b, static_cast<int>(tokens), static_cast<int>(n_in), static_cast<int>(n_out), wide};
+    return dtype == MEGA_BF16 ? few_tokens<MEGA_BF16>(p, s) : few_tokens<MEGA_F16>(p, s);
   }
   const Forward f(tokens, n_in, n_out);
   MEGA_CHECK_ARG(workspace != nullptr || f.bytes == 0, "mega_gated_linear_fwd: null workspace");
@@ -310,22 +367,23 @@ extern "C" int mega_gated_linear_fwd(const void* x_, const void* w1_, const void
       rows = at(f.x);
     }
     const bool cut = gated_parts_bytes(n, f.k, n_out) > 0;
-    if (const int rc = gated_product(dtype, rows, w1, w3, n, f.k, n_out, h + t * n_out, a ? a + t * n_out : nullptr, b ? b + t * n_out : nullptr,
-                                     cut ? reinterpret_cast<float*>(ws + f.parts) : nullptr, s);
+    const auto rows_of = [&](void* q) { return q == nullptr ? nullptr : static_cast<char*>(q) + t * n_out * (wide ? 4 : 2); };
+    if (const int rc = gated_product(dtype, rows, w1, w3, n, f.k, n_out, h + t * n_out, rows_of(a), rows_of(b), wide, cut ? reinterpret_cast<float*>(ws + f.parts) : nullptr, s);
         rc != MEGA_OK)
       return rc;
   }
   return MEGA_OK;
 }
 
-extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void* w1_, const void* w3_, const void* a_, const void* b_, int dtype,
+extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void* w1_, const void* w3_, const void* a, const void* b, int kept, int dtype,
                                      int64_t tokens, int64_t n_in, int64_t n_out, void* dx_, void* dw_, void* workspace, void* stream) {
   if (const int rc = check("mega_gated_linear_bwd", dtype, tokens, n_in, n_out); rc != MEGA_OK) return rc;
-  MEGA_CHECK_ARG(dh_ && x_ && w1_ && w3_ && a_ && b_ && workspace, "mega_gated_linear_bwd: null pointer");
+  MEGA_CHECK_ARG(dh_ && x_ && w1_ && w3_ && a && b && workspace, "mega_gated_linear_bwd: null pointer");
+  MEGA_CHECK_ARG(kept == dtype || kept == MEGA_F32, "mega_gated_linear_bwd: the products are kept in the operands' type or in float32");
   for (const void* q : {x_, w1_, w3_, static_cast<const void*>(dx_), static_cast<const void*>(dw_), static_cast<const void*>(workspace)})
     MEGA_CHECK_ARG(aligned16(q), "mega_gated_linear_bwd: misaligned pointer");
   const auto u = [](const void* q) { return static_cast<const uint16_t*>(q); };
-  const uint16_t *dh = u(dh_), *x = u(x_), *w1 = u(w1_), *w3 = u(w3_), *a = u(a_), *b = u(b_);
+  const uint16_t *dh = u(dh_), *x = u(x_), *w1 = u(w1_), *w3 = u(w3_);
   uint16_t *dx = static_cast<uint16_t*>(dx_), *dw = static_cast<uint16_t*>(dw_);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int what = (dx != nullptr) + 2 * (dw != nullptr);
@@ -350,16 +408,19 @@ extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void
     uint16_t *da = at(f.g), *db = f.apart ? da + n * h : da + h;
     const int64_t ld = f.apart ? h : 2 * h, at0 = t * n_out;
     const unsigned grid = pieces_grid(n * (h / 8));
-    if (dtype == MEGA_BF16) gate_grad_kernel<MEGA_BF16><<<grid, kThreads, 0, s>>>(dh + at0, a + at0, b + at0, da, db, n, (int)n_out, (int)h, ld);
-    else gate_grad_kernel<MEGA_F16><<<grid, kThreads, 0, s>>>(dh + at0, a + at0, b + at0, da, db, n, (int)n_out, (int)h, ld);
+    const bool wide = kept == MEGA_F32;
+    const auto rows_of = [&](const void* q) { return static_cast<const char*>(q) + at0 * (wide ? 4 : 2); };
+    const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(dh + at0, rows_of(a), rows_of(b), da, db, n, (int)n_out, (int)h, ld); };
+    if (dtype == MEGA_BF16) wide ? launch(gate_grad_kernel<MEGA_BF16, true>) : launch(gate_grad_kernel<MEGA_BF16, false>);
+    else wide ? launch(gate_grad_kernel<MEGA_F16, true>) : launch(gate_grad_kernel<MEGA_F16, false>);
     MEGA_CHECK_LAUNCH();
     const int64_t both = 2 * h, one[2] = {h, h};
-    const void *gs[2] = {da, db}, *wide = at(f.w);
+    const void *gs[2] = {da, db}, *both_w = at(f.w);
     if (dx != nullptr) {
       uint16_t* const to = k != n_in ? at(f.dx) : dx + t * n_in;
       const void* ws2[2] = {w1, w3};
       const int rc = f.apart ? mega_linear_input_grad(gs, ws2, nullptr, dtype, n, k, 2, one, to, stream)
-                             : mega_linear_input_grad(gs, &wide, nullptr, dtype, n, k, 1, &both, to, stream);
+                             : mega_linear_input_grad(gs, &both_w, nullptr, dtype, n, k, 1, &both, to, stream);
       if (rc != MEGA_OK) return rc;
       if (k != n_in)
         if (const int rc2 = narrow(to, dx + t * n_in, n, k, n_in, s); rc2 != MEGA_OK) return rc2;

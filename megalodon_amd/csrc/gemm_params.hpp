@@ -58,9 +58,10 @@ struct GemmParams {
   int split_ok;  // (the launcher's: there is memory for the parts)
   // GATE: C = silu(A B^T) o (A B2^T), both operands k-contiguous, N = 2 gate_n: a tile of T columns holds T / 2 rows of B and the
   // same T / 2 of B2, in turn 32 by 32, so that a wave has both factors of its elements.  Ca, Cb: the products themselves, or null
+  // (wide: in float32)
   const uint16_t* B2;
-  uint16_t *Ca, *Cb;
-  int gate_n;
+  void *Ca, *Cb;
+  int gate_n, wide;
   int n_group;  // plain schedule: tiles numbered n fastest inside bands of n_group column tiles, then m,
                 // then band (0: one band) -- the 32 tiles an XCD works on at a time then share fewer
                 // distinct operand blocks (4 x 8 instead of 2 x 16 of a 16-column problem)

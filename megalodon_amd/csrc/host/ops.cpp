@@ -782,22 +782,22 @@ std::vector<Tensor> linear_group(const Tensor& x, const std::vector<Tensor>& par
 }
 
 // ---- the gated half of a feed-forward network -------------------------------------------------------
-// silu(x w1^T) (x w3^T), both projections and the gate in one kernel; (h, a, b), the products a and b where they are `kept`
-std::tuple<Tensor, Tensor, Tensor> gated_raw(const Tensor& x, const Tensor& w1, const Tensor& w3, bool kept) {
+// silu(x w1^T) (x w3^T), both projections and the gate in one kernel; (h, a, b), the products a and b where they are `kept`, in that type
+std::tuple<Tensor, Tensor, Tensor> gated_raw(const Tensor& x, const Tensor& w1, const Tensor& w3, std::optional<at::ScalarType> kept) {
   const int64_t n_in = x.size(-1), n_out = w1.size(0), tokens = x.numel() / n_in;
   auto shape = x.sizes().vec();
   shape.back() = n_out;
   Tensor h = at::empty(shape, x.options()), a, b, ws;
-  if (kept) a = at::empty({tokens, n_out}, x.options()), b = at::empty({tokens, n_out}, x.options());
+  if (kept.has_value()) a = at::empty({tokens, n_out}, x.options().dtype(*kept)), b = at::empty_like(a);
   if (tokens == 0) return {h, a, b};
   if (const int64_t size = mega_gated_linear_workspace_bytes(tokens, n_in, n_out, 0); size > 0) ws = bytes(size, x);
-  check(mega_gated_linear_fwd(x.data_ptr(), w1.data_ptr(), w3.data_ptr(), kernel_code(x), tokens, n_in, n_out, h.data_ptr(), ptr(a), ptr(b), ptr(ws), stream_of(x)), "mega_gated_linear_fwd");
+  check(mega_gated_linear_fwd(x.data_ptr(), w1.data_ptr(), w3.data_ptr(), kernel_code(x), tokens, n_in, n_out, h.data_ptr(), ptr(a), ptr(b), code_of(kept.value_or(x.scalar_type())), ptr(ws), stream_of(x)), "mega_gated_linear_fwd");
   return {h, a, b};
 }
 struct GatedFn : Function<GatedFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w1, const Tensor& w3) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w1, const Tensor& w3, at::ScalarType kept) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [h, a, b] = gated_raw(attn_operand(x), attn_operand(w1), attn_operand(w3), true);
+    auto [h, a, b] = gated_raw(attn_operand(x), attn_operand(w1), attn_operand(w3), kept);
     ctx->save_for_backward({x, w1, w3, a, b});
     return h;
   }
@@ -809,7 +809,7 @@ struct GatedFn : Function<GatedFn> {
       const Tensor x = flat(saved[0]), go = flat(g[0]), &w1 = saved[1], &w3 = saved[2];
       const Tensor a = at::mm(x, w1.t()), b = at::mm(x, w3.t()), s = at::sigmoid(a);
       const Tensor da = go * b * s * (1 + a * (1 - s)), db = go * a * s;
-      return {want_x ? (at::mm(da, w1) + at::mm(db, w3)).view(saved[0].sizes()) : Tensor(), want_1 ? at::mm(da.t(), x) : Tensor(), want_3 ? at::mm(db.t(), x) : Tensor()};
+      return {want_x ? (at::mm(da, w1) + at::mm(db, w3)).view(saved[0].sizes()) : Tensor(), want_1 ? at::mm(da.t(), x) : Tensor(), want_3 ? at::mm(db.t(), x) : Tensor(), Tensor()};
     }
     at::AutoDispatchBelowADInplaceOrView below;
     const Tensor x = attn_operand(saved[0]), w1 = attn_operand(saved[1]), w3 = attn_operand(saved[2]), a = saved[3].contiguous(), b = saved[4].contiguous();
@@ -823,23 +823,24 @@ struct GatedFn : Function<GatedFn> {
       if (dw.defined()) dw.zero_();
     } else if (dx.defined() || dw.defined()) {
       const Tensor ws = bytes(mega_gated_linear_workspace_bytes(tokens, n_in, n_out, (dx.defined() ? 1 : 0) + (dw.defined() ? 2 : 0)), x);
-      check(mega_gated_linear_bwd(dh.data_ptr(), x.data_ptr(), w1.data_ptr(), w3.data_ptr(), a.data_ptr(), b.data_ptr(), kernel_code(x), tokens, n_in, n_out, ptr(dx), ptr(dw), ptr(ws), stream_of(x)), "mega_gated_linear_bwd");
+      check(mega_gated_linear_bwd(dh.data_ptr(), x.data_ptr(), w1.data_ptr(), w3.data_ptr(), a.data_ptr(), b.data_ptr(), code_of(a.scalar_type()), kernel_code(x), tokens, n_in, n_out, ptr(dx), ptr(dw), ptr(ws), stream_of(x)), "mega_gated_linear_bwd");
     }
-    return {dx, want_1 ? dw.select(0, 0) : Tensor(), want_3 ? dw.select(0, 1) : Tensor()};
+    return {dx, want_1 ? dw.select(0, 0) : Tensor(), want_3 ? dw.select(0, 1) : Tensor(), Tensor()};
   }
 };
-Tensor gated_linear(const Tensor& x_, const Tensor& w1_, const Tensor& w3_) {
+Tensor gated_linear(const Tensor& x_, const Tensor& w1_, const Tensor& w3_, std::optional<at::ScalarType> kept) {
   need_gpu({&x_, &w1_, &w3_});
   require(x_.dim() >= 1 && w1_.dim() == 2 && w1_.sizes() == w3_.sizes() && w1_.size(1) == x_.size(-1), "gated_linear: x must be (..., n_in), w1 and w3 (n_out, n_in)");
   const auto type = x_.scalar_type();
   require((type == at::kBFloat16 || type == at::kHalf) && w1_.scalar_type() == type && w3_.scalar_type() == type, "gated_linear: x, w1 and w3 must share one dtype, bfloat16 or float16");
   require(w1_.size(0) >= 1 && w1_.size(1) >= 1, "gated_linear: n_in and n_out must be positive");
+  require(!kept.has_value() || *kept == type || *kept == at::kFloat, "gated_linear: kept must be float32 or x's dtype");
   // what watches the thread's operations is shown operations
   if (watched() || !plain(x_) || !plain(w1_) || !plain(w3_)) return at::silu(at::linear(x_, w1_)) * at::linear(x_, w3_);
   const Tensor x = stored(x_), w1 = stored(w1_), w3 = stored(w3_);
   c10::DeviceGuard guard(x.device());
-  if (wants_grad({&x, &w1, &w3})) return GatedFn::apply(x, w1, w3);
-  return std::get<0>(gated_raw(attn_operand(x), attn_operand(w1), attn_operand(w3), false));
+  if (wants_grad({&x, &w1, &w3})) return GatedFn::apply(x, w1, w3, kept.value_or(at::kFloat));
+  return std::get<0>(gated_raw(attn_operand(x), attn_operand(w1), attn_operand(w3), std::nullopt));
 }
 
 }  // namespace
