@@ -573,7 +573,8 @@ int mega_tensors_clip(const mega_tensors* tensors, double max_norm, const void* 
  * (`F.silu(self.fc1(x)) * self.fc3(x)`, megalodon/modules/normalized_feedforward_network.py:82, with both projections.)
  * Tensors of `dtype` (MEGA_BF16 / MEGA_F16), contiguous, of any sizes from 1 (n_in and n_out up to 2^20, the two matrices
  * together, n_in rounded up to 64, below 2^30 elements, tokens below 2^31); x, the matrices and what is written for them on 16-byte boundaries.  Products and gate in float32, h rounded once from them.
- *   fwd: a = x w1^T and b = x w3^T (tokens, n_out) as well, in `kept` (`dtype` or MEGA_F32), or null for both; they are what bwd wants.
+ *   fwd: a = x w1^T and b = x w3^T as well, in `kept` (`dtype` or MEGA_F32), rows of n_out rounded up to 8 elements (what lies
+ *        behind n_out has no meaning), or null for both; they are what bwd wants.
  *   bwd: dx (tokens, n_in) or null; dw (2, n_out, n_in), the gradients of w1 and w3, or null.  The gradients of a and b are
  *        rounded to `dtype`, operands of the matrix cores as they are; sums are float32 and rounded once (dw of more than
  *        2^30 / (2 n_out) tokens: once for each 2^30 / (2 n_out) of them).

@@ -545,7 +545,7 @@ __device__ __forceinline__ uint2 pack4(const float* v) {
 template <int DT, int IT, int ROWS, int COLS, int THREADS>
 __device__ __forceinline__ void store_gate(const floatx16 (&acc)[IT][2], const GemmParams& p, int row0, int col0, int wrow, int wcol, int lane,
                                            int thread, void* stage) {
-  const auto out = [&](auto zero, void* to, auto value) {
+  const auto out = [&](auto zero, void* to, int pitch, auto value) {
     using T = decltype(zero);
     constexpr int kPer = 16 / sizeof(T), EP = COLS + kPer, kPieces = COLS / kPer;
     T* const st = static_cast<T*>(stage);
@@ -561,27 +561,28 @@ __device__ __forceinline__ void store_gate(const floatx16 (&acc)[IT][2], const G
         else *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
       }
     lds_barrier();
-    const bool vec_ok = p.gate_n % kPer == 0 && reinterpret_cast<uintptr_t>(to) % 16 == 0;
 #pragma unroll 4
     for (int c = thread; c < ROWS * kPieces; c += THREADS) {
       const int row = c / kPieces, kc = c % kPieces * kPer, grow = row0 + row, gcol = col0 + kc;
-      if (grow >= p.M || gcol >= p.gate_n) continue;
-      T* const dst = static_cast<T*>(to) + static_cast<int64_t>(grow) * p.gate_n + gcol;
-      if (vec_ok) {
-        *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(st + row * EP + kc);
+      if (grow >= p.M || gcol >= pitch) continue;
+      T* const dst = static_cast<T*>(to) + static_cast<int64_t>(grow) * pitch + gcol;
+      if (gcol + kPer <= pitch) {
+        typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+        *reinterpret_cast<u32x4_any*>(dst) = __builtin_bit_cast(u32x4_any, *reinterpret_cast<const u32x4*>(st + row * EP + kc));
       } else {
         for (int q = 0; q < kPer; ++q)
-          if (gcol + q < p.gate_n) dst[q] = st[row * EP + kc + q];
+          if (gcol + q < pitch) dst[q] = st[row * EP + kc + q];
       }
     }
   };
-  out(uint16_t(), p.C, [](float a, float b) { return gated(a, b); });
+  out(uint16_t(), p.C, p.gate_n, [](float a, float b) { return gated(a, b); });
+  const int kept = static_cast<int>(gated_pitch(p.gate_n));
   if (p.Ca == nullptr) return;
   for (int j = 0; j < 2; ++j) {
     lds_barrier();  // the output before has been read
     const auto one = [j](float a, float b) { return j == 0 ? a : b; };
-    if (p.wide) out(float(), j == 0 ? p.Ca : p.Cb, one);
-    else out(uint16_t(), j == 0 ? p.Ca : p.Cb, one);
+    if (p.wide) out(float(), j == 0 ? p.Ca : p.Cb, kept, one);
+    else out(uint16_t(), j == 0 ? p.Ca : p.Cb, kept, one);
   }
 }
 
@@ -2128,7 +2129,7 @@ int launch_gated(GemmParams q, int cus, hipStream_t s) {
   plan(q, kForward, 1, &both, cus, &small);
   if (!small) {
     const int whole = q.cut > 0 ? q.full : q.items, most = std::max(cus / kXcds, 1) * kXcds;
-    const GatedTiles t{q.A, q.B, q.B2, q.C, q.Ca, q.Cb, q.M, q.K, q.gate_n, q.mt_count, q.nt_count, whole};
+    const GatedTiles t{q.A, q.B, q.B2, q.C, q.Ca, q.Cb, q.M, q.K, q.gate_n, static_cast<int>(gated_pitch(q.gate_n)), q.mt_count, q.nt_count, whole};
     if (whole > 0)
       if (const int rc = gated_tiles(DT, q.Ca == nullptr ? 0 : q.wide ? 2 : 1, t, std::min((whole + kXcds - 1) / kXcds * kXcds, most), s); rc != MEGA_OK) return rc;
     if (q.cut == 0) return MEGA_OK;

@@ -58,7 +58,7 @@ struct FewParams {
   const uint16_t *x, *w1, *w3;
   uint16_t* h;
   void *a, *b;
-  int tokens, n_in, n_out, wide;
+  int tokens, n_in, n_out, wide, pitch;
 };
 
 template <bool WHOLE>
@@ -137,14 +137,14 @@ __global__ __launch_bounds__(kFewWaves * kWave) void gated_few_kernel(const FewP
     for (int q = 1; q < kFewWaves; ++q) a += sums[q][block][at], b += sums[q][block][at + 32];
     const int token = 16 * (block % NT) + r, f = f0 + 8 * (block / NT) + 4 * half;
     if (token >= p.tokens) continue;
-    const int64_t to = static_cast<int64_t>(token) * p.n_out + f;
+    const int64_t to = static_cast<int64_t>(token) * p.n_out + f, kept = static_cast<int64_t>(token) * p.pitch + f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (f + e >= p.n_out) break;
       Elem<DT>::store(p.h + to + e, a[e] * sigmoidf(a[e]) * b[e]);
       if (p.a == nullptr) continue;
-      if (p.wide) static_cast<float*>(p.a)[to + e] = a[e], static_cast<float*>(p.b)[to + e] = b[e];
-      else Elem<DT>::store(static_cast<uint16_t*>(p.a) + to + e, a[e]), Elem<DT>::store(static_cast<uint16_t*>(p.b) + to + e, b[e]);
+      if (p.wide) static_cast<float*>(p.a)[kept + e] = a[e], static_cast<float*>(p.b)[kept + e] = b[e];
+      else Elem<DT>::store(static_cast<uint16_t*>(p.a) + kept + e, a[e]), Elem<DT>::store(static_cast<uint16_t*>(p.b) + kept + e, b[e]);
     }
   }
 }
@@ -179,79 +179,85 @@ int few_tokens(const FewParams& p, hipStream_t s) {
 // ---- rows of whole 16-byte pieces, and back -----------------------------------------------------------
 constexpr int kThreads = 256;
 
-// dst (rows, to) = src (rows, from), zeros behind column `from`; `to` a multiple of 8, dst on 16-byte boundaries
-__global__ __launch_bounds__(kThreads) void widen_kernel(const uint16_t* src, uint16_t* dst, int64_t rows, int from, int to) {
-  const int64_t pieces = rows * (to / 8);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < pieces; i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t row = i / (to / 8);
-    const int k = static_cast<int>(i % (to / 8)) * 8;
-    *reinterpret_cast<u32x4*>(dst + 8 * i) = eight<false>(src + row * from, k, from);
+// Matrices copied in one launch, 16 bytes a thread: dst (rows, to) = src (rows, from), zeros behind column `from`, or (NARROW) its first
+// columns.  The padded side has rows of whole pieces on 16-byte boundaries.
+struct Copies {
+  struct One {
+    const uint16_t* src;
+    uint16_t* dst;
+    int64_t pieces;  // of this one and of those in front
+    int from, to;
+  } one[5];
+  int count;
+  void add(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t from, int64_t to) {
+    if (rows == 0) return;
+    const int64_t before = count > 0 ? one[count - 1].pieces : 0;
+    one[count++] = {src, dst, before + rows * (std::max(from, to) / 8), static_cast<int>(from), static_cast<int>(to)};
   }
-}
-// dst (rows, to) = the first columns of src (rows, from); `from` a multiple of 8
-__global__ __launch_bounds__(kThreads) void narrow_kernel(const uint16_t* src, uint16_t* dst, int64_t rows, int from, int to) {
-  const int64_t pieces = rows * (from / 8);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < pieces; i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t row = i / (from / 8);
-    const int k = static_cast<int>(i % (from / 8)) * 8;
-    const u32x4 v = *reinterpret_cast<const u32x4*>(src + 8 * i);
-    uint16_t* const to_row = dst + row * to;
-    if (k + 8 <= to) {
-      *reinterpret_cast<u32x4_any*>(to_row + k) = __builtin_bit_cast(u32x4_any, v);
+};
+template <bool NARROW>
+__global__ __launch_bounds__(kThreads) void copies_kernel(const Copies c) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < c.one[c.count - 1].pieces; i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    int m = 0;
+    while (i >= c.one[m].pieces) ++m;
+    const Copies::One& o = c.one[m];
+    const int64_t at = m > 0 ? i - c.one[m - 1].pieces : i;
+    const int per = (NARROW ? o.from : o.to) / 8;
+    const int64_t row = at / per;
+    const int k = static_cast<int>(at - row * per) * 8;
+    if constexpr (!NARROW) {
+      *reinterpret_cast<u32x4*>(o.dst + 8 * at) = eight<false>(o.src + row * o.from, k, o.from);
     } else {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(o.src + 8 * at);
+      uint16_t* const to_row = o.dst + row * o.to;
+      if (k + 8 <= o.to) {
+        *reinterpret_cast<u32x4_any*>(to_row + k) = __builtin_bit_cast(u32x4_any, v);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (k + e < to) to_row[k + e] = static_cast<uint16_t>(v[e / 2] >> (16 * (e % 2)));
+        for (int e = 0; e < 8; ++e)
+          if (k + e < o.to) to_row[k + e] = static_cast<uint16_t>(v[e / 2] >> (16 * (e % 2)));
+      }
     }
   }
 }
 unsigned pieces_grid(int64_t pieces) { return static_cast<unsigned>(std::min<int64_t>((pieces + kThreads - 1) / kThreads, 16384)); }
-int widen(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t from, int64_t to, hipStream_t s) {
-  widen_kernel<<<pieces_grid(rows * (to / 8)), kThreads, 0, s>>>(src, dst, rows, static_cast<int>(from), static_cast<int>(to));
-  MEGA_CHECK_LAUNCH();
-  return MEGA_OK;
-}
-int narrow(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t from, int64_t to, hipStream_t s) {
-  narrow_kernel<<<pieces_grid(rows * (from / 8)), kThreads, 0, s>>>(src, dst, rows, static_cast<int>(from), static_cast<int>(to));
+template <bool NARROW>
+int copy_all(const Copies& c, hipStream_t s) {
+  if (c.count == 0) return MEGA_OK;
+  copies_kernel<NARROW><<<pieces_grid(c.one[c.count - 1].pieces), kThreads, 0, s>>>(c);
   MEGA_CHECK_LAUNCH();
   return MEGA_OK;
 }
 
 // ---- the gate's backward --------------------------------------------------------------------------------
-typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 template <int DT, bool WIDE>
-__device__ __forceinline__ void kept_eight(const void* row, int k, int n, float* v) {
+__device__ __forceinline__ void kept_eight(const void* p, int64_t at, float* v) {
   if constexpr (!WIDE) {
-    unpack8<DT>(__builtin_bit_cast(uint4, eight<false>(static_cast<const uint16_t*>(row), k, n)), v);
+    unpack8<DT>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at), v);
   } else {
-    const float* const p = static_cast<const float*>(row) + k;
-    if (k + 8 <= n) {
-      const f32x4_any lo = *reinterpret_cast<const f32x4_any*>(p), hi = *reinterpret_cast<const f32x4_any*>(p + 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = k + e < n ? p[e] : 0.f;
-    }
+    const float4 lo = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at), hi = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4);
+    v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
   }
 }
-// da, db (tokens, ld) from dh, a, b (tokens, n): 8 elements a thread, zeros from column n to `to`
+// da, db (tokens, ld) from dh (tokens, n) and a, b (tokens, pitch): 8 elements a thread, zeros from column n to `to`
 template <int DT, bool WIDE>
 __global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh, const void* a, const void* b, uint16_t* da, uint16_t* db,
-                                                            int64_t tokens, int n, int to, int64_t ld) {
+                                                            int64_t tokens, int n, int pitch, int to, int64_t ld) {
   const int64_t pieces = tokens * (to / 8);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < pieces; i += static_cast<int64_t>(gridDim.x) * kThreads) {
     const int64_t row = i / (to / 8);
-    const int k = static_cast<int>(i % (to / 8)) * 8;
+    const int k = static_cast<int>(i - row * (to / 8)) * 8;
     float g[8], u[8], v[8], du[8], dv[8];
-    unpack8<DT>(__builtin_bit_cast(uint4, eight<false>(dh + row * n, k, n)), g);
-    kept_eight<DT, WIDE>(static_cast<const char*>(a) + row * n * (WIDE ? 4 : 2), k, n, u);
-    kept_eight<DT, WIDE>(static_cast<const char*>(b) + row * n * (WIDE ? 4 : 2), k, n, v);
+    if (k < pitch) {
+      unpack8<DT>(__builtin_bit_cast(uint4, eight<false>(dh + row * n, k, n)), g);
+      kept_eight<DT, WIDE>(a, row * pitch + k, u);
+      kept_eight<DT, WIDE>(b, row * pitch + k, v);
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float s = sigmoidf(u[e]);
-      dv[e] = g[e] * u[e] * s;
-      du[e] = g[e] * v[e] * s * (1.f + u[e] * (1.f - s));
+      dv[e] = k + e < n ? g[e] * u[e] * s : 0.f;
+      du[e] = k + e < n ? g[e] * v[e] * s * (1.f + u[e] * (1.f - s)) : 0.f;
     }
     *reinterpret_cast<uint4*>(da + row * ld + k) = pack8<DT>(du);
     *reinterpret_cast<uint4*>(db + row * ld + k) = pack8<DT>(dv);
@@ -298,7 +304,7 @@ struct Backward {
   int64_t g, w, x, dx, dw, parts, bytes;
   Backward(int64_t tokens, int64_t n_in, int64_t n_out, int what) {
     Room room;
-    apart = n_out % 64 == 0 && n_in % 8 == 0 && static_cast<double>(tokens) * n_in * n_out <= 0x1p33;
+    apart = n_out % 64 == 0 && n_in % 8 == 0 && static_cast<double>(tokens) * n_in * n_out <= 0x1p33 && tokens * std::max(2 * n_out, n_in) < kMost;
     h = apart ? n_out : up(n_out, 32), k = up(n_in, 8);
     rows = std::min(tokens, std::max<int64_t>((kMost - 1) / std::max(2 * h, k) / 256 * 256, 256));
     g = room.take(2 * rows * 2 * h);
@@ -346,7 +352,7 @@ extern "C" int mega_gated_linear_fwd(const void* x_, const void* w1_, const void
   const bool wide = kept == MEGA_F32;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (few(tokens, n_in, n_out)) {
-    const FewParams p{x, w1, w3, h, a, b, static_cast<int>(tokens), static_cast<int>(n_in), static_cast<int>(n_out), wide};
+    const FewParams p{x, w1, w3, h, a, b, static_cast<int>(tokens), static_cast<int>(n_in), static_cast<int>(n_out), wide, static_cast<int>(gated_pitch(n_out))};
     return dtype == MEGA_BF16 ? few_tokens<MEGA_BF16>(p, s) : few_tokens<MEGA_F16>(p, s);
   }
   const Forward f(tokens, n_in, n_out);
@@ -354,20 +360,22 @@ extern "C" int mega_gated_linear_fwd(const void* x_, const void* w1_, const void
   char* const ws = static_cast<char*>(workspace);
   const auto at = [&](int64_t offset) { return reinterpret_cast<uint16_t*>(ws + offset); };
   const bool padded = f.k != n_in;
-  if (padded) {
-    if (const int rc = widen(w1, at(f.w1), n_out, n_in, f.k, s); rc != MEGA_OK) return rc;
-    if (const int rc = widen(w3, at(f.w3), n_out, n_in, f.k, s); rc != MEGA_OK) return rc;
-    w1 = at(f.w1), w3 = at(f.w3);
-  }
   for (int64_t t = 0; t < tokens; t += f.rows) {
     const int64_t n = std::min(f.rows, tokens - t);
     const uint16_t* rows = x + t * n_in;
     if (padded) {
-      if (const int rc = widen(rows, at(f.x), n, n_in, f.k, s); rc != MEGA_OK) return rc;
+      Copies c{};
+      c.add(rows, at(f.x), n, n_in, f.k);
+      if (t == 0) {
+        c.add(w1, at(f.w1), n_out, n_in, f.k);
+        c.add(w3, at(f.w3), n_out, n_in, f.k);
+        w1 = at(f.w1), w3 = at(f.w3);
+      }
+      if (const int rc = copy_all<false>(c, s); rc != MEGA_OK) return rc;
       rows = at(f.x);
     }
     const bool cut = gated_parts_bytes(n, f.k, n_out) > 0;
-    const auto rows_of = [&](void* q) { return q == nullptr ? nullptr : static_cast<char*>(q) + t * n_out * (wide ? 4 : 2); };
+    const auto rows_of = [&](void* q) { return q == nullptr ? nullptr : static_cast<char*>(q) + t * gated_pitch(n_out) * (wide ? 4 : 2); };
     if (const int rc = gated_product(dtype, rows, w1, w3, n, f.k, n_out, h + t * n_out, rows_of(a), rows_of(b), wide, cut ? reinterpret_cast<float*>(ws + f.parts) : nullptr, s);
         rc != MEGA_OK)
       return rc;
@@ -392,25 +400,30 @@ extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void
   char* const ws = static_cast<char*>(workspace);
   const auto at = [&](int64_t offset) { return reinterpret_cast<uint16_t*>(ws + offset); };
   const int64_t h = f.h, k = f.k;
-  if (dx != nullptr && !f.apart) {
-    if (const int rc = widen(w1, at(f.w), n_out, n_in, k, s); rc != MEGA_OK) return rc;
-    if (const int rc = widen(w3, at(f.w) + h * k, n_out, n_in, k, s); rc != MEGA_OK) return rc;
-    // (features behind the last meet gradients that are zero: they have to be finite)
-    if (h != n_out) {
-      MEGA_CHECK_ARG(h - n_out < 32, "mega_gated_linear_bwd: padding");
-      if (const int rc = widen(w1, at(f.w) + n_out * k, h - n_out, 0, k, s); rc != MEGA_OK) return rc;
-      if (const int rc = widen(w3, at(f.w) + (h + n_out) * k, h - n_out, 0, k, s); rc != MEGA_OK) return rc;
-    }
-  }
   uint16_t* const dw_at = dw != nullptr && (k != n_in || h != n_out) ? at(f.dw) : dw;
   for (int64_t t = 0; t < tokens; t += f.rows) {
     const int64_t n = std::min(f.rows, tokens - t);
     uint16_t *da = at(f.g), *db = f.apart ? da + n * h : da + h;
-    const int64_t ld = f.apart ? h : 2 * h, at0 = t * n_out;
+    const int64_t ld = f.apart ? h : 2 * h, pitch = gated_pitch(n_out), at0 = t * n_out;
+    Copies c{}, back{};
+    if (dx != nullptr && !f.apart && t == 0) {
+      uint16_t *const u1 = at(f.w), *const u3 = u1 + h * k;
+      c.add(w1, u1, n_out, n_in, k);
+      c.add(w3, u3, n_out, n_in, k);
+      // (features behind the last meet gradients that are zero: they have to be finite)
+      c.add(w1, u1 + n_out * k, h - n_out, 0, k);
+      c.add(w3, u3 + n_out * k, h - n_out, 0, k);
+    }
+    const uint16_t* rows = x + t * n_in;
+    if (dw != nullptr && k != n_in) {
+      c.add(rows, at(f.x), n, n_in, k);
+      rows = at(f.x);
+    }
+    if (const int rc = copy_all<false>(c, s); rc != MEGA_OK) return rc;
     const unsigned grid = pieces_grid(n * (h / 8));
     const bool wide = kept == MEGA_F32;
-    const auto rows_of = [&](const void* q) { return static_cast<const char*>(q) + at0 * (wide ? 4 : 2); };
-    const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(dh + at0, rows_of(a), rows_of(b), da, db, n, (int)n_out, (int)h, ld); };
+    const auto rows_of = [&](const void* q) { return static_cast<const char*>(q) + t * pitch * (wide ? 4 : 2); };
+    const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(dh + at0, rows_of(a), rows_of(b), da, db, n, (int)n_out, (int)pitch, (int)h, ld); };
     if (dtype == MEGA_BF16) wide ? launch(gate_grad_kernel<MEGA_BF16, true>) : launch(gate_grad_kernel<MEGA_BF16, false>);
     else wide ? launch(gate_grad_kernel<MEGA_F16, true>) : launch(gate_grad_kernel<MEGA_F16, false>);
     MEGA_CHECK_LAUNCH();
@@ -422,15 +435,9 @@ extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void
       const int rc = f.apart ? mega_linear_input_grad(gs, ws2, nullptr, dtype, n, k, 2, one, to, stream)
                              : mega_linear_input_grad(gs, &both_w, nullptr, dtype, n, k, 1, &both, to, stream);
       if (rc != MEGA_OK) return rc;
-      if (k != n_in)
-        if (const int rc2 = narrow(to, dx + t * n_in, n, k, n_in, s); rc2 != MEGA_OK) return rc2;
+      if (k != n_in) back.add(to, dx + t * n_in, n, k, n_in);
     }
     if (dw != nullptr) {
-      const uint16_t* rows = x + t * n_in;
-      if (k != n_in) {
-        if (const int rc = widen(rows, at(f.x), n, n_in, k, s); rc != MEGA_OK) return rc;
-        rows = at(f.x);
-      }
       const bool cut = mega_linear_workspace_bytes(2, n, k, f.apart ? 2 : 1, f.apart ? one : &both) > 0;
       float* const parts = cut ? reinterpret_cast<float*>(ws + f.parts) : nullptr;
       void* to[2] = {dw_at, dw_at + h * k};
@@ -438,11 +445,12 @@ extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void
       const int rc = f.apart ? mega_linear_weight_grads(gs, rows, dtype, n, k, 2, one, to, parts, stream)
                              : weight_grad_onto(dtype, da, rows, n, k, both, t > 0 ? dw_at : nullptr, dw_at, parts, s);
       if (rc != MEGA_OK) return rc;
+      if (dw_at != dw && t + n == tokens) {
+        back.add(dw_at, dw, n_out, k, n_in);
+        back.add(dw_at + h * k, dw + n_out * n_in, n_out, k, n_in);
+      }
     }
-  }
-  if (dw != nullptr && dw_at != dw) {
-    if (const int rc = narrow(dw_at, dw, n_out, k, n_in, s); rc != MEGA_OK) return rc;
-    return narrow(dw_at + h * k, dw + n_out * n_in, n_out, k, n_in, s);
+    if (const int rc = copy_all<true>(back, s); rc != MEGA_OK) return rc;
   }
   return MEGA_OK;
 }

@@ -18,6 +18,7 @@ namespace {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -190,48 +191,50 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
       stage ^= 1;
     }
     // the tile's elements: lane l has row l % 32 of a block of 32, register e the column 8 (e / 4) + 4 (l / 32) + e % 4
-    const bool whole = m0 + kRows <= p.tokens && h0 + kCols <= p.n_out && p.n_out % 8 == 0;
     const int col0 = h0 + wn * 32;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = m0 + wm * 128 + i * 32 + r;
-      const int64_t at = static_cast<int64_t>(row) * p.n_out + col0;
-      if (whole) {
+      if (row >= p.tokens) continue;
+      uint16_t* const h = p.h + static_cast<int64_t>(row) * p.n_out;
+      const int64_t at = static_cast<int64_t>(row) * p.pitch;
 #pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-          uint2 v[2];
+      for (int q = 0; q < 4; q += 2) {
+        uint2 v[2];
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const int e = 4 * (q + t);
-            v[t] = pack4<DT>(gated(acc[i][0][e], acc[i][1][e]), gated(acc[i][0][e + 1], acc[i][1][e + 1]),
-                             gated(acc[i][0][e + 2], acc[i][1][e + 2]), gated(acc[i][0][e + 3], acc[i][1][e + 3]));
-          }
-          *reinterpret_cast<u32x4*>(p.h + at + 8 * (q + g)) = rows_of_eight(v[0], v[1]);
+        for (int t = 0; t < 2; ++t) {
+          const int e = 4 * (q + t);
+          v[t] = pack4<DT>(gated(acc[i][0][e], acc[i][1][e]), gated(acc[i][0][e + 1], acc[i][1][e + 1]),
+                           gated(acc[i][0][e + 2], acc[i][1][e + 2]), gated(acc[i][0][e + 3], acc[i][1][e + 3]));
         }
+        const u32x4 eight = rows_of_eight(v[0], v[1]);
+        const int col = col0 + 8 * (q + g);
+        if (col + 8 <= p.n_out) {
+          *reinterpret_cast<u32x4_any*>(h + col) = eight;
+        } else {
 #pragma unroll
-        for (int j = 0; j < 2 && KEEP == 1; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; q += 2) {
-            const auto four = [&](int e) { return pack4<DT>(acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]); };
-            *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(j ? p.b : p.a) + at + 8 * (q + g)) = rows_of_eight(four(4 * q), four(4 * q + 4));
-          }
-#pragma unroll
-        for (int j = 0; j < 2 && KEEP == 2; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<float4*>(static_cast<float*>(j ? p.b : p.a) + at + 8 * q + 4 * g) =
-                make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-      } else if (row < p.tokens) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int col = 8 * (e / 4) + 4 * g + e % 4;
-          if (col0 + col >= p.n_out) continue;
-          const float a = acc[i][0][e], b = acc[i][1][e];
-          Elem<DT>::store(p.h + at + col, gated(a, b));
-          if constexpr (KEEP == 1) Elem<DT>::store(static_cast<uint16_t*>(p.a) + at + col, a), Elem<DT>::store(static_cast<uint16_t*>(p.b) + at + col, b);
-          if constexpr (KEEP == 2) static_cast<float*>(p.a)[at + col] = a, static_cast<float*>(p.b)[at + col] = b;
+          for (int e = 0; e < 8; ++e)
+            if (col + e < p.n_out) h[col + e] = static_cast<uint16_t>(eight[e / 2] >> (16 * (e % 2)));
         }
       }
+#pragma unroll
+      for (int j = 0; j < 2 && KEEP == 1; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          const auto four = [&](int e) { return pack4<DT>(acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]); };
+          const u32x4 eight = rows_of_eight(four(4 * q), four(4 * q + 4));
+          const int col = col0 + 8 * (q + g);
+          if (col < p.pitch) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(j ? p.b : p.a) + at + col) = eight;
+        }
+#pragma unroll
+      for (int j = 0; j < 2 && KEEP == 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int col = col0 + 8 * q + 4 * g;
+          if (col < p.pitch)
+            *reinterpret_cast<float4*>(static_cast<float*>(j ? p.b : p.a) + at + col) =
+                make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+        }
     }
     item += it_step;
     if (item >= it_hi) break;

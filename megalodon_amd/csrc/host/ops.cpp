@@ -788,7 +788,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_raw(const Tensor& x, const Tensor& w1, 
   auto shape = x.sizes().vec();
   shape.back() = n_out;
   Tensor h = at::empty(shape, x.options()), a, b, ws;
-  if (kept.has_value()) a = at::empty({tokens, n_out}, x.options().dtype(*kept)), b = at::empty_like(a);
+  if (kept.has_value()) a = at::empty({tokens, (n_out + 7) / 8 * 8}, x.options().dtype(*kept)), b = at::empty_like(a);
   if (tokens == 0) return {h, a, b};
   if (const int64_t size = mega_gated_linear_workspace_bytes(tokens, n_in, n_out, 0); size > 0) ws = bytes(size, x);
   check(mega_gated_linear_fwd(x.data_ptr(), w1.data_ptr(), w3.data_ptr(), kernel_code(x), tokens, n_in, n_out, h.data_ptr(), ptr(a), ptr(b), code_of(kept.value_or(x.scalar_type())), ptr(ws), stream_of(x)), "mega_gated_linear_fwd");
