@@ -530,8 +530,8 @@ __device__ __forceinline__ void store_tile(const floatx16 (&acc)[IT][2], const G
   }
 }
 
-// silu(a) b and two of them in 16 bits.  (The quotient is IEEE's: exp(-a) may be infinite, then the result is 0 times b.)
-__device__ __forceinline__ float gated(float a, float b) { return a / (1.f + __expf(-a)) * b; }
+// silu(a) b, and four values in 16 bits
+__device__ __forceinline__ float gated(float a, float b) { return a * fast_sigmoid(a) * b; }
 template <int DT>
 __device__ __forceinline__ uint2 pack4(const float* v) {
   if (DT == MEGA_BF16) return uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};

@@ -1,14 +1,18 @@
 // The gated product of many tokens in tiles of 256 tokens x 128 features of both matrices (gated_linear.hip has the formulas).
 //
 // Eight waves of 128 x 64 accumulators: 32 features of w1 and the same 32 of w3 beside each other, so that a lane has a and b
-// of its elements.  Slabs of 64 k go from memory straight into LDS (two buffers of 64 KB), a wave's products are 32 x 32 x 16;
-// the layouts in LDS are those of the product kernels with two k-contiguous operands (attention.hip): rows of 128 bytes, whose
-// 16-byte chunk c lies at position c ^ ((row >> 1) & 7).
+// of its elements.  Slabs of 64 k go from memory straight into LDS, a wave's products are 32 x 32 x 16; the layouts in LDS are those of
+// the product kernels with two k-contiguous operands (attention.hip): rows of 128 bytes, whose 16-byte chunk c lies at position
+// c ^ ((row >> 1) & 7); the rows of the two matrices lie 32 by 32 in turn.
 //
-// What is particular to this kernel: it is persistent, and a workgroup's tiles are one line of slabs.  While a tile's last two slabs
-// are worked on, the first two of the next one are on their way, and the gate and the stores of a tile, taken straight from the accumulators
-// without LDS, run while they land.  With a pipeline that drains at the end of each tile and an epilogue through LDS, training on 32768
-// tokens x 4096 x 11008 took 5.2 ms for this product, 1531 tokens without gradients 239 us for the two whole rounds.
+// A workgroup's tiles are one line of slabs: the first slabs of a tile are on their way while the last ones of the tile before are
+// worked on, and the gate and the stores, taken straight from the accumulators, run meanwhile.  The slabs of x and of the matrices go
+// round in five buffers of 32 KB, all of the LDS, so that the requests of a slab can be spread over three of its four steps: a request
+// of 1 KB takes the CU's memory path 16 cycles, the 64 of a slab half of its time, and sent under one step, as two buffers for whole slabs
+// want it, they hold up the waves.  32768 tokens, 4096 -> 11008, nothing kept: 4.23 ms, 1.40 PFLOP/s, the matrix pipe 86 % busy at the
+// 1.53 GHz that the power limit leaves (two buffers 4.43 ms, 75 % at 1.66; the library's product alone, without gate and at
+// the same time, 3.86 ms, 86 % at 1.65).  Four waves of 128 x 128, with a third fewer reads of LDS, take the same time.
+// What remains exposed are the stores: a and b in float32 0.75 ms.
 #include "common.hpp"
 #include "gated.hpp"
 #include "gemm_params.hpp"
@@ -31,8 +35,9 @@ __device__ __forceinline__ floatx16 mma32(u32x4 a, u32x4 b, floatx16 c) {
 }
 
 constexpr int kThreads = 512, kRows = 256, kCols = 128, kK = 64;
-constexpr uint32_t kOperandBytes = 256 * kK * 2, kStageBytes = 2 * kOperandBytes;  // A, then the two matrices' rows 32 by 32 in turn
-constexpr size_t kLds = 2 * kStageBytes;
+constexpr uint32_t kOperandBytes = 256 * kK * 2, kRing = 5 * kOperandBytes;
+constexpr size_t kLds = kRing;
+static_assert(kLds <= 160 * 1024, "fits the LDS");
 
 // 64 lanes' 16 bytes from base + offset to 1 KB of LDS (its address in M0).  Assembly, since the compiler would wait for all of
 // them in front of every read of LDS; the waits are the explicit ones below.
@@ -40,7 +45,7 @@ __device__ __forceinline__ void load_to_lds16(const char* base, uint32_t offset,
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds_dst));
 }
 
-__device__ __forceinline__ float gated(float a, float b) { return a / (1.f + __expf(-a)) * b; }
+__device__ __forceinline__ float gated(float a, float b) { return a * fast_sigmoid(a) * b; }
 template <int DT>
 __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
   if constexpr (DT == MEGA_BF16) return uint2{pack_bf16x2(a, b), pack_bf16x2(c, d)};
@@ -97,22 +102,20 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
   };
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(smem))));
   const uint32_t lds_wave = lds0 + wave * 1024;
-  // request n (0 .. 7) of a slab: even ones of x, odd ones of the matrix
-  const auto request = [&](uint32_t slab, uint32_t stage, int n) {
-    const uint32_t dst = lds_wave + stage * kStageBytes + (n / 2) * 8192 + (n & 1) * kOperandBytes;
-    if (n & 1) load_to_lds16(wb + slab * 128, offw[n / 2], dst);
-    else load_to_lds16(xb + slab * 128, offx[n / 2], dst);
-  };
+  // the ring: operand slabs x 0, matrices 0, x 1, matrices 1, .. in buffers 0 .. 4 in turn
+  const auto behind = [&](uint32_t at, uint32_t buffers) { return at + buffers * kOperandBytes >= kRing ? at + buffers * kOperandBytes - kRing : at + buffers * kOperandBytes; };
+  const auto request_x = [&](uint32_t slab, uint32_t to, int i) { load_to_lds16(xb + slab * 128, offx[i], lds_wave + to + i * 8192); };
+  const auto request_w = [&](uint32_t slab, uint32_t to, int i) { load_to_lds16(wb + slab * 128, offw[i], lds_wave + to + i * 8192); };
 
   // fragment side: k-step `set` of a slab takes k = 16 set + 8 g + e; its chunk 2 set + g lies at (g ^ swizzle) ^ 2 set
-  uint32_t fra = lds0 + (wm * 128 + r) * 128 + (g ^ (r >> 1 & 7)) * 16, frb = fra - wm * 128 * 128 + kOperandBytes + wn * 64 * 128;
+  const uint32_t fra = (wm * 128 + r) * 128 + (g ^ (r >> 1 & 7)) * 16, frb = (wn * 64 + r) * 128 + (g ^ (r >> 1 & 7)) * 16;
   const auto read = [&](uint32_t at) {
     return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(static_cast<uintptr_t>(at));
   };
   u32x4 fa0[4], fb0[2], fa1[4], fb1[2];
-  const auto fread = [&](u32x4* fa, u32x4* fb, int set, int i) {
-    fa[i] = read((fra ^ (set * 32)) + i * 32 * 128);
-    if (i < 2) fb[i] = read((frb ^ (set * 32)) + i * 32 * 128);
+  const auto fread = [&](u32x4* fa, u32x4* fb, uint32_t in_x, uint32_t in_w, int set, int i) {
+    fa[i] = read((fra ^ (set * 32)) + lds0 + in_x + i * 32 * 128);
+    if (i < 2) fb[i] = read((frb ^ (set * 32)) + lds0 + in_w + i * 32 * 128);
   };
   floatx16 acc[4][2];
   const auto mma = [&](const u32x4* fa, const u32x4* fb, int n) { acc[n / 2][n % 2] = mma32<DT>(fb[n % 2], fa[n / 2], acc[n / 2][n % 2]); };
@@ -121,42 +124,47 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
   int m0, h0;
   place(item, &m0, &h0);
   offsets(m0, h0);
-#pragma unroll
-  for (int n = 0; n < 8; ++n) request(0, 0, n);
-  uint32_t ahead = 1, stage = 0;  // the next slab to be asked for, and the buffer of the one that is worked on
-  int next = item + it_step;      // ... of which tile from `slabs` on
-  if (slabs > 1) {
-#pragma unroll
-    for (int n = 0; n < 8; ++n) request(1, 1, n);
-  } else {
-    // a tile of one slab: the second one is the next tile's (or, behind the last, once more this one's)
+  // `ahead`: the slab that is asked for next, of a tile `next` further on once it has reached `slabs` (behind the last tile the
+  // same one again, which nobody reads)
+  int ahead = 0, next = item + it_step;
+  const auto turn = [&]() {
+    if (ahead < slabs) return;
+    ahead = 0;
     if (next < it_hi) {
       int m, h;
       place(next, &m, &h);
       offsets(m, h);
     }
     next += it_step;
+  };
+  uint32_t in_x = 0;  // the buffer of x's slab that is worked on; its matrices' is the next, then come the next slab's
 #pragma unroll
-    for (int n = 0; n < 8; ++n) request(0, 1, n);
-    ahead = 0;
+  for (int q = 0; q < 2; ++q) {
+    turn();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) request_x(ahead, 2 * q * kOperandBytes, i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) request_w(ahead, (2 * q + 1) * kOperandBytes, i);
+    ++ahead;
   }
-  ++ahead;
   asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 4; ++i) fread(fa0, fb0, 0, i);
+  for (int i = 0; i < 4; ++i) fread(fa0, fb0, 0, kOperandBytes, 0, i);
 
+  // A slab's four k-steps.  The fragments of the next step are read under the products of the current one.  The slab behind the
+  // next: x's under the first two steps, into the buffer that the last slab's matrices have left; the matrices' under the last one,
+  // into the buffer of this slab's x, which all waves have read by then.  (Requests for 1 KB keep the memory path 16 cycles each, all 64 of a slab half the
+  // slab's time: sent under one step, as with two buffers for whole slabs, they hold up the waves.)
 #define MEGA_SGB(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
-#define MEGA_KSTEP(FA, FB, NFA, NFB, SET)                                   \
-  {                                                                        \
-    _Pragma("unroll") for (int i = 0; i < 4; ++i) fread(NFA, NFB, (SET) + 1, i); \
-    _Pragma("unroll") for (int n = 0; n < 8; ++n) mma(FA, FB, n);           \
-    _Pragma("unroll") for (int sg = 0; sg < 4; ++sg) {                     \
+#define MEGA_READ_AND_MULTIPLY(FA, FB, NFA, NFB, SET)                      \
+    _Pragma("unroll") for (int i = 0; i < 4; ++i) fread(NFA, NFB, in_x, in_w, (SET) + 1, i); \
+    _Pragma("unroll") for (int n = 0; n < 4; ++n) mma(FA, FB, n);          \
+    _Pragma("unroll") for (int sg = 0; sg < 3; ++sg) {                     \
       MEGA_SGB(0x008, 1);                                                  \
       MEGA_SGB(0x100, 2);                                                  \
     }                                                                      \
-    MEGA_SGB(0x008, 4);                                                    \
-    __builtin_amdgcn_sched_barrier(0);                                     \
-  }
+    MEGA_SGB(0x008, 1);                                                    \
+    __builtin_amdgcn_sched_barrier(0);
   while (true) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -165,30 +173,37 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     for (int s = 0; s < slabs; ++s) {
-      MEGA_KSTEP(fa0, fb0, fa1, fb1, 0)
-      MEGA_KSTEP(fa1, fb1, fa0, fb0, 1)
-      MEGA_KSTEP(fa0, fb0, fa1, fb1, 2)
-      if (static_cast<int>(ahead) == slabs) {  // from here on the next tile's (behind the last tile: this one's again, not read)
-        ahead = 0;
-        if (next < it_hi) {
-          int m, h;
-          place(next, &m, &h);
-          offsets(m, h);
-        }
-        next += it_step;
+      const uint32_t in_w = behind(in_x, 1), next_x = behind(in_x, 2), next_w = behind(in_x, 3), last_w = behind(in_x, 4);
+      turn();
+      MEGA_READ_AND_MULTIPLY(fa0, fb0, fa1, fb1, 0)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        if (n < 2) request_x(ahead, last_w, n);
+        mma(fa0, fb0, 4 + n);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      // the wave's pieces of the next slab have landed, its reads of this one have returned
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      fra ^= kStageBytes, frb ^= kStageBytes;
+      MEGA_READ_AND_MULTIPLY(fa1, fb1, fa0, fb0, 1)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        if (n < 2) request_x(ahead, last_w, 2 + n);
+        mma(fa1, fb1, 4 + n);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      MEGA_READ_AND_MULTIPLY(fa0, fb0, fa1, fb1, 2)
+#pragma unroll
+      for (int n = 4; n < 8; ++n) mma(fa0, fb0, n);
+      __builtin_amdgcn_sched_barrier(0);
+      // the wave's pieces of the next slab have landed (x's of the one behind it may be on their way), its reads of this one have returned
+      asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
-        if (n < 4) fread(fa0, fb0, 0, n);
-        request(ahead, stage, n);
+        if (n < 4) fread(fa0, fb0, next_x, next_w, 0, n);
+        if (n % 2 == 1) request_w(ahead, in_x, n / 2);
         mma(fa1, fb1, n);
         __builtin_amdgcn_sched_barrier(0);
       }
       ++ahead;
-      stage ^= 1;
+      in_x = next_x;
     }
     // the tile's elements: lane l has row l % 32 of a block of 32, register e the column 8 (e / 4) + 4 (l / 32) + e % 4
     const int col0 = h0 + wn * 32;
@@ -240,7 +255,7 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
     if (item >= it_hi) break;
     place(item, &m0, &h0);
   }
-#undef MEGA_KSTEP
+#undef MEGA_READ_AND_MULTIPLY
 #undef MEGA_SGB
   // (nothing may land in LDS that is another workgroup's by then)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
