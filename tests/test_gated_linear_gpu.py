@@ -105,6 +105,11 @@ def test_few_tokens(tokens, n_in, n_out, dtype):
     (1531, 4096, 11008, torch.bfloat16),   # the last round's cut along k
     (257, 4095, 300, torch.float16),
     (2500, 512, 4100, torch.float16),
+    (30000, 64, 2000, torch.bfloat16),     # several tiles of 256 for a workgroup, of one slab,
+    (30011, 128, 1999, torch.float16),     # two,
+    (30000, 192, 2000, torch.bfloat16),    # three
+    (20000, 320, 2100, torch.bfloat16),    # and five
+    (200, 4096, 2048, torch.bfloat16),
 ])
 def test_tiles(tokens, n_in, n_out, dtype):
     check(*operands(tokens, n_in, n_out, dtype))
