@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kGroups = 2048;  // workgroups of a launch: eight of four waves for each CU
-constexpr int kPerLaunch = 160;
+constexpr int kPerLaunch = 160, kStarts = 16;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
@@ -24,7 +24,7 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 struct Tensors {
   const void* from[kPerLaunch];
   void* to[kPerLaunch];  // (scaling only)
-  uint32_t start[kPerLaunch + 1];
+  uint32_t start[kPerLaunch + kStarts + 1];  // (behind the end: the largest number)
   uint16_t last[kPerLaunch];  // less one
   uint8_t dtype[kPerLaunch];
   int count, chunk_bytes;
@@ -36,17 +36,15 @@ struct Chunk {
   void* to;
   int n, dtype;
 };
-// (The lanes look at all of the starts at once: a search by halves is a chain of up to eight loads of the arguments, each
-// waited for.)
+// (Sixteen starts at a time in scalar registers: a search by halves is a chain of up to eight loads of the arguments, each waited for, and vector
+// loads of them pass by the scalar cache.)
 __device__ __forceinline__ Chunk chunk_of(const Tensors& t, uint32_t c) {
-  const int lane = threadIdx.x % kWave;
   int at = -1;
+  for (int i = 0; i < t.count; i += kStarts) {
 #pragma unroll
-  for (int q = 0; q < (kPerLaunch + kWave - 1) / kWave; ++q) {
-    const int i = min(q * kWave + lane, kPerLaunch - 1);
-    at += __popcll(__ballot(q * kWave + lane < t.count && t.start[i] <= c));
+    for (int q = 0; q < kStarts; ++q) at += t.start[i + q] <= c;
+    if (t.start[i + kStarts] > c) break;
   }
-  at = __builtin_amdgcn_readfirstlane(at);
   const int dtype = t.dtype[at], size = dtype == MEGA_F32 ? 4 : 2;
   const int64_t offset = static_cast<int64_t>(c - t.start[at]) * t.chunk_bytes;
   const int n = c + 1 == t.start[at + 1] ? t.last[at] + 1 : t.chunk_bytes / size;
@@ -232,6 +230,7 @@ int each_launch(const mega_tensors& t, bool to, F f) {
   a.chunk_bytes = chunk_bytes_of(t);
   const auto flush = [&]() {
     if (a.count == 0) return static_cast<int>(MEGA_OK);
+    for (int i = a.count + 1; i <= kPerLaunch + kStarts; ++i) a.start[i] = 0xffffffffu;
     const int rc = f(a, static_cast<unsigned>(std::min<int64_t>(a.start[a.count], kGroups)));
     a.count = 0;
     return rc;

@@ -18,6 +18,14 @@ from torch import nn
 from .. import _lib
 
 
+def is_bare(layer) -> bool:
+    """Whether calling the layer is nothing but `Linear.forward`: no hooks of its own or for all modules."""
+    every = torch.nn.modules.module
+    return (type(layer) is Linear and "forward" not in layer.__dict__ and not layer._forward_hooks and not layer._forward_pre_hooks
+            and not layer._backward_hooks and not layer._backward_pre_hooks and not every._global_forward_hooks and not every._global_forward_pre_hooks
+            and not every._global_backward_hooks and not every._global_backward_pre_hooks)
+
+
 def linear_group(x: torch.Tensor, layers) -> Tuple[torch.Tensor, ...]:
     """`tuple(layer(x) for layer in layers)` for `Linear` layers that read the same input; on the GPU in
     16 bits their products are one launch where that is the faster form, and with gradients their backward

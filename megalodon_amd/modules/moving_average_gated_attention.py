@@ -137,7 +137,7 @@ class MegaBlock(nn.Module):
                  chunk_size: int, ffn_hidden_dim: int, norm_num_groups: int, swiglu: bool = True,
                  efficient_attn: Optional[str] = "fused", norm_affine: bool = True, norm_eps: float = 1e-5,
                  rescale_nffn: bool = False, layer_id: int = 0, init_std: float = 0.02, dropout: float = 0.0,
-                 attention_dropout: float = 0.0, hidden_dropout: float = 0.0):
+                 attention_dropout: float = 0.0, hidden_dropout: float = 0.0, fused_gate: bool = False):
         super().__init__()
         self.layer_id = layer_id
         self.mega = MovingAverageGatedAttention(
@@ -149,7 +149,7 @@ class MegaBlock(nn.Module):
         self.nffn = NormalizedFeedForwardNetwork(
             model_dim=model_dim, ffn_hidden_dim=ffn_hidden_dim, dropout=dropout, hidden_dropout=hidden_dropout,
             swiglu=swiglu, norm_affine=norm_affine,
-            norm_eps=norm_eps, rescale=rescale, init_std=init_std)
+            norm_eps=norm_eps, rescale=rescale, init_std=init_std, fused_gate=fused_gate)
 
     def forward(self, x: Tensor, freqs_cis: Optional[Tensor] = None, mask: Optional[Tensor] = None, cache=None):
         if (cache is not None and x.dim() == 3 and x.shape[1] == 1 and mask is None and not self.training

@@ -1,20 +1,23 @@
 """`NormalizedFeedForwardNetwork` (megalodon/modules/normalized_feedforward_network.py:15-98)
 for model-parallel world size 1: Column/RowParallelLinear are plain `nn.Linear`
 (megalodon/modules/model_parallel/layers.py:222-235,321-341); the two dropouts
-sit where the reference has them (:83-90)."""
+sit where the reference has them (:83-90).  `fused_gate`: with `swiglu` and 16-bit rows the two projections and the gate
+(:82) are one operator, `fused_ops.gated_linear`, whose gate sees the products in float32; elsewhere, and by default, they are two
+products and `silu_mul`."""
 import torch
 import torch.nn.functional as F
 from torch import nn
 
-from ..fused_ops import memory_efficient_dropout, silu_mul
-from .linear import Linear, linear_group
+from ..fused_ops import gated_linear, memory_efficient_dropout, silu_mul
+from .linear import Linear, is_bare, linear_group
 from .layer_norm import FusedLayerNorm
 
 
 class NormalizedFeedForwardNetwork(nn.Module):
     def __init__(self, model_dim, ffn_hidden_dim, dropout=0.0, hidden_dropout=0.0, swiglu=False,
-                 norm_affine=True, norm_eps=1e-5, rescale=None, init_std=0.02):
+                 norm_affine=True, norm_eps=1e-5, rescale=None, init_std=0.02, fused_gate=False):
         super().__init__()
+        self.fused_gate = fused_gate
         self.dropout = dropout
         self.hidden_dropout = hidden_dropout
         self.model_dim = model_dim
@@ -37,9 +40,17 @@ class NormalizedFeedForwardNetwork(nn.Module):
     def rescale(self, x: torch.Tensor) -> torch.Tensor:
         return x if self.alpha is None else (self.alpha * x)
 
+    def takes_fused_gate(self, x: torch.Tensor) -> bool:
+        """Rows and weights of one 16-bit type on the GPU, and layers whose call is nothing but `Linear.forward`."""
+        layers = (self.fc1, self.fc3)
+        return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and not torch.is_autocast_enabled("cuda")
+                and all(l.weight.dtype == x.dtype and l.bias is None and is_bare(l) for l in layers))
+
     def forward(self, x, residual):
         x = self.norm(x)
-        if self.swiglu:
+        if self.swiglu and self.fused_gate and self.takes_fused_gate(x):
+            hidden = gated_linear(x, self.fc1.weight, self.fc3.weight)
+        elif self.swiglu:
             hidden = silu_mul(*linear_group(x, (self.fc1, self.fc3)))
         else:
             hidden = F.silu(self.fc1(x))
