@@ -9,7 +9,6 @@
 #include "common.hpp"
 
 #include <algorithm>
-#include <vector>
 
 namespace mega {
 namespace {
@@ -223,35 +222,47 @@ int chunk_bytes_of(const mega_tensors& t) {
 }
 constexpr int64_t kMostChunks = 1ll << 31;  // of a launch
 
-// The launches of a call, one after the other: f(tensors, workgroups).
+// The launches of a call, one after the other (`last_first`: from the end): f(tensors, workgroups).
 template <typename F>
-int each_launch(const mega_tensors& t, bool to, F f) {
-  Tensors a{};
-  a.chunk_bytes = chunk_bytes_of(t);
-  const auto flush = [&]() {
-    if (a.count == 0) return static_cast<int>(MEGA_OK);
-    for (int i = a.count + 1; i <= kPerLaunch + kStarts; ++i) a.start[i] = 0xffffffffu;
-    const int rc = f(a, static_cast<unsigned>(std::min<int64_t>(a.start[a.count], kGroups)));
-    a.count = 0;
-    return rc;
+int each_launch(const mega_tensors& t, bool to, bool last_first, F f) {
+  const int chunk_bytes = chunk_bytes_of(t);
+  const auto chunks_of = [&](int64_t i) {
+    const int64_t size = elem_size(t.dtype[i]);
+    return (t.size[i] * size + chunk_bytes - 1) / chunk_bytes;
   };
-  for (int64_t i = 0; i < t.count; ++i) {
-    const int64_t size = elem_size(t.dtype[i]), chunks = (t.size[i] * size + a.chunk_bytes - 1) / a.chunk_bytes;
-    if (chunks == 0) continue;
-    if (a.count == kPerLaunch || (a.count > 0 && a.start[a.count] + chunks > kMostChunks))
-      if (const int rc = flush(); rc != MEGA_OK) return rc;
-    const int k = a.count++;
-    a.from[k] = t.from[i];
-    a.to[k] = to ? t.to[i] : nullptr;
-    a.start[k + 1] = a.start[k] + static_cast<uint32_t>(chunks);
-    a.last[k] = static_cast<uint16_t>(t.size[i] - (chunks - 1) * (a.chunk_bytes / size) - 1);
-    a.dtype[k] = static_cast<uint8_t>(t.dtype[i]);
+  int64_t lo = 0, hi = t.count;  // the tensors that are left
+  while (lo < hi) {
+    // as many of them as a launch takes: [begin, end)
+    int64_t count = 0, chunks = 0, n = 0;
+    for (; n < hi - lo; ++n) {
+      const int64_t one = chunks_of(last_first ? hi - 1 - n : lo + n);
+      if (one == 0) continue;
+      if (count == kPerLaunch || (count > 0 && chunks + one > kMostChunks)) break;
+      ++count, chunks += one;
+    }
+    const int64_t begin = last_first ? hi - n : lo, end = begin + n;
+    (last_first ? hi : lo) = last_first ? begin : end;
+    if (count == 0) continue;
+    Tensors a{};
+    a.chunk_bytes = chunk_bytes;
+    for (int64_t i = begin; i < end; ++i) {
+      const int64_t size = elem_size(t.dtype[i]), one = chunks_of(i);
+      if (one == 0) continue;
+      const int k = a.count++;
+      a.from[k] = t.from[i];
+      a.to[k] = to ? t.to[i] : nullptr;
+      a.start[k + 1] = a.start[k] + static_cast<uint32_t>(one);
+      a.last[k] = static_cast<uint16_t>(t.size[i] - (one - 1) * (chunk_bytes / size) - 1);
+      a.dtype[k] = static_cast<uint8_t>(t.dtype[i]);
+    }
+    for (int k = a.count + 1; k <= kPerLaunch + kStarts; ++k) a.start[k] = 0xffffffffu;
+    if (const int rc = f(a, static_cast<unsigned>(std::min<int64_t>(a.start[a.count], kGroups))); rc != MEGA_OK) return rc;
   }
-  return flush();
+  return MEGA_OK;
 }
 int64_t totals_of(const mega_tensors& t) {
   int64_t n = 0;
-  each_launch(t, false, [&](const Tensors&, unsigned groups) { return n += groups, static_cast<int>(MEGA_OK); });
+  each_launch(t, false, false, [&](const Tensors&, unsigned groups) { return n += groups, static_cast<int>(MEGA_OK); });
   return n;
 }
 
@@ -273,7 +284,7 @@ extern "C" int mega_tensors_norm(const mega_tensors* tensors, int kind, float* o
   hipStream_t s = static_cast<hipStream_t>(stream);
   double *const norm = static_cast<double*>(workspace), *const totals = norm + 1;
   int64_t n = 0;
-  const int rc = each_launch(*tensors, false, [&](const Tensors& t, unsigned groups) {
+  const int rc = each_launch(*tensors, false, false, [&](const Tensors& t, unsigned groups) {
     if (kind == MEGA_NORM_2) norm_kernel<false><<<groups, kThreads, 0, s>>>(t, totals + n);
     else norm_kernel<true><<<groups, kThreads, 0, s>>>(t, totals + n);
     MEGA_CHECK_LAUNCH();
@@ -292,7 +303,7 @@ extern "C" int mega_tensors_clip(const mega_tensors* tensors, double max_norm, c
   MEGA_CHECK_ARG(max_norm >= 0, "mega_tensors_clip: max_norm must not be negative");
   MEGA_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 8 == 0, "mega_tensors_clip: null or misaligned pointer");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return each_launch(*tensors, true, [&](const Tensors& t, unsigned groups) {
+  return each_launch(*tensors, true, true, [&](const Tensors& t, unsigned groups) {
     scale_kernel<<<groups, kThreads, 0, s>>>(t, static_cast<const double*>(workspace), max_norm);
     MEGA_CHECK_LAUNCH();
     return static_cast<int>(MEGA_OK);
