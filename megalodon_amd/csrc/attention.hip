@@ -1038,10 +1038,8 @@ __global__ __launch_bounds__(2 * T) void gemm_dma64_kernel(const GemmParams p) {
     else if (GATE) offb[i] = static_cast<uint32_t>((static_cast<int64_t>(min(n0 / 2 + (pc >> 3) * 32 + (row & 31), p.gate_n - 1)) * p.ldb + kb + ck * 8) * 2);
     else offb[i] = static_cast<uint32_t>((static_cast<int64_t>(min(n0 + row, t.N - 1)) * p.ldb + kb + ck * 8) * 2);
   }
-  // GATE: pieces of 8 rows, four of one matrix and four of the other: eight waves have one matrix each, four waves send them in turn
-  static_assert(!GATE || (!TA && !TB), "two k-contiguous operands");
-  const uint16_t* const b_odd = !GATE ? nullptr : NW == 8 && (__builtin_amdgcn_readfirstlane(wave) & 4) == 0 ? p.B : p.B2;
-  if constexpr (GATE && NW == 8) B = b_odd;
+  // GATE: pieces of 8 rows, four of one matrix and four of the other, which the four waves send in turn
+  static_assert(!GATE || (!TA && !TB && NW == 4), "two k-contiguous operands, tiles of 128");
   const uint32_t stepa = static_cast<uint32_t>((TA ? t.lda : 1) * kSlab64 * 2);
   const uint32_t stepb = static_cast<uint32_t>((TB ? p.ldb : 1) * kSlab64 * 2);
   const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(
@@ -1050,7 +1048,7 @@ __global__ __launch_bounds__(2 * T) void gemm_dma64_kernel(const GemmParams p) {
   auto request_one = [&](int s, int stage, int n) {
     const uint32_t sc = static_cast<uint32_t>(min(s, nslab - 1));
     const uint32_t dst = lds_wave + static_cast<uint32_t>(stage * kStage + (n >> 1) * NW * 512 + (n & 1) * kOperand) * 2;
-    if (n & 1) load_to_lds16(GATE && NW == 4 && (n >> 1) % 2 == 1 ? b_odd : B, offb[n >> 1] + sc * stepb, dst);
+    if (n & 1) load_to_lds16(GATE && (n >> 1) % 2 == 1 ? p.B2 : B, offb[n >> 1] + sc * stepb, dst);
     else load_to_lds16(A, offa[n >> 1] + sc * stepa, dst);
   };
   auto request = [&](int s, int stage) {
@@ -2120,9 +2118,9 @@ int launch_linear(GemmParams q, int kind, int count, const int64_t* sizes, hipSt
   return launch_tiles<gemm_dma_kernel<DT, true, true, false, kSmall, true>>(q, grid, threads, lds, s);
 }
 
-// Forward products of two layers that meet in silu(a) b: planned as one layer of 2 n_out features.  A single row of large tiles
-// (which the estimate takes for 4096 -> 11008 from 140 tokens on) leaves the chip to the weights' stream: us, small / large, 200 tokens,
-// 4096 -> 11008 53 / 70, 2048 -> 5504 20 / 35.  Of 100 sizes (65 to 8192 tokens, five networks) the choice is then at most 15 %
+// Forward products of two layers that meet in silu(a) b: planned as one layer of 2 n_out features, small tiles here or those of gated_tiles.hip.  A single
+// row of large tiles (which the estimate takes for 4096 -> 11008 from 140 tokens on) leaves the chip to the weights' stream: us, small / large,
+// 200 tokens, 2048 -> 5504 20 / 27, 1024 -> 2752 9 / 24.  Of 75 sizes (65 to 8192 tokens, five networks) the choice is then at most 15 %
 // off the better one, 1 % in the mean.
 bool plan_gated(GemmParams& q, int cus) {
   const int64_t both = q.N;
@@ -2139,16 +2137,8 @@ template <int DT>
 int launch_gated(GemmParams q, int cus, hipStream_t s) {
   q.nh = 1; q.alpha = 1.f; q.n_group = 8;
   const bool small = plan_gated(q, cus);
-  if (!small) {
-    const int whole = q.cut > 0 ? q.full : q.items, most = std::max(cus / kXcds, 1) * kXcds;
-    const GatedTiles t{q.A, q.B, q.B2, q.C, q.Ca, q.Cb, q.M, q.K, q.gate_n, static_cast<int>(gated_pitch(q.gate_n)), q.mt_count, q.nt_count, whole};
-    if (whole > 0)
-      if (const int rc = gated_tiles(DT, q.Ca == nullptr ? 0 : q.wide ? 2 : 1, t, std::min((whole + kXcds - 1) / kXcds * kXcds, most), s); rc != MEGA_OK) return rc;
-    if (q.cut == 0) return MEGA_OK;
-    const int left = q.items - q.full, grid = (left * q.cut + kXcds - 1) / kXcds * kXcds;
-    if (const int rc = launch_tiles<gemm_dma64_kernel<DT, false, false, kTile, false, true, true>>(q, grid, 2 * kTile, kDmaLds, s); rc != MEGA_OK) return rc;
-    return launch_tiles<linear_parts_kernel<DT, kTile, false, false, true>>(q, left * 32, kWave, 0, s);
-  }
+  if (!small) return gated_tiles(DT, q.A, q.B, q.B2, q.M, q.K, q.gate_n, q.C, q.Ca, q.Cb, q.wide != 0, q.parts, s);
+  if (q.cut > 0 && q.parts == nullptr) return set_error(MEGA_ERR_INVALID_ARG, "gated_linear: null workspace");
   const size_t lds = sizeof(uint16_t) * kStages * 2 * kSmall * kSlab;
   const int grid = (q.items * std::max(q.cut, 1) + kXcds - 1) / kXcds * kXcds;
   if (q.cut > 0) {
@@ -2166,18 +2156,8 @@ int64_t gated_parts_bytes(int64_t tokens, int64_t n_in, int64_t n_out) {
   if (compute_units(&cus) != MEGA_OK) return 0;
   const int64_t both = 2 * n_out;
   GemmParams q = linear_sizes(kForward, tokens, n_in, 1, &both);
-  const int64_t tile = plan_gated(q, cus) ? kSmall : kTile;
-  return static_cast<int64_t>(q.items - q.full) * q.cut * tile * tile * static_cast<int64_t>(sizeof(float));
-}
-
-int weight_grad_onto(int dtype, const uint16_t* dy, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, const uint16_t* add,
-                     uint16_t* dw, float* parts, hipStream_t s) {
-  GemmParams g{};
-  g.A = dy; g.B = x; g.C = dw; g.add = add;
-  g.M = (int)n_out; g.N = (int)n_in; g.K = (int)tokens;
-  g.lda = n_out; g.ldb = n_in; g.ldc = n_in; g.ta = 1; g.tb = 1;
-  g.parts = parts; g.split_ok = parts != nullptr;
-  return dtype == MEGA_BF16 ? launch_linear<MEGA_BF16>(g, kWeightGrad, 1, &n_out, s) : launch_linear<MEGA_F16>(g, kWeightGrad, 1, &n_out, s);
+  if (!plan_gated(q, cus)) return gated_tiles_bytes(0, tokens, n_in, n_out);
+  return static_cast<int64_t>(q.items) * q.cut * kSmall * kSmall * static_cast<int64_t>(sizeof(float));
 }
 
 int gated_product(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
@@ -2186,7 +2166,7 @@ int gated_product(int dtype, const uint16_t* x, const uint16_t* w1, const uint16
   g.A = x; g.B = w1; g.B2 = w3; g.C = h; g.Ca = a; g.Cb = b; g.wide = wide;
   g.M = (int)tokens; g.N = (int)(2 * n_out); g.K = (int)n_in; g.gate_n = (int)n_out;
   g.lda = g.ldb = n_in; g.ldc = n_out;
-  g.parts = parts; g.split_ok = parts != nullptr;
+  g.parts = parts; g.split_ok = 1;
   int cus = 0;
   if (const int rc = compute_units(&cus); rc != MEGA_OK) return rc;
   return dtype == MEGA_BF16 ? launch_gated<MEGA_BF16>(g, cus, s) : launch_gated<MEGA_F16>(g, cus, s);

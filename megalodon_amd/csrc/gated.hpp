@@ -17,17 +17,31 @@ __device__ __forceinline__ float fast_sigmoid(float a) {
 __device__ float fast_sigmoid(float a);
 #endif
 
-// h = silu(x w1^T) o (x w3^T), and the two products where they are kept (a and b; null: they are not); tokens * n_in and n_out * n_in
-// below 2^30, n_in a multiple of 64, rows of x, w1 and w3 on 16-byte boundaries.
-// Rows of a and b are `pitch` elements apart, n_out rounded up to 8; what lies behind n_out is of no meaning.
-// Tiles 0 .. tiles - 1 of 256 tokens x 128 features, in bands of eight columns of tiles, row by row in each.
+// A launch of gated_tiles.hip: C (m, n) of operands A and B along k, as its modes read them.
 struct GatedTiles {
-  const uint16_t *x, *w1, *w3;
-  uint16_t* h;
-  void *a, *b;
-  int tokens, n_in, n_out, pitch, row_tiles, col_tiles, tiles;
+  const uint16_t *a, *b, *b2;
+  uint32_t a_bytes, b_bytes;  // where the operands end
+  int m, n, k, lda, ldb;
+  int seg;                    // kInput: slabs of 64 features of b, those behind them are b2's
+  uint16_t* c;
+  void *kept_a, *kept_b;      // kGate: rows of `pitch` elements, n rounded up to 8; what lies behind n is of no meaning
+  int pitch;
+  int cols, n_out, add;       // kInput, kWeight: columns of c; kWeight: rows of either half of c, and whether they are added to
+  int row_tiles, col_tiles;
+  int full, left, cut;        // tiles as a whole, then some whose slabs are cut into `cut` pieces, which go to parts
+  float* parts;
 };
-int gated_tiles(int dtype, int keep, const GatedTiles& p, int grid, hipStream_t s);
+// Operands of fewer than 2^30 elements on 16-byte boundaries; parts: gated_tiles_bytes (kind: 0, 1, 2 as they stand here), or null for none.
+// h = silu(x w1^T) o (x w3^T); a and b may be null; n_in a multiple of 8
+int gated_tiles(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
+                uint16_t* h, void* a, void* b, bool wide, float* parts, hipStream_t s);
+// g (tokens, 2 half), half n_out rounded up to 64: the gradients of a and, from column half on, of b, zeros behind n_out.  Rows of x, w1, w3 `ld`
+// elements apart, a multiple of 8.  dx (tokens, n_in), dw (2, n_out, n_in) of any pitch; add: dw is added to
+int gated_tiles_input(int dtype, const uint16_t* g, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld,
+                      uint16_t* dx, float* parts, hipStream_t s);
+int gated_tiles_weight(int dtype, const uint16_t* g, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld, bool add,
+                       uint16_t* dw, float* parts, hipStream_t s);
+int64_t gated_tiles_bytes(int kind, int64_t tokens, int64_t n_in, int64_t n_out);
 
 // parts: gated_parts_bytes, or null; wide: a and b in float32
 int gated_product(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,

@@ -8,18 +8,14 @@
 // cores) and of the results.  (Gradients in 16 bits off by 1.4 roundings where
 // float32 is kept, by 1.8 where not; training on 32768 tokens, 4096 -> 11008, takes 5 % longer with it.)
 //
-// Many tokens: the product kernels of attention.hip with a gate for an epilogue (gated_product).  Few: the weights' stream from memory is all
-// the time there is, and the kernel below reads them once, straight into the operand registers of the matrix cores.
+// Many tokens: tiles with the gate for an epilogue (gated_product of attention.hip, gated_tiles.hip).  Few: the weights' stream from
+// memory is all the time there is, and the kernel below reads them once, straight into the operand registers of the matrix cores.
 #include "common.hpp"
 #include "gated.hpp"
 
 #include <algorithm>
 
 namespace mega {
-
-// dw (n_out, n_in) = dy^T x + add; sizes as mega_linear_weight_grads takes them (attention.hip)
-int weight_grad_onto(int dtype, const uint16_t* dy, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, const uint16_t* add,
-                     uint16_t* dw, float* parts, hipStream_t s);
 
 namespace {
 
@@ -176,55 +172,37 @@ int few_tokens(const FewParams& p, hipStream_t s) {
   return few_of<DT, 4, 2>(p, cus, s);
 }
 
-// ---- rows of whole 16-byte pieces, and back -----------------------------------------------------------
+// ---- rows of whole 16-byte pieces -----------------------------------------------------------------------
 constexpr int kThreads = 256;
 
-// Matrices copied in one launch, 16 bytes a thread: dst (rows, to) = src (rows, from), zeros behind column `from`, or (NARROW) its first
-// columns.  The padded side has rows of whole pieces on 16-byte boundaries.
+// Matrices copied in one launch, 16 bytes a thread: dst (rows, to) = src (rows, from), zeros behind column `from`; `to` whole
+// pieces, dst on 16-byte boundaries.
 struct Copies {
   struct One {
     const uint16_t* src;
     uint16_t* dst;
     int64_t pieces;  // of this one and of those in front
     int from, to;
-  } one[5];
+  } one[3];
   int count;
   void add(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t from, int64_t to) {
-    if (rows == 0) return;
     const int64_t before = count > 0 ? one[count - 1].pieces : 0;
-    one[count++] = {src, dst, before + rows * (std::max(from, to) / 8), static_cast<int>(from), static_cast<int>(to)};
+    one[count++] = {src, dst, before + rows * (to / 8), static_cast<int>(from), static_cast<int>(to)};
   }
 };
-template <bool NARROW>
 __global__ __launch_bounds__(kThreads) void copies_kernel(const Copies c) {
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < c.one[c.count - 1].pieces; i += static_cast<int64_t>(gridDim.x) * kThreads) {
     int m = 0;
     while (i >= c.one[m].pieces) ++m;
     const Copies::One& o = c.one[m];
-    const int64_t at = m > 0 ? i - c.one[m - 1].pieces : i;
-    const int per = (NARROW ? o.from : o.to) / 8;
-    const int64_t row = at / per;
-    const int k = static_cast<int>(at - row * per) * 8;
-    if constexpr (!NARROW) {
-      *reinterpret_cast<u32x4*>(o.dst + 8 * at) = eight<false>(o.src + row * o.from, k, o.from);
-    } else {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(o.src + 8 * at);
-      uint16_t* const to_row = o.dst + row * o.to;
-      if (k + 8 <= o.to) {
-        *reinterpret_cast<u32x4_any*>(to_row + k) = __builtin_bit_cast(u32x4_any, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (k + e < o.to) to_row[k + e] = static_cast<uint16_t>(v[e / 2] >> (16 * (e % 2)));
-      }
-    }
+    const int64_t at = m > 0 ? i - c.one[m - 1].pieces : i, row = at / (o.to / 8);
+    *reinterpret_cast<u32x4*>(o.dst + 8 * at) = eight<false>(o.src + row * o.from, static_cast<int>(at - row * (o.to / 8)) * 8, o.from);
   }
 }
 unsigned pieces_grid(int64_t pieces) { return static_cast<unsigned>(std::min<int64_t>((pieces + kThreads - 1) / kThreads, 16384)); }
-template <bool NARROW>
 int copy_all(const Copies& c, hipStream_t s) {
   if (c.count == 0) return MEGA_OK;
-  copies_kernel<NARROW><<<pieces_grid(c.one[c.count - 1].pieces), kThreads, 0, s>>>(c);
+  copies_kernel<<<pieces_grid(c.one[c.count - 1].pieces), kThreads, 0, s>>>(c);
   MEGA_CHECK_LAUNCH();
   return MEGA_OK;
 }
@@ -239,14 +217,14 @@ __device__ __forceinline__ void kept_eight(const void* p, int64_t at, float* v) 
     v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
   }
 }
-// da, db (tokens, ld) from dh (tokens, n) and a, b (tokens, pitch): 8 elements a thread, zeros from column n to `to`
+// da | db (tokens, 2 h) from dh (tokens, n) and a, b (tokens, pitch): 8 elements a thread, zeros from column n on
 template <int DT, bool WIDE>
-__global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh, const void* a, const void* b, uint16_t* da, uint16_t* db,
-                                                            int64_t tokens, int n, int pitch, int to, int64_t ld) {
-  const int64_t pieces = tokens * (to / 8);
+__global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh, const void* a, const void* b, uint16_t* g2,
+                                                            int64_t tokens, int n, int pitch, int h) {
+  const int64_t pieces = tokens * (h / 8);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < pieces; i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t row = i / (to / 8);
-    const int k = static_cast<int>(i - row * (to / 8)) * 8;
+    const int64_t row = i / (h / 8);
+    const int k = static_cast<int>(i - row * (h / 8)) * 8;
     float g[8], u[8], v[8], du[8], dv[8];
     if (k < pitch) {
       unpack8<DT>(__builtin_bit_cast(uint4, eight<false>(dh + row * n, k, n)), g);
@@ -259,8 +237,9 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh,
       dv[e] = k + e < n ? g[e] * u[e] * s : 0.f;
       du[e] = k + e < n ? g[e] * v[e] * s * (1.f + u[e] * (1.f - s)) : 0.f;
     }
-    *reinterpret_cast<uint4*>(da + row * ld + k) = pack8<DT>(du);
-    *reinterpret_cast<uint4*>(db + row * ld + k) = pack8<DT>(dv);
+    uint16_t* const to = g2 + row * 2 * h + k;
+    *reinterpret_cast<uint4*>(to) = pack8<DT>(du);
+    *reinterpret_cast<uint4*>(to + h) = pack8<DT>(dv);
   }
 }
 
@@ -296,28 +275,25 @@ struct Forward {
     bytes = room.bytes;
   }
 };
-// Backward: the gradients of a and b beside each other, (tokens, 2 h), are one operand of both products, w1 on w3 (2 h, k) the
-// other of dx.  Few enough products, and weights whose rows the products take as they are: apart (the weights are not copied).
+// Backward: the gradients of a and b beside each other, (tokens, 2 h), for gated_tiles.hip.  (Small sizes too: networks of 1024 -> 2752
+// and up are faster so than by the products of attention.hip, whose tiles are small, by 10 to 50 % up to 1024 tokens; 512 -> 1408 up to 20 % slower from
+// 512 tokens on.)
 struct Backward {
-  bool apart;
   int64_t h, k, rows;  // n_out and n_in with their padding, tokens of a launch
-  int64_t g, w, x, dx, dw, parts, bytes;
+  int64_t g, w1, w3, x, parts, bytes;
   Backward(int64_t tokens, int64_t n_in, int64_t n_out, int what) {
     Room room;
-    apart = n_out % 64 == 0 && n_in % 8 == 0 && static_cast<double>(tokens) * n_in * n_out <= 0x1p33 && tokens * std::max(2 * n_out, n_in) < kMost;
-    h = apart ? n_out : up(n_out, 32), k = up(n_in, 8);
+    h = up(n_out, 64), k = up(n_in, 8);
     rows = std::min(tokens, std::max<int64_t>((kMost - 1) / std::max(2 * h, k) / 256 * 256, 256));
     g = room.take(2 * rows * 2 * h);
-    w = (what & 1) && !apart ? room.take(2 * 2 * h * k) : 0;
+    w1 = (what & 1) && k != n_in ? room.take(2 * n_out * k) : 0;
+    w3 = (what & 1) && k != n_in ? room.take(2 * n_out * k) : 0;
     x = (what & 2) && k != n_in ? room.take(2 * rows * k) : 0;
-    dx = (what & 1) && k != n_in ? room.take(2 * rows * k) : 0;
-    dw = (what & 2) && (k != n_in || h != n_out) ? room.take(2 * 2 * h * k) : 0;
-    parts = 0;
-    if (what & 2) {
-      const int64_t both = 2 * h, one[2] = {h, h}, rest = std::max<int64_t>(tokens % rows, 1);
-      const auto want = [&](int64_t n) { return mega_linear_workspace_bytes(2, n, k, apart ? 2 : 1, apart ? one : &both); };
-      parts = room.take(std::max(want(rows), want(rest)));
-    }
+    // (the products run one after the other)
+    int64_t most = 0;
+    for (int kind = 1; kind <= 2; ++kind)
+      if (what & kind) most = std::max({most, gated_tiles_bytes(kind, rows, n_in, n_out), gated_tiles_bytes(kind, std::max<int64_t>(tokens % rows, 1), n_in, n_out)});
+    parts = room.take(most);
     bytes = room.bytes;
   }
 };
@@ -325,7 +301,7 @@ struct Backward {
 int check(const char* who, int dtype, int64_t tokens, int64_t n_in, int64_t n_out) {
   MEGA_CHECK_ARG(dtype == MEGA_BF16 || dtype == MEGA_F16, "%s: bfloat16 or float16 tensors", who);
   MEGA_CHECK_ARG(tokens >= 1 && n_in >= 1 && n_out >= 1 && tokens < (1ll << 31) && n_in <= (1 << 20) && n_out <= (1 << 20) &&
-                     up(n_in, 64) * 2 * up(n_out, 32) < kMost,
+                     up(n_in, 64) * 2 * up(n_out, 64) < kMost,
                  "%s: bad sizes", who);
   return MEGA_OK;
 }
@@ -337,7 +313,7 @@ bool aligned16(const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0;
 using namespace mega;
 
 extern "C" int64_t mega_gated_linear_workspace_bytes(int64_t tokens, int64_t n_in, int64_t n_out, int backward) {
-  if (tokens < 1 || n_in < 1 || n_out < 1 || n_in > (1 << 20) || n_out > (1 << 20) || tokens >= (1ll << 31) || up(n_in, 64) * 2 * up(n_out, 32) >= kMost) return 0;
+  if (tokens < 1 || n_in < 1 || n_out < 1 || n_in > (1 << 20) || n_out > (1 << 20) || tokens >= (1ll << 31) || up(n_in, 64) * 2 * up(n_out, 64) >= kMost) return 0;
   return backward == 0 ? Forward(tokens, n_in, n_out).bytes : Backward(tokens, n_in, n_out, backward).bytes;
 }
 
@@ -371,12 +347,11 @@ extern "C" int mega_gated_linear_fwd(const void* x_, const void* w1_, const void
         c.add(w3, at(f.w3), n_out, n_in, f.k);
         w1 = at(f.w1), w3 = at(f.w3);
       }
-      if (const int rc = copy_all<false>(c, s); rc != MEGA_OK) return rc;
+      if (const int rc = copy_all(c, s); rc != MEGA_OK) return rc;
       rows = at(f.x);
     }
-    const bool cut = gated_parts_bytes(n, f.k, n_out) > 0;
     const auto rows_of = [&](void* q) { return q == nullptr ? nullptr : static_cast<char*>(q) + t * gated_pitch(n_out) * (wide ? 4 : 2); };
-    if (const int rc = gated_product(dtype, rows, w1, w3, n, f.k, n_out, h + t * n_out, rows_of(a), rows_of(b), wide, cut ? reinterpret_cast<float*>(ws + f.parts) : nullptr, s);
+    if (const int rc = gated_product(dtype, rows, w1, w3, n, f.k, n_out, h + t * n_out, rows_of(a), rows_of(b), wide, reinterpret_cast<float*>(ws + f.parts), s);
         rc != MEGA_OK)
       return rc;
   }
@@ -400,57 +375,33 @@ extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void
   char* const ws = static_cast<char*>(workspace);
   const auto at = [&](int64_t offset) { return reinterpret_cast<uint16_t*>(ws + offset); };
   const int64_t h = f.h, k = f.k;
-  uint16_t* const dw_at = dw != nullptr && (k != n_in || h != n_out) ? at(f.dw) : dw;
   for (int64_t t = 0; t < tokens; t += f.rows) {
     const int64_t n = std::min(f.rows, tokens - t);
-    uint16_t *da = at(f.g), *db = f.apart ? da + n * h : da + h;
-    const int64_t ld = f.apart ? h : 2 * h, pitch = gated_pitch(n_out), at0 = t * n_out;
-    Copies c{}, back{};
-    if (dx != nullptr && !f.apart && t == 0) {
-      uint16_t *const u1 = at(f.w), *const u3 = u1 + h * k;
-      c.add(w1, u1, n_out, n_in, k);
-      c.add(w3, u3, n_out, n_in, k);
-      // (features behind the last meet gradients that are zero: they have to be finite)
-      c.add(w1, u1 + n_out * k, h - n_out, 0, k);
-      c.add(w3, u3 + n_out * k, h - n_out, 0, k);
-    }
+    uint16_t* const g = at(f.g);
+    const int64_t pitch = gated_pitch(n_out), at0 = t * n_out;
     const uint16_t* rows = x + t * n_in;
-    if (dw != nullptr && k != n_in) {
-      c.add(rows, at(f.x), n, n_in, k);
-      rows = at(f.x);
+    if (k != n_in) {
+      Copies c{};
+      if (dx != nullptr && t == 0) {
+        c.add(w1, at(f.w1), n_out, n_in, k);
+        c.add(w3, at(f.w3), n_out, n_in, k);
+        w1 = at(f.w1), w3 = at(f.w3);
+      }
+      if (dw != nullptr) c.add(rows, at(f.x), n, n_in, k), rows = at(f.x);
+      if (const int rc = copy_all(c, s); rc != MEGA_OK) return rc;
     }
-    if (const int rc = copy_all<false>(c, s); rc != MEGA_OK) return rc;
     const unsigned grid = pieces_grid(n * (h / 8));
     const bool wide = kept == MEGA_F32;
     const auto rows_of = [&](const void* q) { return static_cast<const char*>(q) + t * pitch * (wide ? 4 : 2); };
-    const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(dh + at0, rows_of(a), rows_of(b), da, db, n, (int)n_out, (int)pitch, (int)h, ld); };
+    const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(dh + at0, rows_of(a), rows_of(b), g, n, (int)n_out, (int)pitch, (int)h); };
     if (dtype == MEGA_BF16) wide ? launch(gate_grad_kernel<MEGA_BF16, true>) : launch(gate_grad_kernel<MEGA_BF16, false>);
     else wide ? launch(gate_grad_kernel<MEGA_F16, true>) : launch(gate_grad_kernel<MEGA_F16, false>);
     MEGA_CHECK_LAUNCH();
-    const int64_t both = 2 * h, one[2] = {h, h};
-    const void *gs[2] = {da, db}, *both_w = at(f.w);
-    if (dx != nullptr) {
-      uint16_t* const to = k != n_in ? at(f.dx) : dx + t * n_in;
-      const void* ws2[2] = {w1, w3};
-      const int rc = f.apart ? mega_linear_input_grad(gs, ws2, nullptr, dtype, n, k, 2, one, to, stream)
-                             : mega_linear_input_grad(gs, &both_w, nullptr, dtype, n, k, 1, &both, to, stream);
-      if (rc != MEGA_OK) return rc;
-      if (k != n_in) back.add(to, dx + t * n_in, n, k, n_in);
-    }
-    if (dw != nullptr) {
-      const bool cut = mega_linear_workspace_bytes(2, n, k, f.apart ? 2 : 1, f.apart ? one : &both) > 0;
-      float* const parts = cut ? reinterpret_cast<float*>(ws + f.parts) : nullptr;
-      void* to[2] = {dw_at, dw_at + h * k};
-      // (apart: all of the tokens in one launch)
-      const int rc = f.apart ? mega_linear_weight_grads(gs, rows, dtype, n, k, 2, one, to, parts, stream)
-                             : weight_grad_onto(dtype, da, rows, n, k, both, t > 0 ? dw_at : nullptr, dw_at, parts, s);
-      if (rc != MEGA_OK) return rc;
-      if (dw_at != dw && t + n == tokens) {
-        back.add(dw_at, dw, n_out, k, n_in);
-        back.add(dw_at + h * k, dw + n_out * n_in, n_out, k, n_in);
-      }
-    }
-    if (const int rc = copy_all<true>(back, s); rc != MEGA_OK) return rc;
+    float* const parts = reinterpret_cast<float*>(ws + f.parts);
+    if (dx != nullptr)
+      if (const int rc = gated_tiles_input(dtype, g, w1, w3, n, n_in, n_out, k, dx + t * n_in, parts, s); rc != MEGA_OK) return rc;
+    if (dw != nullptr)
+      if (const int rc = gated_tiles_weight(dtype, g, rows, n, n_in, n_out, k, t > 0, dw, parts, s); rc != MEGA_OK) return rc;
   }
   return MEGA_OK;
 }

@@ -45,10 +45,8 @@ def formula(x, w1, w3, dh, dtype, kept=None):
     eda = dh.abs() * ((slope.abs() + 0.5 * ea) * eb + 0.5 * ea * b.abs() + exp * b.abs() * 2)
     edb = dh.abs() * (1.1 * ea + exp * (g.abs() + ea))
     eda, edb = eda + half(da.abs() + eda, dtype), edb + half(db.abs() + edb, dtype)
-    first = da @ w1
-    dx = first + db @ w3
+    dx = da @ w1 + db @ w3
     edx = product(da, eda, w1, none(w1), 2 * H) + product(db, edb, w3, none(w3), 2 * H)
-    edx = edx + half(first.abs() + edx, dtype)  # (two layers one after the other: rounded between them)
     out.append((dx, edx + half(dx.abs() + edx, dtype)))
     for d, e in ((da, eda), (db, edb)):
         w, ew = d.t() @ x, product(d.t(), e.t(), x, none(x), T)
@@ -110,9 +108,30 @@ def test_few_tokens(tokens, n_in, n_out, dtype):
     (30000, 192, 2000, torch.bfloat16),    # three
     (20000, 320, 2100, torch.bfloat16),    # and five
     (200, 4096, 2048, torch.bfloat16),
+    (5000, 520, 1032, torch.bfloat16),     # both gradients' sums in pieces
+    (20000, 264, 72, torch.float16),       # dw of two tiles, many pieces
+    (700, 24, 130000, torch.bfloat16),     # dx of three
+    (66000, 40, 40, torch.float16),        # a tile more than the chip has units
 ])
 def test_tiles(tokens, n_in, n_out, dtype):
     check(*operands(tokens, n_in, n_out, dtype))
+
+
+def test_tokens_of_several_launches():
+    """An operand of 2^30 elements and more: launch by launch, the weights' gradients added to."""
+    one = ((1 << 30) - 1) // 1024 // 256 * 256  # tokens of a launch
+    tokens, n_in, n_out = one + 300, 1024, 8
+    x, w1, w3, dh = operands(tokens, n_in, n_out, torch.bfloat16)
+    want = formula(x, w1, w3, dh, x.dtype)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w1, w3)]
+    h = fused_ops.gated_linear(*leaves)
+    close(h, want[0])
+    dx, *dw = torch.autograd.grad(h, leaves, dh)
+    close(dx, want[1])
+    del dx, h
+    first = formula(x[:one], w1, w3, dh[:one], x.dtype)
+    for got, (value, bar), (part, off) in zip(dw, want[2:], first[2:]):
+        close(got, (value, bar + half(part.abs() + off, x.dtype)))  # (the first launch's sum was rounded)
 
 
 @pytest.mark.parametrize("tokens", [5, 200])
