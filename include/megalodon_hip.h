@@ -572,19 +572,20 @@ int mega_tensors_clip(const mega_tensors* tensors, double max_norm, const void* 
  *
  * (`F.silu(self.fc1(x)) * self.fc3(x)`, megalodon/modules/normalized_feedforward_network.py:82, with both projections.)
  * Tensors of `dtype` (MEGA_BF16 / MEGA_F16), contiguous, of any sizes from 1 (n_in and n_out up to 2^20, the two matrices
- * together, n_in rounded up to 64, below 2^30 elements, tokens below 2^31); x, the matrices and what is written for them on 16-byte boundaries.  Products and gate in float32, h rounded once from them.
+ * together, n_in and n_out rounded up to 64, below 2^30 elements, tokens below 2^31); x, the matrices, a and b on 16-byte
+ * boundaries.  Products and gate in float32, h rounded once from them.
  *   fwd: a = x w1^T and b = x w3^T as well, in `kept` (`dtype` or MEGA_F32), rows of n_out rounded up to 8 elements (what lies
  *        behind n_out has no meaning), or null for both; they are what bwd wants.
- *   bwd: dx (tokens, n_in) or null; dw (2, n_out, n_in), the gradients of w1 and w3, or null.  The gradients of a and b are
- *        rounded to `dtype`, operands of the matrix cores as they are; sums are float32 and rounded once (dw of more than
+ *   bwd: dx (tokens, n_in), dw1 and dw3 (n_out, n_in); null: not wanted.  The gradients of a and b are
+ *        rounded to `dtype`, operands of the matrix cores as they are; sums are float32 and rounded once (dw1 and dw3 of more than
  *        2^30 / (2 n_out) tokens: once for each 2^30 / (2 n_out) of them).
  * Sizes whose rows are no whole 16-byte pieces are laid out anew in `workspace`.  It holds the mega_gated_linear_workspace_bytes
- * (backward = 0, or bits: 1 for dx, 2 for dw) bytes that the call wants, on a 16-byte boundary. */
+ * (backward = 0, or bits: 1 for dx, 2 for dw1, 4 for dw3) bytes that the call wants, on a 16-byte boundary. */
 int64_t mega_gated_linear_workspace_bytes(int64_t tokens, int64_t n_in, int64_t n_out, int backward);
 int mega_gated_linear_fwd(const void* x, const void* w1, const void* w3, int dtype, int64_t tokens, int64_t n_in, int64_t n_out,
                           void* h, void* a, void* b, int kept, void* workspace, void* stream);
 int mega_gated_linear_bwd(const void* dh, const void* x, const void* w1, const void* w3, const void* a, const void* b, int kept, int dtype,
-                          int64_t tokens, int64_t n_in, int64_t n_out, void* dx, void* dw, void* workspace, void* stream);
+                          int64_t tokens, int64_t n_in, int64_t n_out, void* dx, void* dw1, void* dw3, void* workspace, void* stream);
 
 /* ------------------------------------------------------------------------
  * LayerNorm / RMSNorm over the last axis, stored weight = gamma - 1.

@@ -23,25 +23,25 @@ struct GatedTiles {
   uint32_t a_bytes, b_bytes;  // where the operands end
   int m, n, k, lda, ldb;
   int seg;                    // kInput: slabs of 64 features of b, those behind them are b2's
-  uint16_t* c;
+  uint16_t *c, *c2;           // (kWeight: the gradient of w1 or of the only matrix, of w3)
   void *kept_a, *kept_b;      // kGate: rows of `pitch` elements, n rounded up to 8; what lies behind n is of no meaning
   int pitch;
-  int cols, n_out, add;       // kInput, kWeight: columns of c; kWeight: rows of either half of c, and whether they are added to
+  int cols, half, n_out, add; // kInput, kWeight: columns of c; kWeight: columns of a half of A, rows of c, and whether they are added to
   int row_tiles, col_tiles;
   int full, left, cut;        // tiles as a whole, then some whose slabs are cut into `cut` pieces, which go to parts
   float* parts;
 };
 // Operands of fewer than 2^30 elements on 16-byte boundaries; parts: gated_tiles_bytes (kind: 0, 1, 2 as they stand here), or null for none.
-// h = silu(x w1^T) o (x w3^T); a and b may be null; n_in a multiple of 8
+// h = silu(x w1^T) o (x w3^T); a and b may be null; n_in a multiple of 64
 int gated_tiles(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
                 uint16_t* h, void* a, void* b, bool wide, float* parts, hipStream_t s);
 // g (tokens, 2 half), half n_out rounded up to 64: the gradients of a and, from column half on, of b, zeros behind n_out.  Rows of x, w1, w3 `ld`
-// elements apart, a multiple of 8.  dx (tokens, n_in), dw (2, n_out, n_in) of any pitch; add: dw is added to
+// elements apart, a multiple of 8.  dx (tokens, n_in), dw1 and dw3 (n_out, n_in), one of them or both, of any pitch; add: they are added to
 int gated_tiles_input(int dtype, const uint16_t* g, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld,
                       uint16_t* dx, float* parts, hipStream_t s);
 int gated_tiles_weight(int dtype, const uint16_t* g, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld, bool add,
-                       uint16_t* dw, float* parts, hipStream_t s);
-int64_t gated_tiles_bytes(int kind, int64_t tokens, int64_t n_in, int64_t n_out);
+                       uint16_t* dw1, uint16_t* dw3, float* parts, hipStream_t s);
+int64_t gated_tiles_bytes(int kind, int64_t tokens, int64_t n_in, int64_t n_out, int matrices = 2);
 
 // parts: gated_parts_bytes, or null; wide: a and b in float32
 int gated_product(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,

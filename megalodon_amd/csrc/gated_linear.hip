@@ -281,18 +281,20 @@ struct Forward {
 struct Backward {
   int64_t h, k, rows;  // n_out and n_in with their padding, tokens of a launch
   int64_t g, w1, w3, x, parts, bytes;
-  Backward(int64_t tokens, int64_t n_in, int64_t n_out, int what) {
+  Backward(int64_t tokens, int64_t n_in, int64_t n_out, int what) {  // (what: 1 dx, 2 dw1, 4 dw3)
     Room room;
     h = up(n_out, 64), k = up(n_in, 8);
     rows = std::min(tokens, std::max<int64_t>((kMost - 1) / std::max(2 * h, k) / 256 * 256, 256));
     g = room.take(2 * rows * 2 * h);
     w1 = (what & 1) && k != n_in ? room.take(2 * n_out * k) : 0;
     w3 = (what & 1) && k != n_in ? room.take(2 * n_out * k) : 0;
-    x = (what & 2) && k != n_in ? room.take(2 * rows * k) : 0;
+    x = what > 1 && k != n_in ? room.take(2 * rows * k) : 0;
     // (the products run one after the other)
     int64_t most = 0;
-    for (int kind = 1; kind <= 2; ++kind)
-      if (what & kind) most = std::max({most, gated_tiles_bytes(kind, rows, n_in, n_out), gated_tiles_bytes(kind, std::max<int64_t>(tokens % rows, 1), n_in, n_out)});
+    for (const int64_t n : {rows, std::max<int64_t>(tokens % rows, 1)}) {
+      if (what & 1) most = std::max(most, gated_tiles_bytes(1, n, n_in, n_out));
+      if (what > 1) most = std::max(most, gated_tiles_bytes(2, n, n_in, n_out, what >= 6 ? 2 : 1));
+    }
     parts = room.take(most);
     bytes = room.bytes;
   }
@@ -322,7 +324,7 @@ extern "C" int mega_gated_linear_fwd(const void* x_, const void* w1_, const void
   if (const int rc = check("mega_gated_linear_fwd", dtype, tokens, n_in, n_out); rc != MEGA_OK) return rc;
   MEGA_CHECK_ARG(x_ && w1_ && w3_ && h_ && (a == nullptr) == (b == nullptr), "mega_gated_linear_fwd: null pointer");
   MEGA_CHECK_ARG(kept == dtype || kept == MEGA_F32, "mega_gated_linear_fwd: the products are kept in the operands' type or in float32");
-  for (const void* q : {x_, w1_, w3_, static_cast<const void*>(workspace)}) MEGA_CHECK_ARG(aligned16(q), "mega_gated_linear_fwd: misaligned pointer");
+  for (const void* q : {x_, w1_, w3_, static_cast<const void*>(a), static_cast<const void*>(b), static_cast<const void*>(workspace)}) MEGA_CHECK_ARG(aligned16(q), "mega_gated_linear_fwd: misaligned pointer");
   const uint16_t *x = static_cast<const uint16_t*>(x_), *w1 = static_cast<const uint16_t*>(w1_), *w3 = static_cast<const uint16_t*>(w3_);
   uint16_t* h = static_cast<uint16_t*>(h_);
   const bool wide = kept == MEGA_F32;
@@ -359,17 +361,17 @@ extern "C" int mega_gated_linear_fwd(const void* x_, const void* w1_, const void
 }
 
 extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void* w1_, const void* w3_, const void* a, const void* b, int kept, int dtype,
-                                     int64_t tokens, int64_t n_in, int64_t n_out, void* dx_, void* dw_, void* workspace, void* stream) {
+                                     int64_t tokens, int64_t n_in, int64_t n_out, void* dx_, void* dw1_, void* dw3_, void* workspace, void* stream) {
   if (const int rc = check("mega_gated_linear_bwd", dtype, tokens, n_in, n_out); rc != MEGA_OK) return rc;
   MEGA_CHECK_ARG(dh_ && x_ && w1_ && w3_ && a && b && workspace, "mega_gated_linear_bwd: null pointer");
   MEGA_CHECK_ARG(kept == dtype || kept == MEGA_F32, "mega_gated_linear_bwd: the products are kept in the operands' type or in float32");
-  for (const void* q : {x_, w1_, w3_, static_cast<const void*>(dx_), static_cast<const void*>(dw_), static_cast<const void*>(workspace)})
+  for (const void* q : {x_, w1_, w3_, a, b, static_cast<const void*>(workspace)})
     MEGA_CHECK_ARG(aligned16(q), "mega_gated_linear_bwd: misaligned pointer");
   const auto u = [](const void* q) { return static_cast<const uint16_t*>(q); };
   const uint16_t *dh = u(dh_), *x = u(x_), *w1 = u(w1_), *w3 = u(w3_);
-  uint16_t *dx = static_cast<uint16_t*>(dx_), *dw = static_cast<uint16_t*>(dw_);
+  uint16_t *dx = static_cast<uint16_t*>(dx_), *dw1 = static_cast<uint16_t*>(dw1_), *dw3 = static_cast<uint16_t*>(dw3_);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int what = (dx != nullptr) + 2 * (dw != nullptr);
+  const int what = (dx != nullptr) + 2 * (dw1 != nullptr) + 4 * (dw3 != nullptr);
   if (what == 0) return MEGA_OK;
   const Backward f(tokens, n_in, n_out, what);
   char* const ws = static_cast<char*>(workspace);
@@ -387,7 +389,7 @@ extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void
         c.add(w3, at(f.w3), n_out, n_in, k);
         w1 = at(f.w1), w3 = at(f.w3);
       }
-      if (dw != nullptr) c.add(rows, at(f.x), n, n_in, k), rows = at(f.x);
+      if (what > 1) c.add(rows, at(f.x), n, n_in, k), rows = at(f.x);
       if (const int rc = copy_all(c, s); rc != MEGA_OK) return rc;
     }
     const unsigned grid = pieces_grid(n * (h / 8));
@@ -400,8 +402,8 @@ extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void
     float* const parts = reinterpret_cast<float*>(ws + f.parts);
     if (dx != nullptr)
       if (const int rc = gated_tiles_input(dtype, g, w1, w3, n, n_in, n_out, k, dx + t * n_in, parts, s); rc != MEGA_OK) return rc;
-    if (dw != nullptr)
-      if (const int rc = gated_tiles_weight(dtype, g, rows, n, n_in, n_out, k, t > 0, dw, parts, s); rc != MEGA_OK) return rc;
+    if (what > 1)
+      if (const int rc = gated_tiles_weight(dtype, g, rows, n, n_in, n_out, k, t > 0, dw1, dw3, parts, s); rc != MEGA_OK) return rc;
   }
   return MEGA_OK;
 }

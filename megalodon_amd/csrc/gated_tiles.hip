@@ -115,10 +115,10 @@ __device__ __forceinline__ void finish(const GatedTiles& p, const f32x4* acc, in
       }
   } else {
     // kWeight: rows behind n_out of either half are padding
-    const bool second = MODE == kWeight && row >= p.m / 2;
-    const int in_half = second ? row - p.m / 2 : row;
+    const bool second = MODE == kWeight && row >= p.half;
+    const int in_half = second ? row - p.half : row;
     if (MODE == kWeight && in_half >= p.n_out) return;
-    uint16_t* const to = p.c + (second ? static_cast<int64_t>(p.n_out) + in_half : static_cast<int64_t>(in_half)) * p.cols;
+    uint16_t* const to = (second ? p.c2 : p.c) + static_cast<int64_t>(in_half) * p.cols;
 #pragma unroll
     for (int f = 0; f < 4; f += 2) {
       uint2 v[2];
@@ -193,12 +193,8 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
   const uint32_t lds_wave = lds0 + wave * 1024;
   // the ring: operand slabs A 0, B 0, A 1, B 1, .. in buffers 0 .. 4 in turn
   const auto behind = [&](uint32_t at, uint32_t buffers) { return at + buffers * kOperandBytes >= kRing ? at + buffers * kOperandBytes - kRing : at + buffers * kOperandBytes; };
-  // (kGate: chunks behind the last k are zeros, of both operands)
-  const int k_last = p.k - (slabs - 1) * kK;
-  const auto along = [&](uint32_t offset, int slab) { return slab == slabs - 1 && 8 * chunk8 >= k_last ? 0xfffffff0u : offset + slab * 128; };
   const auto request_a = [&](int slab, uint32_t to, int i) {
-    const uint32_t offset = kRowsA ? off_a[i] + slab * kK * pitch_a : MODE == kGate ? along(off_a[i], slab) : off_a[i] + slab * 128;
-    load_to_lds16(buf_a, offset, lds_wave + to + i * 8192);
+    load_to_lds16(buf_a, off_a[i] + slab * (kRowsA ? kK * pitch_a : kK * 2), lds_wave + to + i * 8192);
   };
   const auto request_b = [&](int slab, uint32_t to, int i) {
     if constexpr (MODE == kInput) {
@@ -206,7 +202,7 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
       const u32x4 buf = second ? buf_b2 : buf_b;
       load_to_lds16(buf, off_b[i] + (second ? slab - p.seg : slab) * kK * pitch_b, lds_wave + to + i * 8192);
     } else {
-      load_to_lds16(buf_b, kRowsB ? off_b[i] + slab * kK * pitch_b : along(off_b[i], slab), lds_wave + to + i * 8192);
+      load_to_lds16(buf_b, off_b[i] + slab * (kRowsB ? kK * pitch_b : kK * 2), lds_wave + to + i * 8192);
     }
   };
 
@@ -415,13 +411,15 @@ int launch(GatedTiles p, int most, hipStream_t s) {
   MEGA_CHECK_LAUNCH();
   return MEGA_OK;
 }
+int64_t half_of(int64_t n_out) { return (n_out + kK - 1) / kK * kK; }
 // the last byte of `rows` rows of `n` elements
 uint32_t bytes_of(int64_t rows, int64_t pitch, int64_t n) { return static_cast<uint32_t>(2 * ((rows - 1) * pitch + n)); }
-GatedTiles sizes_of(int mode, int64_t tokens, int64_t n_in, int64_t n_out, int64_t half) {
+GatedTiles sizes_of(int mode, int64_t tokens, int64_t n_in, int64_t n_out, int matrices) {
   GatedTiles p{};
-  p.m = static_cast<int>(mode == kWeight ? 2 * half : tokens), p.k = static_cast<int>(mode == kGate ? n_in : mode == kInput ? 2 * half : tokens);
+  const int64_t half = half_of(n_out);
+  p.m = static_cast<int>(mode == kWeight ? matrices * half : tokens), p.k = static_cast<int>(mode == kGate ? n_in : mode == kInput ? 2 * half : tokens);
   p.row_tiles = (p.m + kTileRows - 1) / kTileRows, p.col_tiles = static_cast<int>(mode == kGate ? (n_out + 127) / 128 : (n_in + 255) / 256);
-  p.n_out = static_cast<int>(n_out), p.cols = static_cast<int>(n_in), p.seg = static_cast<int>(half / kK);
+  p.n_out = static_cast<int>(n_out), p.half = static_cast<int>(half), p.cols = static_cast<int>(n_in), p.seg = static_cast<int>(half / kK);
   return p;
 }
 template <int MODE, int KEEP>
@@ -433,21 +431,20 @@ int launch_of(int dtype, GatedTiles p, float* parts, hipStream_t s) {
   if (p.left > 0 && parts == nullptr) return set_error(MEGA_ERR_INVALID_ARG, "gated_linear: null workspace");
   return dtype == MEGA_BF16 ? launch<MEGA_BF16, MODE, KEEP>(p, most, s) : launch<MEGA_F16, MODE, KEEP>(p, most, s);
 }
-int64_t half_of(int64_t n_out) { return (n_out + kK - 1) / kK * kK; }
 
 }  // namespace
 
-int64_t gated_tiles_bytes(int kind, int64_t tokens, int64_t n_in, int64_t n_out) {
+int64_t gated_tiles_bytes(int kind, int64_t tokens, int64_t n_in, int64_t n_out, int matrices) {
   int most = 0;
   if (workgroups(&most) != MEGA_OK) return 0;
-  GatedTiles p = sizes_of(kind, tokens, n_in, n_out, half_of(n_out));
+  GatedTiles p = sizes_of(kind, tokens, n_in, n_out, matrices);
   cut_last(p, most);
   return static_cast<int64_t>(p.left) * p.cut * kPieceBytes;
 }
 
 int gated_tiles(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
                 uint16_t* h, void* a, void* b, bool wide, float* parts, hipStream_t s) {
-  GatedTiles p = sizes_of(kGate, tokens, n_in, n_out, half_of(n_out));
+  GatedTiles p = sizes_of(kGate, tokens, n_in, n_out, 2);
   p.a = x, p.b = w1, p.b2 = w3, p.a_bytes = bytes_of(tokens, n_in, n_in), p.b_bytes = bytes_of(n_out, n_in, n_in);
   p.n = static_cast<int>(n_out), p.lda = p.ldb = static_cast<int>(n_in);
   p.c = h, p.kept_a = a, p.kept_b = b, p.pitch = static_cast<int>(gated_pitch(n_out));
@@ -458,18 +455,19 @@ int gated_tiles(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t
 int gated_tiles_input(int dtype, const uint16_t* g, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld,
                       uint16_t* dx, float* parts, hipStream_t s) {
   const int64_t both = 2 * half_of(n_out);
-  GatedTiles p = sizes_of(kInput, tokens, n_in, n_out, both / 2);
+  GatedTiles p = sizes_of(kInput, tokens, n_in, n_out, 2);
   p.a = g, p.b = w1, p.b2 = w3, p.a_bytes = bytes_of(tokens, both, both), p.b_bytes = bytes_of(n_out, ld, ld);
   p.n = static_cast<int>(ld), p.lda = static_cast<int>(both), p.ldb = static_cast<int>(ld), p.c = dx;
   return launch_of<kInput, 0>(dtype, p, parts, s);
 }
 
 int gated_tiles_weight(int dtype, const uint16_t* g, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld, bool add,
-                       uint16_t* dw, float* parts, hipStream_t s) {
+                       uint16_t* dw1, uint16_t* dw3, float* parts, hipStream_t s) {
   const int64_t both = 2 * half_of(n_out);
-  GatedTiles p = sizes_of(kWeight, tokens, n_in, n_out, both / 2);
-  p.a = g, p.b = p.b2 = x, p.a_bytes = bytes_of(tokens, both, both), p.b_bytes = bytes_of(tokens, ld, ld);
-  p.n = static_cast<int>(ld), p.lda = static_cast<int>(both), p.ldb = static_cast<int>(ld), p.c = dw, p.add = add;
+  GatedTiles p = sizes_of(kWeight, tokens, n_in, n_out, dw1 != nullptr && dw3 != nullptr ? 2 : 1);
+  const int64_t from = dw1 != nullptr ? 0 : both / 2;
+  p.a = g + from, p.b = p.b2 = x, p.a_bytes = bytes_of(tokens, both, both - from), p.b_bytes = bytes_of(tokens, ld, ld);
+  p.n = static_cast<int>(ld), p.lda = static_cast<int>(both), p.ldb = static_cast<int>(ld), p.c = dw1 != nullptr ? dw1 : dw3, p.c2 = dw3, p.add = add;
   return launch_of<kWeight, 0>(dtype, p, parts, s);
 }
 

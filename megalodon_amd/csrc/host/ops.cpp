@@ -812,20 +812,25 @@ struct GatedFn : Function<GatedFn> {
       return {want_x ? (at::mm(da, w1) + at::mm(db, w3)).view(saved[0].sizes()) : Tensor(), want_1 ? at::mm(da.t(), x) : Tensor(), want_3 ? at::mm(db.t(), x) : Tensor(), Tensor()};
     }
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor x = attn_operand(saved[0]), w1 = attn_operand(saved[1]), w3 = attn_operand(saved[2]), a = saved[3].contiguous(), b = saved[4].contiguous();
-    const Tensor dh = g[0].contiguous();
+    const Tensor x = attn_operand(saved[0]), w1 = attn_operand(saved[1]), w3 = attn_operand(saved[2]), a = attn_operand(saved[3]), b = attn_operand(saved[4]);
+    const Tensor dh = stored(g[0]).contiguous();
     require(dh.scalar_type() == x.scalar_type(), "gated_linear: the output's gradient must have x's dtype");
     const int64_t n_in = x.size(-1), n_out = w1.size(0), tokens = x.numel() / n_in;
-    Tensor dx, dw;
+    // (saved-tensor hooks may hand back anything)
+    require(w1.sizes() == w3.sizes() && w1.size(1) == n_in && dh.numel() == tokens * n_out && a.numel() == tokens * ((n_out + 7) / 8 * 8) && a.sizes() == b.sizes() && a.scalar_type() == b.scalar_type(),
+            "gated_linear: a saved tensor has another shape than it was saved with");
+    Tensor dx, d1, d3;
     if (want_x) dx = at::empty_like(x);
-    if (want_1 || want_3) dw = at::empty({2, n_out, n_in}, x.options());
+    if (want_1) d1 = at::empty_like(w1);
+    if (want_3) d3 = at::empty_like(w3);
     if (tokens == 0) {
-      if (dw.defined()) dw.zero_();
-    } else if (dx.defined() || dw.defined()) {
-      const Tensor ws = bytes(mega_gated_linear_workspace_bytes(tokens, n_in, n_out, (dx.defined() ? 1 : 0) + (dw.defined() ? 2 : 0)), x);
-      check(mega_gated_linear_bwd(dh.data_ptr(), x.data_ptr(), w1.data_ptr(), w3.data_ptr(), a.data_ptr(), b.data_ptr(), code_of(a.scalar_type()), kernel_code(x), tokens, n_in, n_out, ptr(dx), ptr(dw), ptr(ws), stream_of(x)), "mega_gated_linear_bwd");
+      if (want_1) d1.zero_();
+      if (want_3) d3.zero_();
+    } else {
+      const Tensor ws = bytes(mega_gated_linear_workspace_bytes(tokens, n_in, n_out, want_x + 2 * want_1 + 4 * want_3), x);
+      check(mega_gated_linear_bwd(dh.data_ptr(), x.data_ptr(), w1.data_ptr(), w3.data_ptr(), a.data_ptr(), b.data_ptr(), code_of(a.scalar_type()), kernel_code(x), tokens, n_in, n_out, ptr(dx), ptr(d1), ptr(d3), ptr(ws), stream_of(x)), "mega_gated_linear_bwd");
     }
-    return {dx, want_1 ? dw.select(0, 0) : Tensor(), want_3 ? dw.select(0, 1) : Tensor(), Tensor()};
+    return {dx, d1, d3, Tensor()};
   }
 };
 Tensor gated_linear(const Tensor& x_, const Tensor& w1_, const Tensor& w3_, std::optional<at::ScalarType> kept) {

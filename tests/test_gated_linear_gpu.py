@@ -165,6 +165,39 @@ def test_some_gradients(tokens):
             close(g, want[i])
 
 
+def test_gradients_are_tensors_of_their_own():
+    x, w1, w3, dh = operands(70, 72, 40, torch.bfloat16)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w1, w3)]
+    grads = torch.autograd.grad(fused_ops.gated_linear(*leaves), leaves, dh)
+    assert all(g.untyped_storage().nbytes() == 2 * g.numel() and g.is_contiguous() for g in grads)
+
+
+@pytest.mark.parametrize("tokens", [9, 130])
+def test_output_gradient_negated_on_reading(tokens):
+    x, w1, w3, dh = operands(tokens, 72, 40, torch.float16)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w1, w3)]
+    h = fused_ops.gated_linear(*leaves)
+    want = torch.autograd.grad(h, leaves, dh, retain_graph=True)
+    for got, w in zip(torch.autograd.grad(h, leaves, torch._neg_view(-dh)), want):
+        assert torch.equal(got, w)
+
+
+def test_saved_tensors_through_hooks():
+    """What is saved may travel (host memory, another boundary); of another shape it is refused."""
+    x, w1, w3, dh = operands(70, 72, 36, torch.bfloat16)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w1, w3)]
+    want = torch.autograd.grad(fused_ops.gated_linear(*leaves), leaves, dh)
+    shifted = lambda t: torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), shifted):
+        h = fused_ops.gated_linear(*leaves)
+    for got, w in zip(torch.autograd.grad(h, leaves, dh), want):
+        assert torch.equal(got, w)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[: t.shape[0] // 2]):
+        h = fused_ops.gated_linear(*leaves)
+    with pytest.raises(RuntimeError, match="saved tensor"):
+        torch.autograd.grad(h, leaves, dh)
+
+
 def test_no_tokens():
     _, w1, w3, _ = operands(1, 64, 32, torch.float16)
     x = torch.empty(0, 64, dtype=torch.float16, device="cuda", requires_grad=True)
@@ -187,6 +220,12 @@ def test_rows_do_not_touch_each_other(tokens, n_in):
     columns = [i for i in range(40) if i != 7]
     assert torch.equal(got[rows][:, columns], clean[rows][:, columns])
     assert got[1].isnan().all() and not got[2].isfinite().all()
+    dh = torch.ones_like(clean)
+    grads = []
+    for t in (x, x2):
+        leaf = t.clone().requires_grad_(True)
+        grads.append(torch.autograd.grad(fused_ops.gated_linear(leaf, w1, w3), leaf, dh)[0])
+    assert torch.equal(grads[1][rows], grads[0][rows]) and grads[1][1].isnan().all()
 
 
 def test_large_arguments():
