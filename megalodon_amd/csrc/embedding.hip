@@ -141,8 +141,9 @@ __global__ __launch_bounds__(kRankWaves * kWave) void rank_kernel(const Token* t
   order[count] = static_cast<uint32_t>(i);
 }
 
-// More: digits from the lowest up, each a stable move of all positions; a workgroup has kSortBlock of them.
-constexpr int kSortThreads = 512, kSortWaves = kSortThreads / kWave, kSortEach = 4, kSortBlock = kSortThreads * kSortEach, kMostDigits = 2048;
+// More: digits from the lowest up, each a stable move of all positions; a workgroup has `tiles` times kSortBlock of them, one after the other (every workgroup
+// reads the counts of all: there are kSortGroups at most).
+constexpr int kSortThreads = 512, kSortWaves = kSortThreads / kWave, kSortEach = 4, kSortBlock = kSortThreads * kSortEach, kMostDigits = 2048, kSortGroups = 1024;
 
 // what the passes move: in the first, the tokens themselves
 template <typename Token>
@@ -154,14 +155,16 @@ struct Positions {
 };
 
 template <typename Token>
-__global__ __launch_bounds__(kSortThreads) void count_kernel(const Positions<Token> from, int64_t n, int shift, int digits, uint32_t* counts) {
+__global__ __launch_bounds__(kSortThreads) void count_kernel(const Positions<Token> from, int64_t n, int tiles, int shift, int digits, uint32_t* counts) {
   __shared__ uint32_t seen[kMostDigits];
   for (int d = threadIdx.x; d < digits; d += kSortThreads) seen[d] = 0;
   __syncthreads();
+  for (int tile = 0; tile < tiles; ++tile) {
 #pragma unroll
-  for (int q = 0; q < kSortEach; ++q) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kSortBlock + q * kSortThreads + threadIdx.x;
-    if (i < n) atomicAdd(&seen[from.key(i) >> shift & (digits - 1)], 1u);
+    for (int q = 0; q < kSortEach; ++q) {
+      const int64_t i = (static_cast<int64_t>(blockIdx.x) * tiles + tile) * kSortBlock + q * kSortThreads + threadIdx.x;
+      if (i < n) atomicAdd(&seen[from.key(i) >> shift & (digits - 1)], 1u);
+    }
   }
   __syncthreads();
   for (int d = threadIdx.x; d < digits; d += kSortThreads) counts[static_cast<int64_t>(blockIdx.x) * digits + d] = seen[d];
@@ -170,14 +173,13 @@ __global__ __launch_bounds__(kSortThreads) void count_kernel(const Positions<Tok
 // A digit's first place for this workgroup: all smaller digits, and its own of the workgroups in front.  A wave has 256 consecutive
 // positions, 64 at a time: lanes of one digit find each other by ballots, one of them advances the wave's count of it.
 template <typename Token>
-__global__ __launch_bounds__(kSortThreads) void move_kernel(const Positions<Token> from, int64_t n, int shift, int bits, const uint32_t* counts,
+__global__ __launch_bounds__(kSortThreads) void move_kernel(const Positions<Token> from, int64_t n, int tiles, int shift, int bits, const uint32_t* counts,
                                                            uint32_t* keys, uint32_t* order) {
   extern __shared__ uint32_t lds[];
   const int digits = 1 << bits, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   uint32_t* const begins = lds;                  // [digits]
   uint32_t* const seen = lds + digits;           // [wave][digits]
   __shared__ uint32_t wave_sums[kSortWaves];
-  for (int d = threadIdx.x; d < digits * kSortWaves; d += kSortThreads) seen[d] = 0;
   // neighbouring digits a thread: their totals and those in front
   constexpr int kEach = kMostDigits / kSortThreads;
   uint32_t total[kEach] = {}, before[kEach] = {}, sum = 0;
@@ -209,10 +211,12 @@ __global__ __launch_bounds__(kSortThreads) void move_kernel(const Positions<Toke
     if (kEach * static_cast<int>(threadIdx.x) + q < digits) begins[kEach * threadIdx.x + q] = at + before[q];
     at += total[q];
   }
+  for (int tile = 0; tile < tiles; ++tile) {
+  for (int d = threadIdx.x; d < digits * kSortWaves; d += kSortThreads) seen[d] = 0;
   __syncthreads();
   uint32_t key[kSortEach], rank[kSortEach];
   volatile uint32_t* const mine = seen + wave * digits;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortBlock + wave * (kWave * kSortEach) + lane;
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * tiles + tile) * kSortBlock + wave * (kWave * kSortEach) + lane;
 #pragma unroll
   for (int q = 0; q < kSortEach; ++q) key[q] = first + q * kWave < n ? from.key(first + q * kWave) : 0;
 #pragma unroll
@@ -241,6 +245,7 @@ __global__ __launch_bounds__(kSortThreads) void move_kernel(const Positions<Toke
       seen[w * digits + d] = place;
       place += c;
     }
+    begins[d] = place;
   }
   __syncthreads();
 #pragma unroll
@@ -250,6 +255,8 @@ __global__ __launch_bounds__(kSortThreads) void move_kernel(const Positions<Toke
     const uint32_t to = seen[wave * digits + (key[q] >> shift & (digits - 1))] + rank[q];
     keys[to] = key[q];
     order[to] = from.tokens != nullptr ? static_cast<uint32_t>(i) : from.order[i];
+  }
+  __syncthreads();
   }
 }
 
@@ -394,7 +401,7 @@ bool whole_lines(const void* p, int64_t width, int dtype) { return reinterpret_c
 int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct Sizes {
-  int bits, passes;  // of a sorting pass, and how many
+  int bits, passes, tiles;  // of a sorting pass, and how many
   int slices, per_piece;
   int64_t blocks, pieces, bytes, keys[2], order[2], counts, open;  // (offsets into the workspace)
   Sizes(int dtype, int64_t n, int64_t vocab, int64_t width) {
@@ -402,7 +409,9 @@ struct Sizes {
     while ((vocab >> all) > 0) ++all;  // of keys up to `vocab`
     passes = (all + 10) / 11;
     bits = (all + passes - 1) / passes;
-    blocks = (n + kSortBlock - 1) / kSortBlock;
+    const int64_t lines = (n + kSortBlock - 1) / kSortBlock;
+    tiles = static_cast<int>((lines + kSortGroups - 1) / kSortGroups);
+    blocks = tiles > 0 ? (lines + tiles - 1) / tiles : 0;
     const int per = kThreads * (dtype == MEGA_F32 ? 4 : 8);
     slices = static_cast<int>((width + per - 1) / per);
     per_piece = 16;
@@ -452,9 +461,9 @@ int sort_positions(const Token* tokens, int64_t n, int64_t vocab, int64_t paddin
   MEGA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&move_kernel<Token>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
   for (int pass = 0; pass < z.passes; ++pass) {
     uint32_t *to_keys = at(z.keys[pass & 1]), *to_order = at(z.order[pass & 1]);
-    count_kernel<Token><<<static_cast<unsigned>(z.blocks), kSortThreads, 0, s>>>(from, n, pass * z.bits, 1 << z.bits, at(z.counts));
+    count_kernel<Token><<<static_cast<unsigned>(z.blocks), kSortThreads, 0, s>>>(from, n, z.tiles, pass * z.bits, 1 << z.bits, at(z.counts));
     MEGA_CHECK_LAUNCH();
-    move_kernel<Token><<<static_cast<unsigned>(z.blocks), kSortThreads, lds, s>>>(from, n, pass * z.bits, z.bits, at(z.counts), to_keys, to_order);
+    move_kernel<Token><<<static_cast<unsigned>(z.blocks), kSortThreads, lds, s>>>(from, n, z.tiles, pass * z.bits, z.bits, at(z.counts), to_keys, to_order);
     MEGA_CHECK_LAUNCH();
     from = Positions<Token>{nullptr, to_keys, to_order, vocab, padding};
   }

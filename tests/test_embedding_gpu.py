@@ -85,6 +85,12 @@ def test_many_tokens(n, V):
     check(text(n, V, n + V), table(V, 72, torch.bfloat16), 0.5)
 
 
+@pytest.mark.parametrize("V", [900, 70001])
+def test_several_lines_of_positions_for_a_workgroup(V):
+    g = torch.Generator("cuda").manual_seed(V)  # (no frequent ones: the oracle adds up in 64 bits one by one)
+    check(torch.randint(V, (2048 * 1024 * 2 + 12345,), generator=g, device="cuda", dtype=torch.int32), table(V, 4, torch.bfloat16))
+
+
 def test_three_passes():
     V = (1 << 22) + 77
     n = 9000
