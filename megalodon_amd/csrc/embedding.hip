@@ -1,12 +1,14 @@
 // Embedding for gfx950: rows of a table by token, and the table's gradient.
 //   y[r] = s W[t_r]                      (float32 / bfloat16 / float16, rounded once)
-//   dW[v] = s sum over r with t_r = v of dy[r]   (float32 sums, in an order that the sizes alone set)
+//   dW[v] = s sum over r with t_r = v of dy[r]   (float32 sums, in an order that sizes and tokens alone set)
 // A token that is no row of the table gives zeros and takes no gradient; the padding token gives its row and takes none.
 //
 // Both are bound by the bytes they move.  The gradient sorts the positions by token (stable), cuts the sorted line into equal pieces, so that
 // no frequent token keeps one workgroup, and sums each piece's runs of one token in registers.  A run that ends inside its piece is a row
 // of dW; runs over a piece's ends leave float32 sums that a second kernel adds up in their order.  Rows without a token are
-// zeroed by the same launch.  No atomics: the same call gives the same bits.
+// zeroed by the same launch.  The only atomics count integers: the same call gives the same bits.
+// Narrow rows leave a piece few threads, so that a workgroup has several pieces (bfloat16 gradients of 262144 tokens, us, one / several: 64 columns,
+// 1000 rows 169 / 67, 1048576 tokens 675 / 128).  32768 tokens, 32000 rows of 4096: sums 100 us of 126, 5.3 TB/s.
 #include "common.hpp"
 
 #include <algorithm>
@@ -141,9 +143,12 @@ __global__ __launch_bounds__(kRankWaves * kWave) void rank_kernel(const Token* t
   order[count] = static_cast<uint32_t>(i);
 }
 
-// More: digits from the lowest up, each a stable move of all positions; a workgroup has `tiles` times kSortBlock of them, one after the other (every workgroup
-// reads the counts of all: there are kSortGroups at most).
-constexpr int kSortThreads = 512, kSortWaves = kSortThreads / kWave, kSortEach = 4, kSortBlock = kSortThreads * kSortEach, kMostDigits = 2048, kSortGroups = 1024;
+// More: digits from the lowest up, each a stable move of all positions; a workgroup has `tiles` times kSortBlock of them, one after the other.  Few
+// workgroups read each other's counts where they need them, more than kSortAlone have them added up by a launch between (their reads grow with
+// the square: 262144 positions, two digits, us without / with: 160 / 45).  Positions of a thread, us for all of the gradient at 1, 2, 4:
+// 8193 tokens of 64 columns 37, 41, 44, 65536 49, 49, 52, 1048576 158, 158, 153.
+constexpr int kSortThreads = 512, kSortWaves = kSortThreads / kWave, kSortEach = 2, kSortBlock = kSortThreads * kSortEach, kMostDigits = 2048;
+constexpr int kSortAlone = 64, kSortGroups = 1024;
 
 // what the passes move: in the first, the tokens themselves
 template <typename Token>
@@ -170,32 +175,69 @@ __global__ __launch_bounds__(kSortThreads) void count_kernel(const Positions<Tok
   for (int d = threadIdx.x; d < digits; d += kSortThreads) counts[static_cast<int64_t>(blockIdx.x) * digits + d] = seen[d];
 }
 
-// A digit's first place for this workgroup: all smaller digits, and its own of the workgroups in front.  A wave has 256 consecutive
+// counts [group][digit] to those of the groups in front, and behind them the totals: a lane has a digit, the waves have a sixteenth of the groups each
+constexpr int kScanWaves = 16;
+__global__ __launch_bounds__(kScanWaves * kWave) void scan_kernel(uint32_t* counts, int groups, int digits) {
+  __shared__ uint32_t sums[kScanWaves][kWave];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, d = blockIdx.x * kWave + lane;
+  const int lo = groups * wave / kScanWaves, hi = groups * (wave + 1) / kScanWaves;
+  uint32_t sum = 0;
+  if (d < digits) {
+#pragma unroll 8
+    for (int g = lo; g < hi; ++g) sum += counts[static_cast<int64_t>(g) * digits + d];
+  }
+  sums[wave][lane] = sum;
+  __syncthreads();
+  if (d >= digits) return;
+  uint32_t at = 0;
+  for (int w = 0; w < wave; ++w) at += sums[w][lane];
+#pragma unroll 8
+  for (int g = lo; g < hi; ++g) {
+    const uint32_t c = counts[static_cast<int64_t>(g) * digits + d];
+    counts[static_cast<int64_t>(g) * digits + d] = at;
+    at += c;
+  }
+  if (wave == kScanWaves - 1) counts[static_cast<int64_t>(groups) * digits + d] = at;
+}
+
+// A digit's first place for this workgroup: all smaller digits, and its own of the workgroups in front.  A wave has 64 kSortEach consecutive
 // positions, 64 at a time: lanes of one digit find each other by ballots, one of them advances the wave's count of it.
 template <typename Token>
 __global__ __launch_bounds__(kSortThreads) void move_kernel(const Positions<Token> from, int64_t n, int tiles, int shift, int bits, const uint32_t* counts,
                                                            uint32_t* keys, uint32_t* order) {
   extern __shared__ uint32_t lds[];
-  const int digits = 1 << bits, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int digits = 1 << bits, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, groups = static_cast<int>(gridDim.x);
   uint32_t* const begins = lds;                  // [digits]
   uint32_t* const seen = lds + digits;           // [wave][digits]
-  __shared__ uint32_t wave_sums[kSortWaves];
-  // neighbouring digits a thread: their totals and those in front
-  constexpr int kEach = kMostDigits / kSortThreads;
-  uint32_t total[kEach] = {}, before[kEach] = {}, sum = 0;
-#pragma unroll
-  for (int q = 0; q < kEach; ++q) {
-    const int d = kEach * threadIdx.x + q;
-    if (d < digits) {
-#pragma unroll 8
-      for (unsigned b = 0; b < gridDim.x; ++b) {
-        const uint32_t c = counts[static_cast<int64_t>(b) * digits + d];
-        if (b < blockIdx.x) before[q] += c;
-        total[q] += c;
-      }
+  __shared__ uint32_t totals[kMostDigits], wave_sums[kSortWaves];
+  if (groups > kSortAlone) {
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) {
+      begins[d] = counts[static_cast<int64_t>(blockIdx.x) * digits + d];
+      totals[d] = counts[static_cast<int64_t>(groups) * digits + d];
     }
-    sum += total[q];
+  } else {
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) begins[d] = totals[d] = 0;
+    __syncthreads();
+    const int parts = max(kSortThreads / digits, 1);  // threads of a digit
+    for (int i = threadIdx.x; i < digits * parts; i += kSortThreads) {
+      const int d = i % digits;
+      uint32_t before = 0, total = 0;
+#pragma unroll 8
+      for (int g = i / digits; g < groups; g += parts) {
+        const uint32_t c = counts[g * digits + d];
+        if (g < static_cast<int>(blockIdx.x)) before += c;
+        total += c;
+      }
+      atomicAdd(&begins[d], before);
+      atomicAdd(&totals[d], total);
+    }
   }
+  __syncthreads();
+  // neighbouring digits a thread
+  const int each = (digits + kSortThreads - 1) / kSortThreads;
+  uint32_t sum = 0;
+  for (int q = 0; q < each; ++q)
+    if (const int d = each * threadIdx.x + q; d < digits) sum += totals[d];
   const uint32_t own = sum;
 #pragma unroll
   for (int step = 1; step < kWave; step *= 2) {
@@ -206,11 +248,8 @@ __global__ __launch_bounds__(kSortThreads) void move_kernel(const Positions<Toke
   __syncthreads();
   uint32_t at = sum - own;
   for (int w = 0; w < wave; ++w) at += wave_sums[w];
-#pragma unroll
-  for (int q = 0; q < kEach; ++q) {
-    if (kEach * static_cast<int>(threadIdx.x) + q < digits) begins[kEach * threadIdx.x + q] = at + before[q];
-    at += total[q];
-  }
+  for (int q = 0; q < each; ++q)
+    if (const int d = each * threadIdx.x + q; d < digits) begins[d] += at, at += totals[d];
   for (int tile = 0; tile < tiles; ++tile) {
   for (int d = threadIdx.x; d < digits * kSortWaves; d += kSortThreads) seen[d] = 0;
   __syncthreads();
@@ -253,6 +292,7 @@ __global__ __launch_bounds__(kSortThreads) void move_kernel(const Positions<Toke
     const int64_t i = first + q * kWave;
     if (i >= n) break;
     const uint32_t to = seen[wave * digits + (key[q] >> shift & (digits - 1))] + rank[q];
+    if (to >= n) break;  // (tokens that somebody wrote since they were counted: no order, but nothing outside the workspace)
     keys[to] = key[q];
     order[to] = from.tokens != nullptr ? static_cast<uint32_t>(i) : from.order[i];
   }
@@ -267,13 +307,13 @@ struct SumParams {
   const uint32_t *keys, *order;
   float* open;      // [piece][2][width]: sums of runs that begin in front of the piece, and of those that go on behind it
   int64_t n, vocab;
-  int width, per_piece, slices;
-  int64_t pieces;
+  int width, per_piece, slices, threads;  // threads: of a piece (narrow rows: several pieces to a workgroup)
+  int64_t pieces, groups;                 // groups: workgroups of a slice
   float scale;
   bool streaming;
 };
 constexpr int kZeroRows = 16;  // rows of dW that a workgroup looks at
-constexpr int kMostPiece = 1024;
+constexpr int kMostPiece = 1024;  // positions of a workgroup
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
@@ -281,10 +321,10 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
   using T = typename Elem<DT>::type;
   constexpr int kPer = R::kPer, kAhead = 8;
   const int tid = threadIdx.x;
-  if (blockIdx.x >= p.pieces * p.slices) {
+  if (blockIdx.x >= p.groups * p.slices) {
     // rows without a token: lanes look for 16 rows' keys, the workgroup writes
     __shared__ uint32_t empty;
-    const int64_t begin = blockIdx.x - p.pieces * p.slices, step = gridDim.x - p.pieces * p.slices;
+    const int64_t begin = blockIdx.x - p.groups * p.slices, step = gridDim.x - p.groups * p.slices;
     for (int64_t v0 = begin * kZeroRows; v0 < p.vocab; v0 += step * kZeroRows) {
     if (tid < kWave) {
       const int64_t v = v0 + tid;
@@ -311,17 +351,21 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
     }
     return;
   }
-  const int64_t piece = blockIdx.x / p.slices, first = piece * p.per_piece;
-  const int k = (blockIdx.x % p.slices * kThreads + tid) * kPer, left = p.width - k;
-  const int count = static_cast<int>(min(static_cast<int64_t>(p.per_piece), p.n - first));
-  __shared__ uint32_t keys[kMostPiece + 2], order[kMostPiece];  // keys[0] and keys[count + 1]: the neighbours'
-  for (int i = tid; i < count + 2; i += kThreads) {
+  const int each = kThreads / p.threads, own = tid / p.threads;  // pieces of the workgroup, the thread's among them
+  const int64_t piece0 = blockIdx.x / p.slices * each, first = piece0 * p.per_piece, piece = piece0 + own;
+  const int k = (blockIdx.x % p.slices * kThreads + tid % p.threads) * kPer, left = p.width - k;
+  const int all = static_cast<int>(min(static_cast<int64_t>(p.per_piece) * each, p.n - first));
+  __shared__ uint32_t all_keys[kMostPiece + 2], all_order[kMostPiece];  // all_keys[0] and [all + 1]: the neighbours'
+  for (int i = tid; i < all + 2; i += kThreads) {
     const int64_t at = first + i - 1;
-    keys[i] = at >= 0 && at < p.n ? p.keys[at] : 0xffffffffu;
-    if (i < count) order[i] = p.order[first + i];
+    all_keys[i] = at >= 0 && at < p.n ? p.keys[at] : 0xffffffffu;
+    if (i < all) all_order[i] = min(p.order[first + i], static_cast<uint32_t>(p.n - 1));  // (as above)
   }
   __syncthreads();
-  if (keys[1] >= p.vocab || left <= 0) return;
+  const int count = min(p.per_piece, all - own * p.per_piece);
+  if (own >= each || count <= 0 || left <= 0) return;
+  const uint32_t *const keys = all_keys + own * p.per_piece, *const order = all_order + own * p.per_piece;  // keys[0] and keys[count + 1]: the neighbours'
+  if (keys[1] >= p.vocab) return;
   const T* const dy = static_cast<const T*>(p.dy) + k;
   T* const dw = static_cast<T*>(p.dw) + k;
   float* const open = p.open + piece * 2 * p.width + k;
@@ -360,39 +404,60 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
   }
 }
 
-// Runs over the end of the piece that they begin in: the parts of it and of the pieces behind, in their order.
+// Runs over the end of the piece that they begin in: the parts of it and of the pieces behind, in their order; `columns` (16 .. 256, a power of two) to
+// a workgroup, whose threads have equal shares of a column's parts.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void join_kernel(const SumParams p) {
-  const unsigned slices = (p.width + kThreads - 1) / kThreads, piece = blockIdx.x / slices;
-  const int k = static_cast<int>(blockIdx.x % slices) * kThreads + threadIdx.x;
+__global__ __launch_bounds__(kThreads) void join_kernel(const SumParams p, int columns) {
+  const unsigned slices = (p.width + columns - 1) / columns, piece = blockIdx.x / slices;
+  const int tid = threadIdx.x, k = static_cast<int>(blockIdx.x % slices) * columns + tid % columns, share = tid / columns, shares = kThreads / columns;
   const int64_t first = static_cast<int64_t>(piece) * p.per_piece, behind = first + p.per_piece;
   if (behind >= p.n) return;
   const uint32_t key = p.keys[behind], last = p.keys[behind - 1], head = p.keys[first], ahead = first > 0 ? p.keys[first - 1] : 0xffffffffu;
   if (key >= p.vocab || last != key) return;
   if (head == key && ahead == key) return;  // begins further in front
-  // pieces behind whose first position is of the run
+  // pieces behind whose first position is of the run, 256 at a time
   int parts = 0;
   for (bool more = true; more; ) {
-    const int64_t at = behind + static_cast<int64_t>(parts + threadIdx.x % kWave) * p.per_piece;
-    const uint64_t in = __ballot(at < p.n && p.keys[min(at, p.n - 1)] == key);
-    const int run = in == ~0ull ? kWave : __builtin_ctzll(~in);
-    parts += run;
-    more = run == kWave;
+    uint64_t in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t at = behind + static_cast<int64_t>(parts + j * kWave + tid % kWave) * p.per_piece;
+      in[j] = __ballot(at < p.n && p.keys[min(at, p.n - 1)] == key);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int run = in[j] == ~0ull ? kWave : __builtin_ctzll(~in[j]);
+      if (more) parts += run;
+      more = more && run == kWave;
+    }
   }
-  if (k >= p.width) return;
   const int64_t step = 2 * static_cast<int64_t>(p.width);
-  const float* open = p.open + piece * step + k;
-  float sum = open[p.width];
-  constexpr int kAhead = 16;  // parts in flight
-  for (; parts >= kAhead; parts -= kAhead) {
-    float v[kAhead];
+  int left = static_cast<int>(static_cast<int64_t>(parts) * (share + 1) / shares);
+  const int begin = static_cast<int>(static_cast<int64_t>(parts) * share / shares);
+  left -= begin;
+  float sum = 0.f;
+  if (k < p.width) {
+    const float* open = p.open + piece * step + k;
+    if (share == 0) sum = open[p.width];
+    open += begin * step;
+    constexpr int kAhead = 16;  // parts in flight
+    for (; left >= kAhead; left -= kAhead) {
+      float v[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) v[i] = *(open += step);
+      for (int i = 0; i < kAhead; ++i) v[i] = *(open += step);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) sum += v[i];
+      for (int i = 0; i < kAhead; ++i) sum += v[i];
+    }
+    for (; left > 0; --left) sum += *(open += step);
   }
-  for (; parts > 0; --parts) sum += *(open += step);
-  Elem<DT>::store(static_cast<typename Elem<DT>::type*>(p.dw) + static_cast<int64_t>(key) * p.width + k, sum * p.scale);
+  if (shares > 1) {
+    __shared__ float sums[kThreads];
+    sums[tid] = sum;
+    __syncthreads();
+    if (share > 0) return;
+    for (int i = 1; i < shares; ++i) sum += sums[i * columns + tid];
+  }
+  if (k < p.width) Elem<DT>::store(static_cast<typename Elem<DT>::type*>(p.dw) + static_cast<int64_t>(key) * p.width + k, sum * p.scale);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------
@@ -402,8 +467,8 @@ int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct Sizes {
   int bits, passes, tiles;  // of a sorting pass, and how many
-  int slices, per_piece;
-  int64_t blocks, pieces, bytes, keys[2], order[2], counts, open;  // (offsets into the workspace)
+  int slices, per_piece, threads;
+  int64_t blocks, pieces, groups, bytes, keys[2], order[2], counts, open;  // (offsets into the workspace)
   Sizes(int dtype, int64_t n, int64_t vocab, int64_t width) {
     int all = 1;
     while ((vocab >> all) > 0) ++all;  // of keys up to `vocab`
@@ -414,14 +479,16 @@ struct Sizes {
     blocks = tiles > 0 ? (lines + tiles - 1) / tiles : 0;
     const int per = kThreads * (dtype == MEGA_F32 ? 4 : 8);
     slices = static_cast<int>((width + per - 1) / per);
-    per_piece = 16;
-    while (per_piece < kMostPiece && per_piece * 1024ll < n * slices) per_piece *= 2;
-    pieces = (n + per_piece - 1) / per_piece;
+    threads = slices > 1 ? kThreads : static_cast<int>((width + per / kThreads - 1) / (per / kThreads));
+    const int each = kThreads / threads;
+    per_piece = each <= kMostPiece / 16 ? 16 : kMostPiece / each;
+    while (2 * per_piece * each <= kMostPiece && per_piece * each * 1024ll < n * slices) per_piece *= 2;
+    pieces = (n + per_piece - 1) / per_piece, groups = (pieces + each - 1) / each;
     const bool sorts = n > kRankTokens;
     bytes = 0;
     const auto take = [&](int64_t size) { const int64_t at = bytes; bytes += up(size); return at; };
     for (int i = 0; i < 2; ++i) keys[i] = i == 0 || sorts ? take(4 * n) : 0, order[i] = i == 0 || sorts ? take(4 * n) : 0;
-    counts = sorts ? take(4 * (blocks << bits)) : 0;
+    counts = sorts ? take(4 * ((blocks + 1) << bits)) : 0;
     open = take(4 * pieces * 2 * width);
   }
 };
@@ -463,6 +530,10 @@ int sort_positions(const Token* tokens, int64_t n, int64_t vocab, int64_t paddin
     uint32_t *to_keys = at(z.keys[pass & 1]), *to_order = at(z.order[pass & 1]);
     count_kernel<Token><<<static_cast<unsigned>(z.blocks), kSortThreads, 0, s>>>(from, n, z.tiles, pass * z.bits, 1 << z.bits, at(z.counts));
     MEGA_CHECK_LAUNCH();
+    if (z.blocks > kSortAlone) {
+      scan_kernel<<<((1 << z.bits) + kWave - 1) / kWave, kScanWaves * kWave, 0, s>>>(at(z.counts), static_cast<int>(z.blocks), 1 << z.bits);
+      MEGA_CHECK_LAUNCH();
+    }
     move_kernel<Token><<<static_cast<unsigned>(z.blocks), kSortThreads, lds, s>>>(from, n, z.tiles, pass * z.bits, z.bits, at(z.counts), to_keys, to_order);
     MEGA_CHECK_LAUNCH();
     from = Positions<Token>{nullptr, to_keys, to_order, vocab, padding};
@@ -476,17 +547,19 @@ int table_grad(const void* dy, const void* tokens, int token_bits, int64_t n, in
   const Sizes z(DT, n, vocab, width);
   SumParams p{};
   p.dy = dy, p.dw = dw, p.open = reinterpret_cast<float*>(ws + z.open);
-  p.n = n, p.vocab = vocab, p.width = static_cast<int>(width), p.per_piece = z.per_piece, p.slices = z.slices, p.pieces = z.pieces, p.scale = scale, p.streaming = whole_lines(dw, width, DT);
+  p.n = n, p.vocab = vocab, p.width = static_cast<int>(width), p.per_piece = z.per_piece, p.slices = z.slices, p.threads = z.threads, p.pieces = z.pieces, p.groups = z.groups, p.scale = scale, p.streaming = whole_lines(dw, width, DT);
   if (n > 0) {
     const int rc = token_bits == 64 ? sort_positions(static_cast<const int64_t*>(tokens), n, vocab, padding, z, ws, &p.keys, &p.order, s)
                                     : sort_positions(static_cast<const int32_t*>(tokens), n, vocab, padding, z, ws, &p.keys, &p.order, s);
     if (rc != MEGA_OK) return rc;
   }
-  const int64_t groups = p.pieces * p.slices + std::min<int64_t>((vocab + kZeroRows - 1) / kZeroRows, 1 << 20);  // (2^32 threads are the most)
+  const int64_t groups = p.groups * p.slices + std::min<int64_t>((vocab + kZeroRows - 1) / kZeroRows, 1 << 20);  // (2^32 threads are the most)
   sum_kernel<DT><<<static_cast<unsigned>(groups), kThreads, 0, s>>>(p);
   MEGA_CHECK_LAUNCH();
   if (p.pieces > 1) {
-    join_kernel<DT><<<static_cast<unsigned>(p.pieces * ((width + kThreads - 1) / kThreads)), kThreads, 0, s>>>(p);
+    int columns = 16;
+    while (columns < kThreads && columns < width) columns *= 2;
+    join_kernel<DT><<<static_cast<unsigned>(p.pieces * ((width + columns - 1) / columns)), kThreads, 0, s>>>(p, columns);
     MEGA_CHECK_LAUNCH();
   }
   return MEGA_OK;

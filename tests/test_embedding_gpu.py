@@ -110,6 +110,16 @@ def test_runs_over_many_pieces(n, dtype):
     check((torch.arange(n, device="cuda") >= n - 3).long() * 8, weight)
 
 
+@pytest.mark.parametrize("D", [1, 9, 64, 500, 1100])
+@pytest.mark.parametrize("n", [3000, 100001])
+def test_narrow_rows(n, D):
+    """Several pieces to a workgroup; one token has most of the positions, one the last of each hundred, the others few."""
+    tokens = torch.full((n,), 5, device="cuda")
+    tokens[99::100] = 2
+    tokens[7::10000] = torch.arange(len(tokens[7::10000]), device="cuda") % 6
+    check(tokens, table(7, D, torch.bfloat16))
+
+
 @pytest.mark.parametrize("n", [700, 9001])
 def test_sums_run_in_order(n):
     """The sums are those of one order, whatever the other tokens are: small numbers behind a large one come out the same."""
