@@ -65,7 +65,10 @@ __device__ __forceinline__ u32x4 eight(const uint16_t* row, int k, int n) {
   }
   uint32_t e[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = k + i < n ? row[k + i] : 0u;
+  for (int i = 0; i < 8; ++i) {  // (all of them asked for together)
+    const uint32_t v = row[min(k + i, n - 1)];
+    e[i] = k + i < n ? v : 0u;
+  }
   return u32x4{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
 }
 
@@ -181,28 +184,29 @@ struct Copies {
   struct One {
     const uint16_t* src;
     uint16_t* dst;
-    int64_t pieces;  // of this one and of those in front
+    uint32_t pieces, blocks;  // (operands have fewer than 2^30 elements); workgroups of this one and of those in front
     int from, to;
   } one[3];
   int count;
   void add(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t from, int64_t to) {
-    const int64_t before = count > 0 ? one[count - 1].pieces : 0;
-    one[count++] = {src, dst, before + rows * (to / 8), static_cast<int>(from), static_cast<int>(to)};
+    const uint32_t before = count > 0 ? one[count - 1].blocks : 0, pieces = static_cast<uint32_t>(rows * (to / 8));
+    one[count++] = {src, dst, pieces, before + (pieces + kThreads - 1) / kThreads, static_cast<int>(from), static_cast<int>(to)};
   }
 };
 __global__ __launch_bounds__(kThreads) void copies_kernel(const Copies c) {
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < c.one[c.count - 1].pieces; i += static_cast<int64_t>(gridDim.x) * kThreads) {
+  for (uint32_t block = blockIdx.x; block < c.one[c.count - 1].blocks; block += gridDim.x) {
     int m = 0;
-    while (i >= c.one[m].pieces) ++m;
+    while (block >= c.one[m].blocks) ++m;
     const Copies::One& o = c.one[m];
-    const int64_t at = m > 0 ? i - c.one[m - 1].pieces : i, row = at / (o.to / 8);
-    *reinterpret_cast<u32x4*>(o.dst + 8 * at) = eight<false>(o.src + row * o.from, static_cast<int>(at - row * (o.to / 8)) * 8, o.from);
+    const uint32_t at = (m > 0 ? block - c.one[m - 1].blocks : block) * kThreads + threadIdx.x, per = static_cast<uint32_t>(o.to) / 8, row = at / per;
+    if (at < o.pieces)
+      *reinterpret_cast<u32x4*>(o.dst + 8 * static_cast<int64_t>(at)) = eight<false>(o.src + static_cast<int64_t>(row) * o.from, static_cast<int>(at - row * per) * 8, o.from);
   }
 }
-unsigned pieces_grid(int64_t pieces) { return static_cast<unsigned>(std::min<int64_t>((pieces + kThreads - 1) / kThreads, 16384)); }
+constexpr unsigned kMostBlocks = 16384;
 int copy_all(const Copies& c, hipStream_t s) {
   if (c.count == 0) return MEGA_OK;
-  copies_kernel<<<pieces_grid(c.one[c.count - 1].pieces), kThreads, 0, s>>>(c);
+  copies_kernel<<<std::min(c.one[c.count - 1].blocks, kMostBlocks), kThreads, 0, s>>>(c);
   MEGA_CHECK_LAUNCH();
   return MEGA_OK;
 }
@@ -221,10 +225,10 @@ __device__ __forceinline__ void kept_eight(const void* p, int64_t at, float* v) 
 template <int DT, bool WIDE>
 __global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh, const void* a, const void* b, uint16_t* g2,
                                                             int64_t tokens, int n, int pitch, int h) {
-  const int64_t pieces = tokens * (h / 8);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < pieces; i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t row = i / (h / 8);
-    const int k = static_cast<int>(i - row * (h / 8)) * 8;
+  const uint32_t per = static_cast<uint32_t>(h) / 8, pieces = static_cast<uint32_t>(tokens) * per;  // (fewer than 2^30 elements of da | db)
+  for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < pieces; i += gridDim.x * kThreads) {
+    const int64_t row = i / per;
+    const int k = static_cast<int>(i % per) * 8;
     float g[8], u[8], v[8], du[8], dv[8];
     if (k < pitch) {
       unpack8<DT>(__builtin_bit_cast(uint4, eight<false>(dh + row * n, k, n)), g);
@@ -392,7 +396,7 @@ extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void
       if (what > 1) c.add(rows, at(f.x), n, n_in, k), rows = at(f.x);
       if (const int rc = copy_all(c, s); rc != MEGA_OK) return rc;
     }
-    const unsigned grid = pieces_grid(n * (h / 8));
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n * (h / 8) + kThreads - 1) / kThreads, kMostBlocks));
     const bool wide = kept == MEGA_F32;
     const auto rows_of = [&](const void* q) { return static_cast<const char*>(q) + t * pitch * (wide ? 4 : 2); };
     const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(dh + at0, rows_of(a), rows_of(b), g, n, (int)n_out, (int)pitch, (int)h); };
