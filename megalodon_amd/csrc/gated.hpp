@@ -35,13 +35,14 @@ struct GatedTiles {
 // h = silu(x w1^T) o (x w3^T); a and b may be null; n_in a multiple of 64
 int gated_tiles(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
                 uint16_t* h, void* a, void* b, bool wide, float* parts, hipStream_t s);
-// g (tokens, 2 half), half n_out rounded up to 64: the gradients of a and, from column half on, of b, zeros behind n_out.  Rows of x, w1, w3 `ld`
-// elements apart, a multiple of 8.  dx (tokens, n_in), dw1 and dw3 (n_out, n_in), one of them or both, of any pitch; add: they are added to
+// g (tokens, terms, 2 half), half n_out rounded up to 64: the gradients of a and, from column half on, of b, zeros behind n_out, as sums of one or two
+// terms; for dw each row of x stands there `terms` times.  Rows of x, w1, w3 `ld` elements apart, a multiple of 8.
+// dx (tokens, n_in), dw1 and dw3 (n_out, n_in), one of them or both, of any pitch; add: they are added to
 int gated_tiles_input(int dtype, const uint16_t* g, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld,
-                      uint16_t* dx, float* parts, hipStream_t s);
+                      int terms, uint16_t* dx, float* parts, hipStream_t s);
 int gated_tiles_weight(int dtype, const uint16_t* g, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld, bool add,
-                       uint16_t* dw1, uint16_t* dw3, float* parts, hipStream_t s);
-int64_t gated_tiles_bytes(int kind, int64_t tokens, int64_t n_in, int64_t n_out, int matrices = 2);
+                       int terms, uint16_t* dw1, uint16_t* dw3, float* parts, hipStream_t s);
+int64_t gated_tiles_bytes(int kind, int64_t tokens, int64_t n_in, int64_t n_out, int matrices = 2, int terms = 1);
 
 // parts: gated_parts_bytes, or null; wide: a and b in float32
 int gated_product(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,

@@ -5,8 +5,8 @@
 // One kernel has both projections: a wave's accumulators hold a and b of the same elements, and the gate is taken from them
 // in float32, so that neither product goes through memory.  Training keeps both for the backward, in float32 or rounded to the
 // operands' type: half the memory, and a third rounding of the gradients besides those of da and db (operands of the matrix
-// cores) and of the results.  (Gradients in 16 bits off by 1.4 roundings where
-// float32 is kept, by 1.8 where not; training on 32768 tokens, 4096 -> 11008, takes 5 % longer with it.)
+// cores) and of the results.  (Gradients in 16 bits are off by 1.4 times what rounding them once takes where
+// float32 is kept, by 1.8 where not; training on 32768 tokens, 4096 -> 11008, takes 5 % longer with it, 4084 tokens, 2048 -> 5504, 8 %.)
 //
 // Many tokens: tiles with the gate for an epilogue (gated_product of attention.hip, gated_tiles.hip).  Few: the weights' stream from
 // memory is all the time there is, and the kernel below reads them once, straight into the operand registers of the matrix cores.
@@ -14,6 +14,7 @@
 #include "gated.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mega {
 
@@ -178,19 +179,19 @@ int few_tokens(const FewParams& p, hipStream_t s) {
 // ---- rows of whole 16-byte pieces -----------------------------------------------------------------------
 constexpr int kThreads = 256;
 
-// Matrices copied in one launch, 16 bytes a thread: dst (rows, to) = src (rows, from), zeros behind column `from`; `to` whole
+// Matrices copied in one launch, 16 bytes a thread: dst (rows, times, to) = src (rows, from), zeros behind column `from`; `to` whole
 // pieces, dst on 16-byte boundaries.
 struct Copies {
   struct One {
     const uint16_t* src;
     uint16_t* dst;
     uint32_t pieces, blocks;  // (operands have fewer than 2^30 elements); workgroups of this one and of those in front
-    int from, to;
+    int from, to, times;
   } one[3];
   int count;
-  void add(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t from, int64_t to) {
-    const uint32_t before = count > 0 ? one[count - 1].blocks : 0, pieces = static_cast<uint32_t>(rows * (to / 8));
-    one[count++] = {src, dst, pieces, before + (pieces + kThreads - 1) / kThreads, static_cast<int>(from), static_cast<int>(to)};
+  void add(const uint16_t* src, uint16_t* dst, int64_t rows, int64_t from, int64_t to, int times = 1) {
+    const uint32_t before = count > 0 ? one[count - 1].blocks : 0, pieces = static_cast<uint32_t>(rows * times * (to / 8));
+    one[count++] = {src, dst, pieces, before + (pieces + kThreads - 1) / kThreads, static_cast<int>(from), static_cast<int>(to), times};
   }
 };
 __global__ __launch_bounds__(kThreads) void copies_kernel(const Copies c) {
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void copies_kernel(const Copies c) {
     const Copies::One& o = c.one[m];
     const uint32_t at = (m > 0 ? block - c.one[m - 1].blocks : block) * kThreads + threadIdx.x, per = static_cast<uint32_t>(o.to) / 8, row = at / per;
     if (at < o.pieces)
-      *reinterpret_cast<u32x4*>(o.dst + 8 * static_cast<int64_t>(at)) = eight<false>(o.src + static_cast<int64_t>(row) * o.from, static_cast<int>(at - row * per) * 8, o.from);
+      *reinterpret_cast<u32x4*>(o.dst + 8 * static_cast<int64_t>(at)) = eight<false>(o.src + static_cast<int64_t>(row / o.times) * o.from, static_cast<int>(at - row * per) * 8, o.from);
   }
 }
 constexpr unsigned kMostBlocks = 16384;
@@ -221,8 +222,15 @@ __device__ __forceinline__ void kept_eight(const void* p, int64_t at, float* v) 
     v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
   }
 }
-// da | db (tokens, 2 h) from dh (tokens, n) and a, b (tokens, pitch): 8 elements a thread, zeros from column n on
-template <int DT, bool WIDE>
+// What rounding v to the type has left of it (none where that is no number)
+template <int DT>
+__device__ __forceinline__ void remainders(const float* v, uint4 rounded, float* r) {
+  unpack8<DT>(rounded, r);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = fabsf(r[e]) < __builtin_inff() ? v[e] - r[e] : 0.f;
+}
+// da | db (tokens, TERMS, 2 h) from dh (tokens, n) and a, b (tokens, pitch): 8 elements a thread, zeros from column n on
+template <int DT, bool WIDE, int TERMS>
 __global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh, const void* a, const void* b, uint16_t* g2,
                                                             int64_t tokens, int n, int pitch, int h) {
   const uint32_t per = static_cast<uint32_t>(h) / 8, pieces = static_cast<uint32_t>(tokens) * per;  // (fewer than 2^30 elements of da | db)
@@ -241,9 +249,16 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh,
       dv[e] = k + e < n ? g[e] * u[e] * s : 0.f;
       du[e] = k + e < n ? g[e] * v[e] * s * (1.f + u[e] * (1.f - s)) : 0.f;
     }
-    uint16_t* const to = g2 + row * 2 * h + k;
-    *reinterpret_cast<uint4*>(to) = pack8<DT>(du);
-    *reinterpret_cast<uint4*>(to + h) = pack8<DT>(dv);
+    uint16_t* const to = g2 + row * (TERMS * 2) * h + k;
+    const uint4 a16 = pack8<DT>(du), b16 = pack8<DT>(dv);
+    *reinterpret_cast<uint4*>(to) = a16;
+    *reinterpret_cast<uint4*>(to + h) = b16;
+    if constexpr (TERMS == 2) {
+      remainders<DT>(du, a16, g);
+      remainders<DT>(dv, b16, u);
+      *reinterpret_cast<uint4*>(to + 2 * h) = pack8<DT>(g);
+      *reinterpret_cast<uint4*>(to + 3 * h) = pack8<DT>(u);
+    }
   }
 }
 
@@ -282,22 +297,28 @@ struct Forward {
 // Backward: the gradients of a and b beside each other, (tokens, 2 h), for gated_tiles.hip.  (Small sizes too: networks of 1024 -> 2752
 // and up are faster so than by the products of attention.hip, whose tiles are small, by 10 to 50 % up to 1024 tokens; 512 -> 1408 up to 20 % slower from
 // 512 tokens on.)
+// Few tokens: two terms each, what rounding left beside the rounded, so that the results are as good as rounded once; the roundings of few values
+// average out less.  (us, one / two terms, dx and dw of 16 tokens: 1024 -> 2752 27 / 34, 2048 -> 5504 41 / 50, 4096 -> 11008 99 / 120, beside some 60 of
+// the host's.)
+constexpr int64_t kTwoTerms = 64;
 struct Backward {
+  int terms;
   int64_t h, k, rows;  // n_out and n_in with their padding, tokens of a launch
   int64_t g, w1, w3, x, parts, bytes;
   Backward(int64_t tokens, int64_t n_in, int64_t n_out, int what) {  // (what: 1 dx, 2 dw1, 4 dw3)
     Room room;
+    terms = tokens <= kTwoTerms ? 2 : 1;
     h = up(n_out, 64), k = up(n_in, 8);
     rows = std::min(tokens, std::max<int64_t>((kMost - 1) / std::max(2 * h, k) / 256 * 256, 256));
-    g = room.take(2 * rows * 2 * h);
+    g = room.take(2 * rows * terms * 2 * h);
     w1 = (what & 1) && k != n_in ? room.take(2 * n_out * k) : 0;
     w3 = (what & 1) && k != n_in ? room.take(2 * n_out * k) : 0;
-    x = what > 1 && k != n_in ? room.take(2 * rows * k) : 0;
+    x = what > 1 && (k != n_in || terms > 1) ? room.take(2 * terms * rows * k) : 0;
     // (the products run one after the other)
     int64_t most = 0;
     for (const int64_t n : {rows, std::max<int64_t>(tokens % rows, 1)}) {
-      if (what & 1) most = std::max(most, gated_tiles_bytes(1, n, n_in, n_out));
-      if (what > 1) most = std::max(most, gated_tiles_bytes(2, n, n_in, n_out, what >= 6 ? 2 : 1));
+      if (what & 1) most = std::max(most, gated_tiles_bytes(1, n, n_in, n_out, 2, terms));
+      if (what > 1) most = std::max(most, gated_tiles_bytes(2, n, n_in, n_out, what >= 6 ? 2 : 1, terms));
     }
     parts = room.take(most);
     bytes = room.bytes;
@@ -386,28 +407,33 @@ extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void
     uint16_t* const g = at(f.g);
     const int64_t pitch = gated_pitch(n_out), at0 = t * n_out;
     const uint16_t* rows = x + t * n_in;
-    if (k != n_in) {
+    if (k != n_in || f.terms > 1) {
       Copies c{};
-      if (dx != nullptr && t == 0) {
+      if (dx != nullptr && t == 0 && k != n_in) {
         c.add(w1, at(f.w1), n_out, n_in, k);
         c.add(w3, at(f.w3), n_out, n_in, k);
         w1 = at(f.w1), w3 = at(f.w3);
       }
-      if (what > 1) c.add(rows, at(f.x), n, n_in, k), rows = at(f.x);
+      if (what > 1) c.add(rows, at(f.x), n, n_in, k, f.terms), rows = at(f.x);
       if (const int rc = copy_all(c, s); rc != MEGA_OK) return rc;
     }
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n * (h / 8) + kThreads - 1) / kThreads, kMostBlocks));
     const bool wide = kept == MEGA_F32;
     const auto rows_of = [&](const void* q) { return static_cast<const char*>(q) + t * pitch * (wide ? 4 : 2); };
     const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(dh + at0, rows_of(a), rows_of(b), g, n, (int)n_out, (int)pitch, (int)h); };
-    if (dtype == MEGA_BF16) wide ? launch(gate_grad_kernel<MEGA_BF16, true>) : launch(gate_grad_kernel<MEGA_BF16, false>);
-    else wide ? launch(gate_grad_kernel<MEGA_F16, true>) : launch(gate_grad_kernel<MEGA_F16, false>);
+    const auto of_type = [&](auto dt, auto is_wide) {
+      if (f.terms == 2) launch(gate_grad_kernel<decltype(dt)::value, decltype(is_wide)::value, 2>);
+      else launch(gate_grad_kernel<decltype(dt)::value, decltype(is_wide)::value, 1>);
+    };
+    const auto of_width = [&](auto dt) { wide ? of_type(dt, std::true_type()) : of_type(dt, std::false_type()); };
+    if (dtype == MEGA_BF16) of_width(std::integral_constant<int, MEGA_BF16>());
+    else of_width(std::integral_constant<int, MEGA_F16>());
     MEGA_CHECK_LAUNCH();
     float* const parts = reinterpret_cast<float*>(ws + f.parts);
     if (dx != nullptr)
-      if (const int rc = gated_tiles_input(dtype, g, w1, w3, n, n_in, n_out, k, dx + t * n_in, parts, s); rc != MEGA_OK) return rc;
+      if (const int rc = gated_tiles_input(dtype, g, w1, w3, n, n_in, n_out, k, f.terms, dx + t * n_in, parts, s); rc != MEGA_OK) return rc;
     if (what > 1)
-      if (const int rc = gated_tiles_weight(dtype, g, rows, n, n_in, n_out, k, t > 0, dw1, dw3, parts, s); rc != MEGA_OK) return rc;
+      if (const int rc = gated_tiles_weight(dtype, g, rows, n, n_in, n_out, k, t > 0, f.terms, dw1, dw3, parts, s); rc != MEGA_OK) return rc;
   }
   return MEGA_OK;
 }

@@ -198,9 +198,10 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
   };
   const auto request_b = [&](int slab, uint32_t to, int i) {
     if constexpr (MODE == kInput) {
-      const bool second = slab >= p.seg;
+      const int of = slab >= 2 * p.seg ? slab - 2 * p.seg : slab;  // (the second terms' products meet the matrices again)
+      const bool second = of >= p.seg;
       const u32x4 buf = second ? buf_b2 : buf_b;
-      load_to_lds16(buf, off_b[i] + (second ? slab - p.seg : slab) * kK * pitch_b, lds_wave + to + i * 8192);
+      load_to_lds16(buf, off_b[i] + (second ? of - p.seg : of) * kK * pitch_b, lds_wave + to + i * 8192);
     } else {
       load_to_lds16(buf_b, off_b[i] + slab * (kRowsB ? kK * pitch_b : kK * 2), lds_wave + to + i * 8192);
     }
@@ -414,10 +415,10 @@ int launch(GatedTiles p, int most, hipStream_t s) {
 int64_t half_of(int64_t n_out) { return (n_out + kK - 1) / kK * kK; }
 // the last byte of `rows` rows of `n` elements
 uint32_t bytes_of(int64_t rows, int64_t pitch, int64_t n) { return static_cast<uint32_t>(2 * ((rows - 1) * pitch + n)); }
-GatedTiles sizes_of(int mode, int64_t tokens, int64_t n_in, int64_t n_out, int matrices) {
+GatedTiles sizes_of(int mode, int64_t tokens, int64_t n_in, int64_t n_out, int matrices, int terms) {
   GatedTiles p{};
   const int64_t half = half_of(n_out);
-  p.m = static_cast<int>(mode == kWeight ? matrices * half : tokens), p.k = static_cast<int>(mode == kGate ? n_in : mode == kInput ? 2 * half : tokens);
+  p.m = static_cast<int>(mode == kWeight ? matrices * half : tokens), p.k = static_cast<int>(mode == kGate ? n_in : mode == kInput ? terms * 2 * half : terms * tokens);
   p.row_tiles = (p.m + kTileRows - 1) / kTileRows, p.col_tiles = static_cast<int>(mode == kGate ? (n_out + 127) / 128 : (n_in + 255) / 256);
   p.n_out = static_cast<int>(n_out), p.half = static_cast<int>(half), p.cols = static_cast<int>(n_in), p.seg = static_cast<int>(half / kK);
   return p;
@@ -434,17 +435,17 @@ int launch_of(int dtype, GatedTiles p, float* parts, hipStream_t s) {
 
 }  // namespace
 
-int64_t gated_tiles_bytes(int kind, int64_t tokens, int64_t n_in, int64_t n_out, int matrices) {
+int64_t gated_tiles_bytes(int kind, int64_t tokens, int64_t n_in, int64_t n_out, int matrices, int terms) {
   int most = 0;
   if (workgroups(&most) != MEGA_OK) return 0;
-  GatedTiles p = sizes_of(kind, tokens, n_in, n_out, matrices);
+  GatedTiles p = sizes_of(kind, tokens, n_in, n_out, matrices, terms);
   cut_last(p, most);
   return static_cast<int64_t>(p.left) * p.cut * kPieceBytes;
 }
 
 int gated_tiles(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
                 uint16_t* h, void* a, void* b, bool wide, float* parts, hipStream_t s) {
-  GatedTiles p = sizes_of(kGate, tokens, n_in, n_out, 2);
+  GatedTiles p = sizes_of(kGate, tokens, n_in, n_out, 2, 1);
   p.a = x, p.b = w1, p.b2 = w3, p.a_bytes = bytes_of(tokens, n_in, n_in), p.b_bytes = bytes_of(n_out, n_in, n_in);
   p.n = static_cast<int>(n_out), p.lda = p.ldb = static_cast<int>(n_in);
   p.c = h, p.kept_a = a, p.kept_b = b, p.pitch = static_cast<int>(gated_pitch(n_out));
@@ -453,20 +454,20 @@ int gated_tiles(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t
 }
 
 int gated_tiles_input(int dtype, const uint16_t* g, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld,
-                      uint16_t* dx, float* parts, hipStream_t s) {
-  const int64_t both = 2 * half_of(n_out);
-  GatedTiles p = sizes_of(kInput, tokens, n_in, n_out, 2);
-  p.a = g, p.b = w1, p.b2 = w3, p.a_bytes = bytes_of(tokens, both, both), p.b_bytes = bytes_of(n_out, ld, ld);
-  p.n = static_cast<int>(ld), p.lda = static_cast<int>(both), p.ldb = static_cast<int>(ld), p.c = dx;
+                      int terms, uint16_t* dx, float* parts, hipStream_t s) {
+  const int64_t all = terms * 2 * half_of(n_out);
+  GatedTiles p = sizes_of(kInput, tokens, n_in, n_out, 2, terms);
+  p.a = g, p.b = w1, p.b2 = w3, p.a_bytes = bytes_of(tokens, all, all), p.b_bytes = bytes_of(n_out, ld, ld);
+  p.n = static_cast<int>(ld), p.lda = static_cast<int>(all), p.ldb = static_cast<int>(ld), p.c = dx;
   return launch_of<kInput, 0>(dtype, p, parts, s);
 }
 
 int gated_tiles_weight(int dtype, const uint16_t* g, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld, bool add,
-                       uint16_t* dw1, uint16_t* dw3, float* parts, hipStream_t s) {
+                       int terms, uint16_t* dw1, uint16_t* dw3, float* parts, hipStream_t s) {
   const int64_t both = 2 * half_of(n_out);
-  GatedTiles p = sizes_of(kWeight, tokens, n_in, n_out, dw1 != nullptr && dw3 != nullptr ? 2 : 1);
+  GatedTiles p = sizes_of(kWeight, tokens, n_in, n_out, dw1 != nullptr && dw3 != nullptr ? 2 : 1, terms);
   const int64_t from = dw1 != nullptr ? 0 : both / 2;
-  p.a = g + from, p.b = p.b2 = x, p.a_bytes = bytes_of(tokens, both, both - from), p.b_bytes = bytes_of(tokens, ld, ld);
+  p.a = g + from, p.b = p.b2 = x, p.a_bytes = bytes_of(terms * tokens, both, both - from), p.b_bytes = bytes_of(terms * tokens, ld, ld);
   p.n = static_cast<int>(ld), p.lda = static_cast<int>(both), p.ldb = static_cast<int>(ld), p.c = dw1 != nullptr ? dw1 : dw3, p.c2 = dw3, p.add = add;
   return launch_of<kWeight, 0>(dtype, p, parts, s);
 }
