@@ -213,13 +213,25 @@ int copy_all(const Copies& c, hipStream_t s) {
 }
 
 // ---- the gate's backward --------------------------------------------------------------------------------
-template <int DT, bool WIDE>
+// STREAM: what is read once and written past the memory-side cache
+template <bool STREAM, typename T>
+__device__ __forceinline__ T read(const void* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(static_cast<const T*>(p));
+  else return *static_cast<const T*>(p);
+}
+template <bool STREAM>
+__device__ __forceinline__ void write(uint16_t* p, uint4 v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4*>(p));
+  else *reinterpret_cast<uint4*>(p) = v;
+}
+template <int DT, bool WIDE, bool STREAM>
 __device__ __forceinline__ void kept_eight(const void* p, int64_t at, float* v) {
   if constexpr (!WIDE) {
-    unpack8<DT>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at), v);
+    unpack8<DT>(__builtin_bit_cast(uint4, read<STREAM, u32x4>(static_cast<const uint16_t*>(p) + at)), v);
   } else {
-    const float4 lo = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at), hi = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4);
-    v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+    const f32x4 lo = read<STREAM, f32x4>(static_cast<const float*>(p) + at), hi = read<STREAM, f32x4>(static_cast<const float*>(p) + at + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
   }
 }
 // What rounding v to the type has left of it (none where that is no number)
@@ -230,7 +242,7 @@ __device__ __forceinline__ void remainders(const float* v, uint4 rounded, float*
   for (int e = 0; e < 8; ++e) r[e] = fabsf(r[e]) < __builtin_inff() ? v[e] - r[e] : 0.f;
 }
 // da | db (tokens, TERMS, 2 h) from dh (tokens, n) and a, b (tokens, pitch): 8 elements a thread, zeros from column n on
-template <int DT, bool WIDE, int TERMS>
+template <int DT, bool WIDE, int TERMS, bool STREAM>
 __global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh, const void* a, const void* b, uint16_t* g2,
                                                             int64_t tokens, int n, int pitch, int h) {
   const uint32_t per = static_cast<uint32_t>(h) / 8, pieces = static_cast<uint32_t>(tokens) * per;  // (fewer than 2^30 elements of da | db)
@@ -240,8 +252,8 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh,
     float g[8], u[8], v[8], du[8], dv[8];
     if (k < pitch) {
       unpack8<DT>(__builtin_bit_cast(uint4, eight<false>(dh + row * n, k, n)), g);
-      kept_eight<DT, WIDE>(a, row * pitch + k, u);
-      kept_eight<DT, WIDE>(b, row * pitch + k, v);
+      kept_eight<DT, WIDE, STREAM>(a, row * pitch + k, u);
+      kept_eight<DT, WIDE, STREAM>(b, row * pitch + k, v);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -251,13 +263,13 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(const uint16_t* dh,
     }
     uint16_t* const to = g2 + row * (TERMS * 2) * h + k;
     const uint4 a16 = pack8<DT>(du), b16 = pack8<DT>(dv);
-    *reinterpret_cast<uint4*>(to) = a16;
-    *reinterpret_cast<uint4*>(to + h) = b16;
+    write<STREAM>(to, a16);
+    write<STREAM>(to + h, b16);
     if constexpr (TERMS == 2) {
       remainders<DT>(du, a16, g);
       remainders<DT>(dv, b16, u);
-      *reinterpret_cast<uint4*>(to + 2 * h) = pack8<DT>(g);
-      *reinterpret_cast<uint4*>(to + 3 * h) = pack8<DT>(u);
+      write<STREAM>(to + 2 * h, pack8<DT>(g));
+      write<STREAM>(to + 3 * h, pack8<DT>(u));
     }
   }
 }
@@ -301,6 +313,9 @@ struct Forward {
 // average out less.  (us, one / two terms, dx and dw of 16 tokens: 1024 -> 2752 27 / 34, 2048 -> 5504 41 / 50, 4096 -> 11008 99 / 120, beside some 60 of
 // the host's.)
 constexpr int64_t kTwoTerms = 64;
+// Beyond the memory-side cache nothing of the gate's pass is worth keeping (us with the gradient of narrow rows, kept / past it: 32768 x 11008 1355 / 1260, 8192 x 5504
+// 174 / 162, 4084 x 2752 51 / 54).
+constexpr int64_t kCacheBytes = 256 << 20;
 struct Backward {
   int terms;
   int64_t h, k, rows;  // n_out and n_in with their padding, tokens of a launch
@@ -422,8 +437,11 @@ extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void
     const auto rows_of = [&](const void* q) { return static_cast<const char*>(q) + t * pitch * (wide ? 4 : 2); };
     const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(dh + at0, rows_of(a), rows_of(b), g, n, (int)n_out, (int)pitch, (int)h); };
     const auto of_type = [&](auto dt, auto is_wide) {
-      if (f.terms == 2) launch(gate_grad_kernel<decltype(dt)::value, decltype(is_wide)::value, 2>);
-      else launch(gate_grad_kernel<decltype(dt)::value, decltype(is_wide)::value, 1>);
+      constexpr int DT = decltype(dt)::value;
+      constexpr bool WIDE = decltype(is_wide)::value;
+      if (f.terms == 2) launch(gate_grad_kernel<DT, WIDE, 2, false>);
+      else if (n * h * (WIDE ? 14 : 10) > kCacheBytes) launch(gate_grad_kernel<DT, WIDE, 1, true>);
+      else launch(gate_grad_kernel<DT, WIDE, 1, false>);
     };
     const auto of_width = [&](auto dt) { wide ? of_type(dt, std::true_type()) : of_type(dt, std::false_type()); };
     if (dtype == MEGA_BF16) of_width(std::integral_constant<int, MEGA_BF16>());

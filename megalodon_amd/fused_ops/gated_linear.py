@@ -14,5 +14,7 @@ def gated_linear(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, kept: Opti
 
     bfloat16 or float16, one dtype for all three, any sizes; the products and the gate in float32, one rounding.  With gradients
     the two products are kept in `kept`: float32 (the default), or x's dtype for half the memory and one rounding more on the
-    gradients' way.  The gradients of the products are rounded to x's dtype before theirs are formed (up to 64 tokens to two terms, which is as good as not).  The two matrices together hold fewer than 2 ** 30 elements (n_in and n_out rounded up to 64)."""
+    gradients' way.  The products' gradients are rounded to x's dtype before those of x and the weights are formed from them (up to 64
+    tokens: to two terms, so that the results are off by their own rounding alone).  The two matrices together hold fewer than
+    2 ** 30 elements (n_in and n_out rounded up to 64)."""
     return _lib.host().gated_linear(x, w1, w3, kept)
