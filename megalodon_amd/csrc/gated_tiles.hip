@@ -15,7 +15,7 @@
 // as two buffers for whole slabs want it, they hold up the waves (the matrix pipe 75 % busy, 86 % so).
 // The products are 16 x 16 x 32: the power limit sets the clock, and 32 x 32 x 16 move twice the accumulators for the same operations
 // (1.43 against 1.54 PFLOP/s).  32768 tokens, 4096 -> 11008, 5.9 TFLOP each: kGate 3.85 ms, as long as a general library takes for the two products
-// without the gate (4.57 with a and b kept in float32: the stores of all units' tiles come together, 12 us of 100), kInput 4.08, kWeight 4.2 (twice
+// without the gate (4.57 with a and b kept in float32: the stores of all units' tiles come together, 12 us of 100), kInput 3.8, kWeight 4.2 (twice
 // the reads of LDS, 8 bytes each, for an operand whose rows are k).
 #include "common.hpp"
 #include "gated.hpp"
