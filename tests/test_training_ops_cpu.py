@@ -36,11 +36,11 @@ def refused(name, *args):
 def test_gated_linear_sizes(dtype, tokens, n_in, n_out, word):
     sizes = (ctypes.c_int(dtype), I64(tokens), I64(n_in), I64(n_out))
     assert word in refused("mega_gated_linear_fwd", SOME, SOME, SOME, *sizes, SOME, NULL, NULL, ctypes.c_int(dtype), SOME, NULL)
-    assert word in refused("mega_gated_linear_bwd", SOME, SOME, SOME, SOME, SOME, SOME, ctypes.c_int(dtype), *sizes, SOME, SOME, SOME, NULL)
+    assert word in refused("mega_gated_linear_bwd", SOME, SOME, SOME, SOME, SOME, SOME, ctypes.c_int(dtype), *sizes, SOME, SOME, SOME, SOME, NULL)
     fn = _lib.load().mega_gated_linear_workspace_bytes
     fn.restype = I64
     if word == b"sizes":
-        assert fn(*sizes[1:], 0) == 0 and fn(*sizes[1:], 3) == 0
+        assert fn(*sizes[1:], 0) == 0 and fn(*sizes[1:], 7) == 0
 
 
 def test_gated_linear_pointers():
@@ -50,9 +50,10 @@ def test_gated_linear_pointers():
     assert b"null" in refused("mega_gated_linear_fwd", SOME, SOME, SOME, *sizes, SOME, SOME, NULL, ctypes.c_int(1), NULL, NULL)   # one product kept
     assert b"misaligned" in refused("mega_gated_linear_fwd", odd, SOME, SOME, *sizes, SOME, NULL, NULL, ctypes.c_int(1), NULL, NULL)
     assert b"kept" in refused("mega_gated_linear_fwd", SOME, SOME, SOME, *sizes, SOME, SOME, SOME, ctypes.c_int(2), NULL, NULL)
-    assert b"null" in refused("mega_gated_linear_bwd", SOME, SOME, SOME, SOME, SOME, SOME, ctypes.c_int(0), *sizes, SOME, SOME, NULL, NULL)
-    assert b"kept" in refused("mega_gated_linear_bwd", SOME, SOME, SOME, SOME, SOME, SOME, ctypes.c_int(2), *sizes, SOME, SOME, SOME, NULL)
-    assert b"misaligned" in refused("mega_gated_linear_bwd", SOME, SOME, SOME, SOME, SOME, SOME, ctypes.c_int(0), *sizes, odd, SOME, SOME, NULL)
+    assert b"null" in refused("mega_gated_linear_bwd", SOME, SOME, SOME, SOME, SOME, SOME, ctypes.c_int(0), *sizes, SOME, SOME, SOME, NULL, NULL)
+    assert b"kept" in refused("mega_gated_linear_bwd", SOME, SOME, SOME, SOME, SOME, SOME, ctypes.c_int(2), *sizes, SOME, SOME, SOME, SOME, NULL)
+    assert b"misaligned" in refused("mega_gated_linear_bwd", SOME, SOME, SOME, SOME, odd, SOME, ctypes.c_int(0), *sizes, SOME, SOME, SOME, SOME, NULL)
+    assert b"misaligned" in refused("mega_gated_linear_bwd", SOME, SOME, SOME, SOME, SOME, SOME, ctypes.c_int(0), *sizes, SOME, SOME, SOME, odd, NULL)
 
 
 @pytest.mark.parametrize("dtype,bits,n,vocab,width,word", [
