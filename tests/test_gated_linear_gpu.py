@@ -254,9 +254,10 @@ def test_differentiated_twice():
         assert (g.double().cpu() - w).norm() <= 0.05 * w.norm()
 
 
-def test_captured():
+@pytest.mark.parametrize("sizes", [(96, 256, 160), (7, 250, 90), (4500, 500, 1410)])
+def test_captured(sizes):
     """Forward and backward in a graph whose replays follow new operands, the program's own work between them."""
-    x, w1, w3, dh = operands(96, 256, 160, torch.bfloat16)
+    x, w1, w3, dh = operands(*sizes, torch.bfloat16)
     leaves = [t.clone().requires_grad_(True) for t in (x, w1, w3)]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -273,7 +274,7 @@ def test_captured():
     with torch.cuda.graph(graph, stream=side):
         outs = step()
     for seed in range(3):
-        new = operands(96, 256, 160, torch.bfloat16, seed)
+        new = operands(*sizes, torch.bfloat16, seed)
         with torch.no_grad():
             for t, v in zip((*leaves, dh), new):
                 t.copy_(v)
@@ -281,6 +282,26 @@ def test_captured():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_two_streams():
+    """Calls on two streams at once have workspaces of their own."""
+    many = [operands(2500, 500, 1410, torch.bfloat16, seed) for seed in range(4)]
+
+    def one(x, w1, w3, dh):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w1, w3)]
+        h = fused_ops.gated_linear(*leaves)
+        return (h.detach(), *torch.autograd.grad(h, leaves, dh))
+
+    want = [one(*m) for m in many]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [None] * 4
+    for i, m in enumerate(many):
+        with torch.cuda.stream(streams[i % 2]):
+            got[i] = one(*m)
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
 
 
 def test_against_differences():
