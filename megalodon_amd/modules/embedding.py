@@ -15,6 +15,12 @@ class Embedding(nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
         self.scale = scale
 
+    @classmethod
+    def from_pretrained(cls, embeddings: torch.Tensor, freeze: bool = True, padding_idx: Optional[int] = None, scale: float = 1.0):
+        layer = cls(*embeddings.shape, padding_idx=padding_idx, scale=scale, device="meta")
+        layer.weight = nn.Parameter(embeddings, requires_grad=not freeze)
+        return layer
+
     def forward(self, tokens: torch.Tensor) -> torch.Tensor:
         return embedding(tokens, self.weight, self.scale, self.padding_idx)
 

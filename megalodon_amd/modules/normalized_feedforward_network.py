@@ -14,6 +14,8 @@ from .layer_norm import FusedLayerNorm
 
 
 class NormalizedFeedForwardNetwork(nn.Module):
+    fused_gate = False  # (modules that were pickled without it)
+
     def __init__(self, model_dim, ffn_hidden_dim, dropout=0.0, hidden_dropout=0.0, swiglu=False,
                  norm_affine=True, norm_eps=1e-5, rescale=None, init_std=0.02, fused_gate=False):
         super().__init__()
@@ -41,9 +43,10 @@ class NormalizedFeedForwardNetwork(nn.Module):
         return x if self.alpha is None else (self.alpha * x)
 
     def takes_fused_gate(self, x: torch.Tensor) -> bool:
-        """Rows and weights of one 16-bit type on the GPU, and layers whose call is nothing but `Linear.forward`."""
+        """Rows and weights of one 16-bit type on the GPU, of sizes that the operator takes, and layers whose call is nothing but `Linear.forward`."""
         layers = (self.fc1, self.fc3)
-        return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and not torch.is_autocast_enabled("cuda")
+        n_out, n_in = (-(-n // 64) * 64 for n in self.fc1.weight.shape)
+        return (2 * n_in * n_out < 1 << 30 and max(n_in, n_out) <= 1 << 20 and x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and not torch.is_autocast_enabled("cuda")
                 and all(l.weight.dtype == x.dtype and l.bias is None and is_bare(l) for l in layers))
 
     def forward(self, x, residual):

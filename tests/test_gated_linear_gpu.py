@@ -118,10 +118,11 @@ def test_tiles(tokens, n_in, n_out, dtype):
     check(*operands(tokens, n_in, n_out, dtype))
 
 
-def test_tokens_of_several_launches():
+@pytest.mark.parametrize("n_in", [1024, 1001])
+def test_tokens_of_several_launches(n_in):
     """An operand of 2^30 elements and more: launch by launch, the weights' gradients added to."""
-    one = ((1 << 30) - 1) // 1024 // 256 * 256  # tokens of a launch
-    tokens, n_in, n_out = one + 300, 1024, 8
+    one = ((1 << 30) - 1) // (-(-n_in // 8) * 8) // 256 * 256  # tokens of a launch
+    tokens, n_out = one + 300, 8
     x, w1, w3, dh = operands(tokens, n_in, n_out, torch.bfloat16)
     want = formula(x, w1, w3, dh, x.dtype)
     leaves = [t.clone().requires_grad_(True) for t in (x, w1, w3)]

@@ -1,5 +1,6 @@
 """What the embedding, the gated product and the gradients' norm refuse before any launch (no GPU needed)."""
 import ctypes
+import types
 
 import pytest
 import torch
@@ -124,3 +125,26 @@ def test_network_on_the_host_goes_where_it_did():
     ffn = NormalizedFeedForwardNetwork(16, 32, swiglu=True, fused_gate=True)
     assert not ffn.takes_fused_gate(torch.zeros(2, 16))
     assert set(ffn.state_dict()) == set(NormalizedFeedForwardNetwork(16, 32, swiglu=True).state_dict())
+
+
+def test_embedding_from_a_table():
+    table = torch.randn(5, 3)
+    layer = Embedding.from_pretrained(table, padding_idx=-1, scale=2.0)
+    assert layer.weight.data_ptr() == table.data_ptr() and not layer.weight.requires_grad
+    assert (layer.num_embeddings, layer.embedding_dim, layer.padding_idx, layer.scale) == (5, 3, 4, 2.0)
+    assert Embedding.from_pretrained(table, freeze=False).weight.requires_grad
+    assert list(layer.state_dict()) == ["weight"]
+
+
+def test_which_networks_take_the_fused_gate():
+    """Not those whose sizes the operator refuses, and none that was pickled without the choice."""
+    net = NormalizedFeedForwardNetwork(8, 16, swiglu=True, fused_gate=True)
+    assert not net.takes_fused_gate(torch.zeros(1, 8))
+    x = types.SimpleNamespace(is_cuda=True, dtype=torch.bfloat16)
+    weight = lambda *shape: types.SimpleNamespace(shape=shape, dtype=torch.bfloat16)
+    for (n_out, n_in), takes in (((16, 8), True), ((1 << 13, (1 << 16) - 64), True), ((1 << 13, 1 << 16), False), (((1 << 20) + 1, 8), False)):
+        for layer in (net.fc1, net.fc3):
+            layer._parameters["weight"] = weight(n_out, n_in)
+        assert net.takes_fused_gate(x) == takes
+    del net.__dict__["fused_gate"]
+    assert net.fused_gate is False
