@@ -36,7 +36,7 @@ struct GatedTiles {
 int gated_tiles(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
                 uint16_t* h, void* a, void* b, bool wide, float* parts, hipStream_t s);
 // g (tokens, terms, 2 half), half n_out rounded up to 64: the gradients of a and, from column half on, of b, zeros behind n_out, as sums of one or two
-// terms; for dw each row of x stands there `terms` times.  Rows of x, w1, w3 `ld` elements apart, a multiple of 8.
+// terms (two: up to 64 tokens); for dw each row of x stands there `terms` times.  Rows of x, w1, w3 `ld` elements apart, a multiple of 8.
 // dx (tokens, n_in), dw1 and dw3 (n_out, n_in), one of them or both, of any pitch; add: they are added to
 int gated_tiles_input(int dtype, const uint16_t* g, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld,
                       int terms, uint16_t* dx, float* parts, hipStream_t s);

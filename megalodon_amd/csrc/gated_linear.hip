@@ -310,8 +310,8 @@ struct Forward {
 // and up are faster so than by the products of attention.hip, whose tiles are small, by 10 to 50 % up to 1024 tokens; 512 -> 1408 up to 20 % slower from
 // 512 tokens on.)
 // Few tokens: two terms each, what rounding left beside the rounded, so that the results are as good as rounded once; the roundings of few values
-// average out less.  (us, one / two terms, dx and dw of 16 tokens: 1024 -> 2752 27 / 34, 2048 -> 5504 41 / 50, 4096 -> 11008 99 / 120, beside some 60 of
-// the host's.)
+// average out less.  The second term's rows are beside the first's in dx's tile, which is not full anyway.  (us, one / two terms, dx and dw of 16 tokens:
+// 1024 -> 2752 27 / 29, 2048 -> 5504 41 / 43, 4096 -> 11008 99 / 101.)
 constexpr int64_t kTwoTerms = 64;
 // Beyond the memory-side cache nothing of the gate's pass is worth keeping (us with the gradient of narrow rows, kept / past it: 32768 x 11008 1355 / 1260, 8192 x 5504
 // 174 / 162, 4084 x 2752 51 / 54).

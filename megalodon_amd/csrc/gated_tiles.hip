@@ -42,7 +42,7 @@ __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-enum { kGate, kInput, kWeight };
+enum { kGate, kInput, kWeight, kInputTwo };  // (kInputTwo: kInput of two terms)
 constexpr int kThreads = 512, kTileRows = 256, kK = 64, kBand = 8;
 constexpr uint32_t kOperandBytes = 256 * kK * 2, kRing = 5 * kOperandBytes;
 constexpr size_t kLds = kRing;
@@ -185,6 +185,8 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
     for (int i = 0; i < 4; ++i) {
       if constexpr (kRowsA) off_a[i] = (krow + 16 * i) * pitch_a + min(m0 + ((lane & 31) ^ kswizzle) * 8, p.m - 8) * 2;
       else off_a[i] = static_cast<uint32_t>(m0 + row8 + 64 * i) * pitch_a + chunk8 * 16;
+      // (two terms of up to 64 tokens: 64 rows of the first, 64 of the second, which lies behind it in their row of memory, and none)
+      if constexpr (MODE == kInputTwo) off_a[i] = i < 2 ? row8 * pitch_a + i * (pitch_a / 2) + chunk8 * 16 : p.a_bytes;
       if constexpr (kRowsB) off_b[i] = (krow + 16 * i) * pitch_b + min(n0 + ((lane & 31) ^ kswizzle) * 8, p.n - 8) * 2;
       else off_b[i] = static_cast<uint32_t>(n0 + (row8 & 31) + 32 * i) * pitch_b + chunk8 * 16;
     }
@@ -197,11 +199,10 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
     load_to_lds16(buf_a, off_a[i] + slab * (kRowsA ? kK * pitch_a : kK * 2), lds_wave + to + i * 8192);
   };
   const auto request_b = [&](int slab, uint32_t to, int i) {
-    if constexpr (MODE == kInput) {
-      const int of = slab >= 2 * p.seg ? slab - 2 * p.seg : slab;  // (the second terms' products meet the matrices again)
-      const bool second = of >= p.seg;
+    if constexpr (MODE == kInput || MODE == kInputTwo) {
+      const bool second = slab >= p.seg;
       const u32x4 buf = second ? buf_b2 : buf_b;
-      load_to_lds16(buf, off_b[i] + (second ? of - p.seg : of) * kK * pitch_b, lds_wave + to + i * 8192);
+      load_to_lds16(buf, off_b[i] + (second ? slab - p.seg : slab) * kK * pitch_b, lds_wave + to + i * 8192);
     } else {
       load_to_lds16(buf_b, off_b[i] + slab * (kRowsB ? kK * pitch_b : kK * 2), lds_wave + to + i * 8192);
     }
@@ -339,6 +340,12 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
       ++ahead;
       in_a = next_a;
     }
+    if constexpr (MODE == kInputTwo) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] += acc[i + 4][j];
+    }
     if (at.piece >= 0) {
       f32x4* const to = reinterpret_cast<f32x4*>(p.parts) + (static_cast<int64_t>(at.piece) * 8 + wave) * (8 * 4 * kWave) + lane;
 #pragma unroll
@@ -418,7 +425,7 @@ uint32_t bytes_of(int64_t rows, int64_t pitch, int64_t n) { return static_cast<u
 GatedTiles sizes_of(int mode, int64_t tokens, int64_t n_in, int64_t n_out, int matrices, int terms) {
   GatedTiles p{};
   const int64_t half = half_of(n_out);
-  p.m = static_cast<int>(mode == kWeight ? matrices * half : tokens), p.k = static_cast<int>(mode == kGate ? n_in : mode == kInput ? terms * 2 * half : terms * tokens);
+  p.m = static_cast<int>(mode == kWeight ? matrices * half : tokens), p.k = static_cast<int>(mode == kGate ? n_in : mode == kInput ? 2 * half : terms * tokens);
   p.row_tiles = (p.m + kTileRows - 1) / kTileRows, p.col_tiles = static_cast<int>(mode == kGate ? (n_out + 127) / 128 : (n_in + 255) / 256);
   p.n_out = static_cast<int>(n_out), p.half = static_cast<int>(half), p.cols = static_cast<int>(n_in), p.seg = static_cast<int>(half / kK);
   return p;
@@ -459,7 +466,7 @@ int gated_tiles_input(int dtype, const uint16_t* g, const uint16_t* w1, const ui
   GatedTiles p = sizes_of(kInput, tokens, n_in, n_out, 2, terms);
   p.a = g, p.b = w1, p.b2 = w3, p.a_bytes = bytes_of(tokens, all, all), p.b_bytes = bytes_of(n_out, ld, ld);
   p.n = static_cast<int>(ld), p.lda = static_cast<int>(all), p.ldb = static_cast<int>(ld), p.c = dx;
-  return launch_of<kInput, 0>(dtype, p, parts, s);
+  return terms == 2 ? launch_of<kInputTwo, 0>(dtype, p, parts, s) : launch_of<kInput, 0>(dtype, p, parts, s);
 }
 
 int gated_tiles_weight(int dtype, const uint16_t* g, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld, bool add,
