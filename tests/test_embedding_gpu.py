@@ -163,6 +163,19 @@ def test_every_row_is_written():
         assert dw[[0, 500, 999]].eq(1).all() and dw.sum() == 72
 
 
+@pytest.mark.parametrize("V,D,dtype", [(40001, 1001, torch.float32), (70003, 1003, torch.bfloat16), (33, 3, torch.bfloat16)])
+def test_rows_without_tokens(V, D, dtype):
+    """Lines of rows of any width and boundary, in tables that a cache holds and in larger ones."""
+    tokens = torch.tensor([0, V - 1, 17, 18, 5, 5, V // 2], device="cuda")
+    leaf = table(V, D, dtype).requires_grad_(True)
+    junk = torch.full((V * D + 16,), 7.0, dtype=dtype, device="cuda")  # (what the gradient's memory held)
+    del junk
+    dy = torch.ones(len(tokens), D, dtype=dtype, device="cuda")
+    dw, = torch.autograd.grad(fused_ops.embedding(tokens, leaf), leaf, dy)
+    want = torch.bincount(tokens, minlength=V).to(dtype)
+    assert torch.equal(dw, want[:, None].expand(V, D))
+
+
 def test_no_tokens():
     weight = table(10, 16, torch.float16).requires_grad_(True)
     for shape in ((0,), (3, 0)):
