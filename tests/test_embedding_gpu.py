@@ -110,7 +110,7 @@ def test_runs_over_many_pieces(n, dtype):
     check((torch.arange(n, device="cuda") >= n - 3).long() * 8, weight)
 
 
-@pytest.mark.parametrize("D", [1, 9, 64, 500, 1100])
+@pytest.mark.parametrize("D", [1, 9, 64, 500, 1100, 1030])
 @pytest.mark.parametrize("n", [3000, 100001])
 def test_narrow_rows(n, D):
     """Several pieces to a workgroup; one token has most of the positions, one the last of each hundred, the others few."""
