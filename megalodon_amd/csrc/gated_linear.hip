@@ -149,6 +149,87 @@ __global__ __launch_bounds__(kFewWaves * kWave) void gated_few_kernel(const FewP
   }
 }
 
+// 9 to 16 tokens with their rows in LDS: a workgroup for each CU walks the groups of 8 features, and the next group's weights are on their way into registers
+// while the current one's products run and the waves' sums meet.  Read again for every group, as above, so many tokens are half as many bytes as the weights
+// and more; fewer cost less than the part-filled last walk here.  (us, above / here, 8, 12, 16 tokens: 4096 -> 11008 47 / 47, 50 / 47.5, 52.8 / 48.6, 2048 -> 5504 12.4 / 13.5,
+// 13.8 / 13.9, 15.8 / 14.3, 1536 -> 40000 63 / 60, 67 / 62, 70 / 62; 1024 -> 2752 the same.)  STEPS: of 32 k for each wave, at most.
+// A row's chunk c of 16 bytes is at c ^ row: sixteen lanes on different banks.
+constexpr int kRestWaves = 16;
+__host__ __device__ constexpr int resident_pitch(int n_in) { return (n_in + 127) / 128 * 128; }
+template <int DT, int STEPS>
+__global__ __launch_bounds__(kRestWaves * kWave) void gated_resident_kernel(const FewParams p, int groups) {
+  extern __shared__ __align__(16) char smem[];
+  constexpr int kThreadsHere = kRestWaves * kWave;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave), r = lane % 16, g = lane / 16;
+  f32x4* const sums = reinterpret_cast<f32x4*>(smem);  // [2][wave][lane]
+  uint16_t* const rows = reinterpret_cast<uint16_t*>(smem + 2 * kRestWaves * kWave * sizeof(f32x4));
+  const int pitch = resident_pitch(p.n_in), steps = (p.n_in + 31) / 32;
+  const auto weights = [&](int group, u32x4* w) {
+    const uint16_t* const row = (r < 8 ? p.w1 : p.w3) + static_cast<int64_t>(min(8 * group + r % 8, p.n_out - 1)) * p.n_in;
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) {
+      const int k = 32 * (wave + j * kRestWaves) + 8 * g;
+      w[j] = k < p.n_in ? *reinterpret_cast<const u32x4*>(row + k) : u32x4{0, 0, 0, 0};
+    }
+  };
+  u32x4 w[STEPS], next[STEPS];
+  int group = blockIdx.x;
+  weights(group, w);
+  const int per = p.n_in / 8;
+  for (int i = tid; i < p.tokens * per; i += kThreadsHere) {
+    const int t = i / per, c = i - t * per;
+    *reinterpret_cast<u32x4*>(rows + t * pitch + 8 * (c ^ t)) = *reinterpret_cast<const u32x4*>(p.x + static_cast<int64_t>(t) * p.n_in + 8 * c);
+  }
+  __syncthreads();
+  const int token = min(r, p.tokens - 1);
+  const uint16_t* const x = rows + token * pitch;
+  for (int turn = 0; group < groups; turn ^= 1) {
+    const int ahead = group + static_cast<int>(gridDim.x);
+    if (ahead < groups) weights(ahead, next);
+    f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) {
+      const int s = wave + j * kRestWaves;
+      if (s >= steps) break;
+      const int k = 32 * s;
+      const u32x4 v = k + 8 * g < p.n_in ? *reinterpret_cast<const u32x4*>(x + 8 * ((4 * s + g) ^ token)) : u32x4{0, 0, 0, 0};
+      acc = mma16<DT>(w[j], v, acc);
+    }
+    f32x4* const mine = sums + turn * kRestWaves * kWave;
+    mine[wave * kWave + lane] = acc;
+    __syncthreads();
+    // values 0 .. 3 of lanes 0 .. 31 are a, of lanes 32 on b
+    if (tid < 128) {
+      const float* const from = reinterpret_cast<const float*>(mine) + tid;
+      float a = 0.f, b = 0.f;
+#pragma unroll
+      for (int q = 0; q < kRestWaves; ++q) a += from[q * 4 * kWave], b += from[q * 4 * kWave + 128];
+      const int t = tid / 4 % 16, f = 8 * group + 4 * (tid / 64) + tid % 4;
+      if (t < p.tokens && f < p.n_out) {
+        Elem<DT>::store(p.h + static_cast<int64_t>(t) * p.n_out + f, a * fast_sigmoid(a) * b);
+        if (p.a != nullptr) {
+          const int64_t kept = static_cast<int64_t>(t) * p.pitch + f;
+          if (p.wide) static_cast<float*>(p.a)[kept] = a, static_cast<float*>(p.b)[kept] = b;
+          else Elem<DT>::store(static_cast<uint16_t*>(p.a) + kept, a), Elem<DT>::store(static_cast<uint16_t*>(p.b) + kept, b);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) w[j] = next[j];
+    group = ahead;
+  }
+}
+constexpr size_t resident_lds(int tokens, int n_in) { return 2 * kRestWaves * kWave * sizeof(f32x4) + static_cast<size_t>(tokens) * resident_pitch(n_in) * 2; }
+template <int DT, int STEPS>
+int launch_resident(const FewParams& p, int cus, hipStream_t s) {
+  const size_t lds = resident_lds(p.tokens, p.n_in);
+  const int groups = (p.n_out + 7) / 8;
+  MEGA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&gated_resident_kernel<DT, STEPS>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+  gated_resident_kernel<DT, STEPS><<<std::min(groups, cus), kRestWaves * kWave, lds, s>>>(p, groups);
+  MEGA_CHECK_LAUNCH();
+  return MEGA_OK;
+}
+
 template <int DT, int NT, int FT>
 int launch_few(const FewParams& p, hipStream_t s) {
   const dim3 grid((p.n_out + 8 * FT - 1) / (8 * FT)), block(kFewWaves * kWave);
@@ -171,6 +252,8 @@ int few_tokens(const FewParams& p, hipStream_t s) {
   int dev = 0, cus = 0;
   MEGA_CHECK_HIP(hipGetDevice(&dev));
   MEGA_CHECK_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+  static_assert(resident_lds(16, 4096) <= 160 * 1024, "fits the LDS");
+  if (p.tokens > 8 && p.tokens <= 16 && p.n_in % 8 == 0 && p.n_in > 1024 && p.n_in <= 4096) return p.n_in <= 2048 ? launch_resident<DT, 4>(p, cus, s) : launch_resident<DT, 8>(p, cus, s);
   if (p.tokens <= 16) return few_of<DT, 1, 1>(p, cus, s);
   if (p.tokens <= 32) return few_of<DT, 2, 2>(p, cus, s);
   return few_of<DT, 4, 2>(p, cus, s);

@@ -92,6 +92,13 @@ def test_few_tokens(tokens, n_in, n_out, dtype):
     check(*operands(tokens, n_in, n_out, dtype))
 
 
+@pytest.mark.parametrize("tokens", [8, 9, 13, 16])
+@pytest.mark.parametrize("n_in,n_out,dtype", [(2048, 5504, torch.float16), (4096, 333, torch.bfloat16), (1544, 4100, torch.float16), (1032, 8, torch.bfloat16), (3000, 17, torch.bfloat16)])
+def test_tokens_in_lds(tokens, n_in, n_out, dtype):
+    """Rows of whole and part-filled steps, last groups of features that are not whole, workgroups without a second group."""
+    check(*operands(tokens, n_in, n_out, dtype))
+
+
 @pytest.mark.parametrize("tokens,n_in,n_out,dtype", [
     (65, 64, 8, torch.bfloat16),           # part of a tile
     (65, 1, 1, torch.float16),             # rows and columns laid out anew
@@ -210,7 +217,7 @@ def test_no_tokens():
     assert dx.shape == x.shape and not dw.any()
 
 
-@pytest.mark.parametrize("tokens,n_in", [(4, 64), (130, 64), (130, 60)])
+@pytest.mark.parametrize("tokens,n_in", [(4, 64), (130, 64), (130, 60), (11, 1288)])
 def test_rows_do_not_touch_each_other(tokens, n_in):
     """An infinity or a NaN in one token's row, or in a feature's weights, stays there."""
     x, w1, w3, _ = operands(tokens, n_in, 40, torch.bfloat16)
