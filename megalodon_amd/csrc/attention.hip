@@ -2153,6 +2153,7 @@ int launch_gated(GemmParams q, int cus, hipStream_t s) {
 
 int64_t gated_parts_bytes(int64_t tokens, int64_t n_in, int64_t n_out) {
   int cus = 0;
+  if (n_in % 64 != 0) return gated_tiles_bytes(0, tokens, n_in, n_out);
   if (compute_units(&cus) != MEGA_OK) return 0;
   const int64_t both = 2 * n_out;
   GemmParams q = linear_sizes(kForward, tokens, n_in, 1, &both);
@@ -2162,6 +2163,9 @@ int64_t gated_parts_bytes(int64_t tokens, int64_t n_in, int64_t n_out) {
 
 int gated_product(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
                   uint16_t* h, void* a, void* b, bool wide, float* parts, hipStream_t s) {
+  // The small tiles want slabs of 64 k: rows of other lengths would be laid out anew for them.  (us, so / large tiles, 65, 256, 512, 1024 tokens: 4088 -> 11008 127 / 74, 153 / 87,
+  // 162 / 112, 220 / 181, 2056 -> 5504 36 / 30, 42 / 37, 49 / 58, 64 / 58, 1000 -> 2736 22 / 19, 23 / 25, 23 / 31, 29 / 30)
+  if (n_in % 64 != 0) return gated_tiles(dtype, x, w1, w3, tokens, n_in, n_out, h, a, b, wide, parts, s);
   GemmParams g{};
   g.A = x; g.B = w1; g.B2 = w3; g.C = h; g.Ca = a; g.Cb = b; g.wide = wide;
   g.M = (int)tokens; g.N = (int)(2 * n_out); g.K = (int)n_in; g.gate_n = (int)n_out;

@@ -32,7 +32,7 @@ struct GatedTiles {
   float* parts;
 };
 // Operands of fewer than 2^30 elements on 16-byte boundaries; parts: gated_tiles_bytes (kind: 0, 1, 2 as they stand here), or null for none.
-// h = silu(x w1^T) o (x w3^T); a and b may be null; n_in a multiple of 64
+// h = silu(x w1^T) o (x w3^T); a and b may be null; n_in a multiple of 8
 int gated_tiles(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
                 uint16_t* h, void* a, void* b, bool wide, float* parts, hipStream_t s);
 // g (tokens, terms, 2 half), half n_out rounded up to 64: the gradients of a and, from column half on, of b, zeros behind n_out, as sums of one or two

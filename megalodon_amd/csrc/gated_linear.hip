@@ -44,7 +44,7 @@ constexpr int kFewWaves = 8;
 
 // Which calls go here: up to 16 tokens all; then the tokens, read again for every few features, cost more than the tiles' second launch
 // the more the larger the weights are (us, here / tiles: 4096 -> 11008 16 tokens 47 / 50, 24 53 / 51, 64 80 / 54; 2048 -> 5504
-// 16 15 / 19, 48 20.2 / 20.7, 64 21.9 / 20.8; 1024 -> 2752 64 8.4 / 12.7).  Rows that the tiles need laid out anew: up to 64.
+// 16 15 / 19, 48 20.2 / 20.7, 64 21.9 / 20.8; 1024 -> 2752 64 8.4 / 12.7).  Rows that the small tiles do not take: up to 64.
 bool few(int64_t tokens, int64_t n_in, int64_t n_out) {
   if (tokens <= 16 || tokens > 64) return tokens <= 16;
   return n_in % 64 != 0 || static_cast<double>(tokens - 16) * n_in * n_out <= 4e8;
@@ -377,7 +377,7 @@ struct Forward {
     Room room;
     k = n_in, rows = tokens, x = w1 = w3 = parts = 0;
     if (!few(tokens, n_in, n_out)) {
-      k = up(n_in, 64);
+      k = n_in % 8 == 0 ? n_in : up(n_in, 64);
       rows = std::min(tokens, std::max<int64_t>((kMost - 1) / k / 256 * 256, 256));
       if (k != n_in) {
         x = room.take(2 * rows * k);

@@ -195,8 +195,11 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
   const uint32_t lds_wave = lds0 + wave * 1024;
   // the ring: operand slabs A 0, B 0, A 1, B 1, .. in buffers 0 .. 4 in turn
   const auto behind = [&](uint32_t at, uint32_t buffers) { return at + buffers * kOperandBytes >= kRing ? at + buffers * kOperandBytes - kRing : at + buffers * kOperandBytes; };
+  // (kGate: chunks behind the last k, where a row goes on with the next one or ends, are asked for behind the operands' ends)
+  const int k_last = p.k - (slabs - 1) * kK;
+  const auto along = [&](uint32_t offset, int slab, uint32_t end) { return MODE == kGate && slab == slabs - 1 && 8 * chunk8 >= k_last ? end : offset + slab * (kK * 2); };
   const auto request_a = [&](int slab, uint32_t to, int i) {
-    load_to_lds16(buf_a, off_a[i] + slab * (kRowsA ? kK * pitch_a : kK * 2), lds_wave + to + i * 8192);
+    load_to_lds16(buf_a, kRowsA ? off_a[i] + slab * kK * pitch_a : along(off_a[i], slab, p.a_bytes), lds_wave + to + i * 8192);
   };
   const auto request_b = [&](int slab, uint32_t to, int i) {
     if constexpr (MODE == kInput || MODE == kInputTwo) {
@@ -204,7 +207,7 @@ __global__ __launch_bounds__(kThreads) void gated_tiles_kernel(const GatedTiles 
       const u32x4 buf = second ? buf_b2 : buf_b;
       load_to_lds16(buf, off_b[i] + (second ? slab - p.seg : slab) * kK * pitch_b, lds_wave + to + i * 8192);
     } else {
-      load_to_lds16(buf_b, off_b[i] + slab * (kRowsB ? kK * pitch_b : kK * 2), lds_wave + to + i * 8192);
+      load_to_lds16(buf_b, kRowsB ? off_b[i] + slab * kK * pitch_b : along(off_b[i], slab, p.b_bytes), lds_wave + to + i * 8192);
     }
   };
 

@@ -120,6 +120,8 @@ def test_tokens_in_lds(tokens, n_in, n_out, dtype):
     (20000, 264, 72, torch.float16),       # dw of two tiles, many pieces
     (700, 24, 130000, torch.bfloat16),     # dx of three
     (66000, 40, 40, torch.float16),        # a tile more than the chip has units
+    (300, 1000, 2736, torch.bfloat16),     # a last slab of 40 k
+    (1500, 3064, 1000, torch.float16),     # of 56, in pieces
 ])
 def test_tiles(tokens, n_in, n_out, dtype):
     check(*operands(tokens, n_in, n_out, dtype))
