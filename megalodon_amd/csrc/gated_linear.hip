@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void gated_few_kernel(const FewP
 
 // 9 to 16 tokens with their rows in LDS: a workgroup for each CU walks the groups of 8 features, and the next group's weights are on their way into registers
 // while the current one's products run and the waves' sums meet.  Read again for every group, as above, so many tokens are half as many bytes as the weights
-// and more; fewer cost less than the part-filled last walk here.  (us, above / here, 8, 12, 16 tokens: 4096 -> 11008 47 / 47, 50 / 47.5, 52.8 / 48.6, 2048 -> 5504 12.4 / 13.5,
+// and more; fewer cost less than the part-filled last walk here.  (us, above / here, weights from memory, 8, 12, 16 tokens: 4096 -> 11008 47 / 47, 50 / 47.5, 52.8 / 48.6, 2048 -> 5504 12.4 / 13.5,
 // 13.8 / 13.9, 15.8 / 14.3, 1536 -> 40000 63 / 60, 67 / 62, 70 / 62; 1024 -> 2752 the same.)  STEPS: of 32 k for each wave, at most.
 // A row's chunk c of 16 bytes is at c ^ row: sixteen lanes on different banks.
 constexpr int kRestWaves = 16;
