@@ -417,12 +417,11 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
 
 // Runs over the end of the piece that they begin in: the parts of it and of the pieces behind, in their order.  A workgroup has `columns` columns, VEC of
 // them a thread (4 in wide rows: a quarter of the workgroups, most of which find nothing to do; 32768 tokens, 4096 columns 10.6 us, 9.0 so); in narrow
-// rows its threads share a column's parts.
+// rows its threads share a column's parts.  `sums`: a number of each thread, for the shares to meet in.
 template <int DT, int VEC>
-__global__ __launch_bounds__(kThreads) void join_kernel(const SumParams p, int columns) {
+__device__ __forceinline__ void join_one(const SumParams& p, int columns, uint32_t piece, uint32_t slice, float* sums_) {
   const int per = columns / VEC;  // threads of the columns
-  const unsigned slices = (p.width + columns - 1) / columns, piece = blockIdx.x / slices;
-  const int tid = threadIdx.x, k = static_cast<int>(blockIdx.x % slices) * columns + tid % per * VEC, share = tid / per, shares = kThreads / per;
+  const int tid = threadIdx.x, k = static_cast<int>(slice) * columns + tid % per * VEC, share = tid / per, shares = kThreads / per;
   const int64_t first = static_cast<int64_t>(piece) * p.per_piece, behind = first + p.per_piece;
   if (behind >= p.n) return;
   const uint32_t key = p.keys[behind], last = p.keys[behind - 1], head = p.keys[first], ahead = first > 0 ? p.keys[first - 1] : 0xffffffffu;
@@ -475,7 +474,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const SumParams p, int c
     for (; left > 0; --left) sum += load(open += step);
   }
   if (shares > 1) {
-    __shared__ Floats sums[kThreads];
+    Floats* const sums = reinterpret_cast<Floats*>(sums_);
     sums[tid] = sum;
     __syncthreads();
     if (share > 0) return;
@@ -485,6 +484,17 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const SumParams p, int c
 #pragma unroll
   for (int e = 0; e < VEC; ++e)
     if (e < columns_left) Elem<DT>::store(to + e, sum[e] * p.scale);
+}
+// (2^32 threads are the most of a launch: narrow rows of 2^26 tokens have more pieces than that many threads)
+constexpr int64_t kMostJoins = 1 << 20;
+template <int DT, int VEC>
+__global__ __launch_bounds__(kThreads) void join_kernel(const SumParams p, int columns, uint32_t items) {
+  __shared__ float sums[kThreads * VEC];
+  const uint32_t slices = (p.width + columns - 1) / columns;
+  for (uint32_t i = blockIdx.x; i < items; i += gridDim.x) {
+    join_one<DT, VEC>(p, columns, i / slices, i % slices, sums);
+    if (i + gridDim.x < items) __syncthreads();  // (the shares' numbers have been read)
+  }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------
@@ -587,9 +597,10 @@ int table_grad(const void* dy, const void* tokens, int token_bits, int64_t n, in
     int columns = 16;
     while (columns < kThreads && columns < width) columns *= 2;
     if (width >= 4 * kThreads) columns = 4 * kThreads;
-    const unsigned grid = static_cast<unsigned>(p.pieces * ((width + columns - 1) / columns));
-    if (columns > kThreads) join_kernel<DT, 4><<<grid, kThreads, 0, s>>>(p, columns);
-    else join_kernel<DT, 1><<<grid, kThreads, 0, s>>>(p, columns);
+    const int64_t items = p.pieces * ((width + columns - 1) / columns);  // (fewer than 2^31 for any gradient that fits a device)
+    const unsigned grid = static_cast<unsigned>(std::min(items, kMostJoins));
+    if (columns > kThreads) join_kernel<DT, 4><<<grid, kThreads, 0, s>>>(p, columns, static_cast<uint32_t>(items));
+    else join_kernel<DT, 1><<<grid, kThreads, 0, s>>>(p, columns, static_cast<uint32_t>(items));
     MEGA_CHECK_LAUNCH();
   }
   return MEGA_OK;
