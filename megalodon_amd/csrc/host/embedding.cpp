@@ -21,6 +21,38 @@ Tensor gather(const Tensor& tokens, const Tensor& table, double scale) {
   return out;
 }
 
+// dW of (..., width) gradients by their tokens
+Tensor table_grad(const Tensor& dy_, const Tensor& tokens, int64_t vocab, double scale, int64_t padding) {
+  const Tensor dy = stored(dy_).contiguous();
+  const int64_t width = dy.size(-1), n = tokens.numel();
+  const int code = code_of(dy.scalar_type());
+  Tensor dw = at::empty({vocab, width}, dy.options());
+  const Tensor ws = at::empty({mega_embedding_workspace_bytes(code, n, vocab, width)}, dy.options().dtype(at::kByte));
+  check(mega_embedding_bwd(dy.data_ptr(), code, tokens.data_ptr(), tokens.scalar_type() == at::kLong ? 64 : 32, n, vocab, width, scale, padding, dw.data_ptr(),
+                           n > 0 ? ws.data_ptr() : nullptr, stream_of(dy)), "mega_embedding_bwd");
+  return dw;
+}
+
+Tensor embedding(const Tensor& tokens, const Tensor& table, double scale, std::optional<int64_t> padding);
+
+// The table's gradient where it is differentiated again: the same kernel, so that the gradient is the same; it is linear in dy, and its own gradient the
+// rows of tokens that have one.
+struct TableGradFn : Function<TableGradFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& dy, const Tensor& tokens, int64_t vocab, double scale, int64_t padding) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return table_grad(dy, tokens, vocab, scale, padding);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const Tensor tokens = ctx->get_saved_variables()[0];
+    const int64_t padding = ctx->saved_data["padding"].toInt();
+    c10::DeviceGuard guard(g[0].device());
+    return {embedding(padding < 0 ? tokens : tokens.masked_fill(tokens.eq(padding), -1), g[0], ctx->saved_data["scale"].toDouble(), std::nullopt), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
 struct EmbeddingFn : Function<EmbeddingFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& tokens, double scale, int64_t padding) {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -35,20 +67,9 @@ struct EmbeddingFn : Function<EmbeddingFn> {
     const double scale = ctx->saved_data["scale"].toDouble();
     const int64_t padding = ctx->saved_data["padding"].toInt(), vocab = ctx->saved_data["vocab"].toInt();
     c10::DeviceGuard guard(g[0].device());
-    const int64_t width = g[0].size(-1), n = tokens.numel();
-    if (at::GradMode::is_enabled()) {  // differentiated again: recorded operations
-      const Tensor t = tokens.reshape({-1}).to(at::kLong), kept = at::logical_and(at::logical_and(t.ge(0), t.lt(vocab)), t.ne(padding));
-      const Tensor rows = at::where(kept.unsqueeze(1), g[0].reshape({-1, width}) * scale, 0);
-      return {at::zeros({vocab, width}, g[0].options()).index_add(0, t.clamp(0, vocab - 1), rows), Tensor(), Tensor(), Tensor()};
-    }
+    if (at::GradMode::is_enabled()) return {TableGradFn::apply(g[0], tokens, vocab, scale, padding), Tensor(), Tensor(), Tensor()};
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor dy = stored(g[0]).contiguous();
-    const int code = code_of(dy.scalar_type());
-    Tensor dw = at::empty({vocab, width}, dy.options());
-    const Tensor ws = at::empty({mega_embedding_workspace_bytes(code, n, vocab, width)}, dy.options().dtype(at::kByte));
-    check(mega_embedding_bwd(dy.data_ptr(), code, tokens.data_ptr(), tokens.scalar_type() == at::kLong ? 64 : 32, n, vocab, width, scale, padding, dw.data_ptr(),
-                             n > 0 ? ws.data_ptr() : nullptr, stream_of(dy)), "mega_embedding_bwd");
-    return {dw, Tensor(), Tensor(), Tensor()};
+    return {table_grad(g[0], tokens, vocab, scale, padding), Tensor(), Tensor(), Tensor()};
   }
 };
 

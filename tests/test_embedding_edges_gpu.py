@@ -25,3 +25,33 @@ def test_more_pieces_than_a_launch_has_threads_for():
     want = torch.stack([torch.bincount(tokens, dy[:, d].double(), minlength=V) for d in range(D)], 1)
     assert want.abs().max() < 1 << 24
     assert torch.equal(dw, want.to(torch.float32).bfloat16())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_gradient_that_is_differentiated_again(dtype):
+    """The gradient is the one without `create_graph`, bit for bit: frequent tokens are summed in float32, in one order, and scaled once.  Its own gradients are
+    the formula's: dW[v] = s sum dy[r], so that a table u of ones' gradients gives s u[t_r] where r counts."""
+    n, V, D, scale, padding = 6000, 50, 24, 3.0, 7
+    g = torch.Generator("cuda").manual_seed(5)
+    tokens = torch.randint(-2, V + 2, (2, n // 2), generator=g, device="cuda")
+    tokens[:, ::2], tokens[:, 1::8] = 11, padding
+    weight = torch.randn(V, D, generator=g, device="cuda").to(dtype).requires_grad_(True)
+    dy = torch.randn(2, n // 2, D, generator=g, device="cuda").abs().to(dtype).requires_grad_(True)
+    y = fused_ops.embedding(tokens, weight, scale, padding)
+    once, = torch.autograd.grad(y, weight, dy.detach(), retain_graph=True)
+    for _ in range(2):
+        again, = torch.autograd.grad(y, weight, dy, create_graph=True)
+        assert torch.equal(again, once) and again.requires_grad
+    kept = (tokens >= 0) & (tokens < V) & (tokens != padding)
+    rows = dy.detach().double()[kept]
+    want = torch.zeros(V, D, dtype=torch.float64, device="cuda").index_add_(0, tokens[kept], rows) * scale
+    # 6000 positive float32 summands, the scale's product, one rounding; whole in float16 (11 has 3000 of |N(0, 1)|, 7200 or so)
+    assert ((again.detach().double() - want).abs() <= (6002 * 2.0 ** -24 + 1.01 * torch.finfo(dtype).eps / 2) * want).all()
+    u = torch.randn(V, D, generator=g, device="cuda").to(dtype).requires_grad_(True)
+    back, = torch.autograd.grad(again, dy, u, create_graph=True)
+    assert torch.equal(back.detach(), torch.where(kept[..., None], (u.detach().float() * scale)[tokens.clamp(0, V - 1)], 0.0).to(dtype))
+    # ... and once more: u's gradient is dW of the gradients of `back`
+    v = torch.randn(2, n // 2, D, generator=g, device="cuda").abs().to(dtype)
+    third, = torch.autograd.grad(back, u, v)
+    want = torch.zeros(V, D, dtype=torch.float64, device="cuda").index_add_(0, tokens[kept], v.double()[kept]) * scale
+    assert ((third.double() - want).abs() <= (6002 * 2.0 ** -24 + 1.01 * torch.finfo(dtype).eps / 2) * want).all()
