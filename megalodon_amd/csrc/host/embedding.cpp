@@ -67,11 +67,25 @@ struct EmbeddingFn : Function<EmbeddingFn> {
     const double scale = ctx->saved_data["scale"].toDouble();
     const int64_t padding = ctx->saved_data["padding"].toInt(), vocab = ctx->saved_data["vocab"].toInt();
     c10::DeviceGuard guard(g[0].device());
+    if (watched() || !plain(g[0])) {  // (several gradients at once)
+      const int64_t width = g[0].size(-1);
+      const Tensor t = tokens.reshape({-1}).to(at::kLong), counts = at::logical_and(at::logical_and(t.ge(0), t.lt(vocab)), t.ne(padding));
+      const Tensor rows = at::where(counts.unsqueeze(1), g[0].reshape({-1, width}).to(at::kFloat), at::zeros({}, g[0].options().dtype(at::kFloat)));
+      return {at::embedding_dense_backward(rows, t.clamp(0, vocab - 1), vocab, -1, false).mul(scale).to(g[0].scalar_type()), Tensor(), Tensor(), Tensor()};
+    }
     if (at::GradMode::is_enabled()) return {TableGradFn::apply(g[0], tokens, vocab, scale, padding), Tensor(), Tensor(), Tensor()};
     at::AutoDispatchBelowADInplaceOrView below;
     return {table_grad(g[0], tokens, vocab, scale, padding), Tensor(), Tensor(), Tensor()};
   }
 };
+
+// The same by the library's operations.
+Tensor recorded(const Tensor& tokens, const Tensor& table, double scale, int64_t padding) {
+  const int64_t vocab = table.size(0);
+  const Tensor there = at::logical_and(tokens.ge(0), tokens.lt(vocab)).unsqueeze(-1);
+  const Tensor rows = at::embedding(table, tokens.clamp(0, vocab - 1), padding);
+  return at::where(there, scale == 1 ? rows : rows.to(at::kFloat).mul(scale).to(table.scalar_type()), at::zeros({}, table.options()));
+}
 
 Tensor embedding(const Tensor& tokens_, const Tensor& table_, double scale, std::optional<int64_t> padding_) {
   require(tokens_.is_cuda() && table_.is_cuda(), "megalodon_amd ops need GPU (HIP) tensors; there is no CPU fallback");
@@ -85,8 +99,11 @@ Tensor embedding(const Tensor& tokens_, const Tensor& table_, double scale, std:
     require(*padding_ >= -vocab && *padding_ < vocab, "embedding: padding_idx must be a row of weight");
     padding = *padding_ < 0 ? *padding_ + vocab : *padding_;
   }
-  c10::DeviceGuard guard(table_.device());
-  const Tensor tokens = tokens_.contiguous(), table = stored(table_);
+  // what watches the thread's operations is shown operations
+  const Tensor given = stored(tokens_), table = stored(table_);
+  if (watched() || !plain(given) || !plain(table)) return recorded(given, table, scale, padding);
+  c10::DeviceGuard guard(table.device());
+  const Tensor tokens = given.contiguous();
   if ((at::GradMode::is_enabled() && table.requires_grad()) || has_tangent(table)) return EmbeddingFn::apply(table, tokens, scale, padding);
   return gather(tokens, table, scale);
 }

@@ -5,6 +5,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -48,6 +49,20 @@ inline Tensor stored(const Tensor& t) { return lazy(t) ? t.resolve_conj().resolv
 
 // whether a forward-mode derivative travels with the tensor
 inline bool has_tangent(const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+
+// Whether the thread shows its operations to something beside autograd: the TorchScript tracer, a mode that counts flops
+// or makes fake tensors, a functorch transform.  A launch is no operation -- a trace of one holds the allocation of its
+// result and nothing that fills it -- so these are given the library's operations.
+inline bool watched() {
+  const auto tls = c10::impl::tls_local_dispatch_key_set();
+  return (tls.included_ - tls.excluded_ - c10::default_included_set).highestFunctionalityKey() != c10::DispatchKey::Undefined;
+}
+// Whether a tensor is what its memory holds and nothing more: dispatch keys of a dense tensor, no subclass, functional
+// wrapper, zeros without memory or batch.
+inline bool plain(const Tensor& t) {
+  constexpr auto usual = c10::default_included_set | c10::autograd_dispatch_keyset | c10::autocast_dispatch_keyset | c10::DispatchKeySet(c10::DispatchKey::Dense);
+  return (t.key_set() - usual).highestFunctionalityKey() == c10::DispatchKey::Undefined && t.has_storage();
+}
 
 void bind_clip(py::module_& m);
 void bind_decode(py::module_& m);

@@ -4,7 +4,6 @@
 #include "host.hpp"
 
 #include <ATen/autocast_mode.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 #include <map>
@@ -491,19 +490,6 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale
 }
 
 // ---- linear layers --------------------------------------------------------------------------------
-// Whether the thread shows its operations to something beside autograd: the TorchScript tracer, a mode that counts flops
-// or makes fake tensors, a functorch transform.  A launch is no operation -- a trace of one holds the allocation of its
-// result and nothing that fills it -- so these are given the library's products.
-bool watched() {
-  const auto tls = c10::impl::tls_local_dispatch_key_set();
-  return (tls.included_ - tls.excluded_ - c10::default_included_set).highestFunctionalityKey() != c10::DispatchKey::Undefined;
-}
-// Whether a tensor is what its memory holds and nothing more: dispatch keys of a dense tensor, no subclass, functional
-// wrapper, zeros without memory or batch.
-bool plain(const Tensor& t) {
-  constexpr auto usual = c10::default_included_set | c10::autograd_dispatch_keyset | c10::autocast_dispatch_keyset | c10::DispatchKeySet(c10::DispatchKey::Dense);
-  return (t.key_set() - usual).highestFunctionalityKey() == c10::DispatchKey::Undefined && t.has_storage();
-}
 // A matrix as the library's products take it: its own memory, whole rows, 16-byte boundary.
 bool dense16(const Tensor& t) {
   if (!plain(t) || watched() || !t.is_contiguous()) return false;

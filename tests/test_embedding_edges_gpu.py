@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from megalodon_amd import fused_ops
+from megalodon_amd.modules import Embedding
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +56,77 @@ def test_gradient_that_is_differentiated_again(dtype):
     third, = torch.autograd.grad(back, u, v)
     want = torch.zeros(V, D, dtype=torch.float64, device="cuda").index_add_(0, tokens[kept], v.double()[kept]) * scale
     assert ((third.double() - want).abs() <= (6002 * 2.0 ** -24 + 1.01 * torch.finfo(dtype).eps / 2) * want).all()
+
+
+class Rows(torch.nn.Module):
+    """Two tables, one scaled and with a padding row."""
+
+    def __init__(self, dtype):
+        super().__init__()
+        self.first = Embedding(40, 16, padding_idx=3, scale=0.5, device="cuda", dtype=dtype)
+        self.second = Embedding(40, 8, device="cuda", dtype=dtype)
+
+    def forward(self, tokens):
+        return self.first(tokens), self.second(tokens)
+
+
+def foreign(seed, shape=(4, 25), V=40, bits=torch.long):
+    """Tokens with some that are no row."""
+    return torch.randint(-3, V + 3, shape, generator=torch.Generator("cuda").manual_seed(seed), device="cuda").to(bits)
+
+
+@pytest.mark.parametrize("gradients", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_traced(dtype, gradients):
+    """A trace holds operations: called with other tokens it gives what the layer gives, and the layer's gradients."""
+    layers = Rows(dtype)
+    with torch.set_grad_enabled(gradients):
+        traced = torch.jit.trace(layers, (foreign(1),), check_trace=False)
+        for seed in (2, 3):
+            tokens = foreign(seed)
+            got, want = traced(tokens), layers(tokens)
+            assert all(torch.equal(a, b) and a.requires_grad == gradients for a, b in zip(got, want))
+    if gradients:
+        dy = [torch.randint(-2, 3, y.shape, device="cuda").to(dtype) for y in want]
+        for a, b in zip(torch.autograd.grad(got, layers.parameters(), dy), torch.autograd.grad(want, layers.parameters(), dy)):
+            assert torch.equal(a, b)  # (whole numbers and halves: exact)
+
+
+def test_fake_tensors():
+    from torch._subclasses import FakeTensorMode
+    with FakeTensorMode():
+        fake = Embedding(40, 16, scale=2.0, device="cuda", dtype=torch.bfloat16)
+        y = fake(torch.zeros(5, 3, device="cuda", dtype=torch.long))
+        assert y.shape == (5, 3, 16) and y.dtype == torch.bfloat16
+        dw, = torch.autograd.grad(y, fake.weight, torch.empty_like(y))
+        assert dw.shape == (40, 16)
+
+
+def test_functions_of_functions():
+    """vmap over tokens and over tables, functionalize, several gradients at once, gradients that are zeros without memory."""
+    layer = Embedding(40, 16, padding_idx=3, scale=0.5, device="cuda", dtype=torch.bfloat16)
+    tokens = foreign(4, (6, 9))
+    with torch.no_grad():
+        want = layer(tokens)
+        assert torch.equal(torch.func.vmap(layer)(tokens), want)
+        tables = torch.stack([layer.weight, -layer.weight])
+        both = torch.func.vmap(lambda w: fused_ops.embedding(tokens, w, 0.5, 3))(tables)
+        assert torch.equal(both, torch.stack([want, -want]))
+        assert torch.equal(torch.func.functionalize(layer)(tokens), want)
+    for bits in (torch.int32, torch.long):
+        y = layer(tokens.to(bits))
+        many = torch.randint(-2, 3, (3, *y.shape), device="cuda").bfloat16()
+        got, = torch.autograd.grad(y, layer.weight, many, is_grads_batched=True, retain_graph=True)
+        assert torch.equal(got, torch.stack([torch.autograd.grad(y, layer.weight, g, retain_graph=True)[0] for g in many]))
+        dw, = torch.autograd.grad(y, layer.weight, torch._efficientzerotensor(tuple(y.shape), dtype=y.dtype, device="cuda"))
+        assert not dw.any()
+    grads = torch.func.grad(lambda w: fused_ops.embedding(tokens, w, 0.5, 3).float().sum())(layer.weight.detach())
+    y = layer(tokens)
+    assert torch.equal(grads, torch.autograd.grad(y, layer.weight, torch.ones_like(y))[0])
+
+
+def test_tokens_and_tables_negated_on_reading():
+    table, tokens = torch.randn(40, 16, device="cuda"), foreign(6)
+    want = fused_ops.embedding(tokens, table, 3.0)
+    assert torch.equal(fused_ops.embedding(torch._neg_view(-tokens), table, 3.0), want)
+    assert torch.equal(fused_ops.embedding(tokens, torch._neg_view(-table), 3.0), want)
