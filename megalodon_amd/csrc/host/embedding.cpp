@@ -63,7 +63,9 @@ struct EmbeddingFn : Function<EmbeddingFn> {
     return gather(tokens, table, scale);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const Tensor tokens = ctx->get_saved_variables()[0].contiguous();  // (saved-tensor hooks may hand back any layout)
+    const Tensor tokens = stored(ctx->get_saved_variables()[0]).contiguous();  // (saved-tensor hooks may hand back anything)
+    require((tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt) && tokens.device() == g[0].device() && tokens.numel() * g[0].size(-1) == g[0].numel(),
+            "embedding: the saved tokens have another type, device or number than they were saved with");
     const double scale = ctx->saved_data["scale"].toDouble();
     const int64_t padding = ctx->saved_data["padding"].toInt(), vocab = ctx->saved_data["vocab"].toInt();
     c10::DeviceGuard guard(g[0].device());

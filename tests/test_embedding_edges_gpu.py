@@ -130,3 +130,26 @@ def test_tokens_and_tables_negated_on_reading():
     want = fused_ops.embedding(tokens, table, 3.0)
     assert torch.equal(fused_ops.embedding(torch._neg_view(-tokens), table, 3.0), want)
     assert torch.equal(fused_ops.embedding(tokens, torch._neg_view(-table), 3.0), want)
+
+
+@pytest.mark.parametrize("back", [lambda t: t.short(), lambda t: t.double(), lambda t: t.cpu(), lambda t: t[:-1], lambda t: torch.cat([t, t])])
+def test_saved_tokens_that_came_back_as_something_else(back):
+    """What hooks hand back is refused where it is not the tokens any more, before anything is launched."""
+    weight = torch.randn(40, 16, device="cuda", requires_grad=True)
+    tokens = foreign(7, (50,))
+    dy = torch.randn(50, 16, device="cuda")
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+        y = fused_ops.embedding(tokens, weight)
+        with pytest.raises(RuntimeError, match="saved tokens"):
+            torch.autograd.grad(y, weight, dy)
+
+
+def test_saved_tokens_in_other_places_and_types():
+    weight = torch.randn(40, 16, device="cuda", requires_grad=True)
+    tokens = foreign(8, (50,))
+    dy = torch.randn(50, 16, device="cuda")
+    want, = torch.autograd.grad(fused_ops.embedding(tokens, weight), weight, dy)
+    for pack, back in ((lambda t: t.cpu(), lambda t: t.cuda()), (lambda t: t.int(), lambda t: t), (lambda t: t.view(5, 10).t().contiguous(), lambda t: t.t()), (lambda t: -t, torch._neg_view)):
+        with torch.autograd.graph.saved_tensors_hooks(pack, back):
+            got, = torch.autograd.grad(fused_ops.embedding(tokens, weight), weight, dy)
+        assert torch.equal(got, want)
