@@ -790,7 +790,16 @@ struct GatedFn : Function<GatedFn> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
     const bool want_x = ctx->needs_input_grad(0), want_1 = ctx->needs_input_grad(1), want_3 = ctx->needs_input_grad(2);
-    c10::DeviceGuard guard(saved[0].device());
+    c10::DeviceGuard guard(g[0].device());
+    // (saved-tensor hooks may hand back anything)
+    const auto type = g[0].scalar_type(), kept = saved[3].scalar_type();
+    for (const Tensor& t : saved) require(t.device() == g[0].device(), "gated_linear: a saved tensor is on another device than it was saved on");
+    require(saved[0].scalar_type() == type && saved[1].scalar_type() == type && saved[2].scalar_type() == type && saved[4].scalar_type() == kept && (kept == type || kept == at::kFloat),
+            "gated_linear: a saved tensor has another type than it was saved with");
+    const int64_t in = saved[0].dim() > 0 ? saved[0].size(-1) : 0, out = g[0].size(-1), rows = g[0].numel() / out;
+    require(in > 0 && saved[0].numel() == rows * in && saved[1].sizes() == at::IntArrayRef({out, in}) && saved[2].sizes() == saved[1].sizes() &&
+                saved[3].numel() == rows * ((out + 7) / 8 * 8) && saved[4].sizes() == saved[3].sizes(),
+            "gated_linear: a saved tensor has another shape than it was saved with");
     if (at::GradMode::is_enabled()) {  // differentiated again: recorded operations, from the operands themselves
       const Tensor x = flat(saved[0]), go = flat(g[0]), &w1 = saved[1], &w3 = saved[2];
       const Tensor a = at::mm(x, w1.t()), b = at::mm(x, w3.t()), s = at::sigmoid(a);
@@ -798,13 +807,9 @@ struct GatedFn : Function<GatedFn> {
       return {want_x ? (at::mm(da, w1) + at::mm(db, w3)).view(saved[0].sizes()) : Tensor(), want_1 ? at::mm(da.t(), x) : Tensor(), want_3 ? at::mm(db.t(), x) : Tensor(), Tensor()};
     }
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor x = attn_operand(saved[0]), w1 = attn_operand(saved[1]), w3 = attn_operand(saved[2]), a = attn_operand(saved[3]), b = attn_operand(saved[4]);
-    const Tensor dh = stored(g[0]).contiguous();
-    require(dh.scalar_type() == x.scalar_type(), "gated_linear: the output's gradient must have x's dtype");
+    const auto operand = [](const Tensor& t) { return attn_operand(stored(t)); };
+    const Tensor x = operand(saved[0]), w1 = operand(saved[1]), w3 = operand(saved[2]), a = operand(saved[3]), b = operand(saved[4]), dh = stored(g[0]).contiguous();
     const int64_t n_in = x.size(-1), n_out = w1.size(0), tokens = x.numel() / n_in;
-    // (saved-tensor hooks may hand back anything)
-    require(w1.sizes() == w3.sizes() && w1.size(1) == n_in && dh.numel() == tokens * n_out && a.numel() == tokens * ((n_out + 7) / 8 * 8) && a.sizes() == b.sizes() && a.scalar_type() == b.scalar_type(),
-            "gated_linear: a saved tensor has another shape than it was saved with");
     Tensor dx, d1, d3;
     if (want_x) dx = at::empty_like(x);
     if (want_1) d1 = at::empty_like(w1);
