@@ -4,8 +4,10 @@
 #include "host.hpp"
 
 #include <ATen/autocast_mode.h>
+#include <torch/csrc/autograd/autograd.h>
 #include <torch/csrc/autograd/custom_function.h>
 
+#include <array>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -780,6 +782,70 @@ std::tuple<Tensor, Tensor, Tensor> gated_raw(const Tensor& x, const Tensor& w1, 
   check(mega_gated_linear_fwd(x.data_ptr(), w1.data_ptr(), w3.data_ptr(), kernel_code(x), tokens, n_in, n_out, h.data_ptr(), ptr(a), ptr(b), code_of(kept.value_or(x.scalar_type())), ptr(ws), stream_of(x)), "mega_gated_linear_fwd");
   return {h, a, b};
 }
+using Wanted = std::array<bool, 3>;  // of x, w1, w3
+// The gradients by the kernels, those that are wanted.
+variable_list gated_grads(const Tensor& dh_, const Tensor& x_, const Tensor& w1_, const Tensor& w3_, const Tensor& a_, const Tensor& b_, Wanted wanted) {
+  const auto [want_x, want_1, want_3] = wanted;
+  const auto operand = [](const Tensor& t) { return attn_operand(stored(t)); };
+  const Tensor x = operand(x_), w1 = operand(w1_), w3 = operand(w3_), a = operand(a_), b = operand(b_), dh = stored(dh_).contiguous();
+  const int64_t n_in = x.size(-1), n_out = w1.size(0), tokens = x.numel() / n_in;
+  Tensor dx, d1, d3;
+  if (want_x) dx = at::empty_like(x);
+  if (want_1) d1 = at::empty_like(w1);
+  if (want_3) d3 = at::empty_like(w3);
+  if (tokens == 0) {
+    if (want_1) d1.zero_();
+    if (want_3) d3.zero_();
+  } else {
+    const Tensor ws = bytes(mega_gated_linear_workspace_bytes(tokens, n_in, n_out, want_x + 2 * want_1 + 4 * want_3), x);
+    check(mega_gated_linear_bwd(dh.data_ptr(), x.data_ptr(), w1.data_ptr(), w3.data_ptr(), a.data_ptr(), b.data_ptr(), code_of(a.scalar_type()), kernel_code(x), tokens, n_in, n_out, ptr(dx), ptr(d1), ptr(d3), ptr(ws), stream_of(x)), "mega_gated_linear_bwd");
+  }
+  return {dx, d1, d3};
+}
+// The same by recorded operations, in float32 from the operands.
+variable_list gated_recorded(const Tensor& dh, const Tensor& x, const Tensor& w1, const Tensor& w3, Wanted wanted) {
+  const auto type = x.scalar_type();
+  const Tensor go = flat(dh).to(at::kFloat), xf = flat(x).to(at::kFloat), f1 = w1.to(at::kFloat), f3 = w3.to(at::kFloat);
+  const Tensor a = at::mm(xf, f1.t()), b = at::mm(xf, f3.t()), s = at::sigmoid(a);
+  const Tensor da = go * b * s * (1 + a * (1 - s)), db = go * a * s;
+  return {wanted[0] ? (at::mm(da, f1) + at::mm(db, f3)).to(type).view(x.sizes()) : Tensor(), wanted[1] ? at::mm(da.t(), xf).to(type) : Tensor(), wanted[2] ? at::mm(db.t(), xf).to(type) : Tensor()};
+}
+variable_list defined_of(const variable_list& all) {
+  variable_list some;
+  for (const Tensor& t : all)
+    if (t.defined()) some.push_back(t);
+  return some;
+}
+// The gradients where they are differentiated again: by the same kernels, so that they are the same; their own gradients are those of the recorded form.
+struct GatedGradFn : Function<GatedGradFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& dh, const Tensor& x, const Tensor& w1, const Tensor& w3, const Tensor& a, const Tensor& b, Wanted wanted) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({dh, x, w1, w3});
+    ctx->saved_data["wanted"] = std::vector<int64_t>(wanted.begin(), wanted.end());
+    return defined_of(gated_grads(dh, x, w1, w3, a, b, wanted));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const bool again = at::GradMode::is_enabled();
+    const auto saved = ctx->get_saved_variables();
+    const auto flags = ctx->saved_data["wanted"].toIntVector();
+    c10::DeviceGuard guard(saved[0].device());
+    at::AutoGradMode on(true);
+    variable_list in, asked, out, from;  // (aliases, so that what one operand has to do with another is none of these gradients)
+    for (size_t i = 0; i < 4; ++i) {
+      in.push_back(at::alias(saved[i]));
+      if (ctx->needs_input_grad(i)) asked.push_back(in[i]);
+    }
+    const variable_list all = defined_of(gated_recorded(in[0], in[1], in[2], in[3], {flags[0] != 0, flags[1] != 0, flags[2] != 0}));
+    for (size_t i = 0; i < all.size(); ++i)
+      if (all[i].requires_grad()) out.push_back(all[i]), from.push_back(g[i]);
+    variable_list grads(7);
+    if (out.empty() || asked.empty()) return grads;
+    const variable_list got = torch::autograd::grad(out, asked, from, again, again, /*allow_unused=*/true);
+    for (size_t i = 0, next = 0; i < 4; ++i)
+      if (ctx->needs_input_grad(i)) grads[i] = got[next++];
+    return grads;
+  }
+};
 struct GatedFn : Function<GatedFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w1, const Tensor& w3, at::ScalarType kept) {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -789,7 +855,7 @@ struct GatedFn : Function<GatedFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
-    const bool want_x = ctx->needs_input_grad(0), want_1 = ctx->needs_input_grad(1), want_3 = ctx->needs_input_grad(2);
+    const Wanted wanted{ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2)};
     c10::DeviceGuard guard(g[0].device());
     // (saved-tensor hooks may hand back anything)
     const auto type = g[0].scalar_type(), kept = saved[3].scalar_type();
@@ -800,28 +866,17 @@ struct GatedFn : Function<GatedFn> {
     require(in > 0 && saved[0].numel() == rows * in && saved[1].sizes() == at::IntArrayRef({out, in}) && saved[2].sizes() == saved[1].sizes() &&
                 saved[3].numel() == rows * ((out + 7) / 8 * 8) && saved[4].sizes() == saved[3].sizes(),
             "gated_linear: a saved tensor has another shape than it was saved with");
-    if (at::GradMode::is_enabled()) {  // differentiated again: recorded operations, from the operands themselves
-      const Tensor x = flat(saved[0]), go = flat(g[0]), &w1 = saved[1], &w3 = saved[2];
-      const Tensor a = at::mm(x, w1.t()), b = at::mm(x, w3.t()), s = at::sigmoid(a);
-      const Tensor da = go * b * s * (1 + a * (1 - s)), db = go * a * s;
-      return {want_x ? (at::mm(da, w1) + at::mm(db, w3)).view(saved[0].sizes()) : Tensor(), want_1 ? at::mm(da.t(), x) : Tensor(), want_3 ? at::mm(db.t(), x) : Tensor(), Tensor()};
+    variable_list grads;
+    if (at::GradMode::is_enabled()) {
+      const variable_list some = GatedGradFn::apply(g[0], saved[0], saved[1], saved[2], saved[3], saved[4], wanted);
+      for (size_t i = 0, next = 0; i < 3; ++i) grads.push_back(wanted[i] ? some[next++] : Tensor());
+      grads.emplace_back();
+      return grads;
     }
     at::AutoDispatchBelowADInplaceOrView below;
-    const auto operand = [](const Tensor& t) { return attn_operand(stored(t)); };
-    const Tensor x = operand(saved[0]), w1 = operand(saved[1]), w3 = operand(saved[2]), a = operand(saved[3]), b = operand(saved[4]), dh = stored(g[0]).contiguous();
-    const int64_t n_in = x.size(-1), n_out = w1.size(0), tokens = x.numel() / n_in;
-    Tensor dx, d1, d3;
-    if (want_x) dx = at::empty_like(x);
-    if (want_1) d1 = at::empty_like(w1);
-    if (want_3) d3 = at::empty_like(w3);
-    if (tokens == 0) {
-      if (want_1) d1.zero_();
-      if (want_3) d3.zero_();
-    } else {
-      const Tensor ws = bytes(mega_gated_linear_workspace_bytes(tokens, n_in, n_out, want_x + 2 * want_1 + 4 * want_3), x);
-      check(mega_gated_linear_bwd(dh.data_ptr(), x.data_ptr(), w1.data_ptr(), w3.data_ptr(), a.data_ptr(), b.data_ptr(), code_of(a.scalar_type()), kernel_code(x), tokens, n_in, n_out, ptr(dx), ptr(d1), ptr(d3), ptr(ws), stream_of(x)), "mega_gated_linear_bwd");
-    }
-    return {dx, d1, d3, Tensor()};
+    grads = gated_grads(g[0], saved[0], saved[1], saved[2], saved[3], saved[4], wanted);
+    grads.emplace_back();
+    return grads;
   }
 };
 Tensor gated_linear(const Tensor& x_, const Tensor& w1_, const Tensor& w3_, std::optional<at::ScalarType> kept) {

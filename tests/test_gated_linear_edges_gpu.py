@@ -52,3 +52,58 @@ def test_saved_tensors_in_other_forms():
         with torch.autograd.graph.saved_tensors_hooks(pack, back):
             got = torch.autograd.grad(fused_ops.gated_linear(*leaves), leaves, dh)
         assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def twice(fn, x, w1, w3, dh, us):
+    """The gradients, and the gradients of (each times a u) by all four operands, once and once more."""
+    grads = torch.autograd.grad(fn(x, w1, w3), (x, w1, w3), dh, create_graph=True)
+    second = torch.autograd.grad(grads, (x, w1, w3, dh), us, create_graph=True)
+    third = torch.autograd.grad(second, (x, w1, w3, dh), [torch.ones_like(t) for t in second])
+    return grads, second, third
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [5, 100])
+def test_gradients_that_are_differentiated_again(tokens, dtype):
+    """The gradients are those without `create_graph`, bit for bit.  Theirs are the formula's in float32, rounded once: a rounding is off by eps / 2 of the
+    value at most, float32's own part (sums of up to 100 numbers, a few steps an element) is below a 64th of that.  Those of the third order add up
+    gradients of second ones that were rounded on the way: four of them."""
+    x, w1, w3, dh = operands(tokens, 40, 24, dtype)
+    us = [torch.randn_like(t) for t in (x, w1, w3)]
+    leaves = leaves_of(x, w1, w3)
+    once = torch.autograd.grad(fused_ops.gated_linear(*leaves), leaves, dh)
+    got = twice(fused_ops.gated_linear, *leaves_of(x, w1, w3, dh), us)
+    assert all(torch.equal(g, w) for g, w in zip(got[0], once))
+    wide = [t.double().cpu().requires_grad_(True) for t in (x, w1, w3, dh)]
+    want = twice(lambda x, w1, w3: torch.nn.functional.silu(x @ w1.t()) * (x @ w3.t()), *wide, [u.double().cpu() for u in us])
+    u = torch.finfo(dtype).eps / 2
+    for order, times in ((1, 1), (2, 4)):
+        for g, w in zip(got[order], want[order]):
+            assert (g.double().cpu() - w).norm() <= times * u * (1 + 1 / 64) * w.norm()
+
+
+def test_second_gradients_of_some_operands():
+    """Only those that are asked for; operands that depend on each other; an output gradient that depends on one."""
+    x, w1, w3, dh = operands(9, 16, 8, torch.bfloat16)
+    us = [torch.randn_like(t) for t in (x, w1, w3)]
+
+    def run(fn, cast, asked, tied):
+        leaves = [cast(t).requires_grad_(i in asked) for i, t in enumerate((x, w1, w3))]
+        w = leaves[1] * 2 if tied else leaves[2]
+        h = fn(leaves[0], leaves[1], w)
+        go = cast(dh) * leaves[1].detach().sum() if not tied else (leaves[1].sum() / 4) * cast(dh)
+        first = torch.autograd.grad(h, [leaves[i] for i in asked], go, create_graph=True)
+        loss = sum((f * cast(us[i])).sum() for f, i in zip(first, asked))
+        if not loss.requires_grad:
+            return []
+        return torch.autograd.grad(loss, [leaves[i] for i in asked], allow_unused=True)
+
+    for asked, tied in (([0], False), ([1], False), ([2], False), ([0, 2], False), ([0, 1], True)):
+        got = run(fused_ops.gated_linear, lambda t: t.detach().clone(), asked, tied)
+        want = run(lambda x, w1, w3: torch.nn.functional.silu(x @ w1.t()) * (x @ w3.t()), lambda t: t.detach().double().cpu(), asked, tied)
+        for g, w in zip(got, want):
+            if w is None or not w.any():
+                assert g is None or not g.any()
+            else:
+                # (a handful of roundings of the program's own around the operator)
+                assert (g.double().cpu() - w).norm() <= 8 * 2.0 ** -8 * w.norm()
