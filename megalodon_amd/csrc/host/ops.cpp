@@ -808,7 +808,7 @@ variable_list gated_recorded(const Tensor& dh, const Tensor& x, const Tensor& w1
   const Tensor go = flat(dh).to(at::kFloat), xf = flat(x).to(at::kFloat), f1 = w1.to(at::kFloat), f3 = w3.to(at::kFloat);
   const Tensor a = at::mm(xf, f1.t()), b = at::mm(xf, f3.t()), s = at::sigmoid(a);
   const Tensor da = go * b * s * (1 + a * (1 - s)), db = go * a * s;
-  return {wanted[0] ? (at::mm(da, f1) + at::mm(db, f3)).to(type).view(x.sizes()) : Tensor(), wanted[1] ? at::mm(da.t(), xf).to(type) : Tensor(), wanted[2] ? at::mm(db.t(), xf).to(type) : Tensor()};
+  return {wanted[0] ? (at::mm(da, f1) + at::mm(db, f3)).to(type).reshape(x.sizes()) : Tensor(), wanted[1] ? at::mm(da.t(), xf).to(type) : Tensor(), wanted[2] ? at::mm(db.t(), xf).to(type) : Tensor()};
 }
 variable_list defined_of(const variable_list& all) {
   variable_list some;
@@ -867,6 +867,11 @@ struct GatedFn : Function<GatedFn> {
                 saved[3].numel() == rows * ((out + 7) / 8 * 8) && saved[4].sizes() == saved[3].sizes(),
             "gated_linear: a saved tensor has another shape than it was saved with");
     variable_list grads;
+    if (watched() || !plain(g[0])) {  // (several gradients at once, zeros without memory)
+      grads = gated_recorded(g[0], saved[0], saved[1], saved[2], wanted);
+      grads.emplace_back();
+      return grads;
+    }
     if (at::GradMode::is_enabled()) {
       const variable_list some = GatedGradFn::apply(g[0], saved[0], saved[1], saved[2], saved[3], saved[4], wanted);
       for (size_t i = 0, next = 0; i < 3; ++i) grads.push_back(wanted[i] ? some[next++] : Tensor());

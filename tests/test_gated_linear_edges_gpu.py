@@ -107,3 +107,20 @@ def test_second_gradients_of_some_operands():
             else:
                 # (a handful of roundings of the program's own around the operator)
                 assert (g.double().cpu() - w).norm() <= 8 * 2.0 ** -8 * w.norm()
+
+
+def test_gradients_of_several_outputs_at_once():
+    """One backward for many output gradients, and gradients that are zeros without memory."""
+    x, w1, w3, _ = operands(40, 24, 16, torch.bfloat16)
+    leaves = leaves_of(x, w1, w3)
+    h = fused_ops.gated_linear(*leaves)
+    many = torch.randn(3, 40, 16, device="cuda").bfloat16()
+    got = torch.autograd.grad(h, leaves, many, is_grads_batched=True, retain_graph=True)
+    wide = [t.double() for t in (x, w1, w3)]
+    for i, dh in enumerate(many):
+        exact = [t.clone().requires_grad_(True) for t in wide]
+        want = torch.autograd.grad(torch.nn.functional.silu(exact[0] @ exact[1].t()) * (exact[0] @ exact[2].t()), exact, dh.double())
+        for g, w in zip(got, want):
+            assert (g[i].double() - w).norm() <= 2.0 ** -8 * (1 + 1 / 64) * w.norm()  # (one rounding of the float32 formula)
+    none = torch.autograd.grad(h, leaves, torch._efficientzerotensor((40, 16), dtype=h.dtype, device="cuda"))
+    assert all(g.shape == t.shape and not g.any() for g, t in zip(none, leaves))
