@@ -69,7 +69,7 @@ struct EmbeddingFn : Function<EmbeddingFn> {
     const double scale = ctx->saved_data["scale"].toDouble();
     const int64_t padding = ctx->saved_data["padding"].toInt(), vocab = ctx->saved_data["vocab"].toInt();
     c10::DeviceGuard guard(g[0].device());
-    if (watched() || !plain(g[0])) {  // (several gradients at once)
+    if (watched() || !plain(stored(g[0]))) {  // (several gradients at once)
       const int64_t width = g[0].size(-1);
       const Tensor t = tokens.reshape({-1}).to(at::kLong), counts = at::logical_and(at::logical_and(t.ge(0), t.lt(vocab)), t.ne(padding));
       const Tensor rows = at::where(counts.unsqueeze(1), g[0].reshape({-1, width}).to(at::kFloat), at::zeros({}, g[0].options().dtype(at::kFloat)));

@@ -867,8 +867,8 @@ struct GatedFn : Function<GatedFn> {
                 saved[3].numel() == rows * ((out + 7) / 8 * 8) && saved[4].sizes() == saved[3].sizes(),
             "gated_linear: a saved tensor has another shape than it was saved with");
     variable_list grads;
-    if (watched() || !plain(g[0])) {  // (several gradients at once, zeros without memory)
-      grads = gated_recorded(g[0], saved[0], saved[1], saved[2], wanted);
+    if (const Tensor dh = stored(g[0]); watched() || !plain(dh)) {  // (several gradients at once, zeros without memory)
+      grads = gated_recorded(dh, saved[0], saved[1], saved[2], wanted);
       grads.emplace_back();
       return grads;
     }

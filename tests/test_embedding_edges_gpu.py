@@ -130,6 +130,10 @@ def test_tokens_and_tables_negated_on_reading():
     want = fused_ops.embedding(tokens, table, 3.0)
     assert torch.equal(fused_ops.embedding(torch._neg_view(-tokens), table, 3.0), want)
     assert torch.equal(fused_ops.embedding(tokens, torch._neg_view(-table), 3.0), want)
+    leaf, dy = table.requires_grad_(True), torch.randn_like(want)
+    y = fused_ops.embedding(tokens, leaf, 3.0)
+    grads = [torch.autograd.grad(y, leaf, g, retain_graph=True)[0] for g in (dy, torch._neg_view(-dy))]
+    assert torch.equal(*grads)
 
 
 @pytest.mark.parametrize("back", [lambda t: t.short(), lambda t: t.double(), lambda t: t.cpu(), lambda t: t[:-1], lambda t: torch.cat([t, t])])
