@@ -26,7 +26,9 @@ struct GatedTiles {
   uint16_t *c, *c2;           // (kWeight: the gradient of w1 or of the only matrix, of w3)
   void *kept_a, *kept_b;      // kGate: rows of `pitch` elements, n rounded up to 8; what lies behind n is of no meaning
   int pitch;
-  int cols, half, n_out, add; // kInput, kWeight: columns of c; kWeight: columns of a half of A, rows of c, and whether they are added to
+  int cols, half, n_out;      // kInput, kWeight: columns of c; kWeight: columns of a half of A, rows of c
+  float* sum;                 // kWeight of more tokens than a launch takes: the sums so far, rows of c, then of c2; null: one launch
+  int first, last;            // kWeight: of the launches: nothing is in the sums yet; c is written, and not the sums
   int row_tiles, col_tiles;
   int full, left, cut;        // tiles as a whole, then some whose slabs are cut into `cut` pieces, which go to parts
   float* parts;
@@ -37,11 +39,12 @@ int gated_tiles(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t
                 uint16_t* h, void* a, void* b, bool wide, float* parts, hipStream_t s);
 // g (tokens, terms, 2 half), half n_out rounded up to 64: the gradients of a and, from column half on, of b, zeros behind n_out, as sums of one or two
 // terms (two: up to 64 tokens); for dw each row of x stands there `terms` times.  Rows of x, w1, w3 `ld` elements apart, a multiple of 8.
-// dx (tokens, n_in), dw1 and dw3 (n_out, n_in), one of them or both, of any pitch; add: they are added to
+// dx (tokens, n_in), dw1 and dw3 (n_out, n_in), one of them or both, of any pitch; sums: of more tokens than a launch takes, (1 or 2, n_out, n_in)
+// numbers that go from the first launch to the last, which writes dw1 and dw3; or null
 int gated_tiles_input(int dtype, const uint16_t* g, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld,
                       int terms, uint16_t* dx, float* parts, hipStream_t s);
-int gated_tiles_weight(int dtype, const uint16_t* g, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld, bool add,
-                       int terms, uint16_t* dw1, uint16_t* dw3, float* parts, hipStream_t s);
+int gated_tiles_weight(int dtype, const uint16_t* g, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld,
+                       int terms, uint16_t* dw1, uint16_t* dw3, float* sums, bool first, bool last, float* parts, hipStream_t s);
 int64_t gated_tiles_bytes(int kind, int64_t tokens, int64_t n_in, int64_t n_out, int matrices = 2, int terms = 1);
 
 // parts: gated_parts_bytes, or null; wide: a and b in float32

@@ -402,7 +402,7 @@ constexpr int64_t kCacheBytes = 256 << 20;
 struct Backward {
   int terms;
   int64_t h, k, rows;  // n_out and n_in with their padding, tokens of a launch
-  int64_t g, w1, w3, x, parts, bytes;
+  int64_t g, w1, w3, x, sums, parts, bytes;  // sums: float32, of the weights' gradients between launches
   Backward(int64_t tokens, int64_t n_in, int64_t n_out, int what) {  // (what: 1 dx, 2 dw1, 4 dw3)
     Room room;
     terms = tokens <= kTwoTerms ? 2 : 1;
@@ -412,6 +412,7 @@ struct Backward {
     w1 = (what & 1) && k != n_in ? room.take(2 * n_out * k) : 0;
     w3 = (what & 1) && k != n_in ? room.take(2 * n_out * k) : 0;
     x = what > 1 && (k != n_in || terms > 1) ? room.take(2 * terms * rows * k) : 0;
+    sums = what > 1 && tokens > rows ? room.take(4 * n_out * n_in * (what >= 6 ? 2 : 1)) : 0;
     // (the products run one after the other)
     int64_t most = 0;
     for (const int64_t n : {rows, std::max<int64_t>(tokens % rows, 1)}) {
@@ -534,7 +535,10 @@ extern "C" int mega_gated_linear_bwd(const void* dh_, const void* x_, const void
     if (dx != nullptr)
       if (const int rc = gated_tiles_input(dtype, g, w1, w3, n, n_in, n_out, k, f.terms, dx + t * n_in, parts, s); rc != MEGA_OK) return rc;
     if (what > 1)
-      if (const int rc = gated_tiles_weight(dtype, g, rows, n, n_in, n_out, k, t > 0, f.terms, dw1, dw3, parts, s); rc != MEGA_OK) return rc;
+      if (const int rc = gated_tiles_weight(dtype, g, rows, n, n_in, n_out, k, f.terms, dw1, dw3, tokens > f.rows ? reinterpret_cast<float*>(ws + f.sums) : nullptr, t == 0,
+                                            t + n == tokens, parts, s);
+          rc != MEGA_OK)
+        return rc;
   }
   return MEGA_OK;
 }

@@ -118,22 +118,28 @@ __device__ __forceinline__ void finish(const GatedTiles& p, const f32x4* acc, in
     const bool second = MODE == kWeight && row >= p.half;
     const int in_half = second ? row - p.half : row;
     if (MODE == kWeight && in_half >= p.n_out) return;
-    uint16_t* const to = (second ? p.c2 : p.c) + static_cast<int64_t>(in_half) * p.cols;
+    const int64_t at = static_cast<int64_t>(in_half) * p.cols;
+    uint16_t* const to = (second ? p.c2 : p.c) + at;
+    float* const sum = p.sum + (MODE == kWeight && second ? at + static_cast<int64_t>(p.n_out) * p.cols : at);
 #pragma unroll
     for (int f = 0; f < 4; f += 2) {
       uint2 v[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         f32x4 c = acc[f + t];
-        if (MODE == kWeight && p.add) {
+        if (MODE == kWeight && p.sum != nullptr) {
           const int col = n0 + wn * 64 + 16 * (f + t) + 4 * g;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (col + e < p.cols) c[e] += Elem<DT>::load(to + col + e);
+          for (int e = 0; e < 4; ++e) {
+            if (col + e >= p.cols) break;
+            if (!p.first) c[e] += sum[col + e];
+            if (!p.last) sum[col + e] = c[e];
+          }
         }
         v[t] = pack4<DT>(c);
       }
       const int col = n0 + wn * 64 + 16 * f + in32;
+      if (MODE == kWeight && !p.last) continue;
       store_eight(to + col, p.cols - col, rows_of_eight(v[0], v[1]));
     }
   }
@@ -472,13 +478,14 @@ int gated_tiles_input(int dtype, const uint16_t* g, const uint16_t* w1, const ui
   return terms == 2 ? launch_of<kInputTwo, 0>(dtype, p, parts, s) : launch_of<kInput, 0>(dtype, p, parts, s);
 }
 
-int gated_tiles_weight(int dtype, const uint16_t* g, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld, bool add,
-                       int terms, uint16_t* dw1, uint16_t* dw3, float* parts, hipStream_t s) {
+int gated_tiles_weight(int dtype, const uint16_t* g, const uint16_t* x, int64_t tokens, int64_t n_in, int64_t n_out, int64_t ld,
+                       int terms, uint16_t* dw1, uint16_t* dw3, float* sums, bool first, bool last, float* parts, hipStream_t s) {
   const int64_t both = 2 * half_of(n_out);
   GatedTiles p = sizes_of(kWeight, tokens, n_in, n_out, dw1 != nullptr && dw3 != nullptr ? 2 : 1, terms);
   const int64_t from = dw1 != nullptr ? 0 : both / 2;
   p.a = g + from, p.b = p.b2 = x, p.a_bytes = bytes_of(terms * tokens, both, both - from), p.b_bytes = bytes_of(terms * tokens, ld, ld);
-  p.n = static_cast<int>(ld), p.lda = static_cast<int>(both), p.ldb = static_cast<int>(ld), p.c = dw1 != nullptr ? dw1 : dw3, p.c2 = dw3, p.add = add;
+  p.n = static_cast<int>(ld), p.lda = static_cast<int>(both), p.ldb = static_cast<int>(ld), p.c = dw1 != nullptr ? dw1 : dw3, p.c2 = dw3;
+  p.sum = sums, p.first = first, p.last = last;
   return launch_of<kWeight, 0>(dtype, p, parts, s);
 }
 

@@ -124,3 +124,27 @@ def test_gradients_of_several_outputs_at_once():
             assert (g[i].double() - w).norm() <= 2.0 ** -8 * (1 + 1 / 64) * w.norm()  # (one rounding of the float32 formula)
     none = torch.autograd.grad(h, leaves, torch._efficientzerotensor((40, 16), dtype=h.dtype, device="cuda"))
     assert all(g.shape == t.shape and not g.any() for g, t in zip(none, leaves))
+
+
+@pytest.mark.parametrize("asked", [(1, 2), (2,)])
+def test_weight_gradients_of_many_launches(asked):
+    """Rows of 2^20 elements: 768 tokens to a launch.  The weights' gradients are summed in float32 through all launches and rounded once: whole numbers
+    whose sums are below 2^24 come out as their sum's rounding."""
+    tokens, n_in, n_out = 3 * 768 + 41, 1 << 20, 5
+    g = torch.Generator("cuda").manual_seed(3)
+    # a = 0 (silu = 0, silu' = 1/2), b = 2^b: da = dh 2^b / 2, db = 0 ... and with w1 of the first feature, where a is large: silu(a) = a
+    x = torch.randint(0, 2, (tokens, n_in), generator=g, device="cuda", dtype=torch.int8).bfloat16()
+    x[:, 0] = 1
+    w1, w3 = torch.zeros(n_out, n_in, device="cuda").bfloat16(), torch.zeros(n_out, n_in, device="cuda").bfloat16()
+    w1[:, 0], w3[:, 0] = 64.0, 1.0  # a = 64, silu(a) = 64 and silu'(a) = 1 in float32, b = 1
+    dh = torch.randint(1, 4, (tokens, n_out), generator=g, device="cuda").bfloat16()
+    leaves = [x, *(w.requires_grad_(i in asked) for i, w in ((1, w1), (2, w3)))]
+    h = fused_ops.gated_linear(*leaves)
+    assert torch.equal(h, torch.full_like(h, 64.0))
+    grads = torch.autograd.grad(h, [leaves[i] for i in asked], dh)
+    for i, got in zip(asked, grads):
+        want = torch.zeros(n_out, n_in, dtype=torch.float64, device="cuda")
+        for at in range(0, tokens, 256):
+            want += (dh[at:at + 256].double() * (1 if i == 1 else 64)).t() @ x[at:at + 256].double()
+        assert want.max() < 1 << 24 and (want.bfloat16().double() != want).any()
+        assert torch.equal(got, want.float().bfloat16())
