@@ -157,8 +157,16 @@ __global__ __launch_bounds__(kTotalThreads) void total_kernel(const double* tota
   *out = static_cast<float>(sum);
 }
 
+// What a gradient is scaled by, in two parts: the ratio is below float32's normal numbers where gradients near the largest ones are clipped to a small norm.
+// (Bit for bit the product with a float32 where that is a normal number.)
+struct Factor {
+  float part;
+  int exponent;
+  __device__ __forceinline__ float times(float v) const { return __builtin_amdgcn_ldexpf(v * part, exponent); }
+};
+
 template <int DT, bool APART>
-__device__ __forceinline__ void scale_chunk(const Chunk& c, float factor) {
+__device__ __forceinline__ void scale_chunk(const Chunk& c, const Factor& factor) {
   using T = typename Elem<DT>::type;
   constexpr int kPer = DT == MEGA_F32 ? 4 : 8, kAhead = 4;
   const T* const p = static_cast<const T*>(c.from);
@@ -168,7 +176,7 @@ __device__ __forceinline__ void scale_chunk(const Chunk& c, float factor) {
     float v[kPer];
     unpack<DT>(q, v);
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) v[e] *= factor;
+    for (int e = 0; e < kPer; ++e) v[e] = factor.times(v[e]);
     uint4 w;
     if constexpr (DT == MEGA_F32) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
     else w = pack8<DT>(v);
@@ -185,18 +193,20 @@ __device__ __forceinline__ void scale_chunk(const Chunk& c, float factor) {
     for (int a = 0; a < kAhead; ++a) scaled(q[a], i + a * kThreads);
   }
   for (; i < whole; i += kThreads) scaled(__builtin_bit_cast(u32x4, *reinterpret_cast<const u32x4_any*>(p + static_cast<int64_t>(i) * kPer)), i);
-  if (const int rest = whole * kPer + threadIdx.x; rest < c.n) Elem<DT>::store(to + rest, Elem<DT>::load(p + rest) * factor);
+  if (const int rest = whole * kPer + threadIdx.x; rest < c.n) Elem<DT>::store(to + rest, factor.times(Elem<DT>::load(p + rest)));
 }
 
 __global__ __launch_bounds__(kThreads) void scale_kernel(const Tensors t, const double* norm, double max_norm) {
   const double ratio = max_norm / (*norm + 1e-6);
-  const float factor = ratio >= 1 ? 1.f : static_cast<float>(ratio);  // (NaN stays NaN)
+  int exponent = 0;
+  const float part = ratio >= 1 ? 1.f : static_cast<float>(frexp(ratio, &exponent));  // (NaN stays NaN)
+  const Factor factor{part, exponent};
   const uint32_t chunks = t.start[t.count];
   for (uint32_t i = blockIdx.x; i < chunks; i += gridDim.x) {
     // (from the end: what the norm read last is the likeliest to be in the memory-side cache)
     const Chunk k = chunk_of(t, chunks - 1 - i);
     const bool apart = k.from != k.to;
-    if (factor == 1.f && !apart) continue;
+    if (part == 1.f && exponent == 0 && !apart) continue;
     const auto run = [&](auto together, auto streaming) { apart ? streaming(k, factor) : together(k, factor); };
     if (k.dtype == MEGA_F32) run(scale_chunk<MEGA_F32, false>, scale_chunk<MEGA_F32, true>);
     else if (k.dtype == MEGA_BF16) run(scale_chunk<MEGA_BF16, false>, scale_chunk<MEGA_BF16, true>);
