@@ -45,9 +45,10 @@ class NormalizedFeedForwardNetwork(nn.Module):
     def takes_fused_gate(self, x: torch.Tensor) -> bool:
         """Rows and weights of one 16-bit type on the GPU, of sizes that the operator takes, and layers whose call is nothing but `Linear.forward`."""
         layers = (self.fc1, self.fc3)
+        if not (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and all(is_bare(l) and l.bias is None and l.weight.dtype == x.dtype for l in layers)):
+            return False
         n_out, n_in = (-(-n // 64) * 64 for n in self.fc1.weight.shape)
-        return (2 * n_in * n_out < 1 << 30 and max(n_in, n_out) <= 1 << 20 and x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and not torch.is_autocast_enabled("cuda")
-                and all(l.weight.dtype == x.dtype and l.bias is None and is_bare(l) for l in layers))
+        return 2 * n_in * n_out < 1 << 30 and max(n_in, n_out) <= 1 << 20 and not torch.is_autocast_enabled("cuda")
 
     def forward(self, x, residual):
         x = self.norm(x)

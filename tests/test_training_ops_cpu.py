@@ -148,3 +148,20 @@ def test_which_networks_take_the_fused_gate():
         assert net.takes_fused_gate(x) == takes
     del net.__dict__["fused_gate"]
     assert net.fused_gate is False
+
+
+def test_fused_gate_beside_layers_of_other_kinds():
+    """A projection that is no `Linear`, and has no weight, goes where it went without the choice."""
+
+    class Halves(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.parts = torch.nn.ModuleList([torch.nn.Linear(8, 8), torch.nn.Linear(8, 8)])
+
+        def forward(self, x):
+            return torch.cat([p(x) for p in self.parts], -1)
+
+    net = NormalizedFeedForwardNetwork(8, 16, swiglu=True, fused_gate=True)
+    net.fc1 = Halves()
+    assert not net.takes_fused_gate(torch.zeros(1, 8))
+    assert not net.takes_fused_gate(types.SimpleNamespace(is_cuda=True, dtype=torch.bfloat16))
