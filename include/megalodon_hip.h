@@ -577,7 +577,8 @@ int mega_tensors_clip(const mega_tensors* tensors, double max_norm, const void* 
  *   fwd: a = x w1^T and b = x w3^T as well, in `kept` (`dtype` or MEGA_F32), rows of n_out rounded up to 8 elements (what lies
  *        behind n_out has no meaning), or null for both; they are what bwd wants.
  *   bwd: dx (tokens, n_in), dw1 and dw3 (n_out, n_in); null: not wanted.  The gradients of a and b are
- *        rounded to `dtype`, operands of the matrix cores as they are (up to 64 tokens: to two terms of it); sums are float32 and rounded once.
+ *        rounded to `dtype`, operands of the matrix cores as they are (up to 64 tokens: to two terms of it; in float16 they are infinite beyond 65504, and the
+ *        gradients of their token and feature not finite); sums are float32 and rounded once.
  * Sizes whose rows are no whole 16-byte pieces are laid out anew in `workspace`.  It holds the mega_gated_linear_workspace_bytes
  * (backward = 0, or bits: 1 for dx, 2 for dw1, 4 for dw3) bytes that the call wants, on a 16-byte boundary. */
 int64_t mega_gated_linear_workspace_bytes(int64_t tokens, int64_t n_in, int64_t n_out, int backward);

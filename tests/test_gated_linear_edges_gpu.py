@@ -148,3 +148,44 @@ def test_weight_gradients_of_many_launches(asked):
             want += (dh[at:at + 256].double() * (1 if i == 1 else 64)).t() @ x[at:at + 256].double()
         assert want.max() < 1 << 24 and (want.bfloat16().double() != want).any()
         assert torch.equal(got, want.float().bfloat16())
+
+
+@pytest.mark.parametrize("tokens", [9, 64, 70, 300])
+def test_float16_gradients_out_of_range(tokens):
+    """The gradients of a and b are float16 numbers on their way: where one is beyond 65504, its token's dx and its feature's dw are not finite, as in a network of
+    separate layers, never finite and wrong.  All others are the formula's."""
+    n_in, n_out = 64, 40
+    x, w1, w3, dh = operands(tokens, n_in, n_out, torch.float16)
+    x[3], w3[5] = 1.0, 2.0  # b = 128 there, a = -64 .. 64
+    w1[5] = 1 / 16  # a = 4: silu(a) = 3.93, silu' = 1.05; da = 1.05 * 128 dh, db = 3.93 dh
+    dh[:, 5] = 0
+    dh[3, 5] = 2000.0  # da = 2.7e5, db = 7900
+    leaves = leaves_of(x, w1, w3)
+    dx, d1, d3 = torch.autograd.grad(fused_ops.gated_linear(*leaves), leaves, dh)
+    others = [i for i in range(tokens) if i != 3]
+    assert not dx[3].isfinite().any() and not d1[5].isfinite().any()
+    assert dx[others].isfinite().all() and d3.isfinite().all() and d1[[i for i in range(n_out) if i != 5]].isfinite().all()
+    dh[3, 5] = 400.0  # da = 54000: a float16 number
+    got = torch.autograd.grad(fused_ops.gated_linear(*leaves), leaves, dh)
+    wide = [t.double().requires_grad_(True) for t in (x, w1, w3)]
+    want = torch.autograd.grad(torch.nn.functional.silu(wide[0] @ wide[1].t()) * (wide[0] @ wide[2].t()), wide, dh.double())
+    for g, w in zip(got, want):
+        assert g.isfinite().all() and (g.double() - w).norm() <= 3 * 2.0 ** -11 * w.norm()  # (da, db, the result)
+
+
+@pytest.mark.parametrize("tokens", [40, 200])
+def test_small_float16_gradients(tokens):
+    """Below 2^-14 float16 numbers lie 2^-24 apart: da and db, and with two terms what they leave, are off by 2^-25 at most, beside half a step."""
+    x, w1, w3, dh = operands(tokens, 64, 40, torch.float16)
+    dh = dh * 2.0 ** -13
+    leaves = leaves_of(x, w1, w3)
+    got = torch.autograd.grad(fused_ops.gated_linear(*leaves), leaves, dh)
+    x, w1, w3, dh = (t.double() for t in (x, w1, w3, dh))
+    a, b = x @ w1.t(), x @ w3.t()
+    s = torch.sigmoid(a)
+    da, db = dh * b * s * (1 + a * (1 - s)), dh * a * s
+    u, least = 2.0 ** -11, 2.0 ** -25
+    off = lambda t: t.abs() * (u + 2.0 ** -16) + least  # (2^-16: float32's part, exp among it)
+    ea, eb = off(da), off(db)
+    for g, w, e in ((got[0], da @ w1 + db @ w3, ea @ w1.abs() + eb @ w3.abs()), (got[1], da.t() @ x, ea.t() @ x.abs()), (got[2], db.t() @ x, eb.t() @ x.abs())):
+        assert ((g.double() - w).abs() <= e * 1.01 + (w.abs() + e) * u + least).all()
