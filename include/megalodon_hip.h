@@ -531,7 +531,7 @@ int mega_silu_mul_bwd(const void* dout, const void* a, const void* b, int dtype,
  * tokens: n numbers of token_bits (32 or 64) bits; table (vocab, width), rows ld elements apart; out, dy (n, width) and dw
  * (vocab, width) contiguous, of `dtype` (MEGA_F32, MEGA_BF16, MEGA_F16), on any element's boundary.  n and vocab below 2^31,
  * width up to 2^20.  A token that is no row of the table gives zeros and has no gradient; padding: a row without a gradient, or -1.
- * Float32 inside, one rounding; sums run in an order that the sizes alone set, without atomics.
+ * Float32 inside, one rounding; sums run in an order that sizes and tokens alone set, without atomics.
  * bwd writes every row of dw and uses mega_embedding_workspace_bytes(...) bytes on a 16-byte boundary. */
 int mega_embedding_fwd(const void* tokens, int token_bits, const void* table, int dtype, int64_t n, int64_t vocab, int64_t width,
                        int64_t ld, double scale, void* out, void* stream);

@@ -2164,7 +2164,8 @@ int64_t gated_parts_bytes(int64_t tokens, int64_t n_in, int64_t n_out) {
 int gated_product(int dtype, const uint16_t* x, const uint16_t* w1, const uint16_t* w3, int64_t tokens, int64_t n_in, int64_t n_out,
                   uint16_t* h, void* a, void* b, bool wide, float* parts, hipStream_t s) {
   // The small tiles want slabs of 64 k: rows of other lengths would be laid out anew for them.  (us, so / large tiles, 65, 256, 512, 1024 tokens: 4088 -> 11008 127 / 74, 153 / 87,
-  // 162 / 112, 220 / 181, 2056 -> 5504 36 / 30, 42 / 37, 49 / 58, 64 / 58, 1000 -> 2736 22 / 19, 23 / 25, 23 / 31, 29 / 30)
+  // 162 / 112, 220 / 181, 2056 -> 5504 36 / 30, 42 / 37, 49 / 58, 64 / 58, 1000 -> 2736 22 / 19, 23 / 25, 23 / 31, 29 / 30: one rule for all, which the middle sizes of the
+  // narrower networks lose by)
   if (n_in % 64 != 0) return gated_tiles(dtype, x, w1, w3, tokens, n_in, n_out, h, a, b, wide, parts, s);
   GemmParams g{};
   g.A = x; g.B = w1; g.B2 = w3; g.C = h; g.Ca = a; g.Cb = b; g.wide = wide;

@@ -44,7 +44,9 @@ constexpr int kFewWaves = 8;
 
 // Which calls go here: up to 16 tokens all; then the tokens, read again for every few features, cost more than the tiles' second launch
 // the more the larger the weights are (us, here / tiles: 4096 -> 11008 16 tokens 47 / 50, 24 53 / 51, 64 80 / 54; 2048 -> 5504
-// 16 15 / 19, 48 20.2 / 20.7, 64 21.9 / 20.8; 1024 -> 2752 64 8.4 / 12.7).  Rows that the small tiles do not take: up to 64.
+// 16 15 / 19, 48 20.2 / 20.7, 64 21.9 / 20.8; 1024 -> 2752 64 8.4 / 12.7).  Rows that the small tiles do not take (n_in no multiple of 64): up to 64, since the large
+// tiles' time hardly falls with the tokens (17, 32, 48, 64 tokens: 1000 -> 2736 6 / 15, 6 / 15, 8 / 16, 8 / 17; 1001 -> 2731 9 / 20, 11 / 20, 15 / 21, 16 / 21; 2056 -> 5504 17 / 27,
+// 19 / 27, 23 / 28, 26 / 28; 4088 -> 11008 58 / 64, 70 / 65, 80 / 66, 90 / 67; 4085 -> 11007 89 / 115, 114 / 119, 149 / 121, 173 / 123: the largest network's 32 to 64 tokens lose by it).
 bool few(int64_t tokens, int64_t n_in, int64_t n_out) {
   if (tokens <= 16 || tokens > 64) return tokens <= 16;
   return n_in % 64 != 0 || static_cast<double>(tokens - 16) * n_in * n_out <= 4e8;
@@ -149,8 +151,10 @@ __global__ __launch_bounds__(kFewWaves * kWave) void gated_few_kernel(const FewP
   }
 }
 
-// 9 to 16 tokens with their rows in LDS: a workgroup for each CU walks the groups of 8 features, and the next group's weights are on their way into registers
-// while the current one's products run and the waves' sums meet.  Read again for every group, as above, so many tokens are half as many bytes as the weights
+// 9 to 16 tokens with their rows in LDS: a workgroup for each CU walks the groups of 8 features.  The next group's weights are asked for in front of the current one's
+// products, but waited for there too: the requests lie behind branches (rows' ends, the last group), and the compiler waits for all that it cannot count.  So a group's
+// time is its weights' way from memory and the waves' meeting, one after the other; the variant of eight steps also keeps three addresses in
+// scratch.  Read again for every group, as above, so many tokens are half as many bytes as the weights
 // and more; fewer cost less than the part-filled last walk here.  (us, above / here, weights from memory, 8, 12, 16 tokens: 4096 -> 11008 47 / 47, 50 / 47.5, 52.8 / 48.6, 2048 -> 5504 12.4 / 13.5,
 // 13.8 / 13.9, 15.8 / 14.3, 1536 -> 40000 63 / 60, 67 / 62, 70 / 62; 1024 -> 2752 the same.)  STEPS: of 32 k for each wave, at most.
 // A row's chunk c of 16 bytes is at c ^ row: sixteen lanes on different banks.

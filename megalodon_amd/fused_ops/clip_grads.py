@@ -30,7 +30,10 @@ def clip_grads(tensors: Sequence[Tensor], max_norm: float, norm_type: float = 2.
 
 
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0) -> Tensor:
-    """`torch.nn.utils.clip_grad_norm_`: clips the `.grad` of the parameters (those that have one) in place, returns their norm."""
+    """`torch.nn.utils.clip_grad_norm_` for what this module takes: clips the `.grad` of the parameters (those that have one) in place, returns their norm.
+
+    Raises for other norms, gradients of float64 or with gaps, and parameters that share a gradient; there is no `error_if_nonfinite`: as
+    nothing synchronises, a norm that is not finite is returned, and the gradients are scaled by it (NaN, or zeros for an infinite norm's finite ones)."""
     parameters = [parameters] if isinstance(parameters, Tensor) else parameters
     grads = [p.grad for p in parameters if p.grad is not None]
     return _lib.host().clip_grads(grads, grads, max_norm, norm_type, True) if grads else torch.tensor(0.0)

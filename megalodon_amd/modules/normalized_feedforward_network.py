@@ -3,7 +3,8 @@ for model-parallel world size 1: Column/RowParallelLinear are plain `nn.Linear`
 (megalodon/modules/model_parallel/layers.py:222-235,321-341); the two dropouts
 sit where the reference has them (:83-90).  `fused_gate`: with `swiglu` and 16-bit rows the two projections and the gate
 (:82) are one operator, `fused_ops.gated_linear`, whose gate sees the products in float32; elsewhere, and by default, they are two
-products and `silu_mul`."""
+products and `silu_mul`.  The operator is ahead without gradients, and with them on ordinary sizes; its products are kept in float32, which costs the largest trainings
+more than the gate's pass (32768 tokens, 4096 -> 11008 13.6 ms forward and backward, 13.0 without; 4096 tokens, 1024 -> 2752 0.197, 0.193)."""
 import torch
 import torch.nn.functional as F
 from torch import nn
