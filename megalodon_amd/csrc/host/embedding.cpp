@@ -10,6 +10,9 @@ using torch::autograd::AutogradContext;
 using torch::autograd::Function;
 using torch::autograd::variable_list;
 
+// (autocast leaves rows of a table in their type)
+bool shown() { return watched(c10::autocast_dispatch_keyset); }
+
 Tensor gather(const Tensor& tokens, const Tensor& table, double scale) {
   const int64_t n = tokens.numel(), width = table.size(1);
   auto shape = tokens.sizes().vec();
@@ -69,7 +72,7 @@ struct EmbeddingFn : Function<EmbeddingFn> {
     const double scale = ctx->saved_data["scale"].toDouble();
     const int64_t padding = ctx->saved_data["padding"].toInt(), vocab = ctx->saved_data["vocab"].toInt();
     c10::DeviceGuard guard(g[0].device());
-    if (watched() || !plain(stored(g[0]))) {  // (several gradients at once)
+    if (shown() || !plain(stored(g[0]))) {  // (several gradients at once)
       const int64_t width = g[0].size(-1);
       const Tensor t = tokens.reshape({-1}).to(at::kLong), counts = at::logical_and(at::logical_and(t.ge(0), t.lt(vocab)), t.ne(padding));
       const Tensor rows = at::where(counts.unsqueeze(1), g[0].reshape({-1, width}).to(at::kFloat), at::zeros({}, g[0].options().dtype(at::kFloat)));
@@ -103,7 +106,7 @@ Tensor embedding(const Tensor& tokens_, const Tensor& table_, double scale, std:
   }
   // what watches the thread's operations is shown operations
   const Tensor given = stored(tokens_), table = stored(table_);
-  if (watched() || !plain(given) || !plain(table)) return recorded(given, table, scale, padding);
+  if (shown() || !plain(given) || !plain(table)) return recorded(given, table, scale, padding);
   c10::DeviceGuard guard(table.device());
   const Tensor tokens = given.contiguous();
   if ((at::GradMode::is_enabled() && table.requires_grad()) || has_tangent(table)) return EmbeddingFn::apply(table, tokens, scale, padding);

@@ -53,9 +53,10 @@ inline bool has_tangent(const Tensor& t) { return t._fw_grad(/*level=*/0).define
 // Whether the thread shows its operations to something beside autograd: the TorchScript tracer, a mode that counts flops
 // or makes fake tensors, a functorch transform.  A launch is no operation -- a trace of one holds the allocation of its
 // result and nothing that fills it -- so these are given the library's operations.
-inline bool watched() {
+// (`but`: what an operator has nothing to show to)
+inline bool watched(c10::DispatchKeySet but = {}) {
   const auto tls = c10::impl::tls_local_dispatch_key_set();
-  return (tls.included_ - tls.excluded_ - c10::default_included_set).highestFunctionalityKey() != c10::DispatchKey::Undefined;
+  return (tls.included_ - tls.excluded_ - c10::default_included_set - but).highestFunctionalityKey() != c10::DispatchKey::Undefined;
 }
 // Whether a tensor is what its memory holds and nothing more: dispatch keys of a dense tensor, no subclass, functional
 // wrapper, zeros without memory or batch.

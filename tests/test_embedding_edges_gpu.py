@@ -157,3 +157,21 @@ def test_saved_tokens_in_other_places_and_types():
         with torch.autograd.graph.saved_tensors_hooks(pack, back):
             got, = torch.autograd.grad(fused_ops.embedding(tokens, weight), weight, dy)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_under_autocast(dtype):
+    """Autocast has nothing to cast: the same kernels, bit for bit, in the table's type."""
+    n, V, D = 9000, 40, 72
+    g = torch.Generator("cuda").manual_seed(2)
+    tokens = foreign(9, (n,))
+    weight = torch.randn(V, D, generator=g, device="cuda").to(dtype).requires_grad_(True)
+    dy = torch.randn(n, D, generator=g, device="cuda").to(dtype)
+    want = fused_ops.embedding(tokens, weight, 3.0)
+    grad, = torch.autograd.grad(want, weight, dy)
+    for cast in (torch.bfloat16, torch.float16):
+        with torch.autocast("cuda", cast):
+            y = fused_ops.embedding(tokens, weight, 3.0)
+            inside, = torch.autograd.grad(y, weight, dy, retain_graph=True)
+        assert y.dtype == dtype and torch.equal(y, want) and type(y.grad_fn) is type(want.grad_fn)
+        assert torch.equal(inside, grad) and torch.equal(torch.autograd.grad(y, weight, dy)[0], grad)
