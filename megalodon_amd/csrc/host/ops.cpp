@@ -802,8 +802,9 @@ variable_list gated_grads(const Tensor& dh_, const Tensor& x_, const Tensor& w1_
   }
   return {dx, d1, d3};
 }
-// The same by recorded operations, in float32 from the operands.
+// The same by recorded operations, in float32 from the operands (autocast would take the products in 16 bits).
 variable_list gated_recorded(const Tensor& dh, const Tensor& x, const Tensor& w1, const Tensor& w3, Wanted wanted) {
+  const c10::impl::ExcludeDispatchKeyGuard uncast(c10::autocast_dispatch_keyset);
   const auto type = x.scalar_type();
   const Tensor go = flat(dh).to(at::kFloat), xf = flat(x).to(at::kFloat), f1 = w1.to(at::kFloat), f3 = w3.to(at::kFloat);
   const Tensor a = at::mm(xf, f1.t()), b = at::mm(xf, f3.t()), s = at::sigmoid(a);
@@ -830,6 +831,7 @@ struct GatedGradFn : Function<GatedGradFn> {
     const auto flags = ctx->saved_data["wanted"].toIntVector();
     c10::DeviceGuard guard(saved[0].device());
     at::AutoGradMode on(true);
+    const c10::impl::ExcludeDispatchKeyGuard uncast(c10::autocast_dispatch_keyset);
     variable_list in, asked, out, from;  // (aliases, so that what one operand has to do with another is none of these gradients)
     for (size_t i = 0; i < 4; ++i) {
       in.push_back(at::alias(saved[i]));
@@ -867,7 +869,7 @@ struct GatedFn : Function<GatedFn> {
                 saved[3].numel() == rows * ((out + 7) / 8 * 8) && saved[4].sizes() == saved[3].sizes(),
             "gated_linear: a saved tensor has another shape than it was saved with");
     variable_list grads;
-    if (const Tensor dh = stored(g[0]); watched() || !plain(dh)) {  // (several gradients at once, zeros without memory)
+    if (const Tensor dh = stored(g[0]); watched(c10::autocast_dispatch_keyset) || !plain(dh)) {  // (several gradients at once, zeros without memory)
       grads = gated_recorded(dh, saved[0], saved[1], saved[2], wanted);
       grads.emplace_back();
       return grads;

@@ -189,3 +189,26 @@ def test_small_float16_gradients(tokens):
     ea, eb = off(da), off(db)
     for g, w, e in ((got[0], da @ w1 + db @ w3, ea @ w1.abs() + eb @ w3.abs()), (got[1], da.t() @ x, ea.t() @ x.abs()), (got[2], db.t() @ x, eb.t() @ x.abs())):
         assert ((g.double() - w).abs() <= e * 1.01 + (w.abs() + e) * u + least).all()
+
+
+def test_gradients_under_autocast():
+    """Autocast has nothing to cast in them: the kernels' gradients, and their own in float32, bit for bit."""
+    x, w1, w3, dh = operands(90, 40, 24, torch.bfloat16)
+    us = [torch.randn_like(t) for t in (x, w1, w3)]
+
+    def run():
+        leaves = leaves_of(x, w1, w3, dh)
+        h = fused_ops.gated_linear(*leaves[:3])
+
+        def grads():
+            once = torch.autograd.grad(h, leaves[:3], dh, retain_graph=True)
+            again = torch.autograd.grad(h, leaves[:3], leaves[3], create_graph=True)
+            many = torch.autograd.grad(h, leaves[:3], torch.stack([dh, -dh]), is_grads_batched=True, retain_graph=True)
+            return [*once, *again, *many, *torch.autograd.grad(again, leaves, us)]
+        return grads
+
+    want = run()()
+    grads = run()
+    with torch.autocast("cuda", torch.float16):
+        got = grads()
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
