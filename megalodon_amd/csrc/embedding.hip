@@ -417,11 +417,12 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
 
 // Runs over the end of the piece that they begin in: the parts of it and of the pieces behind, in their order.  A workgroup has `columns` columns, VEC of
 // them a thread (4 in wide rows: a quarter of the workgroups, most of which find nothing to do; 32768 tokens, 4096 columns 10.6 us, 9.0 so); in narrow
-// rows its threads share a column's parts.  `sums`: a number of each thread, for the shares to meet in.
+// rows its threads share a column's parts.
 template <int DT, int VEC>
-__device__ __forceinline__ void join_one(const SumParams& p, int columns, uint32_t piece, uint32_t slice, float* sums_) {
+__global__ __launch_bounds__(kThreads) void join_kernel(const SumParams p, int columns) {
   const int per = columns / VEC;  // threads of the columns
-  const int tid = threadIdx.x, k = static_cast<int>(slice) * columns + tid % per * VEC, share = tid / per, shares = kThreads / per;
+  const unsigned slices = (p.width + columns - 1) / columns, group = group_number(), piece = group / slices;
+  const int tid = threadIdx.x, k = static_cast<int>(group % slices) * columns + tid % per * VEC, share = tid / per, shares = kThreads / per;
   const int64_t first = static_cast<int64_t>(piece) * p.per_piece, behind = first + p.per_piece;
   if (behind >= p.n) return;
   const uint32_t key = p.keys[behind], last = p.keys[behind - 1], head = p.keys[first], ahead = first > 0 ? p.keys[first - 1] : 0xffffffffu;
@@ -474,7 +475,7 @@ __device__ __forceinline__ void join_one(const SumParams& p, int columns, uint32
     for (; left > 0; --left) sum += load(open += step);
   }
   if (shares > 1) {
-    Floats* const sums = reinterpret_cast<Floats*>(sums_);
+    __shared__ Floats sums[kThreads];
     sums[tid] = sum;
     __syncthreads();
     if (share > 0) return;
@@ -484,17 +485,6 @@ __device__ __forceinline__ void join_one(const SumParams& p, int columns, uint32
 #pragma unroll
   for (int e = 0; e < VEC; ++e)
     if (e < columns_left) Elem<DT>::store(to + e, sum[e] * p.scale);
-}
-// (2^32 threads are the most of a launch: narrow rows of 2^26 tokens have more pieces than that many threads)
-constexpr int64_t kMostJoins = 1 << 20;
-template <int DT, int VEC>
-__global__ __launch_bounds__(kThreads) void join_kernel(const SumParams p, int columns, uint32_t items) {
-  __shared__ float sums[kThreads * VEC];
-  const uint32_t slices = (p.width + columns - 1) / columns;
-  for (uint32_t i = blockIdx.x; i < items; i += gridDim.x) {
-    join_one<DT, VEC>(p, columns, i / slices, i % slices, sums);
-    if (i + gridDim.x < items) __syncthreads();  // (the shares' numbers have been read)
-  }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------
@@ -597,10 +587,9 @@ int table_grad(const void* dy, const void* tokens, int token_bits, int64_t n, in
     int columns = 16;
     while (columns < kThreads && columns < width) columns *= 2;
     if (width >= 4 * kThreads) columns = 4 * kThreads;
-    const int64_t items = p.pieces * ((width + columns - 1) / columns);  // (fewer than 2^31 for any gradient that fits a device)
-    const unsigned grid = static_cast<unsigned>(std::min(items, kMostJoins));
-    if (columns > kThreads) join_kernel<DT, 4><<<grid, kThreads, 0, s>>>(p, columns, static_cast<uint32_t>(items));
-    else join_kernel<DT, 1><<<grid, kThreads, 0, s>>>(p, columns, static_cast<uint32_t>(items));
+    const dim3 grid = grid_of(p.pieces * ((width + columns - 1) / columns));  // (fewer than 2^31 for any gradient that fits a device)
+    if (columns > kThreads) join_kernel<DT, 4><<<grid, kThreads, 0, s>>>(p, columns);
+    else join_kernel<DT, 1><<<grid, kThreads, 0, s>>>(p, columns);
     MEGA_CHECK_LAUNCH();
   }
   return MEGA_OK;
