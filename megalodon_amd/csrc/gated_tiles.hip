@@ -120,7 +120,6 @@ __device__ __forceinline__ void finish(const GatedTiles& p, const f32x4* acc, in
     if (MODE == kWeight && in_half >= p.n_out) return;
     const int64_t at = static_cast<int64_t>(in_half) * p.cols;
     uint16_t* const to = (second ? p.c2 : p.c) + at;
-    float* const sum = p.sum + (MODE == kWeight && second ? at + static_cast<int64_t>(p.n_out) * p.cols : at);
 #pragma unroll
     for (int f = 0; f < 4; f += 2) {
       uint2 v[2];
@@ -128,6 +127,7 @@ __device__ __forceinline__ void finish(const GatedTiles& p, const f32x4* acc, in
       for (int t = 0; t < 2; ++t) {
         f32x4 c = acc[f + t];
         if (MODE == kWeight && p.sum != nullptr) {
+          float* const sum = p.sum + (second ? at + static_cast<int64_t>(p.n_out) * p.cols : at);
           const int col = n0 + wn * 64 + 16 * (f + t) + 4 * g;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
