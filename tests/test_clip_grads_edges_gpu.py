@@ -30,3 +30,16 @@ def test_factors_below_the_normal_numbers(max_norm, dtype, in_place):
         assert bool(((n.double() - v).abs() <= bar).all())
         if max_norm > 1e-30:
             assert n.any()
+
+
+def test_offsets_beyond_32_bits():
+    """A gradient of more than 2^32 elements between small ones: all counted, all scaled."""
+    n = (1 << 32) + 100_001
+    ts = [torch.ones(7, device="cuda"), torch.full((n,), 0.5, dtype=torch.bfloat16, device="cuda"), torch.ones(9, device="cuda")]
+    ts[1][-3:] = 64.0
+    want = (16 + (n - 3) * 0.25 + 3 * 4096) ** 0.5
+    norm, out = fused_ops.clip_grads(ts, want / 4, out=ts)
+    assert abs(norm.item() - want) <= 2 * U * want
+    for t, v in zip(out, (0.25, 0.125, 0.25)):
+        assert (t[:-3] - v).abs().max() <= 2.0 ** -8 * v
+    assert (out[1][-3:] - 16).abs().max() <= 2.0 ** -8 * 16

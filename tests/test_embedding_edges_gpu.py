@@ -175,3 +175,21 @@ def test_under_autocast(dtype):
             inside, = torch.autograd.grad(y, weight, dy, retain_graph=True)
         assert y.dtype == dtype and torch.equal(y, want) and type(y.grad_fn) is type(want.grad_fn)
         assert torch.equal(inside, grad) and torch.equal(torch.autograd.grad(y, weight, dy)[0], grad)
+
+
+def test_offsets_beyond_32_bits():
+    """A table, rows and a gradient of more than 2^32 elements each: the last rows of all three."""
+    V, D, n = 550_007, 8200, 530_000
+    weight = torch.zeros(V, D, dtype=torch.bfloat16, device="cuda")
+    last = torch.arange(V - 50, V, device="cuda")
+    weight[last] = torch.randn(50, D, device="cuda").bfloat16()
+    weight.requires_grad_(True)
+    tokens = torch.arange(n, device="cuda") % (V - 50)  # (each but once; the last 200 positions: the last 50 rows, four times each)
+    tokens[-200:] = last.repeat(4)
+    y = fused_ops.embedding(tokens, weight, 2.0)
+    assert y.numel() > 1 << 32 and torch.equal(y[-200:], 2 * weight.detach()[last].repeat(4, 1)) and not y[:-200][:: 4099].any()
+    dy = torch.ones_like(y)
+    dy[-200:] = torch.randint(-3, 4, (200, D), device="cuda").bfloat16()
+    dw, = torch.autograd.grad(y, weight, dy)
+    assert torch.equal(dw[last], 2 * dy[-200:].view(4, 50, D).float().sum(0).bfloat16())
+    assert dw[: n - 200 : 4099].eq(2).all() and not dw[n - 200 : V - 50].any()

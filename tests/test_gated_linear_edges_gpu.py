@@ -212,3 +212,21 @@ def test_gradients_under_autocast():
     with torch.autocast("cuda", torch.float16):
         got = grads()
     assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_offsets_beyond_32_bits():
+    """h, the kept products and the output gradient of more than 2^32 elements: the last tokens' rows are those of the same tokens alone."""
+    tokens, n_in, n_out, part = 262_200, 72, 16_400, 300
+    x, w1, w3, _ = operands(tokens, n_in, n_out, torch.bfloat16)
+    leaves = leaves_of(x, w1, w3)
+    h = fused_ops.gated_linear(*leaves, torch.bfloat16)
+    assert h.numel() > 1 << 32
+    dh = torch.zeros_like(h)
+    dh[-part:] = torch.randn(part, n_out, device="cuda").bfloat16()
+    dx, d1, d3 = torch.autograd.grad(h, leaves, dh)
+    some = leaves_of(x[-part:], w1, w3)
+    few = fused_ops.gated_linear(*some, torch.bfloat16)
+    assert not dx[:-part].any()
+    # the same formula, roundings that fall the other way where sums run in another order: two of them for h, four for the gradients
+    for got, want, times in ((h[-part:], few, 2), *zip((dx[-part:], d1, d3), torch.autograd.grad(few, some, dh[-part:]), (4, 4, 4))):
+        assert (got.double() - want.double()).norm() <= times * 2.0 ** -8 * want.double().norm()
